@@ -41,6 +41,27 @@ class Config(C.Structure):
                 ("temperature", C.c_float)]
 
 
+class Rows(C.Structure):
+    """boa_rows: a row tensor's first element and strides in elements."""
+    _fields_ = [("d", C.c_void_p), ("lane_stride", C.c_int64), ("row_stride", C.c_int64)]
+
+
+class Scan(C.Structure):
+    """boa_scan: the inputs of the selective scan."""
+    _fields_ = [("lanes", C.c_int32), ("T", C.c_int32), ("channels", C.c_int32),
+                ("d_state", C.c_int32), ("precision", C.c_int32), ("d_lens", C.c_void_p),
+                ("u", Rows), ("delta", Rows), ("z", Rows), ("b", Rows), ("c", Rows),
+                ("d_A", C.c_void_p), ("d_D", C.c_void_p), ("d_delta_bias", C.c_void_p),
+                ("d_state_in", C.c_void_p)]
+
+
+class ScanGrads(C.Structure):
+    """boa_scan_grads: the outputs of the scan's gradient."""
+    _fields_ = [("du", Rows), ("ddelta", Rows), ("dz", Rows), ("db", Rows), ("dc", Rows),
+                ("d_dA", C.c_void_p), ("d_dD", C.c_void_p), ("d_ddelta_bias", C.c_void_p),
+                ("d_dstate_in", C.c_void_p)]
+
+
 def build(clean: bool = False) -> str:
     """Compile libboa_hip.so and the boa CLI for gfx950 (hipcc)."""
     if clean:
@@ -87,6 +108,19 @@ def lib():
             "boa_forward_chunk": (C.c_int, [P, P, i32, i32, P]),
             "boa_step_batch": (C.c_int, [P, P, i32, P, i32]),
             "boa_forward_chunk_noalloc": (C.c_int, [P, P, i32, i32, P]),
+            "boa_device": (C.c_int, [P]),
+            "boa_embed": (C.c_int, [P, P, i64, P, i32, i32, P, i32, i32, f32, C.POINTER(Rows)]),
+            "boa_embed_grad": (C.c_int, [P, P, i64, P, i32, i32, C.POINTER(Rows), i32, i32, f32,
+                                         P, P, i64]),
+            "boa_embed_grad_work_bytes": (i64, [i32, i32, i32]),
+            "boa_selective_scan": (C.c_int, [P, C.POINTER(Scan), C.POINTER(Rows), P, P, P, i64]),
+            "boa_selective_scan_grad": (C.c_int, [P, C.POINTER(Scan), P, C.POINTER(Rows), P,
+                                                  C.POINTER(ScanGrads), P, i64]),
+            "boa_selective_scan_saved_floats": (i64, [i32, i32, i32, i32]),
+            "boa_selective_scan_work_bytes": (i64, [i32, i32, i32, i32, i32]),
+            "boa_next_byte_loss": (C.c_int, [P, C.POINTER(Rows), P, P, i64, P, i32, i32, i32, f32,
+                                             P, P, C.POINTER(Rows), P, P, i64]),
+            "boa_next_byte_loss_work_bytes": (i64, [i32, i32]),
             "boa_cdf_from_logits": (C.c_int, [P, P, P, i32, P]),
             "boa_cdf_from_probs": (C.c_int, [P, P, i32, i32, P]),
             "boa_rc_encode_cdf": (C.c_int, [P, P, P, i32, i32, P, i64, P]),
@@ -120,6 +154,85 @@ def _ptr(x):
     if isinstance(x, int):
         return x
     return x.data_ptr()
+
+
+# ---- training operators: tensors to C arguments
+# (what the C entry points cannot see -- types, shapes, devices -- is checked
+# here; sizes, strides, alignment and workspaces are checked there)
+_PRECISION = {"torch.float32": 0, "torch.bfloat16": 1}
+
+
+def _tensor(t, name, shape, dtype, device, dense=True):
+    """t's pointer (None for None), of this shape and type on this device."""
+    if t is None:
+        return None
+    if tuple(t.shape) != tuple(shape) or str(t.dtype) != dtype:
+        raise ValueError(f"{name}: want {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    if not t.is_cuda or t.device.index != device:
+        raise ValueError(f"{name} is on {t.device}, the context on cuda:{device}")
+    if dense and not t.is_contiguous():
+        raise ValueError(f"{name} has to be contiguous")
+    return t.data_ptr()
+
+
+def _rows(t, name, lanes, T, width, dtype, device):
+    """A [lanes, T, width] tensor, dense in its last dimension, as a Rows."""
+    d = _tensor(t, name, (lanes, T, width), dtype, device, dense=False)
+    if width > 1 and t.stride(2) != 1:
+        raise ValueError(f"{name} has to be dense in its last dimension")
+    return Rows(d, t.stride(0), t.stride(1))
+
+
+def _bytes(t, name, device):
+    """A uint8 [lanes, T] tensor, dense along T: (pointer, stride of a lane, lanes, T)."""
+    if t.dim() != 2:
+        raise ValueError(f"{name}: want [lanes, T], got {tuple(t.shape)}")
+    d = _tensor(t, name, t.shape, "torch.uint8", device, dense=False)
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} has to be dense along T")
+    return d, t.stride(0), t.shape[0], t.shape[1]
+
+
+def _precision(t, name):
+    p = _PRECISION.get(str(t.dtype))
+    if p is None or t.dim() != 3:
+        raise ValueError(f"{name}: want float32 or bfloat16 [lanes, T, width], got {t.dtype} "
+                         f"{tuple(t.shape)}")
+    return p, str(t.dtype)
+
+
+def _work(t, device):
+    """A workspace tensor of any type: (pointer, bytes)."""
+    if t is None:
+        return None, 0
+    n = t.numel() * t.element_size()
+    if n and (not t.is_cuda or t.device.index != device or not t.is_contiguous()):
+        raise ValueError(f"the workspace has to be contiguous, on cuda:{device}")
+    return (t.data_ptr() if n else None), n
+
+
+def _size(n, what):
+    if n < 0:
+        raise ValueError(f"{what}: sizes out of range")
+    return n
+
+
+def embed_grad_work_bytes(lanes, T, width):
+    return _size(lib().boa_embed_grad_work_bytes(lanes, T, width), "embed_grad")
+
+
+def selective_scan_saved_floats(lanes, T, channels, d_state):
+    return _size(lib().boa_selective_scan_saved_floats(lanes, T, channels, d_state),
+                 "selective_scan")
+
+
+def selective_scan_work_bytes(lanes, T, channels, d_state, grad=False):
+    return _size(lib().boa_selective_scan_work_bytes(lanes, T, channels, d_state, int(grad)),
+                 "selective_scan")
+
+
+def next_byte_loss_work_bytes(lanes, T):
+    return _size(lib().boa_next_byte_loss_work_bytes(lanes, T), "next_byte_loss")
 
 
 class Codec:
@@ -190,6 +303,112 @@ class Codec:
         self._check(lib().boa_rc_decode_cdf(self.h, _ptr(d_cdf), n_sym, lanes, _ptr(d_words),
                                             pitch_words, _ptr(d_sizes), _ptr(d_syms)),
                     "rc_decode_cdf")
+
+    # ---- training operators (boa_embed and the calls after it in boa_hip.h):
+    # tensors on the context's device; row tensors [lanes, T, width], float32
+    # or bfloat16, dense in their last dimension; d_lens int32 [lanes] or None
+    def _device(self):
+        return lib().boa_device(self.h)
+
+    def embed(self, d_tokens, d_table, d_out, scale=1.0, d_lens=None):
+        """out = scale * table[tokens]; table [256, width] of out's type."""
+        dev = self._device()
+        tok, stride, lanes, T = _bytes(d_tokens, "tokens", dev)
+        prec, dt = _precision(d_out, "out")
+        width = d_out.shape[2]
+        out = _rows(d_out, "out", lanes, T, width, dt, dev)
+        self._check(lib().boa_embed(
+            self.h, tok, stride, _tensor(d_lens, "lens", (lanes,), "torch.int32", dev), lanes, T,
+            _tensor(d_table, "table", (256, width), dt, dev), width, prec, scale, C.byref(out)),
+            "embed")
+
+    def embed_grad(self, d_tokens, d_dout, d_dtable, d_work=None, scale=1.0, d_lens=None):
+        """dtable (float32 [256, width]) = scale * sums of dout's rows by token."""
+        dev = self._device()
+        tok, stride, lanes, T = _bytes(d_tokens, "tokens", dev)
+        prec, dt = _precision(d_dout, "dout")
+        width = d_dout.shape[2]
+        dout = _rows(d_dout, "dout", lanes, T, width, dt, dev)
+        self._check(lib().boa_embed_grad(
+            self.h, tok, stride, _tensor(d_lens, "lens", (lanes,), "torch.int32", dev), lanes, T,
+            C.byref(dout), width, prec, scale,
+            _tensor(d_dtable, "dtable", (256, width), "torch.float32", dev),
+            *_work(d_work, dev)), "embed_grad")
+
+    def _scan_args(self, u, delta, z, b, c, A, D, delta_bias, state_in, lens):
+        dev, f32 = self._device(), "torch.float32"
+        prec, dt = _precision(u, "u")
+        lanes, T, ch = u.shape
+        if A.dim() != 2:
+            raise ValueError(f"A: want [channels, d_state], got {tuple(A.shape)}")
+        n = A.shape[1]
+        return Scan(lanes, T, ch, n, prec, _tensor(lens, "lens", (lanes,), "torch.int32", dev),
+                    *[_rows(t, k, lanes, T, w, dt, dev) for t, k, w in
+                      ((u, "u", ch), (delta, "delta", ch), (z, "z", ch), (b, "B", n), (c, "C", n))],
+                    _tensor(A, "A", (ch, n), f32, dev), _tensor(D, "D", (ch,), f32, dev),
+                    _tensor(delta_bias, "delta_bias", (ch,), f32, dev),
+                    _tensor(state_in, "state_in", (lanes, ch, n), f32, dev)), dt, dev
+
+    def selective_scan(self, d_u, d_delta, d_z, d_b, d_c, d_A, d_D, d_delta_bias, d_out,
+                       d_work=None, d_state_in=None, d_state_out=None, d_lens=None, d_saved=None):
+        """The gated recurrence; d_saved (selective_scan_saved_floats floats)
+        keeps what its gradient starts from."""
+        s, dt, dev = self._scan_args(d_u, d_delta, d_z, d_b, d_c, d_A, d_D, d_delta_bias,
+                                     d_state_in, d_lens)
+        out = _rows(d_out, "out", s.lanes, s.T, s.channels, dt, dev)
+        self._check(lib().boa_selective_scan(
+            self.h, C.byref(s), C.byref(out),
+            _tensor(d_state_out, "state_out", (s.lanes, s.channels, s.d_state), "torch.float32",
+                    dev),
+            self._saved(d_saved, s, dev), *_work(d_work, dev)), "selective_scan")
+
+    def _saved(self, t, s, dev):
+        if t is None:
+            return None
+        n = lib().boa_selective_scan_saved_floats(s.lanes, s.T, s.channels, s.d_state)
+        if t.numel() < n:
+            raise ValueError(f"saved: want {n} floats, got {t.numel()}")
+        return _tensor(t, "saved", t.shape, "torch.float32", dev)
+
+    def selective_scan_grad(self, d_u, d_delta, d_z, d_b, d_c, d_A, d_D, d_delta_bias, d_saved,
+                            d_dout, d_du, d_ddelta, d_dz, d_db, d_dc, d_dA, d_dD, d_ddelta_bias,
+                            d_work=None, d_state_in=None, d_dstate_out=None, d_dstate_in=None,
+                            d_lens=None):
+        """Gradients of selective_scan, from its inputs, its d_saved and the
+        gradients of its outputs (d_dstate_out None: zero)."""
+        s, dt, dev = self._scan_args(d_u, d_delta, d_z, d_b, d_c, d_A, d_D, d_delta_bias,
+                                     d_state_in, d_lens)
+        f32, ch, n = "torch.float32", s.channels, s.d_state
+        state = (s.lanes, ch, n)
+        dout = _rows(d_dout, "dout", s.lanes, s.T, ch, dt, dev)
+        g = ScanGrads(*[_rows(t, k, s.lanes, s.T, w, dt, dev) for t, k, w in
+                        ((d_du, "du", ch), (d_ddelta, "ddelta", ch), (d_dz, "dz", ch),
+                         (d_db, "dB", n), (d_dc, "dC", n))],
+                      _tensor(d_dA, "dA", (ch, n), f32, dev), _tensor(d_dD, "dD", (ch,), f32, dev),
+                      _tensor(d_ddelta_bias, "ddelta_bias", (ch,), f32, dev),
+                      _tensor(d_dstate_in, "dstate_in", state, f32, dev))
+        self._check(lib().boa_selective_scan_grad(
+            self.h, C.byref(s), self._saved(d_saved, s, dev), C.byref(dout),
+            _tensor(d_dstate_out, "dstate_out", state, f32, dev), C.byref(g),
+            *_work(d_work, dev)), "selective_scan_grad")
+
+    def next_byte_loss(self, d_logits, d_targets, d_loss, d_work=None, d_bias=None, d_total=None,
+                       d_dlogits=None, d_dbias=None, scale=1.0, d_lens=None):
+        """loss [lanes, T] in nats, its sum, and scale times the gradients of
+        the sum; dlogits may be logits."""
+        dev, f32 = self._device(), "torch.float32"
+        prec, dt = _precision(d_logits, "logits")
+        tgt, stride, lanes, T = _bytes(d_targets, "targets", dev)
+        x = _rows(d_logits, "logits", lanes, T, 256, dt, dev)
+        dx = None
+        if d_dlogits is not None:
+            dx = C.byref(_rows(d_dlogits, "dlogits", lanes, T, 256, dt, dev))
+        self._check(lib().boa_next_byte_loss(
+            self.h, C.byref(x), _tensor(d_bias, "bias", (256,), f32, dev), tgt, stride,
+            _tensor(d_lens, "lens", (lanes,), "torch.int32", dev), lanes, T, prec, scale,
+            _tensor(d_loss, "loss", (lanes, T), f32, dev), _tensor(d_total, "total", (1,), f32, dev),
+            dx, _tensor(d_dbias, "dbias", (256,), f32, dev), *_work(d_work, dev)),
+            "next_byte_loss")
 
     def compress_device(self, d_data, n, chunk_size, d_payload, cap_words, max_chunks=0):
         import numpy as np

@@ -23,6 +23,7 @@
 #include "../../include/boa_hip.h"
 #include "boa_kernels.h"
 #include "container.h"
+#include "train_kernels.h"
 
 using namespace boa;
 
@@ -132,6 +133,7 @@ struct boa_ctx {
   int* t_counter = nullptr;     // decode step counter (device)
 
   int n_cus = 0;  // compute units of the device (persistent decode grid)
+  int device = 0;  // the device that was current in boa_create
 
   // decompress: every step is replayed from a HIP graph on dec_stream; the
   // executable graph is kept while the step's launch arguments stay the same
@@ -1044,6 +1046,121 @@ hipError_t decode_steps(boa_ctx* c, int lanes, int maxlen, uint8_t* out, int64_t
   return e ? e : e2;
 }
 
+// ---- training operators: argument checks -----------------------------------
+bool seqs_ok(int64_t lanes, int64_t T) {
+  return lanes >= 1 && lanes <= 65535 && T >= 1 && lanes * T <= ((int64_t)1 << 30);
+}
+bool scan_sizes_ok(int64_t lanes, int64_t T, int64_t channels, int64_t ds) {
+  return seqs_ok(lanes, T) && channels >= 1 && channels <= 4096 && (ds == 16 || ds == 32);
+}
+
+// Collects the first thing that is wrong with a call's arguments.
+struct TrainCheck {
+  const char* bad = nullptr;   // what is wrong
+  const char* of = "";         // with which argument
+  int64_t lanes = 0, T = 0;
+  int size = 4;                // bytes of a row element
+  // keeps every offset of 2^30 rows of 65535 lanes within 63 bits
+  static constexpr int64_t MAX_STRIDE = (int64_t)1 << 32;
+
+  void that(bool ok, const char* why, const char* what = "") {
+    if (!ok && !bad) bad = why, of = what;
+  }
+  void sizes(int64_t lanes_, int64_t T_, int32_t precision) {
+    lanes = lanes_;
+    T = T_;
+    size = precision == 1 ? 2 : 4;
+    that(seqs_ok(lanes, T), "lanes has to be 1 .. 65535, T at least 1, lanes x T at most 2^30");
+    that(precision == 0 || precision == 1, "precision has to be 0 (fp32) or 1 (bf16)");
+  }
+  void floats(const void* p, size_t align, bool may_be_null, const char* what) {
+    that(p || may_be_null, "a required pointer is NULL: ", what);
+    that((uintptr_t)p % align == 0, "a pointer is not aligned: ", what);
+  }
+  void bytes(const uint8_t* p, int64_t stride, const char* what) {
+    that(p != nullptr, "a required pointer is NULL: ", what);
+    that(stride >= 0 && stride <= MAX_STRIDE, "a stride is negative or over 2^32: ", what);
+  }
+  void in(const boa_rows* r, const char* what) {
+    that(r != nullptr && r->d != nullptr, "a required pointer is NULL: ", what);
+    if (bad) return;
+    floats(r->d, size, false, what);
+    that(r->lane_stride >= 0 && r->row_stride >= 0 && r->lane_stride <= MAX_STRIDE &&
+             r->row_stride <= MAX_STRIDE, "a stride is negative or over 2^32: ", what);
+  }
+  // an output's rows may not overlap: one of the two strides spans the other's extent
+  void out(const boa_rows* r, int64_t width, const char* what) {
+    in(r, what);
+    if (bad) return;
+    const int64_t ls = r->lane_stride, rs = r->row_stride;
+    const bool t_in = (T == 1 || rs >= width) && (lanes == 1 || ls >= (T - 1) * rs + width);
+    const bool l_in = (lanes == 1 || ls >= width) && (T == 1 || rs >= (lanes - 1) * ls + width);
+    that(t_in || l_in, "rows overlap: ", what);
+  }
+  void work(const void* p, int64_t have, int64_t need) {
+    if (bad) return;
+    that(have >= need && (p || need == 0), "the workspace is too small");
+    that((uintptr_t)p % 16 == 0, "a pointer is not aligned: ", "work");
+  }
+  static RowsIn from(const boa_rows& r) { return RowsIn{r.d, r.lane_stride, r.row_stride}; }
+  static RowsOut to(const boa_rows& r) { return RowsOut{r.d, r.lane_stride, r.row_stride}; }
+
+  void scan(const boa_scan* s, ScanArgs& a) {
+    that(s != nullptr, "scan is NULL");
+    if (bad) return;
+    sizes(s->lanes, s->T, s->precision);
+    that(scan_sizes_ok(s->lanes, s->T, s->channels, s->d_state),
+         "channels has to be 1 .. 4096, d_state 16 or 32");
+    floats(s->d_lens, 4, true, "lens");
+    in(&s->u, "u");
+    in(&s->delta, "delta");
+    in(&s->z, "z");
+    in(&s->b, "b");
+    in(&s->c, "c");
+    floats(s->d_A, 4, false, "A");
+    floats(s->d_D, 4, false, "D");
+    floats(s->d_delta_bias, 4, false, "delta_bias");
+    floats(s->d_state_in, 4, true, "state_in");
+    a = ScanArgs{};
+    a.q = Seqs{s->lanes, s->T, s->d_lens};
+    a.C = s->channels;
+    a.ds = s->d_state;
+    a.u = from(s->u);
+    a.delta = from(s->delta);
+    a.z = from(s->z);
+    a.b = from(s->b);
+    a.c = from(s->c);
+    a.A = s->d_A;
+    a.D = s->d_D;
+    a.bias = s->d_delta_bias;
+    a.state_in = s->d_state_in;
+    a.bf16 = s->precision == 1;
+  }
+  static bool scan_input(const boa_scan& s, const void* p) {
+    return p == s.u.d || p == s.delta.d || p == s.z.d || p == s.b.d || p == s.c.d || p == s.d_A ||
+           p == s.d_D || p == s.d_delta_bias || p == s.d_state_in;
+  }
+};
+
+// Runs a training operator's checks and launches with the context's device
+// current; no exception leaves it.
+template <class F>
+int train_call(boa_ctx* c, const char* name, F&& f) noexcept {
+  if (!c) return BOA_E_ARG;
+  try {
+    int prev = -1;
+    HIP_TRY(c, hipGetDevice(&prev));
+    if (prev != c->device) HIP_TRY(c, hipSetDevice(c->device));
+    TrainCheck k;
+    const hipError_t e = f(k);
+    if (prev != c->device) (void)hipSetDevice(prev);
+    if (k.bad) return fail(c, BOA_E_ARG, std::string(name) + ": " + k.bad + k.of);
+    return e ? hip_fail(c, e, name) : BOA_OK;
+  } catch (...) {
+    return BOA_E_NOMEM;
+  }
+}
+
 }  // namespace
 
 // ================================================================ C ABI
@@ -1073,6 +1190,7 @@ int boa_create(const boa_config* cfg, boa_ctx** out) {
   {
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) { delete c; return BOA_E_HIP; }
+    c->device = dev;
     std::lock_guard<std::mutex> lock(g_scratch_mu);
     if (dev >= 0 && dev < kScratchDevices) {
       if (!g_scratch_ptr[dev]) {
@@ -1555,6 +1673,161 @@ int boa_step_batch(boa_ctx* c, const uint8_t* d_tokens, int32_t lanes, float* d_
     return fail(c, BOA_E_ARG, "boa_step_batch: bad arguments");
   HIP_TRY(c, step_forward(c, d_tokens, lanes, add_bias != 0, d_logits));
   return BOA_OK;
+}
+
+// ---- training operators ----------------------------------------------------
+
+int boa_device(const boa_ctx* c) { return c ? c->device : BOA_E_ARG; }
+
+int64_t boa_embed_grad_work_bytes(int32_t lanes, int32_t T, int32_t width) {
+  if (!seqs_ok(lanes, T) || width < 1 || width > 512) return -1;
+  return (int64_t)embed_grad_work((int64_t)lanes * T, width);
+}
+
+int64_t boa_selective_scan_saved_floats(int32_t lanes, int32_t T, int32_t channels,
+                                        int32_t d_state) {
+  if (!scan_sizes_ok(lanes, T, channels, d_state)) return -1;
+  return scan_saved_floats(lanes, T, channels, d_state);
+}
+
+int64_t boa_selective_scan_work_bytes(int32_t lanes, int32_t T, int32_t channels, int32_t d_state,
+                                      int32_t grad) {
+  if (!scan_sizes_ok(lanes, T, channels, d_state)) return -1;
+  return (int64_t)scan_work(lanes, T, channels, d_state, grad != 0);
+}
+
+int64_t boa_next_byte_loss_work_bytes(int32_t lanes, int32_t T) {
+  if (!seqs_ok(lanes, T)) return -1;
+  return (int64_t)loss_work((int64_t)lanes * T);
+}
+
+int boa_embed(boa_ctx* c, const uint8_t* d_tokens, int64_t token_stride, const int32_t* d_lens,
+              int32_t lanes, int32_t T, const void* d_table, int32_t width, int32_t precision,
+              float scale, const boa_rows* out) {
+  return train_call(c, "boa_embed", [&](TrainCheck& k) {
+    k.sizes(lanes, T, precision);
+    k.that(width >= 1 && width <= 512, "width has to be 1 .. 512");
+    k.bytes(d_tokens, token_stride, "tokens");
+    k.floats(d_lens, 4, true, "lens");
+    k.floats(d_table, k.size, false, "table");
+    k.out(out, width, "out");
+    k.that(k.bad || out->d != d_table, "out is an input");
+    if (k.bad) return hipSuccess;
+    return launch_embed({Seqs{lanes, T, d_lens}, d_tokens, token_stride, d_table, width, scale,
+                         k.to(*out), precision == 1}, c->stream);
+  });
+}
+
+int boa_embed_grad(boa_ctx* c, const uint8_t* d_tokens, int64_t token_stride,
+                   const int32_t* d_lens, int32_t lanes, int32_t T, const boa_rows* dout,
+                   int32_t width, int32_t precision, float scale, float* d_dtable, void* d_work,
+                   int64_t work_bytes) {
+  return train_call(c, "boa_embed_grad", [&](TrainCheck& k) {
+    k.sizes(lanes, T, precision);
+    k.that(width >= 1 && width <= 512, "width has to be 1 .. 512");
+    k.bytes(d_tokens, token_stride, "tokens");
+    k.floats(d_lens, 4, true, "lens");
+    k.in(dout, "dout");
+    k.floats(d_dtable, 4, false, "dtable");
+    k.that(k.bad || dout->d != d_dtable, "dtable is an input");
+    k.work(d_work, work_bytes, boa_embed_grad_work_bytes(lanes, T, width));
+    if (k.bad) return hipSuccess;
+    return launch_embed_grad({Seqs{lanes, T, d_lens}, d_tokens, token_stride, k.from(*dout), width,
+                              scale, d_dtable, d_work, precision == 1}, c->stream);
+  });
+}
+
+int boa_selective_scan(boa_ctx* c, const boa_scan* s, const boa_rows* out, float* d_state_out,
+                       float* d_saved, void* d_work, int64_t work_bytes) {
+  return train_call(c, "boa_selective_scan", [&](TrainCheck& k) {
+    ScanArgs a{};
+    k.scan(s, a);
+    if (k.bad) return hipSuccess;
+    k.out(out, s->channels, "out");
+    k.floats(d_state_out, 16, true, "state_out");
+    k.floats(d_saved, 16, true, "saved");
+    k.that(k.bad || !k.scan_input(*s, out->d), "out is an input");
+    k.work(d_work, work_bytes,
+           boa_selective_scan_work_bytes(s->lanes, s->T, s->channels, s->d_state, 0));
+    if (k.bad) return hipSuccess;
+    a.out = k.to(*out);
+    a.state_out = d_state_out;
+    a.saved = d_saved;
+    a.work = d_work;
+    return launch_scan(a, c->stream);
+  });
+}
+
+int boa_selective_scan_grad(boa_ctx* c, const boa_scan* s, const float* d_saved,
+                            const boa_rows* dout, const float* d_dstate_out,
+                            const boa_scan_grads* g, void* d_work, int64_t work_bytes) {
+  return train_call(c, "boa_selective_scan_grad", [&](TrainCheck& k) {
+    ScanGradArgs a{};
+    k.scan(s, a.f);
+    k.that(g != nullptr, "grads is NULL");
+    if (k.bad) return hipSuccess;
+    k.floats(d_saved, 16, false, "saved");
+    k.in(dout, "dout");
+    k.floats(d_dstate_out, 4, true, "dstate_out");
+    k.out(&g->du, s->channels, "du");
+    k.out(&g->ddelta, s->channels, "ddelta");
+    k.out(&g->dz, s->channels, "dz");
+    k.out(&g->db, s->d_state, "db");
+    k.out(&g->dc, s->d_state, "dc");
+    k.floats(g->d_dA, 4, false, "dA");
+    k.floats(g->d_dD, 4, false, "dD");
+    k.floats(g->d_ddelta_bias, 4, false, "ddelta_bias");
+    k.floats(g->d_dstate_in, 16, true, "dstate_in");
+    for (const void* p : {(const void*)g->du.d, (const void*)g->ddelta.d, (const void*)g->dz.d,
+                          (const void*)g->db.d, (const void*)g->dc.d})
+      k.that(k.bad || (!k.scan_input(*s, p) && p != dout->d && p != d_saved),
+             "a gradient is an input");
+    k.work(d_work, work_bytes,
+           boa_selective_scan_work_bytes(s->lanes, s->T, s->channels, s->d_state, 1));
+    if (k.bad) return hipSuccess;
+    a.f.saved = const_cast<float*>(d_saved);
+    a.f.work = d_work;
+    a.dout = k.from(*dout);
+    a.dstate_out = d_dstate_out;
+    a.du = k.to(g->du);
+    a.ddelta = k.to(g->ddelta);
+    a.dz = k.to(g->dz);
+    a.db = k.to(g->db);
+    a.dc = k.to(g->dc);
+    a.dA = g->d_dA;
+    a.dD = g->d_dD;
+    a.dbias = g->d_ddelta_bias;
+    a.dstate_in = g->d_dstate_in;
+    return launch_scan_grad(a, c->stream);
+  });
+}
+
+int boa_next_byte_loss(boa_ctx* c, const boa_rows* logits, const float* d_bias,
+                       const uint8_t* d_targets, int64_t target_stride, const int32_t* d_lens,
+                       int32_t lanes, int32_t T, int32_t precision, float scale, float* d_loss,
+                       float* d_total, const boa_rows* dlogits, float* d_dbias, void* d_work,
+                       int64_t work_bytes) {
+  return train_call(c, "boa_next_byte_loss", [&](TrainCheck& k) {
+    k.sizes(lanes, T, precision);
+    k.in(logits, "logits");
+    k.floats(d_bias, 4, true, "bias");
+    k.bytes(d_targets, target_stride, "targets");
+    k.floats(d_lens, 4, true, "lens");
+    k.floats(d_loss, 4, false, "loss");
+    k.floats(d_total, 4, true, "total");
+    if (dlogits) k.out(dlogits, 256, "dlogits");
+    k.floats(d_dbias, 4, true, "dbias");
+    // in place means the same rows
+    k.that(k.bad || !dlogits || dlogits->d != logits->d ||
+               (dlogits->lane_stride == logits->lane_stride &&
+                dlogits->row_stride == logits->row_stride),
+           "dlogits is logits with other strides");
+    k.work(d_work, work_bytes, boa_next_byte_loss_work_bytes(lanes, T));
+    if (k.bad) return hipSuccess;
+    return launch_loss({Seqs{lanes, T, d_lens}, k.from(*logits), d_targets, target_stride, d_bias,
+                        scale, d_loss, d_total, dlogits ? k.to(*dlogits) : RowsOut{nullptr, 0, 0},
+                        d_dbias, d_work, precision == 1}, c->stream);
+  });
 }
 
 int boa_cdf_from_logits(boa_ctx* c, const float* d_logits, const float* d_bias, int32_t rows,

@@ -149,6 +149,105 @@ int boa_forward_chunk_noalloc(boa_ctx* ctx, const uint8_t* d_tokens, int32_t lan
 int boa_step_batch(boa_ctx* ctx, const uint8_t* d_tokens, int32_t lanes, float* d_logits,
                    int32_t add_bias);
 
+/* ---- training operators (device pointers) ------------------------------- */
+/* What a program that fits or adapts the predictor's weights calls beside its
+ * matrix products: the embedding, the selective scan and the next-byte loss
+ * with their gradients (the reference trains in Python, train.py:33-212, with
+ * the recurrence of model.py:1553-1590).  A context gives them its device,
+ * stream and error message; its model, weights and state play no part.
+ *
+ * Rows: `lanes` byte sequences (1 .. 65535) of up to T positions, lanes x T
+ * at most 2^30.  A boa_rows tensor has element i of row (l, t) at
+ * d + l lane_stride + t row_stride + i, in elements, strides 0 .. 2^32; the
+ * rows of an output may not overlap.  precision is the type of the row tensors, 0 fp32 or 1
+ * bf16; weights, states and the gradients of weights are fp32, every sum is
+ * held in fp32 or more, and results are rounded once.  d_lens (device, may be
+ * NULL) has the lanes' lengths, taken as min(max(len, 0), T); NULL is T for
+ * all.  Rows past a lane's length are never read; outputs keep what they held
+ * there, and gradients of rows are set to zero there.
+ *
+ * The calls launch kernels on the context's stream and do nothing else (no
+ * allocation, no synchronisation, no state), so they can be captured into a
+ * HIP graph.  d_work is the caller's workspace, 16-byte aligned, of at least
+ * the size that the _work_bytes function gives (-1: bad sizes; 0: d_work may
+ * be NULL); its content is not kept, and calls that may overlap in time need
+ * one each.  Outputs may not overlap inputs or each other, except that
+ * dlogits may be logits itself.  Results depend on the inputs and sizes only
+ * (no atomics). */
+typedef struct {
+    void* d;
+    int64_t lane_stride, row_stride;
+} boa_rows;
+
+/* The device that the context was created on. */
+int boa_device(const boa_ctx* ctx);
+
+/* out[l][t] = scale * table[token]: d_tokens, token t of lane l at
+ * l token_stride + t; table [256][width], width 1 .. 512. */
+int boa_embed(boa_ctx* ctx, const uint8_t* d_tokens, int64_t token_stride, const int32_t* d_lens,
+              int32_t lanes, int32_t T, const void* d_table, int32_t width, int32_t precision,
+              float scale, const boa_rows* out);
+/* dtable[v] = scale * sum of dout's rows whose token is v; [256][width] fp32,
+ * written whole (zero where a byte does not occur). */
+int boa_embed_grad(boa_ctx* ctx, const uint8_t* d_tokens, int64_t token_stride,
+                   const int32_t* d_lens, int32_t lanes, int32_t T, const boa_rows* dout,
+                   int32_t width, int32_t precision, float scale, float* d_dtable, void* d_work,
+                   int64_t work_bytes);
+int64_t boa_embed_grad_work_bytes(int32_t lanes, int32_t T, int32_t width);
+
+/* The mambav1 recurrence over [lanes][T] rows of `channels` (1 .. 4096), with
+ * d_state (16 or 32) states a channel:
+ *   delta = softplus(x + delta_bias)             x: the rows `delta`
+ *   h[n]  = exp(delta A[n]) h[n] + delta B[n] u
+ *   out   = (sum_n C[n] h[n] + D u) * z sigmoid(z)
+ * B and C rows are d_state wide and shared by the channels.  d_A [channels]
+ * [d_state] (that is -exp(A_log)), d_D and d_delta_bias [channels], states
+ * [lanes][channels][d_state]; d_state_in NULL is zero.  With T = 1 this is a
+ * decode step. */
+typedef struct {
+    int32_t lanes, T, channels, d_state, precision;
+    const int32_t* d_lens;
+    boa_rows u, delta, z, b, c;
+    const float *d_A, *d_D, *d_delta_bias;
+    const float* d_state_in;
+} boa_scan;
+/* Gradients: rows as their inputs', dA [channels][d_state], dD and ddelta_bias
+ * [channels], dstate_in [lanes][channels][d_state] (NULL: not wanted). */
+typedef struct {
+    boa_rows du, ddelta, dz, db, dc;
+    float *d_dA, *d_dD, *d_ddelta_bias;
+    float* d_dstate_in;
+} boa_scan_grads;
+/* d_state_out (may be NULL): the states after each lane's last position; a
+ * lane of length 0 passes its state on.  d_saved: NULL, or where the states
+ * that the gradient starts from are kept (boa_selective_scan_saved_floats
+ * floats).  Both 16-byte aligned.  d_state_out may be d_state_in itself. */
+int boa_selective_scan(boa_ctx* ctx, const boa_scan* s, const boa_rows* out, float* d_state_out,
+                       float* d_saved, void* d_work, int64_t work_bytes);
+/* The gradient of that call, given its inputs, its d_saved, the gradient of
+ * out and (NULL: zero) of state_out. */
+int boa_selective_scan_grad(boa_ctx* ctx, const boa_scan* s, const float* d_saved,
+                            const boa_rows* dout, const float* d_dstate_out,
+                            const boa_scan_grads* grads, void* d_work, int64_t work_bytes);
+int64_t boa_selective_scan_saved_floats(int32_t lanes, int32_t T, int32_t channels,
+                                        int32_t d_state);
+int64_t boa_selective_scan_work_bytes(int32_t lanes, int32_t T, int32_t channels, int32_t d_state,
+                                      int32_t grad);
+
+/* Cross-entropy of the next bytes in nats (what the coder spends on them, but
+ * for its rounding): per row x = logits + bias, loss = log sum exp(x) -
+ * x[target], dlogits = scale (softmax(x) - onehot(target)); total = sum of
+ * loss, dbias = sum of dlogits.  logits rows are 256 wide; d_targets, target t
+ * of lane l at l target_stride + t; d_loss [lanes][T] fp32; d_bias, d_total
+ * [1], dlogits and d_dbias [256] may be NULL.  Logits of -inf are bytes ruled
+ * out; a row of nothing but -inf has loss inf and gradient zero. */
+int boa_next_byte_loss(boa_ctx* ctx, const boa_rows* logits, const float* d_bias,
+                       const uint8_t* d_targets, int64_t target_stride, const int32_t* d_lens,
+                       int32_t lanes, int32_t T, int32_t precision, float scale, float* d_loss,
+                       float* d_total, const boa_rows* dlogits, float* d_dbias, void* d_work,
+                       int64_t work_bytes);
+int64_t boa_next_byte_loss_work_bytes(int32_t lanes, int32_t T);
+
 /* ---- CDF and coder level (device pointers) ------------------------------ */
 /* Integer CDFs of logits rows: d_qcdf [rows][257] with low_k in column k and
  * 2^24 in column 256; d_bias (may be NULL) is added first.  This is the CDF

@@ -1102,6 +1102,10 @@ struct TrainCheck {
     that(have >= need && (p || need == 0), "the workspace is too small");
     that((uintptr_t)p % 16 == 0, "a pointer is not aligned: ", "work");
   }
+  // the scan's rows: 16 of them within 32 bits of bytes
+  void near(const boa_rows* r, const char* what) {
+    that(bad || r->row_stride <= (int64_t)1 << 25, "a row stride is over 2^25: ", what);
+  }
   static RowsIn from(const boa_rows& r) { return RowsIn{r.d, r.lane_stride, r.row_stride}; }
   static RowsOut to(const boa_rows& r) { return RowsOut{r.d, r.lane_stride, r.row_stride}; }
 
@@ -1112,11 +1116,11 @@ struct TrainCheck {
     that(scan_sizes_ok(s->lanes, s->T, s->channels, s->d_state),
          "channels has to be 1 .. 4096, d_state 16 or 32");
     floats(s->d_lens, 4, true, "lens");
-    in(&s->u, "u");
-    in(&s->delta, "delta");
-    in(&s->z, "z");
-    in(&s->b, "b");
-    in(&s->c, "c");
+    in(&s->u, "u"), near(&s->u, "u");
+    in(&s->delta, "delta"), near(&s->delta, "delta");
+    in(&s->z, "z"), near(&s->z, "z");
+    in(&s->b, "b"), near(&s->b, "b");
+    in(&s->c, "c"), near(&s->c, "c");
     floats(s->d_A, 4, false, "A");
     floats(s->d_D, 4, false, "D");
     floats(s->d_delta_bias, 4, false, "delta_bias");
@@ -1743,7 +1747,7 @@ int boa_selective_scan(boa_ctx* c, const boa_scan* s, const boa_rows* out, float
     ScanArgs a{};
     k.scan(s, a);
     if (k.bad) return hipSuccess;
-    k.out(out, s->channels, "out");
+    k.out(out, s->channels, "out"), k.near(out, "out");
     k.floats(d_state_out, 16, true, "state_out");
     k.floats(d_saved, 16, true, "saved");
     k.that(k.bad || !k.scan_input(*s, out->d), "out is an input");
@@ -1767,13 +1771,13 @@ int boa_selective_scan_grad(boa_ctx* c, const boa_scan* s, const float* d_saved,
     k.that(g != nullptr, "grads is NULL");
     if (k.bad) return hipSuccess;
     k.floats(d_saved, 16, false, "saved");
-    k.in(dout, "dout");
+    k.in(dout, "dout"), k.near(dout, "dout");
     k.floats(d_dstate_out, 4, true, "dstate_out");
-    k.out(&g->du, s->channels, "du");
-    k.out(&g->ddelta, s->channels, "ddelta");
-    k.out(&g->dz, s->channels, "dz");
-    k.out(&g->db, s->d_state, "db");
-    k.out(&g->dc, s->d_state, "dc");
+    k.out(&g->du, s->channels, "du"), k.near(&g->du, "du");
+    k.out(&g->ddelta, s->channels, "ddelta"), k.near(&g->ddelta, "ddelta");
+    k.out(&g->dz, s->channels, "dz"), k.near(&g->dz, "dz");
+    k.out(&g->db, s->d_state, "db"), k.near(&g->db, "db");
+    k.out(&g->dc, s->d_state, "dc"), k.near(&g->dc, "dc");
     k.floats(g->d_dA, 4, false, "dA");
     k.floats(g->d_dD, 4, false, "dD");
     k.floats(g->d_ddelta_bias, 4, false, "ddelta_bias");

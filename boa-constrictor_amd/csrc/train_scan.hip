@@ -32,27 +32,42 @@ namespace boa {
 
 namespace {
 
-constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.693147180559945309417f;
 constexpr int CH = 64;  // channels of a block
+constexpr float NEVER = -__builtin_huge_valf();  // the x whose delta is 0
+// Positions whose staged values are read from LDS ahead of their use: left to
+// itself the compiler reads them right before, and waits.
+constexpr int AHEAD = 2;
 
-// log(1 + e^x): e = e^-|x| in (0, 1], log(1 + e) = 2 atanh(s), s = e / (2 + e)
-// <= 1/3, by its odd series to s^15 (the next term is under 2^-27 of the sum)
+// log(1 + e^x) = max(x, 0) + log(1 + e), e = e^-|x| in (0, 1]: the logarithm of
+// y = 1 + e rounded, whose hardware form is good to an ulp down to y = 1, plus
+// what the rounding lost (over y, which is 1 where that counts).  Without
+// branches; x = -inf gives 0.
 __device__ __forceinline__ float softplus_full(float x) {
   const float e = __builtin_amdgcn_exp2f(-__builtin_fabsf(x) * LOG2E);
-  const float s = e * __builtin_amdgcn_rcpf(2.0f + e), s2 = s * s;
-  float p = 0.0666666666666666667f;
-  p = __builtin_fmaf(p, s2, 0.0769230769230769231f);
-  p = __builtin_fmaf(p, s2, 0.0909090909090909091f);
-  p = __builtin_fmaf(p, s2, 0.111111111111111111f);
-  p = __builtin_fmaf(p, s2, 0.142857142857142857f);
-  p = __builtin_fmaf(p, s2, 0.2f);
-  p = __builtin_fmaf(p, s2, 0.333333333333333333f);
-  p = __builtin_fmaf(p * s2, s, s);
-  return __builtin_fmaxf(x, 0.0f) + 2.0f * p;  // a NaN stays one in p
+  const float y = 1.0f + e, lost = e - (y - 1.0f);
+  // max(NaN, 0) is 0, but e is a NaN then
+  return __builtin_fmaxf(x, 0.0f) + __builtin_fmaf(__builtin_amdgcn_logf(y), LN2, lost);
 }
 __device__ __forceinline__ float sigmoid_hw(float x) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * LOG2E));
 }
+
+// The elements of a row tensor that a thread owns: in each tile of lane l the
+// same ones, off elements from the tile's first row.  The tile's address is
+// uniform (scalar registers), a thread keeps 32 bits of its own.
+template <typename P>
+struct Tensor {
+  P* lane;
+  int64_t row;
+  uint32_t off;
+  template <typename R>
+  __device__ __forceinline__ Tensor(const R& r, int l, int t, int i)
+      : lane((P*)r.d + l * r.lane), row(r.row), off((uint32_t)t * (uint32_t)r.row + i) {}
+  __device__ __forceinline__ P* at(int tile) const {
+    return lane + (int64_t)tile * SCAN_TILE * row + off;
+  }
+};
 
 // EV neighbouring elements of a row, as 32-bit words: EV fp32, or EV / 2 pairs of bf16
 template <typename TE, int EV>
@@ -60,12 +75,13 @@ struct Raw {
   uint32_t w[EV * sizeof(TE) / 4];
 };
 template <typename TE, int EV, bool VEC>
-__device__ __forceinline__ Raw<TE, EV> ld_raw(const void* base, int64_t off, int c, int C, bool ok) {
+__device__ __forceinline__ Raw<TE, EV> ld_raw(const Tensor<const TE>& x, int tile, int c, int C,
+                                              bool ok) {
   Raw<TE, EV> r;
   constexpr int W = EV * sizeof(TE) / 4;
 #pragma unroll
   for (int i = 0; i < W; ++i) r.w[i] = 0;
-  const TE* p = (const TE*)base + off + c;
+  const TE* p = x.at(tile);
   if constexpr (VEC) {
     if (ok && c < C) {
       if constexpr (W == 4) {
@@ -94,9 +110,9 @@ __device__ __forceinline__ float raw_at(const Raw<TE, EV>& r, int i) {
   else return u2f(i % 2 ? r.w[i / 2] & 0xFFFF0000u : r.w[i / 2] << 16);
 }
 template <typename TE, int EV, bool VEC>
-__device__ __forceinline__ void st_row(void* base, int64_t off, int c, int C, bool ok,
+__device__ __forceinline__ void st_row(const Tensor<TE>& x, int tile, int c, int C, bool ok,
                                        const float (&v)[EV]) {
-  TE* p = (TE*)base + off + c;
+  TE* p = x.at(tile);
   if constexpr (VEC) {
     if (ok && c < C) {
       constexpr int W = EV * sizeof(TE) / 4;
@@ -134,32 +150,212 @@ __device__ __forceinline__ float sum_states(float x) {
   return x;
 }
 
-// How the blocks divide the work: lane, channel block (and later segment)
+// How the blocks divide the work: lane, segment of the tiles, channel block.
+// Few lanes are cut into segments, so that there are blocks for every CU: a
+// pass over a segment from a zero state gives the state that it adds, the
+// segments' states are chained (their decay is e^(A sum of delta)), and the
+// main pass starts every segment from its own.  That pass costs about half of
+// the main one, so lanes that give every SIMD two waves by themselves stay whole.
 struct Plan {
-  int tiles, cblocks;
+  int tiles, cblocks, segs, seg_tiles;
 };
-Plan scan_plan(int T, int C) {
-  return Plan{(T + SCAN_TILE - 1) / SCAN_TILE, (C + CH - 1) / CH};
+constexpr int WHOLE_WAVES = 2048, SEG_WAVES = 8192, MAX_SEGS = 256;
+Plan scan_plan(int lanes, int T, int C, int ds) {
+  Plan p;
+  p.tiles = (T + SCAN_TILE - 1) / SCAN_TILE;
+  p.cblocks = (C + CH - 1) / CH;
+  const int64_t waves =
+      (int64_t)lanes * p.cblocks * (ds == 16 ? Shape<16>::WAVES : Shape<32>::WAVES);
+  int64_t segs = waves >= WHOLE_WAVES ? 1 : SEG_WAVES / waves;
+  segs = std::min<int64_t>(std::max<int64_t>(segs, 1), std::min(p.tiles, MAX_SEGS));
+  p.seg_tiles = (int)((p.tiles + segs - 1) / segs);
+  p.segs = (p.tiles + p.seg_tiles - 1) / p.seg_tiles;
+  return p;
+}
+// a block's part of it
+struct Part {
+  int l, seg, cb;
+};
+__device__ __forceinline__ Part block_part(const Plan& p, int segs) {
+  const int cb = blockIdx.x % p.cblocks, r = blockIdx.x / p.cblocks;
+  return Part{r / segs, r % segs, cb};
+}
+// the segments' states [lane][seg][C][N] and sums of delta [lane][seg][C]
+struct Carry {
+  float *state, *sum;
+};
+
+// What a segment does to the state that enters it.  Forward: the state that
+// it leaves when it starts from zero.  Backward (REV): the gradient of the
+// state that enters it, when that of the state it leaves is zero.  And the
+// sum of its deltas.
+template <typename TE, int N, bool VEC, bool REV>
+__global__ __launch_bounds__((Shape<N>::BT)) void scan_local_kernel(const ScanGradArgs g, Plan pl,
+                                                                    Carry cy) {
+  using S = Shape<N>;
+  constexpr int TPC = S::TPC, BT = S::BT, EV = S::EV;
+  __shared__ __align__(16) float s_delta[SCAN_TILE][CH], s_x[SCAN_TILE][CH];
+  __shared__ __align__(16) float s_v[SCAN_TILE][N];
+  const ScanArgs& a = g.f;
+  const Part pt = block_part(pl, pl.segs - 1);  // the last (REV: the first) is not asked for
+  const int tid = threadIdx.x, cb = pt.cb, l = pt.l, seg = pt.seg + (REV ? 1 : 0);
+  const int len = seq_len(a.q, l), q = tid % TPC, ch = tid / TPC, c = cb * CH + ch;
+  const int ot = tid / (CH / EV), oc = (tid % (CH / EV)) * EV, gc = cb * CH + oc;
+  float h[4] = {0.0f, 0.0f, 0.0f, 0.0f}, A2[4], sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) A2[i] = c < a.C ? a.A[(size_t)c * N + 4 * q + i] * LOG2E : 0.0f;
+  float bias[EV];
+#pragma unroll
+  for (int j = 0; j < EV; ++j) bias[j] = gc + j < a.C ? a.bias[gc + j] : 0.0f;
+  constexpr int NBC = SCAN_TILE * N / BT;
+  Raw<TE, EV> ru, rx, ro;
+  float rv[NBC];
+  const RowsIn &ri = REV ? a.z : a.u, &rows_v = REV ? a.c : a.b;
+  using In = Tensor<const TE>;
+  const In xu(ri, l, ot, gc), xx(a.delta, l, ot, gc), xo(REV ? g.dout : ri, l, ot, gc);
+  auto fetch = [&](int tile) {
+    const int t = tile * SCAN_TILE + ot;
+    const bool ok = t < len;
+    rx = ld_raw<TE, EV, VEC>(xx, tile, gc, a.C, ok);
+    ru = ld_raw<TE, EV, VEC>(xu, tile, gc, a.C, ok);
+    if constexpr (REV) ro = ld_raw<TE, EV, VEC>(xo, tile, gc, a.C, ok);
+#pragma unroll
+    for (int i = 0; i < NBC; ++i) {
+      const int e = tid + i * BT;
+      rv[i] = tile * SCAN_TILE + e / N < len ? ldv(In(rows_v, l, e / N, e % N).at(tile)) : 0.0f;
+    }
+  };
+  const int all = (len + SCAN_TILE - 1) / SCAN_TILE;
+  const int lo = seg * pl.seg_tiles, n = min(all, lo + pl.seg_tiles) - lo;
+  if (n > 0) fetch(REV ? lo + n - 1 : lo);
+  for (int i = 0; i < n; ++i) {
+    const int tile = REV ? lo + n - 1 - i : lo + i;
+    const bool ok = tile * SCAN_TILE + ot < len;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < EV; ++j) {
+      const float delta = softplus_full(ok ? raw_at(rx, j) + bias[j] : NEVER);
+      float x = raw_at(ru, j);
+      if constexpr (REV) x = raw_at(ro, j) * (x * sigmoid_hw(x));
+      else x = delta * x;
+      s_delta[ot][oc + j] = delta;
+      s_x[ot][oc + j] = x;
+    }
+#pragma unroll
+    for (int j = 0; j < NBC; ++j) (&s_v[0][0])[tid + j * BT] = rv[j];
+    __syncthreads();
+    if (i + 1 < n) fetch(REV ? tile - 1 : tile + 1);
+    float d[2][AHEAD], x[2][AHEAD];
+    float4 V[2][AHEAD];
+    auto read = [&](int p) {
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int k = REV ? SCAN_TILE - 1 - (p * AHEAD + j) : p * AHEAD + j;
+        d[p & 1][j] = s_delta[k][ch];
+        x[p & 1][j] = s_x[k][ch];
+        V[p & 1][j] = *reinterpret_cast<const float4*>(&s_v[k][4 * q]);
+      }
+    };
+    read(0);
+#pragma unroll
+    for (int p = 0; p < SCAN_TILE / AHEAD; ++p) {
+      if (p + 1 < SCAN_TILE / AHEAD) read(p + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const float delta = d[p & 1][j], xk = x[p & 1][j];
+        const float4 V4 = V[p & 1][j];
+        const float v[4] = {V4.x, V4.y, V4.z, V4.w};
+        sum += delta;
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const float e = __builtin_amdgcn_exp2f(delta * A2[m]);
+          h[m] = REV ? e * __builtin_fmaf(v[m], xk, h[m]) : __builtin_fmaf(e, h[m], xk * v[m]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  if (c < a.C) {
+    const size_t at = ((size_t)l * pl.segs + seg) * a.C + c;
+    *reinterpret_cast<float4*>(cy.state + at * N + 4 * q) = make_float4(h[0], h[1], h[2], h[3]);
+    if (q == 0) cy.sum[at] = sum;
+  }
+}
+
+// The state (REV: the gradient) that enters each segment, over what the
+// segments added: chains of segs steps, cut among up to 16 groups of 64 (channel,
+// state) pairs, each of which first finds what its own segments do.
+constexpr int CARRY_GROUPS = 16;  // at most
+template <bool REV>
+__global__ __launch_bounds__(64 * CARRY_GROUPS) void scan_carry_kernel(
+    const float* __restrict__ A, const float* __restrict__ first, int C, int N, int segs,
+    Carry cy) {
+  __shared__ float s_h[CARRY_GROUPS][64], s_sum[CARRY_GROUPS][64];
+  const int width = C * N, cols = (width + 63) / 64, l = blockIdx.x / cols;
+  const int ln = threadIdx.x & 63, g = threadIdx.x >> 6, i = (blockIdx.x % cols) * 64 + ln;
+  const bool on = i < width;
+  const int c = on ? i / N : 0;
+  const float A2 = on ? A[i] * LOG2E : 0.0f;
+  const int groups = blockDim.x >> 6, per = (segs + groups - 1) / groups;
+  const int k0 = min(segs, g * per), k1 = min(segs, k0 + per);
+  // k-th segment of the chain; the last one's effect is not known and not needed
+  auto seg_at = [&](int k) { return (size_t)l * segs + (REV ? segs - 1 - k : k); };
+  float h = 0.0f, sum = 0.0f;
+  if (on)
+#pragma unroll 4
+    for (int k = k0; k < min(k1, segs - 1); ++k) {
+      const float d = cy.sum[seg_at(k) * C + c], s = cy.state[seg_at(k) * width + i];
+      h = __builtin_fmaf(__builtin_amdgcn_exp2f(A2 * d), h, s);
+      sum += d;
+    }
+  s_h[g][ln] = h;
+  s_sum[g][ln] = sum;
+  __syncthreads();
+  if (!on) return;
+  h = first ? first[(size_t)l * width + i] : 0.0f;
+  for (int k = 0; k < g; ++k)
+    h = __builtin_fmaf(__builtin_amdgcn_exp2f(A2 * s_sum[k][ln]), h, s_h[k][ln]);
+  for (int k = k0; k < k1; ++k) {
+    float d = 0.0f, s = 0.0f;
+    float* p = cy.state + seg_at(k) * width + i;
+    if (k < segs - 1) {
+      d = cy.sum[seg_at(k) * C + c];
+      s = *p;
+    }
+    *p = h;
+    h = __builtin_fmaf(__builtin_amdgcn_exp2f(A2 * d), h, s);
+  }
 }
 
 // ---------------------------------------------------------------- forward
 template <typename TE, int N, bool VEC>
-__global__ __launch_bounds__((Shape<N>::BT)) void scan_kernel(const ScanArgs a, Plan pl) {
+__global__ __launch_bounds__((Shape<N>::BT)) void scan_kernel(const ScanArgs a, Plan pl,
+                                                              const float* carry) {
   using S = Shape<N>;
   constexpr int TPC = S::TPC, BT = S::BT, EV = S::EV, YS = CH + 16;
   __shared__ __align__(16) float s_delta[SCAN_TILE][CH], s_du[SCAN_TILE][CH];
   __shared__ __align__(16) float s_b[SCAN_TILE][N], s_c[SCAN_TILE][N];
   __shared__ __align__(16) float s_y[SCAN_TILE][YS];  // stride: the lanes of a channel on other banks
-  const int tid = threadIdx.x, cb = blockIdx.x % pl.cblocks, l = blockIdx.x / pl.cblocks;
+  const Part pt = block_part(pl, pl.segs);
+  const int tid = threadIdx.x, cb = pt.cb, l = pt.l;
   const int len = seq_len(a.q, l), q = tid % TPC, ch = tid / TPC, c = cb * CH + ch;
+  const int all = (len + SCAN_TILE - 1) / SCAN_TILE, first = pt.seg * pl.seg_tiles;
+  if (pt.seg > 0 && first >= all) return;  // past the lane's end
+  const int tiles = min(all, first + pl.seg_tiles);
   // the row elements that this thread owns: position ot of the tile, channels oc ..
   const int ot = tid / (CH / EV), oc = (tid % (CH / EV)) * EV, gc = cb * CH + oc;
   float h[4], A2[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     A2[i] = c < a.C ? a.A[(size_t)c * N + 4 * q + i] * LOG2E : 0.0f;
-    h[i] = c < a.C && a.state_in ? a.state_in[((size_t)l * a.C + c) * N + 4 * q + i] : 0.0f;
+    h[i] = 0.0f;
   }
+  const float* enter = carry ? carry + ((size_t)l * pl.segs + pt.seg) * a.C * N
+                       : a.state_in ? a.state_in + (size_t)l * a.C * N : nullptr;
+  if (enter && c < a.C)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = enter[c * N + 4 * q + i];
   float bias[EV], D[EV];
 #pragma unroll
   for (int j = 0; j < EV; ++j) {
@@ -169,22 +365,25 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_kernel(const ScanArgs a, 
   constexpr int NBC = SCAN_TILE * N / BT;  // elements of B (and of C) a thread stages
   Raw<TE, EV> ru, rx, rz;
   float rb[NBC], rc[NBC];
+  using In = Tensor<const TE>;
+  const In xu(a.u, l, ot, gc), xx(a.delta, l, ot, gc), xz(a.z, l, ot, gc);
+  const Tensor<TE> xout(a.out, l, ot, gc);
   auto fetch = [&](int tile) {
     const int t = tile * SCAN_TILE + ot;
     const bool ok = t < len;
-    ru = ld_raw<TE, EV, VEC>(a.u.d, l * a.u.lane + t * a.u.row, gc, a.C, ok);
-    rx = ld_raw<TE, EV, VEC>(a.delta.d, l * a.delta.lane + t * a.delta.row, gc, a.C, ok);
-    rz = ld_raw<TE, EV, VEC>(a.z.d, l * a.z.lane + t * a.z.row, gc, a.C, ok);
+    ru = ld_raw<TE, EV, VEC>(xu, tile, gc, a.C, ok);
+    rx = ld_raw<TE, EV, VEC>(xx, tile, gc, a.C, ok);
+    rz = ld_raw<TE, EV, VEC>(xz, tile, gc, a.C, ok);
 #pragma unroll
     for (int i = 0; i < NBC; ++i) {
-      const int e = tid + i * BT, bt = tile * SCAN_TILE + e / N, n = e % N;
-      rb[i] = bt < len ? ldv((const TE*)a.b.d + l * a.b.lane + bt * a.b.row + n) : 0.0f;
-      rc[i] = bt < len ? ldv((const TE*)a.c.d + l * a.c.lane + bt * a.c.row + n) : 0.0f;
+      const int e = tid + i * BT;
+      const bool in = tile * SCAN_TILE + e / N < len;
+      rb[i] = in ? ldv(In(a.b, l, e / N, e % N).at(tile)) : 0.0f;
+      rc[i] = in ? ldv(In(a.c, l, e / N, e % N).at(tile)) : 0.0f;
     }
   };
-  const int tiles = (len + SCAN_TILE - 1) / SCAN_TILE;
-  if (tiles > 0) fetch(0);
-  for (int tile = 0; tile < tiles; ++tile) {
+  if (first < tiles) fetch(first);
+  for (int tile = first; tile < tiles; ++tile) {
     const int t = tile * SCAN_TILE + ot;
     const bool ok = t < len;
     float u[EV], gate[EV];
@@ -194,7 +393,7 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_kernel(const ScanArgs a, 
       const float z = raw_at(rz, j);
       gate[j] = z * sigmoid_hw(z);
       // past the lane's end delta = 0: the state passes unchanged
-      const float delta = ok ? softplus_full(raw_at(rx, j) + bias[j]) : 0.0f;
+      const float delta = softplus_full(ok ? raw_at(rx, j) + bias[j] : NEVER);
       s_delta[ot][oc + j] = delta;
       s_du[ot][oc + j] = delta * u[j];
     }
@@ -211,22 +410,41 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_kernel(const ScanArgs a, 
       *reinterpret_cast<float4*>(p) = make_float4(h[0], h[1], h[2], h[3]);
     }
     float y[SCAN_TILE / TPC];
+    float d[2][AHEAD], x[2][AHEAD];
+    float4 B[2][AHEAD], C[2][AHEAD];
+    auto read = [&](int p) {
 #pragma unroll
-    for (int k = 0; k < SCAN_TILE; ++k) {
-      const float delta = s_delta[k][ch], du = s_du[k][ch];
-      const float4 B = *reinterpret_cast<const float4*>(&s_b[k][4 * q]);
-      const float4 C = *reinterpret_cast<const float4*>(&s_c[k][4 * q]);
-      const float bv[4] = {B.x, B.y, B.z, B.w}, cv[4] = {C.x, C.y, C.z, C.w};
-      float s = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float e = __builtin_amdgcn_exp2f(delta * A2[i]);
-        h[i] = __builtin_fmaf(e, h[i], du * bv[i]);
-        s = __builtin_fmaf(cv[i], h[i], s);
+      for (int j = 0; j < AHEAD; ++j) {
+        const int k = p * AHEAD + j;
+        d[p & 1][j] = s_delta[k][ch];
+        x[p & 1][j] = s_du[k][ch];
+        B[p & 1][j] = *reinterpret_cast<const float4*>(&s_b[k][4 * q]);
+        C[p & 1][j] = *reinterpret_cast<const float4*>(&s_c[k][4 * q]);
       }
-      s = sum_states<TPC>(s);
-      // lane q of the channel keeps the positions q, q + TPC, ...
-      y[k / TPC] = k % TPC == 0 || q == k % TPC ? s : y[k / TPC];
+    };
+    read(0);
+#pragma unroll
+    for (int p = 0; p < SCAN_TILE / AHEAD; ++p) {
+      if (p + 1 < SCAN_TILE / AHEAD) read(p + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int k = p * AHEAD + j;
+        const float delta = d[p & 1][j], du = x[p & 1][j];
+        const float4 B4 = B[p & 1][j], C4 = C[p & 1][j];
+        const float bv[4] = {B4.x, B4.y, B4.z, B4.w}, cv[4] = {C4.x, C4.y, C4.z, C4.w};
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = __builtin_amdgcn_exp2f(delta * A2[i]);
+          h[i] = __builtin_fmaf(e, h[i], du * bv[i]);
+          s = __builtin_fmaf(cv[i], h[i], s);
+        }
+        s = sum_states<TPC>(s);
+        // lane q of the channel keeps the positions q, q + TPC, ...
+        y[k / TPC] = k % TPC == 0 || q == k % TPC ? s : y[k / TPC];
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int k = 0; k < SCAN_TILE / TPC; ++k) s_y[k * TPC + q][ch] = y[k];
@@ -234,64 +452,80 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_kernel(const ScanArgs a, 
     float o[EV];
 #pragma unroll
     for (int j = 0; j < EV; ++j) o[j] = __builtin_fmaf(D[j], u[j], s_y[ot][oc + j]) * gate[j];
-    st_row<TE, EV, VEC>(a.out.d, l * a.out.lane + t * a.out.row, gc, a.C, ok, o);
+    st_row<TE, EV, VEC>(xout, tile, gc, a.C, ok, o);
   }
-  if (a.state_out && c < a.C)
+  if (a.state_out && tiles == all && c < a.C)
     *reinterpret_cast<float4*>(a.state_out + ((size_t)l * a.C + c) * N + 4 * q) =
         make_float4(h[0], h[1], h[2], h[3]);
 }
 
 // --------------------------------------------------------------- backward
-// Partial sums of a block: dA [lane][C][N], dD and dbias [lane][C], and with
-// more than one channel block dB | dC [cblock][row][2 N]
+// Partial sums of a block: dA [lane][seg][C][N], dD and dbias [lane][seg][C],
+// and with more than one channel block dB | dC [cblock][row][2 N]
 struct GradWork {
   float *bc, *da, *dd, *dbias;
 };
 
 template <typename TE, int N, bool VEC>
-__global__ __launch_bounds__((Shape<N>::BT)) void scan_grad_kernel(const ScanGradArgs g, Plan pl,
-                                                                   GradWork wk) {
+__global__ __launch_bounds__((Shape<N>::BT)) __attribute__((amdgpu_waves_per_eu(2, 2))) void scan_grad_kernel(const ScanGradArgs g, Plan pl,
+                                                                   GradWork wk, const float* carry) {
   using S = Shape<N>;
-  constexpr int TPC = S::TPC, BT = S::BT, EV = S::EV, YS = CH + 16;
+  constexpr int TPC = S::TPC, BT = S::BT, EV = S::EV, SUMS = SCAN_TILE * CH + 16;
   __shared__ __align__(16) float s_delta[SCAN_TILE][CH], s_u[SCAN_TILE][CH], s_dy[SCAN_TILE][CH];
   __shared__ __align__(16) float s_b[SCAN_TILE][N], s_c[SCAN_TILE][N];
-  __shared__ __align__(16) float s_y[SCAN_TILE][YS], s_i[SCAN_TILE][YS], s_m[SCAN_TILE][YS];
+  // y, I and sum m A log2(e) of every (position, channel); the three on different banks
+  __shared__ __align__(16) float s_sums[3 * SUMS];
   __shared__ __align__(16) float s_bc[S::WAVES][SCAN_TILE][2 * N];
+  __shared__ __align__(16) float s_dd[SCAN_TILE][CH], s_dbias[SCAN_TILE][CH], s_bias[CH], s_dcoef[CH];
   const ScanArgs& a = g.f;
-  const int tid = threadIdx.x, cb = blockIdx.x % pl.cblocks, l = blockIdx.x / pl.cblocks;
+  const Part pt = block_part(pl, pl.segs);
+  const int tid = threadIdx.x, cb = pt.cb, l = pt.l;
   const int len = seq_len(a.q, l), q = tid % TPC, ch = tid / TPC, c = cb * CH + ch;
   const int ot = tid / (CH / EV), oc = (tid % (CH / EV)) * EV, gc = cb * CH + oc;
   const int w = tid >> 6, ln = tid & 63;
-  float A[4], G[4], dA[4];
+  const int first = pt.seg * pl.seg_tiles, last = min(pl.tiles, first + pl.seg_tiles);
+  float* sums = s_sums + min(q & 3, 2) * SUMS + ch;
+  float A2[4], G[4], dA[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    A[i] = c < a.C ? a.A[(size_t)c * N + 4 * q + i] : 0.0f;
-    G[i] = c < a.C && g.dstate_out ? g.dstate_out[((size_t)l * a.C + c) * N + 4 * q + i] : 0.0f;
-    dA[i] = 0.0f;
+    A2[i] = c < a.C ? a.A[(size_t)c * N + 4 * q + i] * LOG2E : 0.0f;
+    G[i] = dA[i] = 0.0f;
   }
-  float bias[EV], D[EV], dD[EV], dbias[EV];
+  const float* enter = carry ? carry + ((size_t)l * pl.segs + pt.seg) * a.C * N
+                       : g.dstate_out ? g.dstate_out + (size_t)l * a.C * N : nullptr;
+  if (enter && c < a.C)
 #pragma unroll
-  for (int j = 0; j < EV; ++j) {
-    bias[j] = gc + j < a.C ? a.bias[gc + j] : 0.0f;
-    D[j] = gc + j < a.C ? a.D[gc + j] : 0.0f;
-    dD[j] = dbias[j] = 0.0f;
+    for (int i = 0; i < 4; ++i) G[i] = enter[c * N + 4 * q + i];
+  // the owners' parameters and sums live in LDS, to leave the registers to the states
+#pragma unroll
+  for (int j = 0; j < EV; ++j) s_dd[ot][oc + j] = s_dbias[ot][oc + j] = 0.0f;
+  if (tid < CH) {
+    s_bias[tid] = cb * CH + tid < a.C ? a.bias[cb * CH + tid] : 0.0f;
+    s_dcoef[tid] = cb * CH + tid < a.C ? a.D[cb * CH + tid] : 0.0f;
   }
+  __syncthreads();
   constexpr int NBC = SCAN_TILE * N / BT;
   Raw<TE, EV> ru, rx, rz, ro;
   float rb[NBC], rc[NBC];
   float4 rh;
+  using In = Tensor<const TE>;
+  const In xu(a.u, l, ot, gc), xx(a.delta, l, ot, gc), xz(a.z, l, ot, gc);
+  using Out = Tensor<TE>;
+  const In xo(g.dout, l, ot, gc);
+  const Out odu(g.du, l, ot, gc), odx(g.ddelta, l, ot, gc), odz(g.dz, l, ot, gc);
   auto fetch = [&](int tile) {
     const int t = tile * SCAN_TILE + ot;
     const bool ok = t < len;
-    ru = ld_raw<TE, EV, VEC>(a.u.d, l * a.u.lane + t * a.u.row, gc, a.C, ok);
-    rx = ld_raw<TE, EV, VEC>(a.delta.d, l * a.delta.lane + t * a.delta.row, gc, a.C, ok);
-    rz = ld_raw<TE, EV, VEC>(a.z.d, l * a.z.lane + t * a.z.row, gc, a.C, ok);
-    ro = ld_raw<TE, EV, VEC>(g.dout.d, l * g.dout.lane + t * g.dout.row, gc, a.C, ok);
+    ru = ld_raw<TE, EV, VEC>(xu, tile, gc, a.C, ok);
+    rx = ld_raw<TE, EV, VEC>(xx, tile, gc, a.C, ok);
+    rz = ld_raw<TE, EV, VEC>(xz, tile, gc, a.C, ok);
+    ro = ld_raw<TE, EV, VEC>(xo, tile, gc, a.C, ok);
 #pragma unroll
     for (int i = 0; i < NBC; ++i) {
-      const int e = tid + i * BT, bt = tile * SCAN_TILE + e / N, n = e % N;
-      rb[i] = bt < len ? ldv((const TE*)a.b.d + l * a.b.lane + bt * a.b.row + n) : 0.0f;
-      rc[i] = bt < len ? ldv((const TE*)a.c.d + l * a.c.lane + bt * a.c.row + n) : 0.0f;
+      const int e = tid + i * BT;
+      const bool in = tile * SCAN_TILE + e / N < len;
+      rb[i] = in ? ldv(In(a.b, l, e / N, e % N).at(tile)) : 0.0f;
+      rc[i] = in ? ldv(In(a.c, l, e / N, e % N).at(tile)) : 0.0f;
     }
     rh = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (c < a.C)
@@ -310,40 +544,36 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_grad_kernel(const ScanGra
       if (pl.cblocks > 1)
         wk.bc[(((size_t)cb * a.q.lanes + l) * a.q.T + t) * (2 * N) + n] = v;
       else if (n < N)
-        stv((TE*)g.db.d + l * g.db.lane + t * g.db.row + n, v);
+        stv(Out(g.db, l, k, n).at(tile), v);
       else
-        stv((TE*)g.dc.d + l * g.dc.lane + t * g.dc.row + n - N, v);
+        stv(Out(g.dc, l, k, n - N).at(tile), v);
     }
   };
-  const int tiles = (len + SCAN_TILE - 1) / SCAN_TILE;
+  const int tiles = max(first, min(last, (len + SCAN_TILE - 1) / SCAN_TILE));
   // positions past the lane's end take no part: their gradients are zero
-  for (int tile = pl.tiles - 1; tile >= tiles; --tile) {
+  for (int tile = last - 1; tile >= tiles; --tile) {
     const int t = tile * SCAN_TILE + ot;
     const float zero[EV] = {};
     const bool ok = t < a.q.T;
-    st_row<TE, EV, VEC>(g.du.d, l * g.du.lane + t * g.du.row, gc, a.C, ok, zero);
-    st_row<TE, EV, VEC>(g.ddelta.d, l * g.ddelta.lane + t * g.ddelta.row, gc, a.C, ok, zero);
-    st_row<TE, EV, VEC>(g.dz.d, l * g.dz.lane + t * g.dz.row, gc, a.C, ok, zero);
+    st_row<TE, EV, VEC>(odu, tile, gc, a.C, ok, zero);
+    st_row<TE, EV, VEC>(odx, tile, gc, a.C, ok, zero);
+    st_row<TE, EV, VEC>(odz, tile, gc, a.C, ok, zero);
     store_bc(tile, true);
   }
-  if (tiles > 0) fetch(tiles - 1);
-  for (int tile = tiles - 1; tile >= 0; --tile) {
+  if (tiles > first) fetch(tiles - 1);
+  for (int tile = tiles - 1; tile >= first; --tile) {
     const int t = tile * SCAN_TILE + ot;
     const bool ok = t < len;
-    float u[EV], z[EV], sig[EV], dout[EV], dy[EV], delta[EV], xsig[EV];
+    float dzy[EV], xsig[EV];  // dz / y, d delta / dx; the rest is read back from LDS
 #pragma unroll
     for (int j = 0; j < EV; ++j) {
-      u[j] = raw_at(ru, j);
-      z[j] = raw_at(rz, j);
-      dout[j] = raw_at(ro, j);
-      sig[j] = sigmoid_hw(z[j]);
-      dy[j] = dout[j] * (z[j] * sig[j]);
-      const float x = raw_at(rx, j) + bias[j];
-      delta[j] = ok ? softplus_full(x) : 0.0f;
-      xsig[j] = ok ? sigmoid_hw(x) : 0.0f;
-      s_delta[ot][oc + j] = delta[j];
-      s_u[ot][oc + j] = u[j];
-      s_dy[ot][oc + j] = dy[j];
+      const float z = raw_at(rz, j), sig = sigmoid_hw(z), dout = raw_at(ro, j);
+      const float x = ok ? raw_at(rx, j) + s_bias[oc + j] : NEVER;
+      dzy[j] = dout * (sig * __builtin_fmaf(z, 1.0f - sig, 1.0f));
+      xsig[j] = sigmoid_hw(x);
+      s_delta[ot][oc + j] = softplus_full(x);
+      s_u[ot][oc + j] = raw_at(ru, j);
+      s_dy[ot][oc + j] = dout * (z * sig);
     }
 #pragma unroll
     for (int i = 0; i < NBC; ++i) {
@@ -353,100 +583,124 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_grad_kernel(const ScanGra
     }
     const float h0[4] = {rh.x, rh.y, rh.z, rh.w};
     __syncthreads();
-    if (tile > 0) fetch(tile - 1);
-    // the tile's states and decays again
+    // the tile's states and decays again; two positions are read ahead
     float hs[SCAN_TILE][4], es[SCAN_TILE][4];
+    {
+      float d[4], x[4];
+      float4 B[4];
+      auto read = [&](int k) {
+        d[k & 3] = s_delta[k][ch];
+        x[k & 3] = s_u[k][ch];
+        B[k & 3] = *reinterpret_cast<const float4*>(&s_b[k][4 * q]);
+      };
+      read(0), read(1);
 #pragma unroll
-    for (int k = 0; k < SCAN_TILE; ++k) {
-      const float dl = s_delta[k][ch], du = dl * s_u[k][ch];
-      const float4 B = *reinterpret_cast<const float4*>(&s_b[k][4 * q]);
-      const float bv[4] = {B.x, B.y, B.z, B.w};
+      for (int k = 0; k < SCAN_TILE; ++k) {
+        if (k % 2 == 0) {
+          if (k + 2 < SCAN_TILE) read(k + 2), read(k + 3);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        const float dl = d[k & 3], du = dl * x[k & 3];
+        const float bv[4] = {B[k & 3].x, B[k & 3].y, B[k & 3].z, B[k & 3].w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        es[k][i] = __builtin_amdgcn_exp2f(dl * (A[i] * LOG2E));
-        hs[k][i] = __builtin_fmaf(es[k][i], k ? hs[k > 0 ? k - 1 : 0][i] : h0[i], du * bv[i]);
+        for (int i = 0; i < 4; ++i) {
+          es[k][i] = __builtin_amdgcn_exp2f(dl * A2[i]);
+          hs[k][i] = __builtin_fmaf(es[k][i], k ? hs[k > 0 ? k - 1 : 0][i] : h0[i], du * bv[i]);
+        }
       }
     }
-    float ys[SCAN_TILE / TPC], is[SCAN_TILE / TPC], ms[SCAN_TILE / TPC];
+    // and backwards, one position read ahead.  The staged values are read again,
+    // at indices that the compiler does not know to be the same: kept from
+    // above they would take 96 registers
+    int rch = ch, rq = q;
+    asm volatile("" : "+v"(rch), "+v"(rq) : "v"(hs[SCAN_TILE - 1][0]));
+    float d[2], x[2], dys[2];
+    float4 Bs[2], Cs[2];
+    auto read = [&](int k) {
+      d[k & 1] = s_delta[k][rch];
+      x[k & 1] = s_u[k][rch];
+      dys[k & 1] = s_dy[k][rch];
+      Bs[k & 1] = *reinterpret_cast<const float4*>(&s_b[k][4 * rq]);
+      Cs[k & 1] = *reinterpret_cast<const float4*>(&s_c[k][4 * rq]);
+    };
+    read(SCAN_TILE - 1);
 #pragma unroll
     for (int k = SCAN_TILE - 1; k >= 0; --k) {
-      const float dl = s_delta[k][ch], du = dl * s_u[k][ch], dyk = s_dy[k][ch];
-      const float4 B = *reinterpret_cast<const float4*>(&s_b[k][4 * q]);
-      const float4 C = *reinterpret_cast<const float4*>(&s_c[k][4 * q]);
+      if (k > 0) read(k - 1);
+      // the next tile's rows, once half of the states' registers are free
+      if (k == SCAN_TILE / 2 - 1 && tile > first) fetch(tile - 1);
+      __builtin_amdgcn_sched_barrier(0);
+      const float dl = d[k & 1], du = dl * x[k & 1], dyk = dys[k & 1];
+      const float4 B = Bs[k & 1], C = Cs[k & 1];
       const float bv[4] = {B.x, B.y, B.z, B.w}, cv[4] = {C.x, C.y, C.z, C.w};
-      float y = 0.0f, I = 0.0f, M = 0.0f, db[4], dc[4];
+      float y = 0.0f, I = 0.0f, M = 0.0f, v[4];
+      // du and dy of the wave's halves: the lower one sums dB, the upper one dC
+      const auto cf = __builtin_amdgcn_permlane32_swap(f2u(du), f2u(dyk), false, false);
+      const float c0 = u2f(cf[0]), c1 = u2f(cf[1]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float dh = __builtin_fmaf(cv[i], dyk, G[i]);
         y = __builtin_fmaf(cv[i], hs[k][i], y);
         I = __builtin_fmaf(dh, bv[i], I);
-        dc[i] = hs[k][i] * dyk;
-        db[i] = dh * du;
         G[i] = es[k][i] * dh;
         const float m = G[i] * (k ? hs[k > 0 ? k - 1 : 0][i] : h0[i]);
-        M = __builtin_fmaf(m, A[i], M);
+        M = __builtin_fmaf(m, A2[i], M);
         dA[i] = __builtin_fmaf(m, dl, dA[i]);
+        const auto x = __builtin_amdgcn_permlane32_swap(f2u(dh), f2u(hs[k][i]), false, false);
+        v[i] = __builtin_fmaf(u2f(x[1]), c1, u2f(x[0]) * c0);
       }
-      y = sum_states<TPC>(y);
-      I = sum_states<TPC>(I);
-      M = sum_states<TPC>(M);
-      const bool keep = k % TPC == TPC - 1 || q == k % TPC;
-      ys[k / TPC] = keep ? y : ys[k / TPC];
-      is[k / TPC] = keep ? I : is[k / TPC];
-      ms[k / TPC] = keep ? M : ms[k / TPC];
-      // dB, dC over the wave's channels: the halves of the wave take dB and dC,
-      // the odd rows of 16 lanes states 2 and 3, lanes with bit 3 set 1 and 3
-      float v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = fold32(db[i], dc[i]);
+      // the three sums over the channel's lanes, one for each of lanes 0, 1 and 2
+      if constexpr (TPC == 8) {
+        y = dpp_add<DPP_HALF_MIRROR>(y);
+        I = dpp_add<DPP_HALF_MIRROR>(I);
+        M = dpp_add<DPP_HALF_MIRROR>(M);
+      }
+      const float yi = (q & 1 ? I : y) + dpp_move<DPP_XOR1>(q & 1 ? y : I);
+      M = dpp_add<DPP_XOR1>(M);
+      sums[k * CH] = (q & 2 ? M : yi) + dpp_move<DPP_XOR2>(q & 2 ? yi : M);
+      // dB, dC over the wave's channels: the odd rows of 16 lanes take states 2
+      // and 3, lanes with bit 3 set 1 and 3
       const float x0 = fold16(v[0], v[2]), x1 = fold16(v[1], v[3]);
       const bool odd = ln & 8;
       float r = (odd ? x1 : x0) + dpp_move<DPP_ROR8>(odd ? x0 : x1);
       if constexpr (TPC == 4) r = dpp_add<DPP_ROR4>(r);
       s_bc[w][k][(ln >> 5) * N + 4 * q + ((ln >> 4) & 1) * 2 + ((ln >> 3) & 1)] = r;
     }
-#pragma unroll
-    for (int k = 0; k < SCAN_TILE / TPC; ++k) {
-      s_y[k * TPC + q][ch] = ys[k];
-      s_i[k * TPC + q][ch] = is[k];
-      s_m[k * TPC + q][ch] = ms[k];
-    }
     __syncthreads();
     float o_u[EV], o_x[EV], o_z[EV];
 #pragma unroll
     for (int j = 0; j < EV; ++j) {
-      const float I = s_i[ot][oc + j], y = __builtin_fmaf(D[j], u[j], s_y[ot][oc + j]);
-      o_u[j] = __builtin_fmaf(D[j], dy[j], delta[j] * I);
-      o_x[j] = __builtin_fmaf(u[j], I, s_m[ot][oc + j]) * xsig[j];
-      o_z[j] = dout[j] * y * (sig[j] * __builtin_fmaf(z[j], 1.0f - sig[j], 1.0f));
-      dD[j] = __builtin_fmaf(dy[j], u[j], dD[j]);
-      dbias[j] += o_x[j];
+      const int at = ot * CH + oc + j;
+      const float y = s_sums[at], I = s_sums[SUMS + at], M = s_sums[2 * SUMS + at], D = s_dcoef[oc + j], u = s_u[ot][oc + j], dy = s_dy[ot][oc + j];
+      o_u[j] = __builtin_fmaf(D, dy, s_delta[ot][oc + j] * I);
+      o_x[j] = __builtin_fmaf(u, I, M * LN2) * xsig[j];
+      o_z[j] = dzy[j] * __builtin_fmaf(D, u, y);
+      s_dd[ot][oc + j] = __builtin_fmaf(dy, u, s_dd[ot][oc + j]);
+      s_dbias[ot][oc + j] += o_x[j];
     }
     const bool in = t < a.q.T;
-    st_row<TE, EV, VEC>(g.du.d, l * g.du.lane + t * g.du.row, gc, a.C, in, o_u);
-    st_row<TE, EV, VEC>(g.ddelta.d, l * g.ddelta.lane + t * g.ddelta.row, gc, a.C, in, o_x);
-    st_row<TE, EV, VEC>(g.dz.d, l * g.dz.lane + t * g.dz.row, gc, a.C, in, o_z);
+    st_row<TE, EV, VEC>(odu, tile, gc, a.C, in, o_u);
+    st_row<TE, EV, VEC>(odx, tile, gc, a.C, in, o_x);
+    st_row<TE, EV, VEC>(odz, tile, gc, a.C, in, o_z);
     store_bc(tile, false);
+    __syncthreads();
   }
+  const size_t part = (size_t)l * pl.segs + pt.seg;
   if (c < a.C) {
-    const size_t at = ((size_t)l * a.C + c) * N + 4 * q;
-    *reinterpret_cast<float4*>(wk.da + at) = make_float4(dA[0], dA[1], dA[2], dA[3]);
-    if (g.dstate_in)
-      *reinterpret_cast<float4*>(g.dstate_in + at) = make_float4(G[0], G[1], G[2], G[3]);
+    *reinterpret_cast<float4*>(wk.da + (part * a.C + c) * N + 4 * q) =
+        make_float4(dA[0], dA[1], dA[2], dA[3]);
+    if (g.dstate_in && pt.seg == 0)
+      *reinterpret_cast<float4*>(g.dstate_in + ((size_t)l * a.C + c) * N + 4 * q) =
+          make_float4(G[0], G[1], G[2], G[3]);
   }
   // the owners' sums over the tile's positions
-#pragma unroll
-  for (int j = 0; j < EV; ++j) {
-    s_u[ot][oc + j] = dD[j];
-    s_dy[ot][oc + j] = dbias[j];
-  }
   __syncthreads();
   if (tid < 2 * CH) {
     const int cc = tid % CH;
     float s = 0.0f;
-    for (int k = 0; k < SCAN_TILE; ++k) s += tid < CH ? s_u[k][cc] : s_dy[k][cc];
+    for (int k = 0; k < SCAN_TILE; ++k) s += tid < CH ? s_dd[k][cc] : s_dbias[k][cc];
     if (cb * CH + cc < a.C)
-      (tid < CH ? wk.dd : wk.dbias)[(size_t)l * a.C + cb * CH + cc] = s;
+      (tid < CH ? wk.dd : wk.dbias)[part * a.C + cb * CH + cc] = s;
   }
 }
 
@@ -467,20 +721,29 @@ __global__ __launch_bounds__(256) void scan_bc_sum_kernel(const float* __restric
   }
 }
 
-// sums over n partials of `width` values: 64 columns a block, 16 groups of
-// rows, the groups added in order
-__global__ __launch_bounds__(1024) void scan_part_sum_kernel(const float* __restrict__ part, int n,
-                                                             int width, float* __restrict__ out) {
-  __shared__ float sm[16][64];
-  const int col = blockIdx.x * 64 + (threadIdx.x & 63), g = threadIdx.x >> 6;
+// The parameters' gradients, sums over n partials: dA's `width` values, then
+// dD's and dbias's C.  16 columns a block, 16 groups of partials, the groups
+// added in order.
+__global__ __launch_bounds__(256) void scan_part_sum_kernel(GradWork wk, int n, int width, int C,
+                                                            float* __restrict__ dA,
+                                                            float* __restrict__ dD,
+                                                            float* __restrict__ dbias) {
+  __shared__ float sm[16][16];
+  const int ba = (width + 15) / 16, bc = (C + 15) / 16, b = blockIdx.x;
+  const int which = b < ba ? 0 : b < ba + bc ? 1 : 2;
+  const float* part = which == 0 ? wk.da : which == 1 ? wk.dd : wk.dbias;
+  float* out = which == 0 ? dA : which == 1 ? dD : dbias;
+  if (which) width = C;
+  const int i = threadIdx.x & 15, g = threadIdx.x >> 4;
+  const int col = (b - (which == 0 ? 0 : which == 1 ? ba : ba + bc)) * 16 + i;
   float s = 0.0f;
   if (col < width)
 #pragma unroll 8
     for (int k = g; k < n; k += 16) s += part[(size_t)k * width + col];
-  sm[g][threadIdx.x & 63] = s;
+  sm[g][i] = s;
   __syncthreads();
   if (g == 0 && col < width) {
-    for (int k = 1; k < 16; ++k) s += sm[k][threadIdx.x];
+    for (int k = 1; k < 16; ++k) s += sm[k][i];
     out[col] = s;
   }
 }
@@ -497,67 +760,111 @@ int64_t scan_saved_floats(int lanes, int T, int C, int ds) {
   return (int64_t)lanes * ((T + SCAN_TILE - 1) / SCAN_TILE) * C * ds;
 }
 
-size_t scan_work(int lanes, int T, int C, int ds, bool grad) {
-  if (!grad) return 0;
-  const Plan p = scan_plan(T, C);
-  const size_t L = lanes;
-  size_t n = round256(L * C * ds * 4) + 2 * round256(L * C * 4);
-  if (p.cblocks > 1) n += round256((size_t)p.cblocks * L * T * 2 * ds * 4);
-  return n;
+namespace {
+
+// the workspace in 256-byte aligned parts; at null, only their sizes are counted
+struct Take {
+  char* at;
+  size_t used = 0;
+  float* operator()(size_t floats) {
+    float* p = at ? (float*)(at + used) : nullptr;
+    used += round256(floats * 4);
+    return p;
+  }
+};
+Carry take_carry(Take& take, const Plan& p, size_t lanes, size_t C, size_t ds) {
+  if (p.segs == 1) return Carry{};
+  return Carry{take(lanes * p.segs * C * ds), take(lanes * p.segs * C)};
+}
+GradWork take_grad(Take& take, const Plan& p, size_t lanes, size_t T, size_t C, size_t ds) {
+  GradWork w{};
+  w.da = take(lanes * p.segs * C * ds);
+  w.dd = take(lanes * p.segs * C);
+  w.dbias = take(lanes * p.segs * C);
+  if (p.cblocks > 1) w.bc = take(p.cblocks * lanes * T * 2 * ds);
+  return w;
 }
 
+template <bool REV>
+void launch_carry(const ScanArgs& a, const Plan& pl, const float* first, const Carry& cy,
+                  hipStream_t s) {
+  const int groups = std::min(CARRY_GROUPS, (pl.segs + 3) / 4);
+  BOA_LAUNCH(scan_carry_kernel<REV>, dim3((uint32_t)a.q.lanes * ((a.C * a.ds + 63) / 64)),
+             dim3(64 * groups), 0, s, a.A, first, a.C, a.ds, pl.segs, cy);
+}
+
+}  // namespace
+
+size_t scan_work(int lanes, int T, int C, int ds, bool grad) {
+  const Plan p = scan_plan(lanes, T, C, ds);
+  Take take{nullptr};
+  take_carry(take, p, lanes, C, ds);
+  if (grad) take_grad(take, p, lanes, T, C, ds);
+  return take.used;
+}
+
+#define BOA_SCAN_N(TE, V)              \
+  if (a.ds == 16) BOA_SCAN(TE, 16, V); \
+  else BOA_SCAN(TE, 32, V)
+#define BOA_SCAN_ALL                          \
+  if (a.bf16) {                               \
+    if (vec) { BOA_SCAN_N(uint16_t, true); }  \
+    else { BOA_SCAN_N(uint16_t, false); }     \
+  } else {                                    \
+    if (vec) { BOA_SCAN_N(float, true); }     \
+    else { BOA_SCAN_N(float, false); }        \
+  }
+
 hipError_t launch_scan(const ScanArgs& a, hipStream_t s) {
-  const Plan pl = scan_plan(a.q.T, a.C);
+  const Plan pl = scan_plan(a.q.lanes, a.q.T, a.C, a.ds);
   const int ev = a.ds == 16 ? Shape<16>::EV : Shape<32>::EV, size = a.bf16 ? 2 : 4;
   auto ok = [&](const auto& r) { return rows_vec(r.d, r.lane, r.row, ev, size); };
   const bool vec = a.C % ev == 0 && ok(a.u) && ok(a.delta) && ok(a.z) && ok(a.out);
-  const dim3 grid((uint32_t)a.q.lanes * pl.cblocks);
+  Take take{(char*)a.work};
+  const Carry cy = take_carry(take, pl, a.q.lanes, a.C, a.ds);
+  if (pl.segs > 1) {
+    const dim3 grid((uint32_t)a.q.lanes * (pl.segs - 1) * pl.cblocks);
+    ScanGradArgs g{};
+    g.f = a;
 #define BOA_SCAN(TE, N, V) \
-  BOA_LAUNCH((scan_kernel<TE, N, V>), grid, dim3(Shape<N>::BT), 0, s, a, pl)
-#define BOA_SCAN_N(TE, V)             \
-  if (a.ds == 16) BOA_SCAN(TE, 16, V); \
-  else BOA_SCAN(TE, 32, V)
-  if (a.bf16) {
-    if (vec) { BOA_SCAN_N(uint16_t, true); }
-    else { BOA_SCAN_N(uint16_t, false); }
-  } else {
-    if (vec) { BOA_SCAN_N(float, true); }
-    else { BOA_SCAN_N(float, false); }
+  BOA_LAUNCH((scan_local_kernel<TE, N, V, false>), grid, dim3(Shape<N>::BT), 0, s, g, pl, cy)
+    BOA_SCAN_ALL
+#undef BOA_SCAN
+    launch_carry<false>(a, pl, a.state_in, cy, s);
   }
+  const dim3 grid((uint32_t)a.q.lanes * pl.segs * pl.cblocks);
+#define BOA_SCAN(TE, N, V) \
+  BOA_LAUNCH((scan_kernel<TE, N, V>), grid, dim3(Shape<N>::BT), 0, s, a, pl, cy.state)
+  BOA_SCAN_ALL
 #undef BOA_SCAN
   return hipGetLastError();
 }
 
 hipError_t launch_scan_grad(const ScanGradArgs& g, hipStream_t s) {
   const ScanArgs& a = g.f;
-  const Plan pl = scan_plan(a.q.T, a.C);
+  const Plan pl = scan_plan(a.q.lanes, a.q.T, a.C, a.ds);
   const int ev = a.ds == 16 ? Shape<16>::EV : Shape<32>::EV, size = a.bf16 ? 2 : 4;
   auto ok = [&](const auto& r) { return rows_vec(r.d, r.lane, r.row, ev, size); };
   const bool vec = a.C % ev == 0 && ok(a.u) && ok(a.delta) && ok(a.z) && ok(g.dout) && ok(g.du) &&
                    ok(g.ddelta) && ok(g.dz);
-  const size_t L = a.q.lanes, rows = L * a.q.T;
-  char* at = (char*)a.work;
-  auto take = [&](size_t floats) {
-    float* p = (float*)at;
-    at += round256(floats * 4);
-    return p;
-  };
-  GradWork wk{};
-  wk.da = take(L * a.C * a.ds);
-  wk.dd = take(L * a.C);
-  wk.dbias = take(L * a.C);
-  if (pl.cblocks > 1) wk.bc = take((size_t)pl.cblocks * rows * 2 * a.ds);
-  const dim3 grid((uint32_t)a.q.lanes * pl.cblocks);
+  const size_t rows = (size_t)a.q.lanes * a.q.T;
+  Take take{(char*)a.work};
+  const Carry cy = take_carry(take, pl, a.q.lanes, a.C, a.ds);
+  const GradWork wk = take_grad(take, pl, a.q.lanes, a.q.T, a.C, a.ds);
+  if (pl.segs > 1) {
+    const dim3 grid((uint32_t)a.q.lanes * (pl.segs - 1) * pl.cblocks);
 #define BOA_SCAN(TE, N, V) \
-  BOA_LAUNCH((scan_grad_kernel<TE, N, V>), grid, dim3(Shape<N>::BT), 0, s, g, pl, wk)
-  if (a.bf16) {
-    if (vec) { BOA_SCAN_N(uint16_t, true); }
-    else { BOA_SCAN_N(uint16_t, false); }
-  } else {
-    if (vec) { BOA_SCAN_N(float, true); }
-    else { BOA_SCAN_N(float, false); }
-  }
+  BOA_LAUNCH((scan_local_kernel<TE, N, V, true>), grid, dim3(Shape<N>::BT), 0, s, g, pl, cy)
+    BOA_SCAN_ALL
 #undef BOA_SCAN
+    launch_carry<true>(a, pl, g.dstate_out, cy, s);
+  }
+  const dim3 grid((uint32_t)a.q.lanes * pl.segs * pl.cblocks);
+#define BOA_SCAN(TE, N, V) \
+  BOA_LAUNCH((scan_grad_kernel<TE, N, V>), grid, dim3(Shape<N>::BT), 0, s, g, pl, wk, cy.state)
+  BOA_SCAN_ALL
+#undef BOA_SCAN
+#undef BOA_SCAN_ALL
 #undef BOA_SCAN_N
   if (pl.cblocks > 1) {
     const dim3 gb((uint32_t)std::min<size_t>(MAX_BLOCKS, (rows * 2 * a.ds + 255) / 256));
@@ -568,13 +875,9 @@ hipError_t launch_scan_grad(const ScanGradArgs& g, hipStream_t s) {
       BOA_LAUNCH(scan_bc_sum_kernel<float>, gb, dim3(256), 0, s, wk.bc, pl.cblocks, (uint32_t)rows,
                  a.q.T, a.ds, g.db, g.dc);
   }
-  auto sum = [&](const float* p, int width, float* out) {
-    BOA_LAUNCH(scan_part_sum_kernel, dim3((width + 63) / 64), dim3(1024), 0, s, p, (int)L, width,
-               out);
-  };
-  sum(wk.da, a.C * a.ds, g.dA);
-  sum(wk.dd, a.C, g.dD);
-  sum(wk.dbias, a.C, g.dbias);
+  const int width = a.C * a.ds;
+  BOA_LAUNCH(scan_part_sum_kernel, dim3((width + 15) / 16 + 2 * ((a.C + 15) / 16)), dim3(256), 0, s,
+             wk, a.q.lanes * pl.segs, width, a.C, g.dA, g.dD, g.dbias);
   return hipGetLastError();
 }
 

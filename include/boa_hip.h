@@ -202,8 +202,8 @@ int64_t boa_embed_grad_work_bytes(int32_t lanes, int32_t T, int32_t width);
  *   out   = (sum_n C[n] h[n] + D u) * z sigmoid(z)
  * B and C rows are d_state wide and shared by the channels.  d_A [channels]
  * [d_state] (that is -exp(A_log)), d_D and d_delta_bias [channels], states
- * [lanes][channels][d_state]; d_state_in NULL is zero.  With T = 1 this is a
- * decode step. */
+ * [lanes][channels][d_state]; d_state_in NULL is zero.  Row strides of the
+ * scan's tensors are at most 2^25.  With T = 1 this is a decode step. */
 typedef struct {
     int32_t lanes, T, channels, d_state, precision;
     const int32_t* d_lens;

@@ -286,7 +286,8 @@ SCAN = [(1, 1, 1, 16, "dense", "full"), (2, 1, 64, 32, "dense", "full"),
         (3, 31, 67, 16, "odd", "ragged"), (2, 40, 66, 32, "odd", "ragged"),
         (4, 35, 192, 32, "time", "ragged"), (2, 100, 128, 16, "time", "full"),
         (70, 5, 32, 16, "dense", "ragged"), (1, 333, 64, 16, "dense", "full"),
-        (2, 150, 64, 32, "wide", "ragged")]
+        (2, 150, 64, 32, "wide", "ragged"), (1, 1201, 20, 16, "dense", "full"),
+        (3, 700, 64, 32, "dense", "ragged")]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

@@ -159,54 +159,62 @@ def _ptr(x):
 # ---- training operators: tensors to C arguments
 # (what the C entry points cannot see -- types, shapes, devices -- is checked
 # here; sizes, strides, alignment and workspaces are checked there)
-_PRECISION = {"torch.float32": 0, "torch.bfloat16": 1}
-
-
-def _tensor(t, name, shape, dtype, device, dense=True):
-    """t's pointer (None for None), of this shape and type on this device."""
+def _tensor(t, name, shape, dtype, device):
+    """A dense tensor's pointer (None for None), of this shape and type on this device."""
     if t is None:
         return None
-    if tuple(t.shape) != tuple(shape) or str(t.dtype) != dtype:
+    if t.shape != shape or t.dtype != dtype:
         raise ValueError(f"{name}: want {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    if not t.is_cuda or t.device.index != device:
+    if t.get_device() != device or not t.is_cuda:
         raise ValueError(f"{name} is on {t.device}, the context on cuda:{device}")
-    if dense and not t.is_contiguous():
+    if not t.is_contiguous():
         raise ValueError(f"{name} has to be contiguous")
     return t.data_ptr()
 
 
 def _rows(t, name, lanes, T, width, dtype, device):
     """A [lanes, T, width] tensor, dense in its last dimension, as a Rows."""
-    d = _tensor(t, name, (lanes, T, width), dtype, device, dense=False)
-    if width > 1 and t.stride(2) != 1:
+    if t.shape != (lanes, T, width) or t.dtype != dtype:
+        raise ValueError(f"{name}: want {dtype} {(lanes, T, width)}, got {t.dtype} "
+                         f"{tuple(t.shape)}")
+    if t.get_device() != device or not t.is_cuda:
+        raise ValueError(f"{name} is on {t.device}, the context on cuda:{device}")
+    ls, rs, one = t.stride()
+    if one != 1 and width > 1:
         raise ValueError(f"{name} has to be dense in its last dimension")
-    return Rows(d, t.stride(0), t.stride(1))
+    return Rows(t.data_ptr(), ls, rs)
 
 
 def _bytes(t, name, device):
     """A uint8 [lanes, T] tensor, dense along T: (pointer, stride of a lane, lanes, T)."""
-    if t.dim() != 2:
-        raise ValueError(f"{name}: want [lanes, T], got {tuple(t.shape)}")
-    d = _tensor(t, name, t.shape, "torch.uint8", device, dense=False)
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    import torch
+    if t.dim() != 2 or t.dtype != torch.uint8:
+        raise ValueError(f"{name}: want uint8 [lanes, T], got {t.dtype} {tuple(t.shape)}")
+    if t.get_device() != device or not t.is_cuda:
+        raise ValueError(f"{name} is on {t.device}, the context on cuda:{device}")
+    ls, one = t.stride()
+    if one != 1 and t.shape[1] > 1:
         raise ValueError(f"{name} has to be dense along T")
-    return d, t.stride(0), t.shape[0], t.shape[1]
+    return t.data_ptr(), ls, t.shape[0], t.shape[1]
 
 
 def _precision(t, name):
-    p = _PRECISION.get(str(t.dtype))
-    if p is None or t.dim() != 3:
-        raise ValueError(f"{name}: want float32 or bfloat16 [lanes, T, width], got {t.dtype} "
-                         f"{tuple(t.shape)}")
-    return p, str(t.dtype)
+    import torch
+    if t.dim() == 3:
+        if t.dtype == torch.float32:
+            return 0
+        if t.dtype == torch.bfloat16:
+            return 1
+    raise ValueError(f"{name}: want float32 or bfloat16 [lanes, T, width], got {t.dtype} "
+                     f"{tuple(t.shape)}")
 
 
 def _work(t, device):
     """A workspace tensor of any type: (pointer, bytes)."""
     if t is None:
         return None, 0
-    n = t.numel() * t.element_size()
-    if n and (not t.is_cuda or t.device.index != device or not t.is_contiguous()):
+    n = t.nbytes
+    if n and (t.get_device() != device or not t.is_cuda or not t.is_contiguous()):
         raise ValueError(f"the workspace has to be contiguous, on cuda:{device}")
     return (t.data_ptr() if n else None), n
 
@@ -247,6 +255,7 @@ class Codec:
         if rc != BOA_OK:
             raise BoaError(f"boa_create failed ({rc})")
         self.h = h
+        self.device = lib().boa_device(h)
 
     def _check(self, rc, what):
         if rc != BOA_OK:
@@ -307,68 +316,65 @@ class Codec:
     # ---- training operators (boa_embed and the calls after it in boa_hip.h):
     # tensors on the context's device; row tensors [lanes, T, width], float32
     # or bfloat16, dense in their last dimension; d_lens int32 [lanes] or None
-    def _device(self):
-        return lib().boa_device(self.h)
-
     def embed(self, d_tokens, d_table, d_out, scale=1.0, d_lens=None):
         """out = scale * table[tokens]; table [256, width] of out's type."""
-        dev = self._device()
+        import torch
+        dev = self.device
         tok, stride, lanes, T = _bytes(d_tokens, "tokens", dev)
-        prec, dt = _precision(d_out, "out")
-        width = d_out.shape[2]
-        out = _rows(d_out, "out", lanes, T, width, dt, dev)
+        prec, dt, width = _precision(d_out, "out"), d_out.dtype, d_out.shape[2]
         self._check(lib().boa_embed(
-            self.h, tok, stride, _tensor(d_lens, "lens", (lanes,), "torch.int32", dev), lanes, T,
-            _tensor(d_table, "table", (256, width), dt, dev), width, prec, scale, C.byref(out)),
-            "embed")
+            self.h, tok, stride, _tensor(d_lens, "lens", (lanes,), torch.int32, dev), lanes, T,
+            _tensor(d_table, "table", (256, width), dt, dev), width, prec, scale,
+            C.byref(_rows(d_out, "out", lanes, T, width, dt, dev))), "embed")
 
     def embed_grad(self, d_tokens, d_dout, d_dtable, d_work=None, scale=1.0, d_lens=None):
         """dtable (float32 [256, width]) = scale * sums of dout's rows by token."""
-        dev = self._device()
+        import torch
+        dev = self.device
         tok, stride, lanes, T = _bytes(d_tokens, "tokens", dev)
-        prec, dt = _precision(d_dout, "dout")
-        width = d_dout.shape[2]
-        dout = _rows(d_dout, "dout", lanes, T, width, dt, dev)
+        prec, width = _precision(d_dout, "dout"), d_dout.shape[2]
         self._check(lib().boa_embed_grad(
-            self.h, tok, stride, _tensor(d_lens, "lens", (lanes,), "torch.int32", dev), lanes, T,
-            C.byref(dout), width, prec, scale,
-            _tensor(d_dtable, "dtable", (256, width), "torch.float32", dev),
+            self.h, tok, stride, _tensor(d_lens, "lens", (lanes,), torch.int32, dev), lanes, T,
+            C.byref(_rows(d_dout, "dout", lanes, T, width, d_dout.dtype, dev)), width, prec, scale,
+            _tensor(d_dtable, "dtable", (256, width), torch.float32, dev),
             *_work(d_work, dev)), "embed_grad")
 
     def _scan_args(self, u, delta, z, b, c, A, D, delta_bias, state_in, lens):
-        dev, f32 = self._device(), "torch.float32"
-        prec, dt = _precision(u, "u")
-        lanes, T, ch = u.shape
+        import torch
+        dev, f32, prec = self.device, torch.float32, _precision(u, "u")
+        (lanes, T, ch), dt = u.shape, u.dtype
         if A.dim() != 2:
             raise ValueError(f"A: want [channels, d_state], got {tuple(A.shape)}")
         n = A.shape[1]
-        return Scan(lanes, T, ch, n, prec, _tensor(lens, "lens", (lanes,), "torch.int32", dev),
-                    *[_rows(t, k, lanes, T, w, dt, dev) for t, k, w in
-                      ((u, "u", ch), (delta, "delta", ch), (z, "z", ch), (b, "B", n), (c, "C", n))],
+        return Scan(lanes, T, ch, n, prec, _tensor(lens, "lens", (lanes,), torch.int32, dev),
+                    _rows(u, "u", lanes, T, ch, dt, dev),
+                    _rows(delta, "delta", lanes, T, ch, dt, dev),
+                    _rows(z, "z", lanes, T, ch, dt, dev),
+                    _rows(b, "B", lanes, T, n, dt, dev), _rows(c, "C", lanes, T, n, dt, dev),
                     _tensor(A, "A", (ch, n), f32, dev), _tensor(D, "D", (ch,), f32, dev),
                     _tensor(delta_bias, "delta_bias", (ch,), f32, dev),
-                    _tensor(state_in, "state_in", (lanes, ch, n), f32, dev)), dt, dev
+                    _tensor(state_in, "state_in", (lanes, ch, n), f32, dev))
 
     def selective_scan(self, d_u, d_delta, d_z, d_b, d_c, d_A, d_D, d_delta_bias, d_out,
                        d_work=None, d_state_in=None, d_state_out=None, d_lens=None, d_saved=None):
         """The gated recurrence; d_saved (selective_scan_saved_floats floats)
         keeps what its gradient starts from."""
-        s, dt, dev = self._scan_args(d_u, d_delta, d_z, d_b, d_c, d_A, d_D, d_delta_bias,
-                                     d_state_in, d_lens)
-        out = _rows(d_out, "out", s.lanes, s.T, s.channels, dt, dev)
+        s, dev = self._scan_args(d_u, d_delta, d_z, d_b, d_c, d_A, d_D, d_delta_bias, d_state_in,
+                                 d_lens), self.device
+        out = _rows(d_out, "out", s.lanes, s.T, s.channels, d_u.dtype, dev)
         self._check(lib().boa_selective_scan(
             self.h, C.byref(s), C.byref(out),
-            _tensor(d_state_out, "state_out", (s.lanes, s.channels, s.d_state), "torch.float32",
-                    dev),
+            _tensor(d_state_out, "state_out", (s.lanes, s.channels, s.d_state), d_A.dtype, dev),
             self._saved(d_saved, s, dev), *_work(d_work, dev)), "selective_scan")
 
     def _saved(self, t, s, dev):
         if t is None:
             return None
+        import torch
         n = lib().boa_selective_scan_saved_floats(s.lanes, s.T, s.channels, s.d_state)
         if t.numel() < n:
             raise ValueError(f"saved: want {n} floats, got {t.numel()}")
-        return _tensor(t, "saved", t.shape, "torch.float32", dev)
+        return _tensor(t, "saved", t.shape, torch.float32, dev)
 
     def selective_scan_grad(self, d_u, d_delta, d_z, d_b, d_c, d_A, d_D, d_delta_bias, d_saved,
                             d_dout, d_du, d_ddelta, d_dz, d_db, d_dc, d_dA, d_dD, d_ddelta_bias,
@@ -376,36 +382,38 @@ class Codec:
                             d_lens=None):
         """Gradients of selective_scan, from its inputs, its d_saved and the
         gradients of its outputs (d_dstate_out None: zero)."""
-        s, dt, dev = self._scan_args(d_u, d_delta, d_z, d_b, d_c, d_A, d_D, d_delta_bias,
-                                     d_state_in, d_lens)
-        f32, ch, n = "torch.float32", s.channels, s.d_state
-        state = (s.lanes, ch, n)
-        dout = _rows(d_dout, "dout", s.lanes, s.T, ch, dt, dev)
-        g = ScanGrads(*[_rows(t, k, s.lanes, s.T, w, dt, dev) for t, k, w in
-                        ((d_du, "du", ch), (d_ddelta, "ddelta", ch), (d_dz, "dz", ch),
-                         (d_db, "dB", n), (d_dc, "dC", n))],
+        s, dev = self._scan_args(d_u, d_delta, d_z, d_b, d_c, d_A, d_D, d_delta_bias, d_state_in,
+                                 d_lens), self.device
+        f32, dt, lanes, T, ch, n = d_A.dtype, d_u.dtype, s.lanes, s.T, s.channels, s.d_state
+        dout = _rows(d_dout, "dout", lanes, T, ch, dt, dev)
+        g = ScanGrads(_rows(d_du, "du", lanes, T, ch, dt, dev),
+                      _rows(d_ddelta, "ddelta", lanes, T, ch, dt, dev),
+                      _rows(d_dz, "dz", lanes, T, ch, dt, dev),
+                      _rows(d_db, "dB", lanes, T, n, dt, dev),
+                      _rows(d_dc, "dC", lanes, T, n, dt, dev),
                       _tensor(d_dA, "dA", (ch, n), f32, dev), _tensor(d_dD, "dD", (ch,), f32, dev),
                       _tensor(d_ddelta_bias, "ddelta_bias", (ch,), f32, dev),
-                      _tensor(d_dstate_in, "dstate_in", state, f32, dev))
+                      _tensor(d_dstate_in, "dstate_in", (lanes, ch, n), f32, dev))
         self._check(lib().boa_selective_scan_grad(
             self.h, C.byref(s), self._saved(d_saved, s, dev), C.byref(dout),
-            _tensor(d_dstate_out, "dstate_out", state, f32, dev), C.byref(g),
+            _tensor(d_dstate_out, "dstate_out", (lanes, ch, n), f32, dev), C.byref(g),
             *_work(d_work, dev)), "selective_scan_grad")
 
     def next_byte_loss(self, d_logits, d_targets, d_loss, d_work=None, d_bias=None, d_total=None,
                        d_dlogits=None, d_dbias=None, scale=1.0, d_lens=None):
         """loss [lanes, T] in nats, its sum, and scale times the gradients of
         the sum; dlogits may be logits."""
-        dev, f32 = self._device(), "torch.float32"
-        prec, dt = _precision(d_logits, "logits")
+        import torch
+        dev, f32 = self.device, torch.float32
+        prec, dt = _precision(d_logits, "logits"), d_logits.dtype
         tgt, stride, lanes, T = _bytes(d_targets, "targets", dev)
-        x = _rows(d_logits, "logits", lanes, T, 256, dt, dev)
         dx = None
         if d_dlogits is not None:
             dx = C.byref(_rows(d_dlogits, "dlogits", lanes, T, 256, dt, dev))
         self._check(lib().boa_next_byte_loss(
-            self.h, C.byref(x), _tensor(d_bias, "bias", (256,), f32, dev), tgt, stride,
-            _tensor(d_lens, "lens", (lanes,), "torch.int32", dev), lanes, T, prec, scale,
+            self.h, C.byref(_rows(d_logits, "logits", lanes, T, 256, dt, dev)),
+            _tensor(d_bias, "bias", (256,), f32, dev), tgt, stride,
+            _tensor(d_lens, "lens", (lanes,), torch.int32, dev), lanes, T, prec, scale,
             _tensor(d_loss, "loss", (lanes, T), f32, dev), _tensor(d_total, "total", (1,), f32, dev),
             dx, _tensor(d_dbias, "dbias", (256,), f32, dev), *_work(d_work, dev)),
             "next_byte_loss")

@@ -53,26 +53,6 @@ __device__ __forceinline__ float fold16(float x, float y) {
   const auto s = __builtin_amdgcn_permlane16_swap(f2u(x), f2u(y), false, false);
   return u2f(s[0]) + u2f(s[1]);
 }
-// over the 64 lanes, the result in all of them
-__device__ __forceinline__ float wave_sum(float x) {
-  x = dpp_add<DPP_XOR1>(x);
-  x = dpp_add<DPP_XOR2>(x);
-  x = dpp_add<DPP_HALF_MIRROR>(x);
-  x = dpp_add<DPP_MIRROR>(x);
-  x = fold16(x, x);
-  return fold32(x, x);
-}
-__device__ __forceinline__ float wave_max(float x) {
-  x = fmaxf(x, dpp_move<DPP_XOR1>(x));
-  x = fmaxf(x, dpp_move<DPP_XOR2>(x));
-  x = fmaxf(x, dpp_move<DPP_HALF_MIRROR>(x));
-  x = fmaxf(x, dpp_move<DPP_MIRROR>(x));
-  const auto s = __builtin_amdgcn_permlane16_swap(f2u(x), f2u(x), false, false);
-  x = fmaxf(u2f(s[0]), u2f(s[1]));
-  const auto t = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
-  return fmaxf(u2f(t[0]), u2f(t[1]));
-}
-
 // ---- embedding (train_ops.hip) -------------------------------------------
 struct EmbedArgs {
   Seqs q;

@@ -63,26 +63,58 @@ bool rows16(const void* d, int64_t lane, int64_t row, int width, int size) {
 
 // -------------------------------------------------------------- embedding
 // out[r] = scale table[tok[r]], one rounding.  Bound by the writes of the
-// rows: the 256 table rows stay in the L2s.  A thread moves 16 bytes a step,
-// `steps` of them, over per_block consecutive vectors of the output.
-template <typename T, int V>
+// rows: the 256 table rows stay in the L2s.  A block takes whole rows, about
+// 256 U vectors of 16 bytes, U a thread, whose bytes, table rows and stores
+// are each under way together.  inv = ceil(2^32 / vectors a row) divides the
+// block's vectors by a multiplication; a row's lane and position follow from
+// the block's first row's.
+template <typename T, int V, int U>
 __global__ __launch_bounds__(256) void embed_kernel(const EmbedArgs a, uint32_t rows,
-                                                    uint32_t block_rows) {
-  const uint32_t vpr = a.width / V;
-  for (uint64_t r0 = (uint64_t)blockIdx.x * block_rows; r0 < rows;
-       r0 += (uint64_t)gridDim.x * block_rows) {
-    const uint32_t n = (uint32_t)min((uint64_t)block_rows, rows - r0) * vpr;
-    for (uint32_t i = threadIdx.x; i < n; i += 256) {
-      const uint32_t k = i / vpr, col = (i - k * vpr) * V, r = (uint32_t)r0 + k;
-      const uint32_t l = r / (uint32_t)a.q.T, t = r - l * a.q.T;
-      if ((int)t >= seq_len(a.q, l)) continue;
-      const uint32_t byte = a.tok[l * a.tok_lane + t];
-      float v[V];
-      ld_vec<V>((const T*)a.table + (size_t)byte * a.width + col, v);
+                                                    uint32_t block_rows, uint32_t inv) {
+  const uint32_t vpr = a.width / V, len = a.q.T;
+  for (uint64_t b0 = (uint64_t)blockIdx.x * block_rows; b0 < rows;
+       b0 += (uint64_t)gridDim.x * block_rows) {
+    const uint32_t r0 = (uint32_t)b0, l0 = r0 / len, t0 = r0 - l0 * len;
+    const uint32_t n = min(block_rows, rows - r0) * vpr;
+    uint32_t l[U], t[U], col[U], byte[U];
+    bool ok[U];
+    float v[U][V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] *= a.scale;
-      st_vec<V>((T*)a.out.d + l * a.out.lane + t * a.out.row + col, v);
+    for (int u = 0; u < U; ++u) {
+      const uint32_t i = threadIdx.x + 256 * u, k = vpr == 1 ? i : __umulhi(i, inv);
+      col[u] = (i - k * vpr) * V;
+      l[u] = l0;
+      t[u] = t0 + k;
+      if (t[u] >= len) {
+        if (block_rows <= len) {
+          l[u] += 1;
+          t[u] -= len;
+        } else {
+          const uint32_t d = t[u] / len;
+          l[u] += d;
+          t[u] -= d * len;
+        }
+      }
+      ok[u] = i < n;
+      if (!ok[u]) l[u] = t[u] = 0;
     }
+    // no branch lies between loads (each would wait for those before it): what
+    // takes no part reads the table's first byte as its token
+#pragma unroll
+    for (int u = 0; u < U; ++u) ok[u] = ok[u] && (int)t[u] < seq_len(a.q, l[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      byte[u] = *(ok[u] ? a.tok + l[u] * a.tok_lane + t[u] : (const uint8_t*)a.table);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      ld_vec<V>((const T*)a.table + byte[u] * (uint32_t)a.width + col[u], v[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (ok[u]) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[u][j] *= a.scale;
+        st_vec<V>((T*)a.out.d + l[u] * a.out.lane + t[u] * a.out.row + col[u], v[u]);
+      }
   }
 }
 
@@ -92,8 +124,8 @@ __global__ __launch_bounds__(256) void embed_kernel(const EmbedArgs a, uint32_t 
 // `chunk` rows (a stable counting sort in LDS), then its groups of G lanes
 // take equal parts of the sorted rows and sum run by run, so a byte that
 // fills most rows is spread over all groups like any other.  Runs that cross
-// a group's border leave their pieces in LDS, and the group they start in
-// joins them in order.  One partial row per byte that occurs in the chunk
+// a group's border leave their later pieces in LDS, and the group they start
+// in adds them in order.  One partial row per byte that occurs in the chunk
 // goes to the workspace; the second kernel sums a byte's partials over the
 // chunks.  dout is read once; the partials are at most 256 / chunk of it.
 constexpr int EG_THREADS = 512, EG_WAVES = EG_THREADS / 64, EG_MAX_CHUNK = 2048;
@@ -131,7 +163,7 @@ __global__ __launch_bounds__(EG_THREADS) void embed_grad_kernel(
   __shared__ uint64_t list[EG_MAX_CHUNK];  // dout offset, the byte in the top 8 bits
   __shared__ uint16_t start[257], slot[256];
   __shared__ uint32_t wave_tot[4];
-  __shared__ float head[V * NV][EG_THREADS], tail[V * NV][EG_THREADS];
+  __shared__ float head[V * NV][EG_THREADS];
   const int tid = threadIdx.x, w = tid >> 6, ln = tid & 63;
   const uint32_t c = blockIdx.x, r0 = c * (uint32_t)chunk;
 
@@ -146,21 +178,23 @@ __global__ __launch_bounds__(EG_THREADS) void embed_grad_kernel(
   volatile uint32_t* my_hist = hist[w];
 #pragma unroll
   for (int i = 0; i < MB; ++i) {
+    const uint32_t lr = (w * batches + i) * 64 + ln, r = r0 + lr;
     valid[i] = false;
     key[i] = 0;
     rank[i] = 0;
-    if (i < batches) {
-      const int b = w * batches + i;
-      const uint32_t lr = b * 64 + ln, r = r0 + lr;
-      uint32_t byte = 0;
-      if (lr < (uint32_t)chunk && r < rows) {
-        const uint32_t l = r / (uint32_t)a.q.T, t = r - l * a.q.T;
-        if ((int)t < seq_len(a.q, l)) {
-          valid[i] = true;
-          byte = a.tok[l * a.tok_lane + t];
-          key[i] = ((uint64_t)byte << 56) | (uint64_t)(l * a.dout.lane + t * a.dout.row);
-        }
+    if (i < batches && lr < (uint32_t)chunk && r < rows) {
+      const uint32_t l = r / (uint32_t)a.q.T, t = r - l * a.q.T;
+      if ((int)t < seq_len(a.q, l)) {
+        valid[i] = true;
+        key[i] = ((uint64_t)a.tok[l * a.tok_lane + t] << 56) |
+                 (uint64_t)(l * a.dout.lane + t * a.dout.row);
       }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MB; ++i) {
+    if (i < batches) {
+      const uint32_t byte = (uint32_t)(key[i] >> 56);
       uint64_t same = __builtin_amdgcn_ballot_w64(valid[i]);
 #pragma unroll
       for (int bit = 0; bit < 8; ++bit) {
@@ -215,120 +249,139 @@ __global__ __launch_bounds__(EG_THREADS) void embed_grad_kernel(
   const int per = (n + groups - 1) / groups;
   const int p0 = min(n, g * per), p1 = min(n, p0 + per);
   const T* dout = (const T*)a.dout.d;
-  auto store = [&](int byte, const float (&acc)[V * NV]) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int col = (k * G + gl) * V;
-      if (col < a.width) {
-        float v[V];
-        float* dst;
-        if (slot_map) {
-          dst = part + ((size_t)c * slots + slot[byte]) * a.width + col;
-#pragma unroll
-          for (int j = 0; j < V; ++j) v[j] = acc[k * V + j];
-        } else {
-          dst = a.dtable + (size_t)byte * a.width + col;
-#pragma unroll
-          for (int j = 0; j < V; ++j) v[j] = acc[k * V + j] * a.scale;
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) dst[j] = v[j];
-      }
-    }
-  };
   float acc[V * NV];
 #pragma unroll
   for (int j = 0; j < V * NV; ++j) acc[j] = 0.0f;
   int cur = p0 < p1 ? (int)(list[p0] >> 56) : 0;
-  auto flush = [&](int byte) {  // the run of `byte` ends here, or the group's part does
-    if (start[byte] < p0) {
+  // where the run's sum goes: bytes that occur have consecutive slots, in order
+  const bool partial = slot_map != nullptr;
+  const float scale = partial ? 1.0f : a.scale;
+  float* dst = partial ? part + ((size_t)c * slots + slot[cur]) * a.width
+                       : a.dtable + (size_t)cur * a.width;
+  auto store = [&](float* to) {
 #pragma unroll
-      for (int j = 0; j < V * NV; ++j) head[j][tid] = acc[j];
-    } else if (start[byte + 1] > p1) {
+    for (int k = 0; k < NV; ++k) {
+      const int col = (k * G + gl) * V;
+      if (col < a.width) {
+        if constexpr (V > 1) {  // width is a multiple of V, and so of four
 #pragma unroll
-      for (int j = 0; j < V * NV; ++j) tail[j][tid] = acc[j];
-    } else {
-      store(byte, acc);
+          for (int j = 0; j < V; j += 4)
+            *reinterpret_cast<float4*>(to + col + j) =
+                make_float4(acc[k * V + j] * scale, acc[k * V + j + 1] * scale,
+                            acc[k * V + j + 2] * scale, acc[k * V + j + 3] * scale);
+        } else {
+          to[col] = acc[k] * scale;
+        }
+      }
     }
   };
-  constexpr int U = 4;  // rows in flight
-  for (int p = p0; p < p1; p += U) {
-    float v[U][NV][V];
-    int byte[U];
+  bool begun = p0 < p1 && start[cur] < p0;  // the run began in an earlier group
+  auto flush = [&]() {                      // the run ends here
+    if (begun) {
+#pragma unroll
+      for (int j = 0; j < V * NV; ++j) head[j][tid] = acc[j];
+      begun = false;
+    } else {
+      store(dst);
+    }
+  };
+  // U rows are summed while the next U are on their way
+  constexpr int U = V * NV <= 4 ? 8 : 4;
+  float v[2][U][NV][V];
+  int byte[2][U];
+  auto fetch = [&](int p, int h) {
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const uint64_t e = list[min(p + k, p1 - 1)];
-      byte[k] = (int)(e >> 56);
+      byte[h][k] = (int)(e >> 56);
       const T* src = dout + (e & 0x00FFFFFFFFFFFFFFull);
 #pragma unroll
       for (int m = 0; m < NV; ++m) {
-        const int col = (m * G + gl) * V;
-        if (col < a.width) ld_vec<V>(src + col, v[k][m]);
+        // without a branch, which would wait for the loads before it: lanes past
+        // the width read its last vector
+        ld_vec<V>(src + min((m * G + gl) * V, a.width - V), v[h][k][m]);
       }
     }
+  };
+  auto add = [&](int p, int h) {
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       if (p + k < p1) {
-        if (byte[k] != cur) {
-          flush(cur);
-          cur = byte[k];
+        if (byte[h][k] != cur) {
+          flush();
+          dst += (size_t)(partial ? 1 : byte[h][k] - cur) * a.width;
+          cur = byte[h][k];
 #pragma unroll
           for (int j = 0; j < V * NV; ++j) acc[j] = 0.0f;
         }
 #pragma unroll
         for (int m = 0; m < NV; ++m)
-          if ((m * G + gl) * V < a.width)
 #pragma unroll
-            for (int j = 0; j < V; ++j) acc[m * V + j] += v[k][m][j];
+          for (int j = 0; j < V; ++j) acc[m * V + j] += v[h][k][m][j];
       }
     }
+  };
+  if (p0 < p1) fetch(p0, 0);
+  for (int p = p0; p < p1; p += 2 * U) {
+    if (p + U < p1) fetch(p + U, 1);
+    add(p, 0);
+    if (p + 2 * U < p1) fetch(p + 2 * U, 0);
+    if (p + U < p1) add(p + U, 1);
   }
-  if (p0 < p1) flush(cur);
+  const int end = start[cur + 1];
+  const bool goes_on = p0 < p1 && !begun && end > p1;
+  if (p0 < p1 && !goes_on) flush();
   __syncthreads();
   // a run that starts here and goes on: its later pieces are the next groups' heads
-  if (p0 < p1 && start[cur] >= p0 && start[cur + 1] > p1) {
-#pragma unroll
-    for (int j = 0; j < V * NV; ++j) acc[j] = tail[j][tid];
-    const int end = start[cur + 1];
+  if (goes_on) {
     for (int h = g + 1; h < groups && h * per < end; ++h)
 #pragma unroll
       for (int j = 0; j < V * NV; ++j) acc[j] += head[j][h * G + gl];
-    store(cur, acc);
+    store(dst);
   }
-  if (!slot_map)  // the only chunk: bytes that do not occur have no gradient
+  if (!partial)  // the only chunk: bytes that do not occur have no gradient
     for (int i = tid; i < 256 * a.width; i += EG_THREADS)
       if (slot[i / a.width] == 0xFFFF) a.dtable[i] = 0.0f;
 }
 
-// a byte's partial rows summed over the chunks: groups of G lanes take every
-// groups-th chunk, then the groups' sums are added in order
+// a byte's partial rows summed over the chunks: the slots of up to 1024 chunks
+// come to LDS at once, groups of G lanes take every groups-th chunk, and the
+// groups' sums are added in order
+constexpr int EG_SLOTS = 1024;
 template <int V>
 __global__ __launch_bounds__(EG_THREADS) void embed_grad_sum_kernel(
     const float* __restrict__ part, const uint16_t* __restrict__ slot_map, int chunks, int slots,
     int width, int G, float scale, float* __restrict__ dtable) {
   __shared__ float sums[V][EG_THREADS];
+  __shared__ uint16_t map[EG_SLOTS];
   const int byte = blockIdx.x, tid = threadIdx.x, g = tid / G, gl = tid % G, groups = EG_THREADS / G;
   const int col = (blockIdx.y * G + gl) * V;
-  const uint16_t* map = slot_map + (size_t)byte * chunks;
   float acc[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) acc[j] = 0.0f;
-  if (col < width) {
-    constexpr int U = 8;
-    for (int c = g; c < chunks; c += U * groups) {
-      float v[U][V];
+  for (int c0 = 0; c0 < chunks; c0 += EG_SLOTS) {
+    const int n = min(EG_SLOTS, chunks - c0);
+    __syncthreads();
+    for (int i = tid; i < EG_SLOTS; i += EG_THREADS)
+      map[i] = i < n ? slot_map[(size_t)byte * chunks + c0 + i] : 0xFFFF;
+    __syncthreads();
+    if (col < width) {
+      constexpr int U = 8;
+      for (int c = g; c < n; c += U * groups) {
+        float v[U][V];
+        bool on[U];
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const int cc = c + k * groups;
-        const uint32_t s = cc < chunks ? map[cc] : 0xFFFF;
+        for (int k = 0; k < U; ++k) {
+          const int cc = c + k * groups;
+          const uint32_t s = cc < n ? map[cc] : 0xFFFF;
+          on[k] = s != 0xFFFF;  // else the first partial row is read, and not added
+          ld_vec<V>(part + (on[k] ? ((size_t)(c0 + cc) * slots + s) * width : 0) + col, v[k]);
+        }
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[k][j] = 0.0f;
-        if (s != 0xFFFF) ld_vec<V>(part + ((size_t)cc * slots + s) * width + col, v[k]);
+        for (int k = 0; k < U; ++k)
+#pragma unroll
+          for (int j = 0; j < V; ++j) acc[j] += on[k] ? v[k][j] : 0.0f;
       }
-#pragma unroll
-      for (int k = 0; k < U; ++k)
-#pragma unroll
-        for (int j = 0; j < V; ++j) acc[j] += v[k][j];
     }
   }
 #pragma unroll
@@ -344,136 +397,164 @@ __global__ __launch_bounds__(EG_THREADS) void embed_grad_sum_kernel(
 }
 
 // ---------------------------------------------------------- next-byte loss
-// loss = log sum_j e^{x_j} - x_target, dx = scale (softmax - onehot).  A wave
-// holds a row, four logits a lane, so each logit is read once and its
-// gradient written once: bound by those bytes.  The largest logit's own term
-// (1) stays out of the sum: rest = sum of the others, loss = log1p(rest) +
-// (max - x_target), so a byte predicted with near certainty keeps its small
-// loss and gradient, which 1 + rest would round away.
+// loss = log sum_j e^{x_j} - x_target, dx = scale (softmax - onehot).  A row
+// belongs to 16 lanes, 16 logits each, so a wave works on four rows at once:
+// the maximum and the sum take four steps within a DPP row, the logarithm and
+// the reciprocal serve four rows, and the next four rows are on their way
+// meanwhile.  Each logit is read once and its gradient written once: bound by
+// those bytes.  The largest logit's own term (1) stays out of the sum: rest =
+// sum of the others, loss = log1p(rest) + (max - x_target), so a byte
+// predicted with near certainty keeps its small loss and gradient, which 1 +
+// rest would round away.
 constexpr int LOSS_THREADS = 512, LOSS_WAVES = LOSS_THREADS / 64, LOSS_U = 4;
 
-// blocks: four rows at a time for each wave, at most two blocks a CU
+// blocks: four rows at a time for each wave, at most two blocks a CU; few rows
+// stay in one, which needs no second launch
 int loss_blocks(int64_t rows) {
-  return (int)std::min<int64_t>(512, (rows + 63) / 64);
+  return rows <= 128 ? 1 : (int)std::min<int64_t>(512, (rows + 63) / 64);
 }
 
-__device__ __forceinline__ void ld_row4(const float* p, float (&v)[4]) {
-  const float4 t = raw_f4(p);
-  v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+// sum and maximum over the 16 lanes of a DPP row, in all of them
+__device__ __forceinline__ float row_sum(float x) {
+  x = dpp_add<DPP_XOR1>(x);
+  x = dpp_add<DPP_XOR2>(x);
+  x = dpp_add<DPP_HALF_MIRROR>(x);
+  return dpp_add<DPP_MIRROR>(x);
 }
-__device__ __forceinline__ void ld_row4(const uint16_t* p, float (&v)[4]) {
-  const uint2 t = *reinterpret_cast<const uint2*>(p);
-  v[0] = u2f(t.x << 16); v[1] = u2f(t.x & 0xFFFF0000u);
-  v[2] = u2f(t.y << 16); v[3] = u2f(t.y & 0xFFFF0000u);
-}
-__device__ __forceinline__ void st_row4(float* p, const float (&v)[4]) {
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-}
-__device__ __forceinline__ void st_row4(uint16_t* p, const float (&v)[4]) {
-  *reinterpret_cast<uint2*>(p) =
-      make_uint2((uint32_t)f32_to_bf16(v[0]) | ((uint32_t)f32_to_bf16(v[1]) << 16),
-                 (uint32_t)f32_to_bf16(v[2]) | ((uint32_t)f32_to_bf16(v[3]) << 16));
+__device__ __forceinline__ float row_max(float x) {
+  x = fmaxf(x, dpp_move<DPP_XOR1>(x));
+  x = fmaxf(x, dpp_move<DPP_XOR2>(x));
+  x = fmaxf(x, dpp_move<DPP_HALF_MIRROR>(x));
+  return fmaxf(x, dpp_move<DPP_MIRROR>(x));
 }
 
-// log(1 + x), x >= 0: log(y) x / (y - 1) with y = 1 + x rounded corrects y's rounding
-__device__ __forceinline__ float log1p_pos(float x) {
-  const float y = 1.0f + x, d = y - 1.0f;
-  const float r = d > 0.0f ? log_core(y) * (x / d) : x;
-  return y < __builtin_huge_valf() ? r : y;  // inf and NaN
-}
-
-// VEC: rows aligned for a lane's four logits at once
+// VEC: rows aligned for 16-byte accesses.  A lane's logits are V neighbours
+// (16 bytes) of every 16 V.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(LOSS_THREADS) void loss_kernel(const LossArgs a, uint32_t rows,
                                                             float* __restrict__ part_bias,
                                                             double* __restrict__ part_total) {
+  constexpr int V = 16 / sizeof(T), K = 16 / V;
   __shared__ float sm[LOSS_WAVES][256];
   __shared__ double st[LOSS_WAVES];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ln = threadIdx.x & 63;
+  const int i = ln & 15;
   const uint32_t waves = gridDim.x * LOSS_WAVES, me = blockIdx.x * LOSS_WAVES + w;
-  const T* in = (const T*)a.logits.d;
   T* dx = (T*)a.dlogits.d;
-  float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f}, db[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (a.bias)
+  float bias[16], db[16];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) bias[j] = a.bias[4 * ln + j];
-  double total = 0.0;
-  for (uint64_t g = me; g * LOSS_U < rows; g += waves) {
-    float x[LOSS_U][4];
-    uint32_t l[LOSS_U], t[LOSS_U];
-    bool in_rows[LOSS_U], live[LOSS_U];
+  for (int j = 0; j < 16; ++j) {
+    bias[j] = a.bias ? a.bias[16 * V * (j / V) + V * i + j % V] : 0.0f;
+    db[j] = 0.0f;
+  }
+  // the four rows of a group: this lane's row, its raw logits and target
+  struct Group {
+    bool in, live;
+    uint32_t l, t;
+    int tgt;
+    uint32_t raw[K][4];
+  };
+  auto fetch = [&](uint64_t g, Group& r) {
+    const uint64_t row = g * LOSS_U + (ln >> 4);
+    r.in = row < rows;
+    const uint32_t rr = r.in ? (uint32_t)row : 0;
+    r.l = rr / (uint32_t)a.q.T;
+    r.t = rr - r.l * a.q.T;
+    r.live = r.in && (int)r.t < seq_len(a.q, r.l);
+    r.tgt = 0;
+    if (r.live) {
+      r.tgt = a.tgt[r.l * a.tgt_lane + r.t];
+      const T* p = (const T*)a.logits.d + r.l * a.logits.lane + r.t * a.logits.row + V * i;
 #pragma unroll
-    for (int k = 0; k < LOSS_U; ++k) {
-      const uint64_t r = g * LOSS_U + k;
-      in_rows[k] = r < rows;
-      const uint32_t rr = in_rows[k] ? (uint32_t)r : 0;
-      l[k] = rr / (uint32_t)a.q.T;
-      t[k] = rr - l[k] * a.q.T;
-      live[k] = in_rows[k] && (int)t[k] < seq_len(a.q, l[k]);
-      if (live[k]) {
-        const T* p = in + l[k] * a.logits.lane + t[k] * a.logits.row + 4 * ln;
+      for (int k = 0; k < K; ++k) {
         if constexpr (VEC) {
-          ld_row4(p, x[k]);
+          const uint4 v = *reinterpret_cast<const uint4*>(p + 16 * V * k);
+          r.raw[k][0] = v.x; r.raw[k][1] = v.y; r.raw[k][2] = v.z; r.raw[k][3] = v.w;
         } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[k][j] = ldv(p + j);
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (sizeof(T) == 4)
+              r.raw[k][j] = f2u(p[16 * V * k + j]);
+            else
+              r.raw[k][j] = (uint32_t)p[16 * V * k + 2 * j] | (uint32_t)p[16 * V * k + 2 * j + 1] << 16;
+          }
         }
       }
     }
+  };
+  double total = 0.0;
+  Group nx;
+  if ((uint64_t)me * LOSS_U < rows) fetch(me, nx);
+  for (uint64_t g = me; g * LOSS_U < rows; g += waves) {
+    const Group c = nx;
+    float e[16];
 #pragma unroll
-    for (int k = 0; k < LOSS_U; ++k) {
-      if (!in_rows[k]) continue;
-      float gr[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (live[k]) {
-        const int tgt = a.tgt[l[k] * a.tgt_lane + t[k]];
-        float e[4];
+    for (int j = 0; j < 16; ++j) {
+      if constexpr (sizeof(T) == 4) e[j] = u2f(c.raw[j / V][j % V]);
+      else e[j] = u2f(j % 2 ? c.raw[j / V][j % V / 2] & 0xFFFF0000u : c.raw[j / V][j % V / 2] << 16);
+      e[j] += bias[j];
+    }
+    if ((g + waves) * LOSS_U < rows) fetch(g + waves, nx);
+    float m = e[0];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) e[j] = x[k][j] + bias[j];
-        const float m = wave_max(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])));
-        // the value at the target, and the place of the first largest logit
-        const int tj = tgt & 3, tl = tgt >> 2;
-        const float pick = tj == 0 ? e[0] : tj == 1 ? e[1] : tj == 2 ? e[2] : e[3];
-        const float xt = u2f(__builtin_amdgcn_readlane(f2u(pick), tl));
-        const int mj = e[0] == m ? 0 : e[1] == m ? 1 : e[2] == m ? 2 : e[3] == m ? 3 : 4;
-        const uint64_t has = __builtin_amdgcn_ballot_w64(mj < 4);
-        const int ml = has ? __builtin_ctzll(has) : -1;
-        const int top = ml < 0 ? -1 : 4 * ml + __builtin_amdgcn_readlane(mj, ml);
-        float rest = 0.0f;
+    for (int j = 1; j < 16; ++j) m = fmaxf(m, e[j]);
+    m = row_max(m);
+    const bool none = m == -__builtin_huge_valf();  // nothing is allowed
+    m = none ? 0.0f : m;
+    // the target's place among this lane's logits, or none
+    const int at = (c.tgt / V) % 16 == i ? c.tgt / (16 * V) * V + c.tgt % V : -1;
+    float pick = 0.0f, rest = 0.0f, tops = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          e[j] = __builtin_amdgcn_exp2f((e[j] - m) * 1.44269504088896340736f);
-          rest += 4 * ln + j == top ? 0.0f : e[j];
-        }
-        rest = wave_sum(rest);
-        float loss;
-        if (m == -__builtin_huge_valf()) {  // nothing is allowed: no gradient
-          loss = __builtin_huge_valf();
-        } else {
-          loss = log1p_pos(rest) + (m - xt);
-          const float sum = 1.0f + rest, inv = a.scale / sum;
+    for (int j = 0; j < 16; ++j) {
+      const float d = e[j] - m;
+      pick = at == j ? d : pick;
+      e[j] = __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
+      rest += d == 0.0f ? 0.0f : e[j];
+      tops += d == 0.0f ? 1.0f : 0.0f;
+    }
+    const float dt = row_sum(pick);  // x_target - max
+    rest = row_sum(rest) + (row_sum(tops) - 1.0f);
+    // log1p(rest): what 1 + rest loses is put back
+    const float sum = 1.0f + rest, lost = rest - (sum - 1.0f), inv_sum = __builtin_amdgcn_rcpf(sum);
+    float loss = __builtin_fmaf(__builtin_amdgcn_logf(sum), 0.69314718055994530942f,
+                                lost * inv_sum) - dt;
+    loss = none ? __builtin_huge_valf() : loss;
+    const float inv = none || !c.live ? 0.0f : a.scale * inv_sum;
+    const float gt = (dt == 0.0f ? -rest : __builtin_amdgcn_exp2f(dt * 1.44269504088896340736f) - sum) * inv;
+    float gr[16];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            gr[j] = e[j] * inv;
-            if (4 * ln + j == tgt) gr[j] = tgt == top ? -(rest * inv) : (e[j] - sum) * inv;
-            db[j] += gr[j];
-          }
-        }
-        total += (double)loss;
-        if (ln == 0) a.loss[l[k] * (int64_t)a.q.T + t[k]] = loss;
-      }
-      if (dx) {
-        T* p = dx + l[k] * a.dlogits.lane + t[k] * a.dlogits.row + 4 * ln;
+    for (int j = 0; j < 16; ++j) {
+      gr[j] = at == j ? gt : e[j] * inv;
+      gr[j] = c.live ? gr[j] : 0.0f;  // what was not read may be anything
+      db[j] += gr[j];
+    }
+    if (c.live && i == 0) {
+      total += (double)loss;
+      a.loss[c.l * (int64_t)a.q.T + c.t] = loss;
+    }
+    if (dx && c.in) {
+      T* p = dx + c.l * a.dlogits.lane + c.t * a.dlogits.row + V * i;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float v[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = gr[k * V + j];
         if constexpr (VEC) {
-          st_row4(p, gr);
+          st_vec<V>(p + 16 * V * k, v);
         } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) stv(p + j, gr[j]);
+          for (int j = 0; j < V; ++j) stv(p + 16 * V * k + j, v[j]);
         }
       }
     }
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) sm[w][4 * ln + j] = db[j];
+  for (int j = 0; j < 16; ++j) {
+    const float x = fold16(db[j], db[j]), s = fold32(x, x);
+    if (ln < 16) sm[w][16 * V * (j / V) + V * i + j % V] = s;
+  }
+  total += __shfl_xor(total, 16, 64);
+  total += __shfl_xor(total, 32, 64);
   if (ln == 0) st[w] = total;
   __syncthreads();
   const int tid = threadIdx.x;
@@ -539,18 +620,25 @@ hipError_t launch_embed(const EmbedArgs& a, hipStream_t s) {
   const bool vec = rows16(a.out.d, a.out.lane, a.out.row, a.width, size) &&
                    ((uintptr_t)a.table & 15) == 0;
   const uint32_t vpr = vec ? a.width * size / 16 : a.width;
-  // a block's threads take 8 vectors each; with fewer than two blocks a CU, one
-  const uint64_t vecs = (uint64_t)rows * vpr;
-  const uint32_t per = vecs >= 512ull * 2048 ? 2048 : 256;
-  const uint32_t block_rows = std::max<uint32_t>(1, per / vpr);
-  const dim3 grid(std::min<uint32_t>(MAX_BLOCKS, (rows + block_rows - 1) / block_rows));
+  // a block's threads take 4 vectors each; with fewer than two such blocks a CU, one
+  const int u = (uint64_t)rows * vpr >= 512ull * 1024 ? 4 : 1;
+  const uint32_t block_rows = std::max<uint32_t>(1, 256 * u / vpr);
+  const uint32_t blocks = (rows + block_rows - 1) / block_rows;
+  const uint32_t inv = (uint32_t)(((1ull << 32) + vpr - 1) / vpr);
+  const dim3 grid(std::min(MAX_BLOCKS, blocks));
+#define BOA_EMBED(Tv, Vv)                                                                      \
+  if (block_rows * vpr > 256)                                                                  \
+    BOA_LAUNCH((embed_kernel<Tv, Vv, 4>), grid, dim3(256), 0, s, a, rows, block_rows, inv);    \
+  else                                                                                         \
+    BOA_LAUNCH((embed_kernel<Tv, Vv, 1>), grid, dim3(256), 0, s, a, rows, block_rows, inv)
   if (a.bf16) {
-    if (vec) BOA_LAUNCH((embed_kernel<uint16_t, 8>), grid, dim3(256), 0, s, a, rows, block_rows);
-    else BOA_LAUNCH((embed_kernel<uint16_t, 1>), grid, dim3(256), 0, s, a, rows, block_rows);
+    if (vec) { BOA_EMBED(uint16_t, 8); }
+    else { BOA_EMBED(uint16_t, 1); }
   } else {
-    if (vec) BOA_LAUNCH((embed_kernel<float, 4>), grid, dim3(256), 0, s, a, rows, block_rows);
-    else BOA_LAUNCH((embed_kernel<float, 1>), grid, dim3(256), 0, s, a, rows, block_rows);
+    if (vec) { BOA_EMBED(float, 4); }
+    else { BOA_EMBED(float, 1); }
   }
+#undef BOA_EMBED
   return hipGetLastError();
 }
 
@@ -604,9 +692,9 @@ size_t loss_work(int64_t rows) {
 
 hipError_t launch_loss(const LossArgs& a, hipStream_t s) {
   const uint32_t rows = (uint32_t)a.q.lanes * (uint32_t)a.q.T;
-  const int n = loss_blocks(rows), al = a.bf16 ? 8 : 16;
+  const int n = loss_blocks(rows), v = a.bf16 ? 8 : 4;
   auto fits = [&](const void* d, int64_t lane, int64_t row) {
-    return ((uintptr_t)d & (al - 1)) == 0 && lane % 4 == 0 && row % 4 == 0;
+    return ((uintptr_t)d & 15) == 0 && lane % v == 0 && row % v == 0;
   };
   const bool vec = fits(a.logits.d, a.logits.lane, a.logits.row) &&
                    (!a.dlogits.d || fits(a.dlogits.d, a.dlogits.lane, a.dlogits.row));

@@ -141,6 +141,15 @@ struct Shape {
   static constexpr int WAVES = BT / 64;
 };
 
+// a thread's four states, at any float's address; zero where there are none
+typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ void ld_states(const float* p, bool ok, float (&v)[4]) {
+  f4_any t = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (p && ok) t = *reinterpret_cast<const f4_any*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = t[i];
+}
+
 // sum over the TPC lanes of a channel, in all of them
 template <int TPC>
 __device__ __forceinline__ float sum_states(float x) {
@@ -202,14 +211,15 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_local_kernel(const ScanGr
   const int len = seq_len(a.q, l), q = tid % TPC, ch = tid / TPC, c = cb * CH + ch;
   const int ot = tid / (CH / EV), oc = (tid % (CH / EV)) * EV, gc = cb * CH + oc;
   float h[4] = {0.0f, 0.0f, 0.0f, 0.0f}, A2[4], sum = 0.0f;
+  ld_states(a.A + (size_t)c * N + 4 * q, c < a.C, A2);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) A2[i] = c < a.C ? a.A[(size_t)c * N + 4 * q + i] * LOG2E : 0.0f;
+  for (int i = 0; i < 4; ++i) A2[i] *= LOG2E;
   float bias[EV];
 #pragma unroll
   for (int j = 0; j < EV; ++j) bias[j] = gc + j < a.C ? a.bias[gc + j] : 0.0f;
   constexpr int NBC = SCAN_TILE * N / BT;
   Raw<TE, EV> ru, rx, ro;
-  float rv[NBC];
+  TE rv[NBC];  // as they are: to convert them here would wait for every load before
   const RowsIn &ri = REV ? a.z : a.u, &rows_v = REV ? a.c : a.b;
   using In = Tensor<const TE>;
   const In xu(ri, l, ot, gc), xx(a.delta, l, ot, gc), xo(REV ? g.dout : ri, l, ot, gc);
@@ -222,7 +232,7 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_local_kernel(const ScanGr
 #pragma unroll
     for (int i = 0; i < NBC; ++i) {
       const int e = tid + i * BT;
-      rv[i] = tile * SCAN_TILE + e / N < len ? ldv(In(rows_v, l, e / N, e % N).at(tile)) : 0.0f;
+      rv[i] = tile * SCAN_TILE + e / N < len ? *In(rows_v, l, e / N, e % N).at(tile) : TE(0);
     }
   };
   const int all = (len + SCAN_TILE - 1) / SCAN_TILE;
@@ -242,7 +252,7 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_local_kernel(const ScanGr
       s_x[ot][oc + j] = x;
     }
 #pragma unroll
-    for (int j = 0; j < NBC; ++j) (&s_v[0][0])[tid + j * BT] = rv[j];
+    for (int j = 0; j < NBC; ++j) (&s_v[0][0])[tid + j * BT] = ldv(&rv[j]);
     __syncthreads();
     if (i + 1 < n) fetch(REV ? tile - 1 : tile + 1);
     float d[2][AHEAD], x[2][AHEAD];
@@ -346,16 +356,12 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_kernel(const ScanArgs a, 
   // the row elements that this thread owns: position ot of the tile, channels oc ..
   const int ot = tid / (CH / EV), oc = (tid % (CH / EV)) * EV, gc = cb * CH + oc;
   float h[4], A2[4];
+  ld_states(a.A + (size_t)c * N + 4 * q, c < a.C, A2);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    A2[i] = c < a.C ? a.A[(size_t)c * N + 4 * q + i] * LOG2E : 0.0f;
-    h[i] = 0.0f;
-  }
+  for (int i = 0; i < 4; ++i) A2[i] *= LOG2E;
   const float* enter = carry ? carry + ((size_t)l * pl.segs + pt.seg) * a.C * N
                        : a.state_in ? a.state_in + (size_t)l * a.C * N : nullptr;
-  if (enter && c < a.C)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = enter[c * N + 4 * q + i];
+  ld_states(enter ? enter + c * N + 4 * q : nullptr, c < a.C, h);
   float bias[EV], D[EV];
 #pragma unroll
   for (int j = 0; j < EV; ++j) {
@@ -364,7 +370,7 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_kernel(const ScanArgs a, 
   }
   constexpr int NBC = SCAN_TILE * N / BT;  // elements of B (and of C) a thread stages
   Raw<TE, EV> ru, rx, rz;
-  float rb[NBC], rc[NBC];
+  TE rb[NBC], rc[NBC];  // as they are: to convert them here would wait for every load before
   using In = Tensor<const TE>;
   const In xu(a.u, l, ot, gc), xx(a.delta, l, ot, gc), xz(a.z, l, ot, gc);
   const Tensor<TE> xout(a.out, l, ot, gc);
@@ -378,8 +384,8 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_kernel(const ScanArgs a, 
     for (int i = 0; i < NBC; ++i) {
       const int e = tid + i * BT;
       const bool in = tile * SCAN_TILE + e / N < len;
-      rb[i] = in ? ldv(In(a.b, l, e / N, e % N).at(tile)) : 0.0f;
-      rc[i] = in ? ldv(In(a.c, l, e / N, e % N).at(tile)) : 0.0f;
+      rb[i] = in ? *In(a.b, l, e / N, e % N).at(tile) : TE(0);
+      rc[i] = in ? *In(a.c, l, e / N, e % N).at(tile) : TE(0);
     }
   };
   if (first < tiles) fetch(first);
@@ -400,8 +406,8 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_kernel(const ScanArgs a, 
 #pragma unroll
     for (int i = 0; i < NBC; ++i) {
       const int e = tid + i * BT;
-      (&s_b[0][0])[e] = rb[i];
-      (&s_c[0][0])[e] = rc[i];
+      (&s_b[0][0])[e] = ldv(&rb[i]);
+      (&s_c[0][0])[e] = ldv(&rc[i]);
     }
     __syncthreads();
     if (tile + 1 < tiles) fetch(tile + 1);
@@ -486,16 +492,15 @@ __global__ __launch_bounds__((Shape<N>::BT)) __attribute__((amdgpu_waves_per_eu(
   const int first = pt.seg * pl.seg_tiles, last = min(pl.tiles, first + pl.seg_tiles);
   float* sums = s_sums + min(q & 3, 2) * SUMS + ch;
   float A2[4], G[4], dA[4];
+  ld_states(a.A + (size_t)c * N + 4 * q, c < a.C, A2);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    A2[i] = c < a.C ? a.A[(size_t)c * N + 4 * q + i] * LOG2E : 0.0f;
-    G[i] = dA[i] = 0.0f;
+    A2[i] *= LOG2E;
+    dA[i] = 0.0f;
   }
   const float* enter = carry ? carry + ((size_t)l * pl.segs + pt.seg) * a.C * N
                        : g.dstate_out ? g.dstate_out + (size_t)l * a.C * N : nullptr;
-  if (enter && c < a.C)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) G[i] = enter[c * N + 4 * q + i];
+  ld_states(enter ? enter + c * N + 4 * q : nullptr, c < a.C, G);
   // the owners' parameters and sums live in LDS, to leave the registers to the states
 #pragma unroll
   for (int j = 0; j < EV; ++j) s_dd[ot][oc + j] = s_dbias[ot][oc + j] = 0.0f;
@@ -506,7 +511,7 @@ __global__ __launch_bounds__((Shape<N>::BT)) __attribute__((amdgpu_waves_per_eu(
   __syncthreads();
   constexpr int NBC = SCAN_TILE * N / BT;
   Raw<TE, EV> ru, rx, rz, ro;
-  float rb[NBC], rc[NBC];
+  TE rb[NBC], rc[NBC];  // as they are: to convert them here would wait for every load before
   float4 rh;
   using In = Tensor<const TE>;
   const In xu(a.u, l, ot, gc), xx(a.delta, l, ot, gc), xz(a.z, l, ot, gc);
@@ -524,8 +529,8 @@ __global__ __launch_bounds__((Shape<N>::BT)) __attribute__((amdgpu_waves_per_eu(
     for (int i = 0; i < NBC; ++i) {
       const int e = tid + i * BT;
       const bool in = tile * SCAN_TILE + e / N < len;
-      rb[i] = in ? ldv(In(a.b, l, e / N, e % N).at(tile)) : 0.0f;
-      rc[i] = in ? ldv(In(a.c, l, e / N, e % N).at(tile)) : 0.0f;
+      rb[i] = in ? *In(a.b, l, e / N, e % N).at(tile) : TE(0);
+      rc[i] = in ? *In(a.c, l, e / N, e % N).at(tile) : TE(0);
     }
     rh = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (c < a.C)
@@ -578,8 +583,8 @@ __global__ __launch_bounds__((Shape<N>::BT)) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
     for (int i = 0; i < NBC; ++i) {
       const int e = tid + i * BT;
-      (&s_b[0][0])[e] = rb[i];
-      (&s_c[0][0])[e] = rc[i];
+      (&s_b[0][0])[e] = ldv(&rb[i]);
+      (&s_c[0][0])[e] = ldv(&rc[i]);
     }
     const float h0[4] = {rh.x, rh.y, rh.z, rh.w};
     __syncthreads();

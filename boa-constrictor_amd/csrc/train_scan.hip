@@ -465,6 +465,43 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_kernel(const ScanArgs a, 
         make_float4(h[0], h[1], h[2], h[3]);
 }
 
+// One position a lane: the decode step, bound by the states' bytes.  Without
+// tiles a thread computes its channel's delta and gate itself (the lanes of a
+// channel the same ones), every load is under way at once, and a CU holds
+// twice the blocks of the tiled kernel.
+template <typename TE, int N>
+__global__ __launch_bounds__((Shape<N>::BT)) void scan_step_kernel(const ScanArgs a, Plan pl) {
+  constexpr int TPC = Shape<N>::TPC;
+  const Part pt = block_part(pl, 1);
+  const int l = pt.l, q = threadIdx.x % TPC, c = pt.cb * CH + threadIdx.x / TPC;
+  if (c >= a.C) return;
+  using In = Tensor<const TE>;
+  const size_t at = ((size_t)l * a.C + c) * N + 4 * q;
+  const bool on = seq_len(a.q, l) > 0;
+  float h[4], A2[4];
+  ld_states(a.state_in ? a.state_in + at : nullptr, true, h);
+  if (a.saved) *reinterpret_cast<float4*>(a.saved + at) = make_float4(h[0], h[1], h[2], h[3]);
+  if (on) {
+    ld_states(a.A + (size_t)c * N + 4 * q, true, A2);
+    const float u = ldv(In(a.u, l, 0, c).at(0)), z = ldv(In(a.z, l, 0, c).at(0));
+    const float x = ldv(In(a.delta, l, 0, c).at(0)) + a.bias[c], D = a.D[c];
+    const TE *pb = In(a.b, l, 0, 4 * q).at(0), *pc = In(a.c, l, 0, 4 * q).at(0);
+    float b[4], cv[4], y = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = ldv(pb + i), cv[i] = ldv(pc + i);
+    const float delta = softplus_full(x), du = delta * u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float e = __builtin_amdgcn_exp2f(delta * (A2[i] * LOG2E));
+      h[i] = __builtin_fmaf(e, h[i], du * b[i]);
+      y = __builtin_fmaf(cv[i], h[i], y);
+    }
+    y = __builtin_fmaf(D, u, sum_states<TPC>(y)) * (z * sigmoid_hw(z));
+    if (q == 0) stv(Tensor<TE>(a.out, l, 0, c).at(0), y);
+  }
+  if (a.state_out) *reinterpret_cast<float4*>(a.state_out + at) = make_float4(h[0], h[1], h[2], h[3]);
+}
+
 // --------------------------------------------------------------- backward
 // Partial sums of a block: dA [lane][seg][C][N], dD and dbias [lane][seg][C],
 // and with more than one channel block dB | dC [cblock][row][2 N]
@@ -825,6 +862,20 @@ hipError_t launch_scan(const ScanArgs& a, hipStream_t s) {
   const int ev = a.ds == 16 ? Shape<16>::EV : Shape<32>::EV, size = a.bf16 ? 2 : 4;
   auto ok = [&](const auto& r) { return rows_vec(r.d, r.lane, r.row, ev, size); };
   const bool vec = a.C % ev == 0 && ok(a.u) && ok(a.delta) && ok(a.z) && ok(a.out);
+  if (a.q.T == 1) {
+    const dim3 grid((uint32_t)a.q.lanes * pl.cblocks);
+#define BOA_STEP(TE, N) \
+  BOA_LAUNCH((scan_step_kernel<TE, N>), grid, dim3(Shape<N>::BT), 0, s, a, pl)
+    if (a.bf16) {
+      if (a.ds == 16) BOA_STEP(uint16_t, 16);
+      else BOA_STEP(uint16_t, 32);
+    } else {
+      if (a.ds == 16) BOA_STEP(float, 16);
+      else BOA_STEP(float, 32);
+    }
+#undef BOA_STEP
+    return hipGetLastError();
+  }
   Take take{(char*)a.work};
   const Carry cy = take_carry(take, pl, a.q.lanes, a.C, a.ds);
   if (pl.segs > 1) {

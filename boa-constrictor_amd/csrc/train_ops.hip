@@ -55,6 +55,31 @@ __device__ __forceinline__ void st_vec(uint16_t* p, const float (&v)[V]) {
   }
 }
 
+// ... past the caches (stream): rows that the L2s cannot hold until they are
+// read (embedding of 261,000 bf16 rows of 256, 133 MB: 38 us through them, 29
+// past them; loss with 533 MB of gradients: 173, 167)
+template <typename T, int V>
+__device__ __forceinline__ void st_rows(T* p, const float (&v)[V], bool stream) {
+  if constexpr (sizeof(T) * V == 16) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    if (stream) {
+      u4 w;
+      if constexpr (V == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = f2u(v[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          w[i] = (uint32_t)f32_to_bf16(v[2 * i]) | ((uint32_t)f32_to_bf16(v[2 * i + 1]) << 16);
+      }
+      __builtin_nontemporal_store(w, reinterpret_cast<u4*>(p));
+      return;
+    }
+  }
+  st_vec<V>(p, v);
+}
+constexpr size_t CACHED_BYTES = (size_t)32 << 20;  // the eight L2s
+
 // whether rows of `width` elements can be moved 16 bytes at a time
 bool rows16(const void* d, int64_t lane, int64_t row, int width, int size) {
   const int v = 16 / size;
@@ -70,7 +95,7 @@ bool rows16(const void* d, int64_t lane, int64_t row, int width, int size) {
 // the block's first row's.
 template <typename T, int V, int U>
 __global__ __launch_bounds__(256) void embed_kernel(const EmbedArgs a, uint32_t rows,
-                                                    uint32_t block_rows, uint32_t inv) {
+                                                    uint32_t block_rows, uint32_t inv, bool stream) {
   const uint32_t vpr = a.width / V, len = a.q.T;
   for (uint64_t b0 = (uint64_t)blockIdx.x * block_rows; b0 < rows;
        b0 += (uint64_t)gridDim.x * block_rows) {
@@ -113,7 +138,7 @@ __global__ __launch_bounds__(256) void embed_kernel(const EmbedArgs a, uint32_t 
       if (ok[u]) {
 #pragma unroll
         for (int j = 0; j < V; ++j) v[u][j] *= a.scale;
-        st_vec<V>((T*)a.out.d + l[u] * a.out.lane + t[u] * a.out.row + col[u], v[u]);
+        st_rows<T, V>((T*)a.out.d + l[u] * a.out.lane + t[u] * a.out.row + col[u], v[u], stream);
       }
   }
 }
@@ -432,6 +457,7 @@ __device__ __forceinline__ float row_max(float x) {
 // (16 bytes) of every 16 V.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(LOSS_THREADS) void loss_kernel(const LossArgs a, uint32_t rows,
+                                                            bool stream,
                                                             float* __restrict__ part_bias,
                                                             double* __restrict__ part_total) {
   constexpr int V = 16 / sizeof(T), K = 16 / V;
@@ -540,7 +566,7 @@ __global__ __launch_bounds__(LOSS_THREADS) void loss_kernel(const LossArgs a, ui
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] = gr[k * V + j];
         if constexpr (VEC) {
-          st_vec<V>(p + 16 * V * k, v);
+          st_rows<T, V>(p + 16 * V * k, v, stream);
         } else {
 #pragma unroll
           for (int j = 0; j < V; ++j) stv(p + 16 * V * k + j, v[j]);
@@ -626,11 +652,14 @@ hipError_t launch_embed(const EmbedArgs& a, hipStream_t s) {
   const uint32_t blocks = (rows + block_rows - 1) / block_rows;
   const uint32_t inv = (uint32_t)(((1ull << 32) + vpr - 1) / vpr);
   const dim3 grid(std::min(MAX_BLOCKS, blocks));
+  const bool stream = (size_t)rows * a.width * size > CACHED_BYTES;
 #define BOA_EMBED(Tv, Vv)                                                                      \
   if (block_rows * vpr > 256)                                                                  \
-    BOA_LAUNCH((embed_kernel<Tv, Vv, 4>), grid, dim3(256), 0, s, a, rows, block_rows, inv);    \
+    BOA_LAUNCH((embed_kernel<Tv, Vv, 4>), grid, dim3(256), 0, s, a, rows, block_rows, inv,     \
+               stream);                                                                        \
   else                                                                                         \
-    BOA_LAUNCH((embed_kernel<Tv, Vv, 1>), grid, dim3(256), 0, s, a, rows, block_rows, inv)
+    BOA_LAUNCH((embed_kernel<Tv, Vv, 1>), grid, dim3(256), 0, s, a, rows, block_rows, inv,     \
+               stream)
   if (a.bf16) {
     if (vec) { BOA_EMBED(uint16_t, 8); }
     else { BOA_EMBED(uint16_t, 1); }
@@ -698,11 +727,13 @@ hipError_t launch_loss(const LossArgs& a, hipStream_t s) {
   };
   const bool vec = fits(a.logits.d, a.logits.lane, a.logits.row) &&
                    (!a.dlogits.d || fits(a.dlogits.d, a.dlogits.lane, a.dlogits.row));
+  const bool stream = (size_t)rows * 256 * (a.bf16 ? 2 : 4) > CACHED_BYTES;
   // doubles first: the workspace is 8-byte aligned
   double* pt = (double*)a.work;
   float* pb = n == 1 ? nullptr : (float*)(pt + n);
 #define BOA_LOSS(Tv, VECv) \
-  BOA_LAUNCH((loss_kernel<Tv, VECv>), dim3(n), dim3(LOSS_THREADS), 0, s, a, rows, pb, pt)
+  BOA_LAUNCH((loss_kernel<Tv, VECv>), dim3(n), dim3(LOSS_THREADS), 0, s, a, rows, stream, pb, \
+             pt)
   if (a.bf16) {
     if (vec) BOA_LOSS(uint16_t, true);
     else BOA_LOSS(uint16_t, false);

@@ -13,6 +13,7 @@ import ctypes as C
 import os
 import re
 import subprocess
+import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libboa_hip.so")
@@ -165,7 +166,7 @@ def _tensor(t, name, shape, dtype, device):
         return None
     if t.shape != shape or t.dtype != dtype:
         raise ValueError(f"{name}: want {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    if t.get_device() != device or not t.is_cuda:
+    if t.get_device() != device:  # -1 on the CPU
         raise ValueError(f"{name} is on {t.device}, the context on cuda:{device}")
     if not t.is_contiguous():
         raise ValueError(f"{name} has to be contiguous")
@@ -177,7 +178,7 @@ def _rows(t, name, lanes, T, width, dtype, device):
     if t.shape != (lanes, T, width) or t.dtype != dtype:
         raise ValueError(f"{name}: want {dtype} {(lanes, T, width)}, got {t.dtype} "
                          f"{tuple(t.shape)}")
-    if t.get_device() != device or not t.is_cuda:
+    if t.get_device() != device:  # -1 on the CPU
         raise ValueError(f"{name} is on {t.device}, the context on cuda:{device}")
     ls, rs, one = t.stride()
     if one != 1 and width > 1:
@@ -187,10 +188,10 @@ def _rows(t, name, lanes, T, width, dtype, device):
 
 def _bytes(t, name, device):
     """A uint8 [lanes, T] tensor, dense along T: (pointer, stride of a lane, lanes, T)."""
-    import torch
+    torch = sys.modules["torch"]  # there is a tensor, so it is loaded
     if t.dim() != 2 or t.dtype != torch.uint8:
         raise ValueError(f"{name}: want uint8 [lanes, T], got {t.dtype} {tuple(t.shape)}")
-    if t.get_device() != device or not t.is_cuda:
+    if t.get_device() != device:  # -1 on the CPU
         raise ValueError(f"{name} is on {t.device}, the context on cuda:{device}")
     ls, one = t.stride()
     if one != 1 and t.shape[1] > 1:
@@ -199,7 +200,7 @@ def _bytes(t, name, device):
 
 
 def _precision(t, name):
-    import torch
+    torch = sys.modules["torch"]  # there is a tensor, so it is loaded
     if t.dim() == 3:
         if t.dtype == torch.float32:
             return 0
@@ -214,7 +215,7 @@ def _work(t, device):
     if t is None:
         return None, 0
     n = t.nbytes
-    if n and (t.get_device() != device or not t.is_cuda or not t.is_contiguous()):
+    if n and (t.get_device() != device or not t.is_contiguous()):
         raise ValueError(f"the workspace has to be contiguous, on cuda:{device}")
     return (t.data_ptr() if n else None), n
 
@@ -318,7 +319,7 @@ class Codec:
     # or bfloat16, dense in their last dimension; d_lens int32 [lanes] or None
     def embed(self, d_tokens, d_table, d_out, scale=1.0, d_lens=None):
         """out = scale * table[tokens]; table [256, width] of out's type."""
-        import torch
+        torch = sys.modules["torch"]
         dev = self.device
         tok, stride, lanes, T = _bytes(d_tokens, "tokens", dev)
         prec, dt, width = _precision(d_out, "out"), d_out.dtype, d_out.shape[2]
@@ -329,7 +330,7 @@ class Codec:
 
     def embed_grad(self, d_tokens, d_dout, d_dtable, d_work=None, scale=1.0, d_lens=None):
         """dtable (float32 [256, width]) = scale * sums of dout's rows by token."""
-        import torch
+        torch = sys.modules["torch"]
         dev = self.device
         tok, stride, lanes, T = _bytes(d_tokens, "tokens", dev)
         prec, width = _precision(d_dout, "dout"), d_dout.shape[2]
@@ -340,7 +341,7 @@ class Codec:
             *_work(d_work, dev)), "embed_grad")
 
     def _scan_args(self, u, delta, z, b, c, A, D, delta_bias, state_in, lens):
-        import torch
+        torch = sys.modules["torch"]
         dev, f32, prec = self.device, torch.float32, _precision(u, "u")
         (lanes, T, ch), dt = u.shape, u.dtype
         if A.dim() != 2:
@@ -370,7 +371,7 @@ class Codec:
     def _saved(self, t, s, dev):
         if t is None:
             return None
-        import torch
+        torch = sys.modules["torch"]
         n = lib().boa_selective_scan_saved_floats(s.lanes, s.T, s.channels, s.d_state)
         if t.numel() < n:
             raise ValueError(f"saved: want {n} floats, got {t.numel()}")
@@ -403,7 +404,7 @@ class Codec:
                        d_dlogits=None, d_dbias=None, scale=1.0, d_lens=None):
         """loss [lanes, T] in nats, its sum, and scale times the gradients of
         the sum; dlogits may be logits."""
-        import torch
+        torch = sys.modules["torch"]
         dev, f32 = self.device, torch.float32
         prec, dt = _precision(d_logits, "logits"), d_logits.dtype
         tgt, stride, lanes, T = _bytes(d_targets, "targets", dev)

@@ -33,6 +33,13 @@ __device__ __forceinline__ int seq_len(const Seqs& q, int l) {
   return n < 0 ? 0 : (n < q.T ? n : q.T);
 }
 
+// bfloat16 of two floats by one instruction, x in the low half
+__device__ __forceinline__ uint32_t bf16_pair(float x, float y) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{x, y}, b2));
+}
+
 // x + x of the lane that CTRL names within the row of 16 lanes
 constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_HALF_MIRROR = 0x141, DPP_MIRROR = 0x140,
               DPP_ROR4 = 0x124, DPP_ROR8 = 0x128;

@@ -48,7 +48,7 @@ __device__ __forceinline__ void st_vec(uint16_t* p, const float (&v)[V]) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      w[i] = (uint32_t)f32_to_bf16(v[2 * i]) | ((uint32_t)f32_to_bf16(v[2 * i + 1]) << 16);
+      w[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
     *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
     *p = f32_to_bf16(v[0]);
@@ -70,7 +70,7 @@ __device__ __forceinline__ void st_rows(T* p, const float (&v)[V], bool stream) 
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          w[i] = (uint32_t)f32_to_bf16(v[2 * i]) | ((uint32_t)f32_to_bf16(v[2 * i + 1]) << 16);
+          w[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
       }
       __builtin_nontemporal_store(w, reinterpret_cast<u4*>(p));
       return;

@@ -65,7 +65,11 @@ struct Tensor {
   __device__ __forceinline__ Tensor(const R& r, int l, int t, int i)
       : lane((P*)r.d + l * r.lane), row(r.row), off((uint32_t)t * (uint32_t)r.row + i) {}
   __device__ __forceinline__ P* at(int tile) const {
-    return lane + (int64_t)tile * SCAN_TILE * row + off;
+    uint32_t o = off;
+    // not known to be the same in every tile: lane + off would take two
+    // registers for each tensor throughout
+    asm volatile("" : "+v"(o));
+    return lane + (int64_t)tile * SCAN_TILE * row + o;
   }
 };
 
@@ -109,6 +113,22 @@ __device__ __forceinline__ float raw_at(const Raw<TE, EV>& r, int i) {
   if constexpr (sizeof(TE) == 4) return u2f(r.w[i]);
   else return u2f(i % 2 ? r.w[i / 2] & 0xFFFF0000u : r.w[i / 2] << 16);
 }
+// EV neighbouring floats of a staged row
+template <int EV>
+__device__ __forceinline__ void st_lds(float* p, const float (&v)[EV]) {
+  if constexpr (EV == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  else *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+}
+template <int EV>
+__device__ __forceinline__ void ld_lds(const float* p, float (&v)[EV]) {
+  if constexpr (EV == 4) {
+    const float4 t = *reinterpret_cast<const float4*>(p);
+    v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+  } else {
+    const float2 t = *reinterpret_cast<const float2*>(p);
+    v[0] = t.x; v[1] = t.y;
+  }
+}
 template <typename TE, int EV, bool VEC>
 __device__ __forceinline__ void st_row(const Tensor<TE>& x, int tile, int c, int C, bool ok,
                                        const float (&v)[EV]) {
@@ -120,7 +140,7 @@ __device__ __forceinline__ void st_row(const Tensor<TE>& x, int tile, int c, int
 #pragma unroll
       for (int i = 0; i < W; ++i) {
         if constexpr (sizeof(TE) == 4) w[i] = f2u(v[i]);
-        else w[i] = (uint32_t)f32_to_bf16(v[2 * i]) | ((uint32_t)f32_to_bf16(v[2 * i + 1]) << 16);
+        else w[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
       }
       if constexpr (W == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
       else if constexpr (W == 2) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
@@ -242,15 +262,16 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_local_kernel(const ScanGr
     const int tile = REV ? lo + n - 1 - i : lo + i;
     const bool ok = tile * SCAN_TILE + ot < len;
     __syncthreads();
+    float o_d[EV], o_x[EV];
 #pragma unroll
     for (int j = 0; j < EV; ++j) {
-      const float delta = softplus_full(ok ? raw_at(rx, j) + bias[j] : NEVER);
-      float x = raw_at(ru, j);
-      if constexpr (REV) x = raw_at(ro, j) * (x * sigmoid_hw(x));
-      else x = delta * x;
-      s_delta[ot][oc + j] = delta;
-      s_x[ot][oc + j] = x;
+      const float in = raw_at(rx, j) + bias[j], x = raw_at(ru, j);
+      o_d[j] = softplus_full(ok ? in : NEVER);
+      if constexpr (REV) o_x[j] = raw_at(ro, j) * (x * sigmoid_hw(x));
+      else o_x[j] = o_d[j] * x;
     }
+    st_lds(&s_delta[ot][oc], o_d);
+    st_lds(&s_x[ot][oc], o_x);
 #pragma unroll
     for (int j = 0; j < NBC; ++j) (&s_v[0][0])[tid + j * BT] = ldv(&rv[j]);
     __syncthreads();
@@ -392,17 +413,19 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_kernel(const ScanArgs a, 
   for (int tile = first; tile < tiles; ++tile) {
     const int t = tile * SCAN_TILE + ot;
     const bool ok = t < len;
-    float u[EV], gate[EV];
+    float u[EV], gate[EV], o_d[EV], o_x[EV];
 #pragma unroll
     for (int j = 0; j < EV; ++j) {
       u[j] = raw_at(ru, j);
       const float z = raw_at(rz, j);
       gate[j] = z * sigmoid_hw(z);
       // past the lane's end delta = 0: the state passes unchanged
-      const float delta = softplus_full(ok ? raw_at(rx, j) + bias[j] : NEVER);
-      s_delta[ot][oc + j] = delta;
-      s_du[ot][oc + j] = delta * u[j];
+      const float in = raw_at(rx, j) + bias[j];
+      o_d[j] = softplus_full(ok ? in : NEVER);
+      o_x[j] = o_d[j] * u[j];
     }
+    st_lds(&s_delta[ot][oc], o_d);
+    st_lds(&s_du[ot][oc], o_x);
 #pragma unroll
     for (int i = 0; i < NBC; ++i) {
       const int e = tid + i * BT;
@@ -456,8 +479,9 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_kernel(const ScanArgs a, 
     for (int k = 0; k < SCAN_TILE / TPC; ++k) s_y[k * TPC + q][ch] = y[k];
     __syncthreads();
     float o[EV];
+    ld_lds(&s_y[ot][oc], o);
 #pragma unroll
-    for (int j = 0; j < EV; ++j) o[j] = __builtin_fmaf(D[j], u[j], s_y[ot][oc + j]) * gate[j];
+    for (int j = 0; j < EV; ++j) o[j] = __builtin_fmaf(D[j], u[j], o[j]) * gate[j];
     st_row<TE, EV, VEC>(xout, tile, gc, a.C, ok, o);
   }
   if (a.state_out && tiles == all && c < a.C)
@@ -576,8 +600,9 @@ __global__ __launch_bounds__((Shape<N>::BT)) __attribute__((amdgpu_waves_per_eu(
   };
   // dB and dC of a tile: one value of one position a thread
   auto store_bc = [&](int tile, bool zero) {
-    for (int e = tid; e < SCAN_TILE * 2 * N; e += BT) {
-      const int k = e / (2 * N), n = e % (2 * N), t = tile * SCAN_TILE + k;
+#pragma unroll
+    for (int j = 0; j < SCAN_TILE * 2 * N / BT; ++j) {
+      const int e = tid + j * BT, k = e / (2 * N), n = e % (2 * N), t = tile * SCAN_TILE + k;
       if (t >= a.q.T) continue;
       float v = 0.0f;
       if (!zero)
@@ -607,16 +632,23 @@ __global__ __launch_bounds__((Shape<N>::BT)) __attribute__((amdgpu_waves_per_eu(
     const int t = tile * SCAN_TILE + ot;
     const bool ok = t < len;
     float dzy[EV], xsig[EV];  // dz / y, d delta / dx; the rest is read back from LDS
+    float bias[EV], o_d[EV], o_x[EV], o_y[EV];
+    ld_lds(&s_bias[oc], bias);
 #pragma unroll
     for (int j = 0; j < EV; ++j) {
       const float z = raw_at(rz, j), sig = sigmoid_hw(z), dout = raw_at(ro, j);
-      const float x = ok ? raw_at(rx, j) + s_bias[oc + j] : NEVER;
+      const float in = raw_at(rx, j) + bias[j], x = ok ? in : NEVER;
       dzy[j] = dout * (sig * __builtin_fmaf(z, 1.0f - sig, 1.0f));
       xsig[j] = sigmoid_hw(x);
-      s_delta[ot][oc + j] = softplus_full(x);
-      s_u[ot][oc + j] = raw_at(ru, j);
-      s_dy[ot][oc + j] = dout * (z * sig);
+      o_d[j] = softplus_full(x);
+      o_x[j] = raw_at(ru, j);
+      o_y[j] = dout * (z * sig);
+      // now, and not where they are used: that would keep what they are made of
+      asm volatile("" : "+v"(dzy[j]), "+v"(xsig[j]));
     }
+    st_lds(&s_delta[ot][oc], o_d);
+    st_lds(&s_u[ot][oc], o_x);
+    st_lds(&s_dy[ot][oc], o_y);
 #pragma unroll
     for (int i = 0; i < NBC; ++i) {
       const int e = tid + i * BT;
@@ -688,6 +720,8 @@ __global__ __launch_bounds__((Shape<N>::BT)) __attribute__((amdgpu_waves_per_eu(
         const float m = G[i] * (k ? hs[k > 0 ? k - 1 : 0][i] : h0[i]);
         M = __builtin_fmaf(m, A2[i], M);
         dA[i] = __builtin_fmaf(m, dl, dA[i]);
+        // here: put off to the end of the tile these sums would keep 64 m
+        asm volatile("" : "+v"(dA[i]));
         const auto x = __builtin_amdgcn_permlane32_swap(f2u(dh), f2u(hs[k][i]), false, false);
         v[i] = __builtin_fmaf(u2f(x[1]), c1, u2f(x[0]) * c0);
       }
@@ -709,17 +743,21 @@ __global__ __launch_bounds__((Shape<N>::BT)) __attribute__((amdgpu_waves_per_eu(
       s_bc[w][k][(ln >> 5) * N + 4 * q + ((ln >> 4) & 1) * 2 + ((ln >> 3) & 1)] = r;
     }
     __syncthreads();
-    float o_u[EV], o_x[EV], o_z[EV];
+    float o_u[EV], o_z[EV], I[EV], y[EV], M[EV], D[EV], u[EV], dy[EV], dl[EV], sd[EV], sb[EV];
+    const int at = ot * CH + oc;
+    ld_lds(&s_sums[at], y), ld_lds(&s_sums[SUMS + at], I), ld_lds(&s_sums[2 * SUMS + at], M);
+    ld_lds(&s_dcoef[oc], D), ld_lds(&s_u[ot][oc], u), ld_lds(&s_dy[ot][oc], dy);
+    ld_lds(&s_delta[ot][oc], dl), ld_lds(&s_dd[ot][oc], sd), ld_lds(&s_dbias[ot][oc], sb);
 #pragma unroll
     for (int j = 0; j < EV; ++j) {
-      const int at = ot * CH + oc + j;
-      const float y = s_sums[at], I = s_sums[SUMS + at], M = s_sums[2 * SUMS + at], D = s_dcoef[oc + j], u = s_u[ot][oc + j], dy = s_dy[ot][oc + j];
-      o_u[j] = __builtin_fmaf(D, dy, s_delta[ot][oc + j] * I);
-      o_x[j] = __builtin_fmaf(u, I, M * LN2) * xsig[j];
-      o_z[j] = dzy[j] * __builtin_fmaf(D, u, y);
-      s_dd[ot][oc + j] = __builtin_fmaf(dy, u, s_dd[ot][oc + j]);
-      s_dbias[ot][oc + j] += o_x[j];
+      o_u[j] = __builtin_fmaf(D[j], dy[j], dl[j] * I[j]);
+      o_x[j] = __builtin_fmaf(u[j], I[j], M[j] * LN2) * xsig[j];
+      o_z[j] = dzy[j] * __builtin_fmaf(D[j], u[j], y[j]);
+      sd[j] = __builtin_fmaf(dy[j], u[j], sd[j]);
+      sb[j] += o_x[j];
     }
+    st_lds(&s_dd[ot][oc], sd);
+    st_lds(&s_dbias[ot][oc], sb);
     const bool in = t < a.q.T;
     st_row<TE, EV, VEC>(odu, tile, gc, a.C, in, o_u);
     st_row<TE, EV, VEC>(odx, tile, gc, a.C, in, o_x);

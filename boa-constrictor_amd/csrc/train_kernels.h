@@ -33,6 +33,9 @@ __device__ __forceinline__ int seq_len(const Seqs& q, int l) {
   return n < 0 ? 0 : (n < q.T ? n : q.T);
 }
 
+// four floats at any float's address
+typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
+
 // bfloat16 of two floats by one instruction, x in the low half
 __device__ __forceinline__ uint32_t bf16_pair(float x, float y) {
   typedef float f2 __attribute__((ext_vector_type(2)));

@@ -291,9 +291,9 @@ __global__ __launch_bounds__(EG_THREADS) void embed_grad_kernel(
         if constexpr (V > 1) {  // width is a multiple of V, and so of four
 #pragma unroll
           for (int j = 0; j < V; j += 4)
-            *reinterpret_cast<float4*>(to + col + j) =
-                make_float4(acc[k * V + j] * scale, acc[k * V + j + 1] * scale,
-                            acc[k * V + j + 2] * scale, acc[k * V + j + 3] * scale);
+            *reinterpret_cast<f4_any*>(to + col + j) =
+                f4_any{acc[k * V + j] * scale, acc[k * V + j + 1] * scale,
+                       acc[k * V + j + 2] * scale, acc[k * V + j + 3] * scale};
         } else {
           to[col] = acc[k] * scale;
         }

@@ -162,7 +162,6 @@ struct Shape {
 };
 
 // a thread's four states, at any float's address; zero where there are none
-typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
 __device__ __forceinline__ void ld_states(const float* p, bool ok, float (&v)[4]) {
   f4_any t = {0.0f, 0.0f, 0.0f, 0.0f};
   if (p && ok) t = *reinterpret_cast<const f4_any*>(p);

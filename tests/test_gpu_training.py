@@ -287,7 +287,11 @@ SCAN = [(1, 1, 1, 16, "dense", "full"), (2, 1, 64, 32, "dense", "full"),
         (4, 35, 192, 32, "time", "ragged"), (2, 100, 128, 16, "time", "full"),
         (70, 5, 32, 16, "dense", "ragged"), (1, 333, 64, 16, "dense", "full"),
         (2, 150, 64, 32, "wide", "ragged"), (1, 1201, 20, 16, "dense", "full"),
-        (3, 700, 64, 32, "dense", "ragged")]
+        (3, 700, 64, 32, "dense", "ragged"),
+        (520, 19, 16, 16, "dense", "ragged"),    # whole lanes: no segments
+        (264, 17, 12, 32, "time", "ragged"),
+        (1, 4300, 4, 16, "dense", "full"),       # as many segments as there are
+        (2, 5, 4096, 16, "dense", "full"), (1, 18, 4095, 32, "odd", "full")]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -358,6 +362,68 @@ def test_scan_extremes(codec):
     ref.check("state_out", got["state_out"], state)
     for k, want in ref.scan_grad(s, live, kept).items():
         ref.check(k, got[k], want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_scan_of_one_lane_alone(codec, dtype):
+    """A lane's results do not depend on the lanes beside it, nor on NaN there."""
+    s, _ = scan_inputs(4, 40, 96, 16, dtype, "full")
+    a, _ = run_scan(codec, s, None, "dense")
+    t = {k: v.clone() for k, v in s.items()}
+    t["u"][1, 7] = math.nan
+    t["B"][3] = math.inf
+    b, _ = run_scan(codec, t, None, "dense")
+    for k in ("out", "state_out", "du", "ddelta", "dz", "dB", "dC", "dstate_in"):
+        assert torch.equal(a[k][0], b[k][0]) and torch.equal(a[k][2], b[k][2]), k
+
+
+# ------------------------------------------------------------- far addresses
+def far(t, dtype=None, fill=SKIP):
+    """[2, T, width] with 2^31 + 16 elements between the lanes."""
+    lanes, T, width = t.shape
+    step = (1 << 31) + 16
+    buf = torch.empty(step + T * width, dtype=t.dtype, device="cuda")
+    v = torch.as_strided(buf, (lanes, T, width), (step, width, 1))
+    v.copy_(t)
+    return v
+
+
+def test_far_lanes(codec):
+    """Offsets that pass 32 bits: every row tensor in turn."""
+    g = torch.Generator().manual_seed(9)
+    lanes, T, width = 2, 21, 64
+    tok = tokens_of("any", lanes, T, g)
+    live = ref.mask(None, lanes, T)
+    table = torch.randn((256, width), generator=g).to(BF16)
+    out = far(torch.zeros((lanes, T, width), dtype=BF16))
+    codec.embed(dev(tok), dev(table), out)
+    ref.check("out", out, ref.embed(tok, table, 1.0), BF16)
+    del out
+    dout = torch.randn((lanes, T, width), generator=g).to(BF16)
+    dtable = torch.zeros(256 * width + 1, device="cuda")[1:].view(256, width)  # unaligned
+    n = boa_hip.embed_grad_work_bytes(lanes, T, width)
+    codec.embed_grad(dev(tok), far(dout), dtable, work(n))
+    ref.check("dtable", dtable, ref.embed_grad(tok, dout, 1.0, live))
+    x = torch.randn((lanes, T, 256), generator=g).to(BF16)
+    loss = torch.zeros((lanes, T), device="cuda")
+    dx = far(torch.zeros((lanes, T, 256), dtype=BF16))
+    codec.next_byte_loss(far(x), dev(tok), loss, work(boa_hip.next_byte_loss_work_bytes(lanes, T)),
+                         d_dlogits=dx)
+    want = ref.loss(x, None, tok, 1.0, live)
+    ref.check("loss", loss, want[0])
+    ref.check("dlogits", dx, want[2], BF16)
+    del dx
+    s, _ = scan_inputs(lanes, T, 64, 16, BF16, "full")
+    near, _ = run_scan(codec, s, None, "dense")
+    d = {k: v.cuda() for k, v in s.items()}
+    for name in ROWS_IN[:5]:
+        e = dict(d, **{name: far(s[name])})
+        o, st = torch.zeros((lanes, T, 64), dtype=BF16, device="cuda"), torch.zeros_like(d["state_in"])
+        codec.selective_scan(*[e[k] for k in ("u", "delta", "z", "B", "C", "A", "D", "delta_bias")],
+                             o, work(boa_hip.selective_scan_work_bytes(lanes, T, 64, 16)),
+                             d_state_in=d["state_in"], d_state_out=st)
+        assert torch.equal(o, near["out"]) and torch.equal(st, near["state_out"]), name
+        del e
 
 
 # ---------------------------------------------------------- used as they are
@@ -556,6 +622,9 @@ def test_refusals(codec):
     refused(lambda: scan(state_out=z(2049)[1:].view(2, 64, 16)), "aligned")
     refused(lambda: scan(out=d["u"]), "input")
     refused(lambda: scan(out=z(1, 5, 64).expand(2, 5, 64)), "rows overlap")
+    wide = torch.empty(((1 << 25) + 1) * 4 + 128, device="cuda")
+    refused(lambda: scan(u=torch.as_strided(wide, (2, 5, 64), (64, (1 << 25) + 1, 1))), "2^25")
+    del wide
     saved = z(boa_hip.selective_scan_saved_floats(2, 5, 64, 16))
     g = [z(2, 5, 64), z(2, 5, 64), z(2, 5, 64), z(2, 5, 16), z(2, 5, 16), z(64, 16), z(64), z(64)]
     a = [d[k] for k in names]

@@ -146,16 +146,24 @@ __global__ __launch_bounds__(256) void embed_kernel(const EmbedArgs a, uint32_t 
 // ----------------------------------------------------- embedding gradient
 // dtable[v] = scale sum of dout's rows whose token is v, in fp32 and in an
 // order that only the sizes decide (no atomics).  A block sorts the tokens of
-// `chunk` rows (a stable counting sort in LDS), then its groups of G lanes
-// take equal parts of the sorted rows and sum run by run, so a byte that
-// fills most rows is spread over all groups like any other.  Runs that cross
-// a group's border leave their later pieces in LDS, and the group they start
-// in adds them in order.  One partial row per byte that occurs in the chunk
-// goes to the workspace; the second kernel sums a byte's partials over the
-// chunks.  dout is read once; the partials are at most 256 / chunk of it.
-constexpr int EG_THREADS = 512, EG_WAVES = EG_THREADS / 64, EG_MAX_CHUNK = 2048;
+// `chunk` rows by a stable counting sort in LDS.  Then its groups of G lanes
+// take equal parts of the sorted rows and sum run by run, so a byte that fills
+// most rows is spread over all groups like any other.  Runs that cross a
+// group's border leave their later pieces in LDS, and the group they start in
+// adds them in order.  One partial row per byte that occurs in the chunk goes
+// to the workspace; the second kernel sums a byte's partials over the chunks.
+// dout is read once; the partials are at most 256 / chunk of it.  A chunk is
+// batches of 64 rows from all over the sequences, so that blocks come by as
+// many rows within their lanes' lengths.
+// Bound by dout's bytes; 1000 x 521 ragged fp32 rows of 256, most bytes zero
+// (267 MB within the lengths): 88 us with consecutive rows and 512 threads, 81
+// with batches, 75 with 1024 threads (3.6 TB/s; the sort and the runs of single
+// rows, which one wave of a block gets all of, are the rest).
+constexpr int EG_THREADS = 1024, EG_WAVES = EG_THREADS / 64, EG_MAX_CHUNK = 2048;
 
-// rows a block sorts: enough blocks for every CU, few partials
+// Rows a block sorts: at least a block a CU, then as many as there can be, for
+// few partials (twice the blocks of half the rows: as fast at 521,000 rows, and
+// the second kernel takes 11 us and not 7).
 int embed_grad_chunk(int64_t rows) {
   int chunk = 64;
   while (chunk < EG_MAX_CHUNK && rows > (int64_t)chunk * 256) chunk *= 2;
@@ -190,7 +198,7 @@ __global__ __launch_bounds__(EG_THREADS) void embed_grad_kernel(
   __shared__ uint32_t wave_tot[4];
   __shared__ float head[V * NV][EG_THREADS];
   const int tid = threadIdx.x, w = tid >> 6, ln = tid & 63;
-  const uint32_t c = blockIdx.x, r0 = c * (uint32_t)chunk;
+  const uint32_t c = blockIdx.x;
 
   // each wave ranks its own consecutive batches of 64 rows among equal bytes
   for (int i = tid; i < EG_WAVES * 256; i += EG_THREADS) (&hist[0][0])[i] = 0;
@@ -203,11 +211,13 @@ __global__ __launch_bounds__(EG_THREADS) void embed_grad_kernel(
   volatile uint32_t* my_hist = hist[w];
 #pragma unroll
   for (int i = 0; i < MB; ++i) {
-    const uint32_t lr = (w * batches + i) * 64 + ln, r = r0 + lr;
+    const uint32_t b = w * batches + i;
+    const uint64_t r64 = ((uint64_t)b * chunks + c) * 64 + ln;
+    const uint32_t r = (uint32_t)r64;
     valid[i] = false;
     key[i] = 0;
     rank[i] = 0;
-    if (i < batches && lr < (uint32_t)chunk && r < rows) {
+    if (i < batches && b < (uint32_t)chunk / 64 && r64 < rows) {
       const uint32_t l = r / (uint32_t)a.q.T, t = r - l * a.q.T;
       if ((int)t < seq_len(a.q, l)) {
         valid[i] = true;
@@ -311,7 +321,7 @@ __global__ __launch_bounds__(EG_THREADS) void embed_grad_kernel(
     }
   };
   // U rows are summed while the next U are on their way
-  constexpr int U = V * NV <= 4 ? 8 : 4;
+  constexpr int U = V * NV <= 4 ? 8 : V > 1 ? 4 : 2;
   float v[2][U][NV][V];
   int byte[2][U];
   auto fetch = [&](int p, int h) {

@@ -208,10 +208,42 @@ __device__ __forceinline__ Part block_part(const Plan& p, int segs) {
   const int cb = blockIdx.x % p.cblocks, r = blockIdx.x / p.cblocks;
   return Part{r / segs, r % segs, cb};
 }
-// the segments' states [lane][seg][C][N] and sums of delta [lane][seg][C]
+// The segments' states [lane][seg][C][N] and sums of delta [lane][seg][C].  Up
+// to CHAIN_SEGS segments every block of the main pass chains those before its
+// own itself; more would read too much, and a kernel between the passes puts
+// what enters each segment in their place (`entered`).  (4 lanes x 257, 17
+// segments, forward and gradient: 46 us with that kernel, 38 without.)
+constexpr int CHAIN_SEGS = 32;
 struct Carry {
   float *state, *sum;
+  bool entered;
 };
+
+// What enters segment `seg` of lane l for a thread's four states of channel c:
+// the chain from `first` (null: zero) over the segments before it (REV: after
+// it, from the last).
+template <int N, bool REV>
+__device__ __forceinline__ void enter_segment(const Carry& cy, const float* first, int segs, int l,
+                                              int seg, int c, int C, int q, const float (&A2)[4],
+                                              float (&h)[4]) {
+  const bool on = c < C;
+  if (cy.entered) {
+    ld_states(cy.state + (((size_t)l * segs + seg) * C + c) * N + 4 * q, on, h);
+    return;
+  }
+  ld_states(first ? first + ((size_t)l * C + c) * N + 4 * q : nullptr, on, h);
+  if (!on) return;
+  const int n = REV ? segs - 1 - seg : seg;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const size_t at = ((size_t)l * segs + (REV ? segs - 1 - i : i)) * C + c;
+    float s[4];
+    ld_states(cy.state + at * N + 4 * q, true, s);
+    const float d = cy.sum[at];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(A2[j] * d), h[j], s[j]);
+  }
+}
 
 // What a segment does to the state that enters it.  Forward: the state that
 // it leaves when it starts from zero.  Backward (REV): the gradient of the
@@ -361,7 +393,7 @@ __global__ __launch_bounds__(64 * CARRY_GROUPS) void scan_carry_kernel(
 // ---------------------------------------------------------------- forward
 template <typename TE, int N, bool VEC>
 __global__ __launch_bounds__((Shape<N>::BT)) void scan_kernel(const ScanArgs a, Plan pl,
-                                                              const float* carry) {
+                                                              Carry cy) {
   using S = Shape<N>;
   constexpr int TPC = S::TPC, BT = S::BT, EV = S::EV, YS = CH + 16;
   __shared__ __align__(16) float s_delta[SCAN_TILE][CH], s_du[SCAN_TILE][CH];
@@ -379,9 +411,7 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_kernel(const ScanArgs a, 
   ld_states(a.A + (size_t)c * N + 4 * q, c < a.C, A2);
 #pragma unroll
   for (int i = 0; i < 4; ++i) A2[i] *= LOG2E;
-  const float* enter = carry ? carry + ((size_t)l * pl.segs + pt.seg) * a.C * N
-                       : a.state_in ? a.state_in + (size_t)l * a.C * N : nullptr;
-  ld_states(enter ? enter + c * N + 4 * q : nullptr, c < a.C, h);
+  enter_segment<N, false>(cy, a.state_in, pl.segs, l, pt.seg, c, a.C, q, A2, h);
   float bias[EV], D[EV];
 #pragma unroll
   for (int j = 0; j < EV; ++j) {
@@ -534,7 +564,7 @@ struct GradWork {
 
 template <typename TE, int N, bool VEC>
 __global__ __launch_bounds__((Shape<N>::BT)) __attribute__((amdgpu_waves_per_eu(2, 2))) void scan_grad_kernel(const ScanGradArgs g, Plan pl,
-                                                                   GradWork wk, const float* carry) {
+                                                                   GradWork wk, Carry cy) {
   using S = Shape<N>;
   constexpr int TPC = S::TPC, BT = S::BT, EV = S::EV, SUMS = SCAN_TILE * CH + 16;
   __shared__ __align__(16) float s_delta[SCAN_TILE][CH], s_u[SCAN_TILE][CH], s_dy[SCAN_TILE][CH];
@@ -558,9 +588,7 @@ __global__ __launch_bounds__((Shape<N>::BT)) __attribute__((amdgpu_waves_per_eu(
     A2[i] *= LOG2E;
     dA[i] = 0.0f;
   }
-  const float* enter = carry ? carry + ((size_t)l * pl.segs + pt.seg) * a.C * N
-                       : g.dstate_out ? g.dstate_out + (size_t)l * a.C * N : nullptr;
-  ld_states(enter ? enter + c * N + 4 * q : nullptr, c < a.C, G);
+  enter_segment<N, true>(cy, g.dstate_out, pl.segs, l, pt.seg, c, a.C, q, A2, G);
   // the owners' parameters and sums live in LDS, to leave the registers to the states
 #pragma unroll
   for (int j = 0; j < EV; ++j) s_dd[ot][oc + j] = s_dbias[ot][oc + j] = 0.0f;
@@ -783,32 +811,32 @@ __global__ __launch_bounds__((Shape<N>::BT)) __attribute__((amdgpu_waves_per_eu(
   }
 }
 
-// dB and dC over the channel blocks
+// The blocks' sums of the gradient.  The first bc_blocks blocks sum dB and dC
+// over the channel blocks, a value a thread; the others the parameters'
+// gradients over n partials -- dA's `width` values, then dD's and dbias's C --,
+// 16 columns a block, 16 groups of partials, the groups added in order.
 template <typename TE>
-__global__ __launch_bounds__(256) void scan_bc_sum_kernel(const float* __restrict__ part,
-                                                          int cblocks, uint32_t rows, int T, int N,
-                                                          RowsOut db, RowsOut dc) {
-  const uint64_t n = (uint64_t)rows * 2 * N, step = (uint64_t)gridDim.x * 256;
-  for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += step) {
-    float s = 0.0f;
-#pragma unroll 4
-    for (int k = 0; k < cblocks; ++k) s += part[k * n + e];
-    const uint32_t r = (uint32_t)(e / (2 * N)), i = (uint32_t)(e - (uint64_t)r * 2 * N);
-    const uint32_t l = r / (uint32_t)T, t = r - l * T;
-    if (i < (uint32_t)N) stv((TE*)db.d + l * db.lane + t * db.row + i, s);
-    else stv((TE*)dc.d + l * dc.lane + t * dc.row + i - N, s);
-  }
-}
-
-// The parameters' gradients, sums over n partials: dA's `width` values, then
-// dD's and dbias's C.  16 columns a block, 16 groups of partials, the groups
-// added in order.
-__global__ __launch_bounds__(256) void scan_part_sum_kernel(GradWork wk, int n, int width, int C,
-                                                            float* __restrict__ dA,
-                                                            float* __restrict__ dD,
-                                                            float* __restrict__ dbias) {
+__global__ __launch_bounds__(256) void scan_sums_kernel(GradWork wk, uint32_t bc_blocks,
+                                                        int cblocks, uint32_t rows, int T, int N,
+                                                        RowsOut db, RowsOut dc, int n, int width,
+                                                        int C, float* __restrict__ dA,
+                                                        float* __restrict__ dD,
+                                                        float* __restrict__ dbias) {
   __shared__ float sm[16][16];
-  const int ba = (width + 15) / 16, bc = (C + 15) / 16, b = blockIdx.x;
+  if (blockIdx.x < bc_blocks) {
+    const uint64_t all = (uint64_t)rows * 2 * N, step = (uint64_t)bc_blocks * 256;
+    for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < all; e += step) {
+      float s = 0.0f;
+#pragma unroll 4
+      for (int k = 0; k < cblocks; ++k) s += wk.bc[k * all + e];
+      const uint32_t r = (uint32_t)(e / (2 * N)), i = (uint32_t)(e - (uint64_t)r * 2 * N);
+      const uint32_t l = r / (uint32_t)T, t = r - l * T;
+      if (i < (uint32_t)N) stv((TE*)db.d + l * db.lane + t * db.row + i, s);
+      else stv((TE*)dc.d + l * dc.lane + t * dc.row + i - N, s);
+    }
+    return;
+  }
+  const int ba = (width + 15) / 16, bc = (C + 15) / 16, b = blockIdx.x - bc_blocks;
   const int which = b < ba ? 0 : b < ba + bc ? 1 : 2;
   const float* part = which == 0 ? wk.da : which == 1 ? wk.dd : wk.dbias;
   float* out = which == 0 ? dA : which == 1 ? dD : dbias;
@@ -852,8 +880,8 @@ struct Take {
   }
 };
 Carry take_carry(Take& take, const Plan& p, size_t lanes, size_t C, size_t ds) {
-  if (p.segs == 1) return Carry{};
-  return Carry{take(lanes * p.segs * C * ds), take(lanes * p.segs * C)};
+  if (p.segs == 1) return Carry{nullptr, nullptr, false};
+  return Carry{take(lanes * p.segs * C * ds), take(lanes * p.segs * C), p.segs > CHAIN_SEGS};
 }
 GradWork take_grad(Take& take, const Plan& p, size_t lanes, size_t T, size_t C, size_t ds) {
   GradWork w{};
@@ -923,11 +951,11 @@ hipError_t launch_scan(const ScanArgs& a, hipStream_t s) {
   BOA_LAUNCH((scan_local_kernel<TE, N, V, false>), grid, dim3(Shape<N>::BT), 0, s, g, pl, cy)
     BOA_SCAN_ALL
 #undef BOA_SCAN
-    launch_carry<false>(a, pl, a.state_in, cy, s);
+    if (cy.entered) launch_carry<false>(a, pl, a.state_in, cy, s);
   }
   const dim3 grid((uint32_t)a.q.lanes * pl.segs * pl.cblocks);
 #define BOA_SCAN(TE, N, V) \
-  BOA_LAUNCH((scan_kernel<TE, N, V>), grid, dim3(Shape<N>::BT), 0, s, a, pl, cy.state)
+  BOA_LAUNCH((scan_kernel<TE, N, V>), grid, dim3(Shape<N>::BT), 0, s, a, pl, cy)
   BOA_SCAN_ALL
 #undef BOA_SCAN
   return hipGetLastError();
@@ -950,27 +978,25 @@ hipError_t launch_scan_grad(const ScanGradArgs& g, hipStream_t s) {
   BOA_LAUNCH((scan_local_kernel<TE, N, V, true>), grid, dim3(Shape<N>::BT), 0, s, g, pl, cy)
     BOA_SCAN_ALL
 #undef BOA_SCAN
-    launch_carry<true>(a, pl, g.dstate_out, cy, s);
+    if (cy.entered) launch_carry<true>(a, pl, g.dstate_out, cy, s);
   }
   const dim3 grid((uint32_t)a.q.lanes * pl.segs * pl.cblocks);
 #define BOA_SCAN(TE, N, V) \
-  BOA_LAUNCH((scan_grad_kernel<TE, N, V>), grid, dim3(Shape<N>::BT), 0, s, g, pl, wk, cy.state)
+  BOA_LAUNCH((scan_grad_kernel<TE, N, V>), grid, dim3(Shape<N>::BT), 0, s, g, pl, wk, cy)
   BOA_SCAN_ALL
 #undef BOA_SCAN
 #undef BOA_SCAN_ALL
 #undef BOA_SCAN_N
-  if (pl.cblocks > 1) {
-    const dim3 gb((uint32_t)std::min<size_t>(MAX_BLOCKS, (rows * 2 * a.ds + 255) / 256));
-    if (a.bf16)
-      BOA_LAUNCH(scan_bc_sum_kernel<uint16_t>, gb, dim3(256), 0, s, wk.bc, pl.cblocks,
-                 (uint32_t)rows, a.q.T, a.ds, g.db, g.dc);
-    else
-      BOA_LAUNCH(scan_bc_sum_kernel<float>, gb, dim3(256), 0, s, wk.bc, pl.cblocks, (uint32_t)rows,
-                 a.q.T, a.ds, g.db, g.dc);
-  }
   const int width = a.C * a.ds;
-  BOA_LAUNCH(scan_part_sum_kernel, dim3((width + 15) / 16 + 2 * ((a.C + 15) / 16)), dim3(256), 0, s,
-             wk, a.q.lanes * pl.segs, width, a.C, g.dA, g.dD, g.dbias);
+  const uint32_t gb = pl.cblocks == 1 ? 0
+                      : (uint32_t)std::min<size_t>(MAX_BLOCKS, (rows * 2 * a.ds + 255) / 256);
+  const dim3 gs(gb + (width + 15) / 16 + 2 * ((a.C + 15) / 16));
+#define BOA_SUMS(TE)                                                                            \
+  BOA_LAUNCH(scan_sums_kernel<TE>, gs, dim3(256), 0, s, wk, gb, pl.cblocks, (uint32_t)rows,     \
+             a.q.T, a.ds, g.db, g.dc, a.q.lanes * pl.segs, width, a.C, g.dA, g.dD, g.dbias)
+  if (a.bf16) BOA_SUMS(uint16_t);
+  else BOA_SUMS(float);
+#undef BOA_SUMS
   return hipGetLastError();
 }
 

@@ -212,7 +212,9 @@ __device__ __forceinline__ Part block_part(const Plan& p, int segs) {
 // to CHAIN_SEGS segments every block of the main pass chains those before its
 // own itself; more would read too much, and a kernel between the passes puts
 // what enters each segment in their place (`entered`).  (4 lanes x 257, 17
-// segments, forward and gradient: 46 us with that kernel, 38 without.)
+// segments, forward and gradient: 46 us with that kernel, 38 without.)  So does
+// a call whose state is updated in place: a lane's last segment stores it, and
+// blocks of its other segments may not have begun by then.
 constexpr int CHAIN_SEGS = 32;
 struct Carry {
   float *state, *sum;
@@ -879,9 +881,10 @@ struct Take {
     return p;
   }
 };
-Carry take_carry(Take& take, const Plan& p, size_t lanes, size_t C, size_t ds) {
+Carry take_carry(Take& take, const Plan& p, size_t lanes, size_t C, size_t ds, bool in_place) {
   if (p.segs == 1) return Carry{nullptr, nullptr, false};
-  return Carry{take(lanes * p.segs * C * ds), take(lanes * p.segs * C), p.segs > CHAIN_SEGS};
+  return Carry{take(lanes * p.segs * C * ds), take(lanes * p.segs * C),
+               in_place || p.segs > CHAIN_SEGS};
 }
 GradWork take_grad(Take& take, const Plan& p, size_t lanes, size_t T, size_t C, size_t ds) {
   GradWork w{};
@@ -905,7 +908,7 @@ void launch_carry(const ScanArgs& a, const Plan& pl, const float* first, const C
 size_t scan_work(int lanes, int T, int C, int ds, bool grad) {
   const Plan p = scan_plan(lanes, T, C, ds);
   Take take{nullptr};
-  take_carry(take, p, lanes, C, ds);
+  take_carry(take, p, lanes, C, ds, false);
   if (grad) take_grad(take, p, lanes, T, C, ds);
   return take.used;
 }
@@ -942,7 +945,8 @@ hipError_t launch_scan(const ScanArgs& a, hipStream_t s) {
     return hipGetLastError();
   }
   Take take{(char*)a.work};
-  const Carry cy = take_carry(take, pl, a.q.lanes, a.C, a.ds);
+  const Carry cy = take_carry(take, pl, a.q.lanes, a.C, a.ds,
+                              a.state_in && a.state_out == a.state_in);
   if (pl.segs > 1) {
     const dim3 grid((uint32_t)a.q.lanes * (pl.segs - 1) * pl.cblocks);
     ScanGradArgs g{};
@@ -970,7 +974,8 @@ hipError_t launch_scan_grad(const ScanGradArgs& g, hipStream_t s) {
                    ok(g.ddelta) && ok(g.dz);
   const size_t rows = (size_t)a.q.lanes * a.q.T;
   Take take{(char*)a.work};
-  const Carry cy = take_carry(take, pl, a.q.lanes, a.C, a.ds);
+  const Carry cy = take_carry(take, pl, a.q.lanes, a.C, a.ds,
+                              g.dstate_out && g.dstate_in == g.dstate_out);
   const GradWork wk = take_grad(take, pl, a.q.lanes, a.q.T, a.C, a.ds);
   if (pl.segs > 1) {
     const dim3 grid((uint32_t)a.q.lanes * (pl.segs - 1) * pl.cblocks);

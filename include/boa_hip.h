@@ -171,9 +171,10 @@ int boa_step_batch(boa_ctx* ctx, const uint8_t* d_tokens, int32_t lanes, float* 
  * HIP graph.  d_work is the caller's workspace, 16-byte aligned, of at least
  * the size that the _work_bytes function gives (-1: bad sizes; 0: d_work may
  * be NULL); its content is not kept, and calls that may overlap in time need
- * one each.  Outputs may not overlap inputs or each other, except that
- * dlogits may be logits itself.  Results depend on the inputs and sizes only
- * (no atomics). */
+ * one each.  Outputs may not overlap inputs or each other, except where one
+ * may be an input itself (dlogits, d_state_out, dstate_in).  Results depend on
+ * the inputs and sizes only (no atomics), and on whether states are updated in
+ * place. */
 typedef struct {
     void* d;
     int64_t lane_stride, row_stride;
@@ -212,7 +213,8 @@ typedef struct {
     const float* d_state_in;
 } boa_scan;
 /* Gradients: rows as their inputs', dA [channels][d_state], dD and ddelta_bias
- * [channels], dstate_in [lanes][channels][d_state] (NULL: not wanted). */
+ * [channels], dstate_in [lanes][channels][d_state] (NULL: not wanted; it may
+ * be the gradient of state_out itself). */
 typedef struct {
     boa_rows du, ddelta, dz, db, dc;
     float *d_dA, *d_dD, *d_ddelta_bias;

@@ -345,6 +345,32 @@ def test_scan_in_steps(codec):
     ref.check("state", h, state)
 
 
+# lanes that are cut into 2 to 32 segments, with more blocks than start at once
+@pytest.mark.parametrize("lanes,T,ch,n", [(3, 500, 640, 16), (2, 70, 64, 32), (7, 333, 1024, 32)])
+def test_scan_states_in_place(codec, lanes, T, ch, n):
+    """state_out over state_in and dstate_in over dstate_out: what a lane's last
+    segment stores is not what its other segments start from."""
+    s, lens = scan_inputs(lanes, T, ch, n, F32, "ragged")
+    live = ref.mask(lens, lanes, T)
+    want, state, kept = ref.scan(s, live)
+    d = {k: v.cuda() for k, v in s.items()}
+    args = [d[k] for k in ("u", "delta", "z", "B", "C", "A", "D", "delta_bias")]
+    out, h, g = torch.zeros_like(d["u"]), d["state_in"].clone(), d["dstate_out"].clone()
+    saved = torch.empty(boa_hip.selective_scan_saved_floats(lanes, T, ch, n), device="cuda")
+    codec.selective_scan(*args, out, work(boa_hip.selective_scan_work_bytes(lanes, T, ch, n)),
+                         d_state_in=h, d_state_out=h, d_lens=dev(lens), d_saved=saved)
+    ref.check("out", out.cpu()[live], want[live])
+    ref.check("state", h, state)
+    grads = {k: torch.empty_like(d[k]) for k in ("u", "delta", "z", "B", "C", "A", "D",
+                                                 "delta_bias")}
+    codec.selective_scan_grad(*args, saved, d["dout"], *grads.values(),
+                              work(boa_hip.selective_scan_work_bytes(lanes, T, ch, n, grad=True)),
+                              d_state_in=d["state_in"], d_dstate_out=g, d_dstate_in=g,
+                              d_lens=dev(lens))
+    for k, v in ref.scan_grad(s, live, kept).items():
+        ref.check(k, g if k == "dstate_in" else grads[k[1:]], v)
+
+
 def test_scan_extremes(codec):
     """Decays of 0 and 1, gates shut and open wide, delta of 0 and large."""
     s, _ = scan_inputs(2, 20, 64, 16, F32, "full")

@@ -53,6 +53,14 @@ __device__ __forceinline__ float sigmoid_hw(float x) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * LOG2E));
 }
 
+// A in powers of two, kept finite: where delta is 0 (past a lane's end), 0 times
+// an infinity would not leave the state as it is
+__device__ __forceinline__ float rate2(float A) {
+  constexpr float MOST = 3.402823466e38f;
+  const float r = A * LOG2E;
+  return r < -MOST ? -MOST : r > MOST ? MOST : r;  // a NaN stays one
+}
+
 // The elements of a row tensor that a thread owns: in each tile of lane l the
 // same ones, off elements from the tile's first row.  The tile's address is
 // uniform (scalar registers), a thread keeps 32 bits of its own.
@@ -266,7 +274,7 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_local_kernel(const ScanGr
   float h[4] = {0.0f, 0.0f, 0.0f, 0.0f}, A2[4], sum = 0.0f;
   ld_states(a.A + (size_t)c * N + 4 * q, c < a.C, A2);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) A2[i] *= LOG2E;
+  for (int i = 0; i < 4; ++i) A2[i] = rate2(A2[i]);
   float bias[EV];
 #pragma unroll
   for (int j = 0; j < EV; ++j) bias[j] = gc + j < a.C ? a.bias[gc + j] : 0.0f;
@@ -360,7 +368,7 @@ __global__ __launch_bounds__(64 * CARRY_GROUPS) void scan_carry_kernel(
   const int ln = threadIdx.x & 63, g = threadIdx.x >> 6, i = (blockIdx.x % cols) * 64 + ln;
   const bool on = i < width;
   const int c = on ? i / N : 0;
-  const float A2 = on ? A[i] * LOG2E : 0.0f;
+  const float A2 = on ? rate2(A[i]) : 0.0f;
   const int groups = blockDim.x >> 6, per = (segs + groups - 1) / groups;
   const int k0 = min(segs, g * per), k1 = min(segs, k0 + per);
   // k-th segment of the chain; the last one's effect is not known and not needed
@@ -412,7 +420,7 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_kernel(const ScanArgs a, 
   float h[4], A2[4];
   ld_states(a.A + (size_t)c * N + 4 * q, c < a.C, A2);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) A2[i] *= LOG2E;
+  for (int i = 0; i < 4; ++i) A2[i] = rate2(A2[i]);
   enter_segment<N, false>(cy, a.state_in, pl.segs, l, pt.seg, c, a.C, q, A2, h);
   float bias[EV], D[EV];
 #pragma unroll
@@ -547,7 +555,7 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_step_kernel(const ScanArg
     const float delta = softplus_full(x), du = delta * u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float e = __builtin_amdgcn_exp2f(delta * (A2[i] * LOG2E));
+      const float e = __builtin_amdgcn_exp2f(delta * rate2(A2[i]));
       h[i] = __builtin_fmaf(e, h[i], du * b[i]);
       y = __builtin_fmaf(cv[i], h[i], y);
     }
@@ -587,7 +595,7 @@ __global__ __launch_bounds__((Shape<N>::BT)) __attribute__((amdgpu_waves_per_eu(
   ld_states(a.A + (size_t)c * N + 4 * q, c < a.C, A2);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    A2[i] *= LOG2E;
+    A2[i] = rate2(A2[i]);
     dA[i] = 0.0f;
   }
   enter_segment<N, true>(cy, g.dstate_out, pl.segs, l, pt.seg, c, a.C, q, A2, G);
@@ -637,6 +645,7 @@ __global__ __launch_bounds__((Shape<N>::BT)) __attribute__((amdgpu_waves_per_eu(
       if (!zero)
 #pragma unroll
         for (int i = 0; i < S::WAVES; ++i) v += s_bc[i][k][n];
+      v = t < len ? v : 0.0f;
       if (pl.cblocks > 1)
         wk.bc[(((size_t)cb * a.q.lanes + l) * a.q.T + t) * (2 * N) + n] = v;
       else if (n < N)
@@ -782,6 +791,10 @@ __global__ __launch_bounds__((Shape<N>::BT)) __attribute__((amdgpu_waves_per_eu(
       o_u[j] = __builtin_fmaf(D[j], dy[j], dl[j] * I[j]);
       o_x[j] = __builtin_fmaf(u[j], I[j], M[j] * LN2) * xsig[j];
       o_z[j] = dzy[j] * __builtin_fmaf(D[j], u[j], y[j]);
+      // sums of zeros past the lane's end, but for a state that is not finite
+      o_u[j] = ok ? o_u[j] : 0.0f;
+      o_x[j] = ok ? o_x[j] : 0.0f;
+      o_z[j] = ok ? o_z[j] : 0.0f;
       sd[j] = __builtin_fmaf(dy[j], u[j], sd[j]);
       sb[j] += o_x[j];
     }

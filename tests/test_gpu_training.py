@@ -403,6 +403,36 @@ def test_scan_of_one_lane_alone(codec, dtype):
         assert torch.equal(a[k][0], b[k][0]) and torch.equal(a[k][2], b[k][2]), k
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [16, 32])
+def test_scan_past_the_end_of_infinite_states(codec, n, dtype):
+    """Gradients past a lane's length are zero whatever the lane holds."""
+    s, _ = scan_inputs(3, 45, 70, n, dtype, "full")
+    s["state_in"][0, 5, 3] = math.inf
+    s["dstate_out"][1, 9, 2] = math.nan
+    s["u"][2, 4, 60] = -math.inf
+    got, live = run_scan(codec, s, torch.tensor([21, 35, 5], dtype=torch.int32), "wide")
+    for k in ("du", "ddelta", "dz", "dB", "dC"):
+        zeroed(got[k], live, k)
+    untouched(got["out"], live, "out")
+
+
+@pytest.mark.parametrize("T", [1, 3, 40])
+def test_scan_that_forgets_at_once(codec, T):
+    """The largest decays: each state is its last position's, in lanes that end
+    inside a tile or hold nothing as well."""
+    s, _ = scan_inputs(3, T, 64, 16, F32, "full")
+    s["A"][:] = -torch.finfo(F32).max
+    s["A"][:, 1] = -math.inf
+    lens = torch.tensor([T, max(T - 1, 1), 0], dtype=torch.int32)
+    got, live = run_scan(codec, s, lens, "dense", grad=False)
+    # with any large decay the older positions' part is below what fp64 tells apart
+    s["A"][:] = -1e6
+    out, state, _ = ref.scan(s, live)
+    ref.check("out", got["out"].cpu()[live], out[live])
+    ref.check("state_out", got["state_out"], state)
+
+
 # ------------------------------------------------------------- far addresses
 def far(t, dtype=None, fill=SKIP):
     """[2, T, width] with 2^31 + 16 elements between the lanes."""

@@ -214,6 +214,18 @@ def test_loss_of_impossible_rows(codec):
         assert dx[r].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_loss_of_a_nan_among_ruled_out_bytes(codec, dtype):
+    """A NaN is not ruled out: its row's loss is NaN wherever it stands."""
+    x = torch.full((1, 256, 256), -math.inf)
+    x[0, torch.arange(256), torch.arange(256)] = math.nan
+    tgt = torch.full((1, 256), 9, dtype=torch.uint8)
+    loss = torch.zeros((1, 256), device="cuda")
+    codec.next_byte_loss(x.to(dtype).cuda(), dev(tgt), loss,
+                         work(boa_hip.next_byte_loss_work_bytes(1, 256)))
+    assert loss.isnan().all()
+
+
 def test_loss_of_near_certainty(codec):
     """Losses far under fp32's step at 1 keep their digits."""
     x = torch.zeros((1, 4, 256))

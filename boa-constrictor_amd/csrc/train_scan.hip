@@ -357,8 +357,9 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_local_kernel(const ScanGr
 
 // The state (REV: the gradient) that enters each segment, over what the
 // segments added: chains of segs steps, cut among up to 16 groups of 64 (channel,
-// state) pairs, each of which first finds what its own segments do.
-constexpr int CARRY_GROUPS = 16;  // at most
+// state) pairs, each of which first finds what its own segments do.  Bound by
+// latency, so a thread's whole part is under way at once and stays in registers.
+constexpr int CARRY_GROUPS = 16, CARRY_PER = MAX_SEGS / CARRY_GROUPS;  // at most
 template <bool REV>
 __global__ __launch_bounds__(64 * CARRY_GROUPS) void scan_carry_kernel(
     const float* __restrict__ A, const float* __restrict__ first, int C, int N, int segs,
@@ -367,36 +368,39 @@ __global__ __launch_bounds__(64 * CARRY_GROUPS) void scan_carry_kernel(
   const int width = C * N, cols = (width + 63) / 64, l = blockIdx.x / cols;
   const int ln = threadIdx.x & 63, g = threadIdx.x >> 6, i = (blockIdx.x % cols) * 64 + ln;
   const bool on = i < width;
-  const int c = on ? i / N : 0;
-  const float A2 = on ? rate2(A[i]) : 0.0f;
+  const int at = on ? i : 0, c = at / N;
+  const float A2 = rate2(A[at]);
   const int groups = blockDim.x >> 6, per = (segs + groups - 1) / groups;
   const int k0 = min(segs, g * per), k1 = min(segs, k0 + per);
   // k-th segment of the chain; the last one's effect is not known and not needed
   auto seg_at = [&](int k) { return (size_t)l * segs + (REV ? segs - 1 - k : k); };
-  float h = 0.0f, sum = 0.0f;
-  if (on)
-#pragma unroll 4
-    for (int k = k0; k < min(k1, segs - 1); ++k) {
-      const float d = cy.sum[seg_at(k) * C + c], s = cy.state[seg_at(k) * width + i];
-      h = __builtin_fmaf(__builtin_amdgcn_exp2f(A2 * d), h, s);
-      sum += d;
-    }
+  float e[CARRY_PER], s[CARRY_PER], h = 0.0f, sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < CARRY_PER; ++j) {  // without branches: what is not there is read as segment 0
+    const int k = k0 + j < min(k1, segs - 1) ? k0 + j : 0;
+    e[j] = cy.sum[seg_at(k) * C + c];
+    s[j] = cy.state[seg_at(k) * width + at];
+  }
+#pragma unroll
+  for (int j = 0; j < CARRY_PER; ++j) {
+    const bool in = k0 + j < min(k1, segs - 1);
+    sum += in ? e[j] : 0.0f;
+    e[j] = __builtin_amdgcn_exp2f(A2 * (in ? e[j] : 0.0f));
+    s[j] = in ? s[j] : 0.0f;
+    h = __builtin_fmaf(e[j], h, s[j]);
+  }
   s_h[g][ln] = h;
   s_sum[g][ln] = sum;
   __syncthreads();
   if (!on) return;
   h = first ? first[(size_t)l * width + i] : 0.0f;
+#pragma unroll 4
   for (int k = 0; k < g; ++k)
     h = __builtin_fmaf(__builtin_amdgcn_exp2f(A2 * s_sum[k][ln]), h, s_h[k][ln]);
-  for (int k = k0; k < k1; ++k) {
-    float d = 0.0f, s = 0.0f;
-    float* p = cy.state + seg_at(k) * width + i;
-    if (k < segs - 1) {
-      d = cy.sum[seg_at(k) * C + c];
-      s = *p;
-    }
-    *p = h;
-    h = __builtin_fmaf(__builtin_amdgcn_exp2f(A2 * d), h, s);
+#pragma unroll
+  for (int j = 0; j < CARRY_PER; ++j) {
+    if (k0 + j < k1) cy.state[seg_at(k0 + j) * width + i] = h;
+    h = __builtin_fmaf(e[j], h, s[j]);
   }
 }
 

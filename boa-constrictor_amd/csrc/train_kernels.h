@@ -45,7 +45,7 @@ __device__ __forceinline__ uint32_t bf16_pair(float x, float y) {
 
 // x + x of the lane that CTRL names within the row of 16 lanes
 constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_HALF_MIRROR = 0x141, DPP_MIRROR = 0x140,
-              DPP_ROR4 = 0x124, DPP_ROR8 = 0x128;
+              DPP_ROR8 = 0x128;
 template <int CTRL>
 __device__ __forceinline__ float dpp_move(float x) {
   return u2f((uint32_t)__builtin_amdgcn_update_dpp(0, (int)f2u(x), CTRL, 0xF, 0xF, true));

@@ -33,6 +33,7 @@
 // the rows alone would take 72 at the rate of a copy.
 #include <algorithm>
 
+#include "scan_lanes.h"
 #include "train_kernels.h"
 
 namespace boa {
@@ -192,6 +193,25 @@ __device__ __forceinline__ float sum_states(float x) {
   if constexpr (TPC == 8) x = dpp_add<DPP_HALF_MIRROR>(x);
   return x;
 }
+
+// the lane operations of scan_lanes.h
+struct Lanes {
+  int i;
+  struct Pair {
+    float a, b;
+  };
+  __device__ __forceinline__ float xor1(float x) const { return dpp_move<DPP_XOR1>(x); }
+  __device__ __forceinline__ float xor2(float x) const { return dpp_move<DPP_XOR2>(x); }
+  __device__ __forceinline__ float half_mirror(float x) const { return dpp_move<DPP_HALF_MIRROR>(x); }
+  __device__ __forceinline__ float ror8(float x) const { return dpp_move<DPP_ROR8>(x); }
+  __device__ __forceinline__ float fold16(float x, float y) const { return boa::fold16(x, y); }
+  __device__ __forceinline__ Pair swap32(float x, float y) const {
+    const auto s = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(y), false, false);
+    return Pair{u2f(s[0]), u2f(s[1])};
+  }
+  __device__ __forceinline__ float pick(int bit, float x, float y) const { return i & bit ? x : y; }
+  __device__ __forceinline__ float fma(float x, float y, float z) const { return __builtin_fmaf(x, y, z); }
+};
 
 // How the blocks divide the work: lane, segment of the tiles, channel block.
 // Few lanes are cut into segments, so that there are blocks for every CU: a
@@ -606,11 +626,12 @@ __global__ __launch_bounds__((Shape<N>::BT)) __attribute__((amdgpu_waves_per_eu(
   const ScanArgs& a = g.f;
   const Part pt = block_part(pl, pl.segs);
   const int tid = threadIdx.x, cb = pt.cb, l = pt.l;
-  const int len = seq_len(a.q, l), q = tid % TPC, ch = tid / TPC, c = cb * CH + ch;
+  const Lanes lanes{tid & 63};
+  const int len = seq_len(a.q, l), q = lane_states<TPC>(tid), ch = tid / TPC, c = cb * CH + ch;
   const int ot = tid / (CH / EV), oc = (tid % (CH / EV)) * EV, gc = cb * CH + oc;
-  const int w = tid >> 6, ln = tid & 63;
+  const int w = tid >> 6;
   const int first = pt.seg * pl.seg_tiles, last = min(pl.tiles, first + pl.seg_tiles);
-  float* sums = s_sums + min(q & 3, 2) * SUMS + ch;
+  float* sums = s_sums + min(tid & 3, 2) * SUMS + ch;
   float A2[4], G[4], dA[4];
   ld_states(a.A + (size_t)c * N + 4 * q, c < a.C, A2);
 #pragma unroll
@@ -766,9 +787,7 @@ __global__ __launch_bounds__((Shape<N>::BT)) __attribute__((amdgpu_waves_per_eu(
       const float4 B = Bs[k & 1], C = Cs[k & 1];
       const float bv[4] = {B.x, B.y, B.z, B.w}, cv[4] = {C.x, C.y, C.z, C.w};
       float y = 0.0f, I = 0.0f, M = 0.0f, v[4];
-      // du and dy of the wave's halves: the lower one sums dB, the upper one dC
-      const auto cf = __builtin_amdgcn_permlane32_swap(f2u(du), f2u(dyk), false, false);
-      const float c0 = u2f(cf[0]), c1 = u2f(cf[1]);
+      const Lanes::Pair cf = lanes.swap32(du, dyk);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float dh = __builtin_fmaf(cv[i], dyk, G[i]);
@@ -780,25 +799,10 @@ __global__ __launch_bounds__((Shape<N>::BT)) __attribute__((amdgpu_waves_per_eu(
         dA[i] = __builtin_fmaf(m, dl, dA[i]);
         // here: put off to the end of the tile these sums would keep 64 m
         asm volatile("" : "+v"(dA[i]));
-        const auto x = __builtin_amdgcn_permlane32_swap(f2u(dh), f2u(hs[k][i]), false, false);
-        v[i] = __builtin_fmaf(u2f(x[1]), c1, u2f(x[0]) * c0);
+        v[i] = bc_term(lanes, dh, hs[k][i], cf);
       }
-      // the three sums over the channel's lanes, one for each of lanes 0, 1 and 2
-      if constexpr (TPC == 8) {
-        y = dpp_add<DPP_HALF_MIRROR>(y);
-        I = dpp_add<DPP_HALF_MIRROR>(I);
-        M = dpp_add<DPP_HALF_MIRROR>(M);
-      }
-      const float yi = (q & 1 ? I : y) + dpp_move<DPP_XOR1>(q & 1 ? y : I);
-      M = dpp_add<DPP_XOR1>(M);
-      sums[k * CH] = (q & 2 ? M : yi) + dpp_move<DPP_XOR2>(q & 2 ? yi : M);
-      // dB, dC over the wave's channels: the odd rows of 16 lanes take states 2
-      // and 3, lanes with bit 3 set 1 and 3
-      const float x0 = fold16(v[0], v[2]), x1 = fold16(v[1], v[3]);
-      const bool odd = ln & 8;
-      float r = (odd ? x1 : x0) + dpp_move<DPP_ROR8>(odd ? x0 : x1);
-      if constexpr (TPC == 4) r = dpp_add<DPP_ROR4>(r);
-      s_bc[w][k][(ln >> 5) * N + 4 * q + ((ln >> 4) & 1) * 2 + ((ln >> 3) & 1)] = r;
+      sums[k * CH] = channel_sums<TPC>(lanes, y, I, M);
+      s_bc[w][k][bc_slot<TPC>(lanes.i)] = bc_sums<TPC>(lanes, v);
     }
     __syncthreads();
     float o_u[EV], o_z[EV], I[EV], y[EV], M[EV], D[EV], u[EV], dy[EV], dl[EV], sd[EV], sb[EV];

@@ -561,7 +561,8 @@ __global__ __launch_bounds__(LOSS_THREADS) void loss_kernel(const LossArgs a, ui
     float loss = __builtin_fmaf(__builtin_amdgcn_logf(sum), 0.69314718055994530942f,
                                 lost * inv_sum) - dt;
     loss = none ? __builtin_huge_valf() + rest : loss;  // a NaN beside -inf stays one
-    const float inv = none || !c.live ? 0.0f : a.scale * inv_sum;
+    // (rest - rest: 0, or that NaN, which every byte's gradient then is)
+    const float inv = !c.live ? 0.0f : none ? rest - rest : a.scale * inv_sum;
     const float gt = (dt == 0.0f ? -rest : __builtin_amdgcn_exp2f(dt * 1.44269504088896340736f) - sum) * inv;
     float gr[16];
 #pragma unroll

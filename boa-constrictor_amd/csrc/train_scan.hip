@@ -263,6 +263,14 @@ struct Carry {
   bool entered;
 };
 
+// A state after a segment whose decay is 2^x and that adds s to it.  The decay
+// is r^2, r = 2^(x / 2): it may leave fp32's range where the state that goes
+// through it does not, and infinity times a state of zero would be NaN.
+__device__ __forceinline__ float half_decay(float x) { return __builtin_amdgcn_exp2f(0.5f * x); }
+__device__ __forceinline__ float pass_segment(float r, float h, float s) {
+  return h == 0.0f ? s : __builtin_fmaf(r, r * h, s);
+}
+
 // What enters segment `seg` of lane l for a thread's four states of channel c:
 // the chain from `first` (null: zero) over the segments before it (REV: after
 // it, from the last).
@@ -285,7 +293,7 @@ __device__ __forceinline__ void enter_segment(const Carry& cy, const float* firs
     ld_states(cy.state + at * N + 4 * q, true, s);
     const float d = cy.sum[at];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) h[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(A2[j] * d), h[j], s[j]);
+    for (int j = 0; j < 4; ++j) h[j] = pass_segment(half_decay(A2[j] * d), h[j], s[j]);
   }
 }
 
@@ -420,9 +428,9 @@ __global__ __launch_bounds__(64 * CARRY_GROUPS) void scan_carry_kernel(
   for (int j = 0; j < CARRY_PER; ++j) {
     const bool in = k0 + j < min(k1, segs - 1);
     sum += in ? e[j] : 0.0f;
-    e[j] = __builtin_amdgcn_exp2f(A2 * (in ? e[j] : 0.0f));
+    e[j] = half_decay(A2 * (in ? e[j] : 0.0f));
     s[j] = in ? s[j] : 0.0f;
-    h = __builtin_fmaf(e[j], h, s[j]);
+    h = pass_segment(e[j], h, s[j]);
   }
   s_h[g][ln] = h;
   s_sum[g][ln] = sum;
@@ -431,11 +439,11 @@ __global__ __launch_bounds__(64 * CARRY_GROUPS) void scan_carry_kernel(
   h = first ? first[(size_t)l * width + i] : 0.0f;
 #pragma unroll 4
   for (int k = 0; k < g; ++k)
-    h = __builtin_fmaf(__builtin_amdgcn_exp2f(A2 * s_sum[k][ln]), h, s_h[k][ln]);
+    h = pass_segment(half_decay(A2 * s_sum[k][ln]), h, s_h[k][ln]);
 #pragma unroll
   for (int j = 0; j < CARRY_PER; ++j) {
     if (k0 + j < k1) cy.state[seg_at(k0 + j) * width + i] = h;
-    h = __builtin_fmaf(e[j], h, s[j]);
+    h = pass_segment(e[j], h, s[j]);
   }
 }
 

@@ -72,3 +72,58 @@ def test_decay_gradient_beside_infinite_states(codec, ch, n, dtype):  # noqa: F8
     finite = torch.ones((ch, n), dtype=torch.bool)
     finite[9, 2] = False
     ref.check("dA", dA[finite], want[finite])
+
+
+@pytest.mark.parametrize("T", [300, 700])
+def test_growing_states_that_are_zero(codec, T):  # noqa: F811
+    """A > 0 over segments whose decay overflows: a state (and a gradient) of
+    zero stays zero until something enters it."""
+    s, _ = scan_inputs(1, T, 64, 16, F32, "full", state=False)
+    s["A"] = s["A"].abs().clamp(8, 12)
+    s["delta"][:], s["delta_bias"][:] = 0.0, 0.0  # delta = log 2: e^(A delta 16) > 1e38
+    s["u"][:, :-6] = 0.0     # the state is zero until six positions before the end
+    s["dout"][:, 6:] = 0.0   # and its gradient down to the sixth position
+    got, live = run_scan(codec, s, None, "dense")
+    out, state, kept = ref.scan(s, live)
+    ref.check("out", got["out"], out)
+    ref.check("state_out", got["state_out"], state)
+    for k, want in ref.scan_grad(s, live, kept).items():
+        ref.check(k, got[k], want)
+
+
+@pytest.mark.parametrize("T", [30, 600])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_segments_whose_decay_leaves_the_range(codec, sign, T):  # noqa: F811
+    """A segment's decay may overflow (underflow) where the state that goes
+    through it does not."""
+    s, _ = scan_inputs(1, T, 64, 16, F32, "full")
+    size = 2.0 ** 83                                # a segment of 16 positions: 2^(16 * 9) = 2^144
+    s["A"] = torch.full((64, 16), sign * 9.0)
+    s["delta"][:], s["delta_bias"][:] = -200.0, 0.0   # delta = 0
+    s["delta"][:, :16] = 0.0                          # delta = log 2, in the first segment only
+    s["u"][:] = 0.0
+    s["state_in"] = s["state_in"].abs().clamp(0.5, 1.5) * size ** -sign
+    s["dstate_out"] = s["dstate_out"].abs().clamp(0.5, 1.5) * size ** -sign
+    got, live = run_scan(codec, s, None, "dense")
+    out, state, kept = ref.scan(s, live)
+    # the chain's own roundings: 16 deltas added up, the exponent's three, the
+    # two factors' four -- relative to the state, whose exponent is 16 * 9 log 2
+    more = ref.U * ((16 + 3) * 16 * 9 * math.log(2) + 4)
+    state.err = state.err + more * state.val.abs()
+    ref.check("state_out", got["state_out"], state)
+    # dout's terms grow by 2^144 on their way to the first position, so where
+    # A > 0 dstate_in is out of fp32's range
+    want = ref.scan_grad(s, live, kept)["dstate_in"]
+    if sign > 0:
+        assert (want.val.abs() > torch.finfo(F32).max).all()
+        assert torch.equal(got["dstate_in"].cpu().double(), want.val.sign() * math.inf)
+    else:
+        want.err = want.err + more * want.val.abs()
+        ref.check("dstate_in", got["dstate_in"], want)
+    # and without them it is dstate_out times the decay
+    s["dout"][:] = 0.0
+    got, _ = run_scan(codec, s, None, "dense")
+    want = ref.scan_grad(s, live, kept | {"w": dict(kept["w"], dout=ref.V(s["dout"].double()))})
+    want = want["dstate_in"]
+    want.err = want.err + more * want.val.abs()
+    ref.check("dstate_in", got["dstate_in"], want)

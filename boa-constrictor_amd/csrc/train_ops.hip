@@ -148,7 +148,8 @@ __global__ __launch_bounds__(256) void embed_kernel(const EmbedArgs a, uint32_t 
 
 // ----------------------------------------------------- embedding gradient
 // dtable[v] = scale sum of dout's rows whose token is v, in fp32 and in an
-// order that only the sizes decide (no atomics).  A block sorts the tokens of
+// order that the sizes, lengths and tokens decide (no atomics: a call repeated
+// gives the same bits; other tokens elsewhere may change a byte's last bits).  A block sorts the tokens of
 // `chunk` rows by a stable counting sort in LDS.  Then its groups of G lanes
 // take equal parts of the sorted rows and sum run by run, so a byte that fills
 // most rows is spread over all groups like any other.  Runs that cross a

@@ -160,6 +160,13 @@ def _ptr(x):
 # ---- training operators: tensors to C arguments
 # (what the C entry points cannot see -- types, shapes, devices -- is checked
 # here; sizes, strides, alignment and workspaces are checked there)
+def _int32(*n):
+    """Sizes that ctypes can pass as int32 (it would cut larger ones off)."""
+    if max(n) >> 31 or min(n) < 0:
+        raise ValueError(f"sizes out of range: {n}")
+    return n
+
+
 def _tensor(t, name, shape, dtype, device):
     """A dense tensor's pointer (None for None), of this shape and type on this device."""
     if t is None:
@@ -193,10 +200,12 @@ def _bytes(t, name, device):
         raise ValueError(f"{name}: want uint8 [lanes, T], got {t.dtype} {tuple(t.shape)}")
     if t.get_device() != device:  # -1 on the CPU
         raise ValueError(f"{name} is on {t.device}, the context on cuda:{device}")
-    ls, one = t.stride()
-    if one != 1 and t.shape[1] > 1:
+    (ls, one), (lanes, T) = t.stride(), t.shape
+    if one != 1 and T > 1:
         raise ValueError(f"{name} has to be dense along T")
-    return t.data_ptr(), ls, t.shape[0], t.shape[1]
+    if (lanes | T) >> 31:
+        _int32(lanes, T)
+    return t.data_ptr(), ls, lanes, T
 
 
 def _precision(t, name):
@@ -227,21 +236,21 @@ def _size(n, what):
 
 
 def embed_grad_work_bytes(lanes, T, width):
-    return _size(lib().boa_embed_grad_work_bytes(lanes, T, width), "embed_grad")
+    return _size(lib().boa_embed_grad_work_bytes(*_int32(lanes, T, width)), "embed_grad")
 
 
 def selective_scan_saved_floats(lanes, T, channels, d_state):
-    return _size(lib().boa_selective_scan_saved_floats(lanes, T, channels, d_state),
+    return _size(lib().boa_selective_scan_saved_floats(*_int32(lanes, T, channels, d_state)),
                  "selective_scan")
 
 
 def selective_scan_work_bytes(lanes, T, channels, d_state, grad=False):
-    return _size(lib().boa_selective_scan_work_bytes(lanes, T, channels, d_state, int(grad)),
-                 "selective_scan")
+    return _size(lib().boa_selective_scan_work_bytes(*_int32(lanes, T, channels, d_state),
+                                                     int(grad)), "selective_scan")
 
 
 def next_byte_loss_work_bytes(lanes, T):
-    return _size(lib().boa_next_byte_loss_work_bytes(lanes, T), "next_byte_loss")
+    return _size(lib().boa_next_byte_loss_work_bytes(*_int32(lanes, T)), "next_byte_loss")
 
 
 class Codec:
@@ -347,6 +356,7 @@ class Codec:
         if A.dim() != 2:
             raise ValueError(f"A: want [channels, d_state], got {tuple(A.shape)}")
         n = A.shape[1]
+        _int32(lanes, T, ch, n)
         return Scan(lanes, T, ch, n, prec, _tensor(lens, "lens", (lanes,), torch.int32, dev),
                     _rows(u, "u", lanes, T, ch, dt, dev),
                     _rows(delta, "delta", lanes, T, ch, dt, dev),

@@ -105,3 +105,28 @@ def test_binding_refuses_wrong_tensors():
         boa_hip._precision(t.half(), "x")
     with pytest.raises(ValueError):
         boa_hip._bytes(torch.zeros((2, 3)), "tokens", 0)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """What ctypes would cut to 32 bits, to sizes that are in range."""
+    far = 2 ** 32
+    for f, good in ((boa_hip.embed_grad_work_bytes, (1, 1, 64)),
+                    (boa_hip.selective_scan_saved_floats, (1, 5, 64, 16)),
+                    (boa_hip.selective_scan_work_bytes, (1, 5, 64, 16)),
+                    (boa_hip.next_byte_loss_work_bytes, (1, 1))):
+        f(*good)
+        for i in range(len(good)):
+            bad = list(good)
+            bad[i] += far
+            with pytest.raises(ValueError, match="range"):
+                f(*bad)
+    meta = lambda *s, **k: torch.empty(s, device="meta", **k)  # noqa: E731
+    for s in ((1, far + 3), (far + 3, 1)):
+        with pytest.raises(ValueError, match="range"):
+            boa_hip._bytes(meta(*s, dtype=torch.uint8), "tokens", -1)
+    codec = boa_hip.Codec.__new__(boa_hip.Codec)  # no context: the checks before the call
+    codec.h, codec.device = None, -1
+    for lanes, T, ch, n in ((1, far + 5, 64, 16), (1, 5, far + 64, 16), (1, 5, 64, far + 16)):
+        rows, bc, a = meta(lanes, T, ch), meta(lanes, T, n), meta(ch, n)
+        with pytest.raises(ValueError, match="range"):
+            codec._scan_args(rows, rows, rows, bc, bc, a, meta(ch), meta(ch), None, None)

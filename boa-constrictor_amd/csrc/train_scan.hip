@@ -265,10 +265,13 @@ struct Carry {
 
 // A state after a segment whose decay is 2^x and that adds s to it.  The decay
 // is r^2, r = 2^(x / 2): it may leave fp32's range where the state that goes
-// through it does not, and infinity times a state of zero would be NaN.
-__device__ __forceinline__ float half_decay(float x) { return __builtin_amdgcn_exp2f(0.5f * x); }
+// through it does not.  r stays finite, since infinity times a state of zero
+// would be NaN; any other state overflows with the largest r as well.
+__device__ __forceinline__ float half_decay(float x) {
+  return __builtin_fminf(__builtin_amdgcn_exp2f(0.5f * x), 3.402823466e38f);
+}
 __device__ __forceinline__ float pass_segment(float r, float h, float s) {
-  return h == 0.0f ? s : __builtin_fmaf(r, r * h, s);
+  return __builtin_fmaf(r, r * h, s);
 }
 
 // What enters segment `seg` of lane l for a thread's four states of channel c:

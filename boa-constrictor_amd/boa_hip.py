@@ -356,7 +356,8 @@ class Codec:
         if A.dim() != 2:
             raise ValueError(f"A: want [channels, d_state], got {tuple(A.shape)}")
         n = A.shape[1]
-        _int32(lanes, T, ch, n)
+        if (lanes | T | ch | n) >> 31:
+            _int32(lanes, T, ch, n)
         return Scan(lanes, T, ch, n, prec, _tensor(lens, "lens", (lanes,), torch.int32, dev),
                     _rows(u, "u", lanes, T, ch, dt, dev),
                     _rows(delta, "delta", lanes, T, ch, dt, dev),

@@ -25,12 +25,13 @@
 // The backward pass recomputes a tile's states from the one that the forward
 // pass saved at the tile's start and keeps them and the decays in registers.
 //
-// Bound by VALU issue: four states of a position take 22 instructions in the
-// segments' passes, 32 forward and 93 backward, four of them exponentials that
-// take as long as three or four others.  32 lanes x 1024 positions x 512
-// channels of 16 states, bf16, in 8 segments: 52 us and 86 forward (VALU busy
-// 99 and 98 %), 56 and 258 backward (99 and 89 %), 13 for the blocks' sums;
-// the rows alone would take 72 at the rate of a copy.
+// Bound by VALU issue: four states of a position take 23 instructions in the
+// segments' passes, 33 forward and 99 backward, four of them exponentials that
+// take as long as three or four others and, backward, seven lane swaps as long
+// as those.  32 lanes x 1024 positions x 512 channels of 16 states, bf16,
+// in 8 segments: 43 us and 72 forward (VALU busy 100 and 99 %), 46 and 217
+// backward (100 and 90 %), 13 for the blocks' sums; the rows alone would take 72
+// at the rate of a copy.
 #include <algorithm>
 
 #include "scan_lanes.h"
@@ -220,11 +221,12 @@ struct Lanes {
 // main pass starts every segment from its own.  That pass costs about half of
 // the main one, so lanes that give every SIMD two waves by themselves stay whole
 // (512 positions x 512 channels bf16, forward and gradient: 64 lanes whole 315
-// us, in two 374; 32 lanes whole 214, in 8 209).  Up to eight waves a SIMD even
-// out lanes of different lengths (16 x up to 1041 fp32: 248, 234 and 197 us with
-// two, four and eight; even lanes lose up to 4 %), and more segments than 256
-// cost more to chain than they save (1 x 16,001 x 128, forward, the kernels'
-// times: 39, 37 and 42 us with 128, 256 and 512).
+// us, in two 363; 32 lanes whole 224, in 8 215).  Up to eight waves a SIMD even
+// out lanes of different lengths (16 x up to 1041 fp32: 239, 229 and 196 us with
+// two, four and eight); lanes of one length would take four (32 x 512 and 32 x
+// 1024 bf16: 204 and 385 us, with eight 215 and 391).  More segments than 256
+// cost more to chain than they save (1 x 16,001 x 128, forward: 37, 33 and 36 us
+// with 128, 256 and 512).
 struct Plan {
   int tiles, cblocks, segs, seg_tiles;
 };
@@ -253,8 +255,8 @@ __device__ __forceinline__ Part block_part(const Plan& p, int segs) {
 // to CHAIN_SEGS segments every block of the main pass chains those before its
 // own itself; more would read too much, and a kernel between the passes puts
 // what enters each segment in their place (`entered`).  (4 lanes x 257, 17
-// segments, forward and gradient: 46 us with that kernel, 38 without; 4 x 2000
-// and 1 x 16,001 x 128, forward: 25 and 35 us with it, 40 and 55 without.)  So does
+// segments, forward and gradient: 43 us with that kernel, 38 without; 4 x 2000
+// and 1 x 16,001 x 128, forward: 25 and 33 us with it, 50 and 61 without.)  So does
 // a call whose state is updated in place: a lane's last segment stores it, and
 // blocks of its other segments may not have begun by then.
 constexpr int CHAIN_SEGS = 32;
@@ -404,7 +406,7 @@ __global__ __launch_bounds__((Shape<N>::BT)) void scan_local_kernel(const ScanGr
 // segments added: chains of segs steps, cut among up to 16 groups of 64 (channel,
 // state) pairs, each of which first finds what its own segments do.  Bound by
 // latency, so a thread's whole part is under way at once and stays in registers
-// (256 segments: 6 us; four loads at a time, and again for the second walk: 9.5).
+// (251 segments: 7 us; four loads at a time, and again for the second walk: 10).
 constexpr int CARRY_GROUPS = 16, CARRY_PER = MAX_SEGS / CARRY_GROUPS;  // at most
 template <bool REV>
 __global__ __launch_bounds__(64 * CARRY_GROUPS) void scan_carry_kernel(
@@ -912,7 +914,7 @@ __global__ __launch_bounds__(256) void scan_sums_kernel(GradWork wk, uint32_t bc
 }
 
 // whether a thread's elements of a row can be moved at once (32 x 1024 x 512 bf16,
-// forward and gradient: 384 us; element by element 520)
+// forward and gradient: 391 us; element by element 527)
 bool rows_vec(const void* d, int64_t lane, int64_t row, int ev, int size) {
   return ((uintptr_t)d % (ev * size)) == 0 && lane % ev == 0 && row % ev == 0;
 }

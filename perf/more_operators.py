@@ -1,0 +1,594 @@
+"""Performance cases of the operators of a gated-delta-rule byte predictor, in
+training and in serving.
+
+A case is one pass of one of five paths over rows = `lanes` x `T` (byte
+sequences side by side, a row for each byte):
+
+  delta        the gated delta rule forward, state in and out (T = 1: one
+               decode step)
+  delta_train  the rule forward and its gradients, as a training step runs them
+  norm_train   residual addition and root-mean-square norm, and their gradients
+  project      residual addition and norm with rows in 8 bits, and their
+               product with weights in 8 bits: what opens a block in serving
+  sample       logits -> bytes, by temperature, top-k, top-p and min-p, from
+               given random numbers
+
+`precision` is the type of the row tensors ("fp32" or "bf16"); log decays,
+betas, states, weights of norms, scales and the gradients of weights are
+float32.  `ragged` cases have lanes of different lengths, one of them empty:
+rows past a lane's length keep what the output held (zero here), and their
+gradients are zero.
+"""
+import importlib
+import math
+
+import torch
+
+own = False
+
+# heads of a block at the repository's widths: (width, heads of q and k, heads of v, d_k, d_v)
+_MODELS = {"d64": (64, 1, 2, 64, 64), "d80": (80, 1, 2, 80, 80), "d256": (256, 4, 4, 64, 128),
+           "d512": (512, 4, 8, 128, 128)}
+_EPS = 1e-6
+
+
+def _case(name, path, model, lanes, T, precision, ragged=False, mixed=False):
+    c = {"path": path, "model": model, "lanes": lanes, "T": T, "precision": precision,
+         "ragged": ragged, "mixed": mixed}
+    return dict(c, name=name) if name else c
+
+
+def listed():
+    return [
+        # a decode step of a thousand lanes, state in and out
+        _case("delta_step_d256", "delta", "d256", 1000, 1, "fp32"),
+        # scoring one long text: a single sequence
+        _case("delta_long_d64", "delta", "d64", 1, 16001, "fp32"),
+        # the prompts of a batch of requests, of different lengths
+        _case("delta_prefill_d512_bf16", "delta", "d512", 64, 521, "bf16", ragged=True),
+        # fitting a small model to a few texts
+        _case("delta_train_d64", "delta_train", "d64", 4, 257, "fp32"),
+        # a training batch of the middle width
+        _case("delta_train_d256_bf16", "delta_train", "d256", 32, 1024, "bf16"),
+        # a small batch of the large width, two value heads to a key head
+        _case("delta_train_d512_bf16", "delta_train", "d512", 4, 777, "bf16", ragged=True),
+        # a training batch of whole chunks, and a smaller one of the large width
+        _case("norm_train_d256", "norm_train", "d256", 250, 521, "fp32", ragged=True),
+        _case("norm_train_d512_bf16", "norm_train", "d512", 37, 219, "bf16"),
+        # the projection that opens a block: one byte of every live stream, and whole prompts
+        _case("project_step_d256", "project", "d256", 64, 1, "fp32"),
+        _case("project_d512_bf16", "project", "d512", 16, 2085, "bf16"),
+        # the next byte of every live stream, and a thousand requests with settings of their own
+        _case("sample_step", "sample", "d64", 64, 1, "fp32"),
+        _case("sample_large", "sample", "d256", 1000, 65, "fp32", ragged=True, mixed=True),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    path = rng.choice(["delta", "delta", "delta_train", "delta_train", "norm_train", "project",
+                       "sample"])
+    model = rng.choice(sorted(_MODELS))
+    width, _, hv, dk, dv = _MODELS[model]
+    precision = rng.choice(["fp32", "bf16"])
+    mixed = False
+    if path in ("delta", "delta_train"):
+        rows = 32 * 1024 * 4 * 64 * 128 // (hv * dk * dv)  # the largest listed training batch
+        if path == "delta":
+            lanes = _log_int(rng, 1, 1000 if hv * dk * dv <= 4 * 64 * 128 else 250)
+            T = 1 if rng.random() < 0.3 else _log_int(rng, 2, max(2, min(16384, rows // lanes)))
+        else:
+            lanes = _log_int(rng, 1, 128)
+            T = _log_int(rng, 2, max(2, min(4096, rows // lanes)))
+    elif path == "sample":
+        lanes = _log_int(rng, 1, 1000)
+        T = _log_int(rng, 1, 64)
+        mixed = rng.random() < 0.5
+    else:
+        rows = 32768 if path == "project" else 32768 * 512 // width
+        lanes = _log_int(rng, 1, 1000)
+        T = 1 if rng.random() < 0.25 else _log_int(rng, 2, max(2, rows // lanes))
+    return _case(None, path, model, lanes, T, precision,
+                 ragged=lanes > 1 and rng.random() < 0.5, mixed=mixed)
+
+
+# ------------------------------------------------------------------ inputs
+def _tokens(case, g):
+    """[lanes, T] bytes: little-endian float32 records as an instrument writes
+    them, half of them zero."""
+    lanes, T = case["lanes"], case["T"]
+    k = (lanes * T + 3) // 4
+    v = torch.round(torch.randn((k,), generator=g, device="cuda") * 1000) / 1000
+    v = v * (torch.rand((k,), generator=g, device="cuda") < 0.5)
+    return v.view(torch.uint8)[:lanes * T].view(lanes, T)
+
+
+def _lens(case, g):
+    if not case["ragged"]:
+        return None
+    lanes, T = case["lanes"], case["T"]
+    n = torch.randint(0, T + 1, (lanes,), generator=g, device="cuda", dtype=torch.int32)
+    n[0] = T
+    n[-1] = 0
+    return n
+
+
+def _type(case):
+    return torch.bfloat16 if case["precision"] == "bf16" else torch.float32
+
+
+def _columns(case):
+    """Channels of the block's opening product: q, k, v and a gate beside v."""
+    _, h, hv, dk, dv = _MODELS[case["model"]]
+    return 2 * h * dk + 2 * hv * dv
+
+
+def prepare(case, seed):
+    width, h, hv, dk, dv = _MODELS[case["model"]]
+    lanes, T, path, dt = case["lanes"], case["T"], case["path"], _type(case)
+    g = torch.Generator("cuda").manual_seed(seed)
+
+    def randn(*shape):
+        return torch.randn(shape, generator=g, device="cuda")
+
+    s = {"case": case, "lens": _lens(case, g)}
+    if path in ("delta", "delta_train"):
+        # q, k and v side by side, as the product before the rule leaves them; the
+        # same byte has much the same key wherever it stands
+        qkv = randn(lanes, T, 2 * h * dk + hv * dv)
+        qkv[..., h * dk:2 * h * dk] += randn(256, h * dk)[_tokens(case, g).long()]
+        qkv = qkv.to(dt)
+        s["q"], s["k"] = qkv[..., :h * dk], qkv[..., h * dk:2 * h * dk]
+        s["v"] = qkv[..., 2 * h * dk:]
+        rate = torch.exp(math.log(1e-3) + math.log(100.0)
+                         * torch.rand((hv,), generator=g, device="cuda"))
+        decay = 1 + 15 * torch.rand((hv,), generator=g, device="cuda")
+        s["g"] = -decay * rate * torch.exp(0.5 * randn(lanes, T, hv))
+        s["beta"] = torch.sigmoid(randn(lanes, T, hv))
+        s["scale"] = dk ** -0.5
+        s["state_in"] = randn(lanes, hv, dk, dv) * 0.1
+        if path == "delta_train":
+            s["dout"] = (randn(lanes, T, hv * dv) * 1e-2).to(dt)
+            s["dstate_out"] = randn(lanes, hv, dk, dv) * 1e-2
+    elif path == "sample":
+        s["logits"] = (randn(lanes, T, 256) * 3).to(dt)
+        s["bias"] = randn(256) * 0.1
+        s["logits"][:, :, 250:] = -math.inf  # bytes that the format rules out
+        s["uniform"] = torch.rand((lanes, T), generator=g, device="cuda")
+        if case["mixed"]:  # temperature, top_k, top_p, min_p of every lane; some are greedy
+            p = torch.rand((lanes, 4), generator=g, device="cuda")
+            p[:, 0] = torch.where(p[:, 0] < 0.1, torch.zeros_like(p[:, 0]), 0.3 + p[:, 0])
+            p[:, 1] = torch.floor(p[:, 1] * 100)
+            p[:, 2] = 0.5 + 0.6 * p[:, 2]
+            p[:, 3] = (p[:, 3] - 0.5) * 0.1
+            s["params"] = p
+        else:
+            s["params"] = torch.tensor([[0.8, 40.0, 0.95, 0.01]], device="cuda").expand(lanes, 4)
+    else:
+        s["x"], s["residual"] = randn(lanes, T, width).to(dt), (2 * randn(lanes, T, width)).to(dt)
+        s["weight"] = 1 + 0.2 * randn(width)
+        if path == "norm_train":
+            s["dout"] = (randn(lanes, T, width) * 1e-2).to(dt)
+            s["dsum"] = (randn(lanes, T, width) * 1e-2).to(dt)
+        else:
+            n = _columns(case)
+            s["w8"] = torch.clamp(torch.round(randn(n, width) * 36), -127, 127).to(torch.int8)
+            s["wscale"] = (0.5 + torch.rand((n,), generator=g, device="cuda")) / 36 / width ** 0.5
+            s["bias"] = randn(n) * 0.1
+    if own:
+        _own_state(s)
+    return s
+
+
+def _own_state(s):
+    """What a program of this library keeps between calls: a context, outputs,
+    workspaces and weights as the product reads them."""
+    boa = importlib.import_module("boa-constrictor_amd.boa_hip")
+    case = s["case"]
+    width, h, hv, dk, dv = _MODELS[case["model"]]
+    lanes, T, path, dt = case["lanes"], case["T"], case["path"], _type(case)
+
+    def zeros(*shape, dtype=torch.float32):
+        return torch.zeros(shape, dtype=dtype, device="cuda")
+
+    s["codec"] = boa.Codec(64, 1, 16, max_lanes=1)
+    s["codec"].set_stream(torch.cuda.current_stream().cuda_stream)
+    work = 0
+    if path in ("delta", "delta_train"):
+        sizes, train = (lanes, T, h, hv, dk, dv), path == "delta_train"
+        s["out"] = zeros(lanes, T, hv * dv, dtype=dt)
+        s["state_out"] = zeros(lanes, hv, dk, dv)
+        work = boa.delta_rule_work_bytes(*sizes, grad=train)
+        if train:
+            s["saved"] = zeros(boa.delta_rule_saved_floats(*sizes))
+            d = zeros(lanes, T, 2 * h * dk + hv * dv, dtype=dt)
+            s["dq"], s["dk"] = d[..., :h * dk], d[..., h * dk:2 * h * dk]
+            s["dv"] = d[..., 2 * h * dk:]
+            s["dg"], s["dbeta"] = zeros(lanes, T, hv), zeros(lanes, T, hv)
+            s["dstate_in"] = zeros(lanes, hv, dk, dv)
+    elif path == "sample":
+        s["bytes"], s["logp"] = zeros(lanes, T, dtype=torch.uint8), zeros(lanes, T)
+    else:
+        s["sum"] = zeros(lanes, T, width, dtype=dt)
+        if path == "norm_train":
+            s["out"], s["dx"] = zeros(lanes, T, width, dtype=dt), zeros(lanes, T, width, dtype=dt)
+            s["dweight"] = zeros(width)
+            work = boa.rms_norm_grad_work_bytes(lanes, T, width)
+        else:
+            n = _columns(case)
+            s["x8"], s["scale8"] = zeros(lanes, T, width, dtype=torch.int8), zeros(lanes, T)
+            s["packed"] = zeros(boa.int8_pack_bytes(n, width), dtype=torch.uint8)
+            s["codec"].int8_pack(s["w8"], s["packed"])
+            s["out"] = zeros(lanes, T, n, dtype=dt)
+    s["work"] = zeros(work, dtype=torch.uint8)
+
+
+# ---------------------------------------------------------------- one pass
+def run(state):
+    path = state["case"]["path"]
+    if own:
+        return _run_own(state, path)
+    return {"delta": _delta, "delta_train": _delta, "norm_train": _norm_train,
+            "project": _project, "sample": _sample}[path](state)
+
+
+def _run_own(s, path):
+    codec = s["codec"]
+    if path == "sample":
+        if s["case"]["mixed"]:
+            how = {"d_params": s["params"]}
+        else:
+            how = {"temperature": 0.8, "top_k": 40, "top_p": 0.95, "min_p": 0.01}
+        codec.sample_bytes(s["logits"], s["uniform"], s["bytes"], d_bias=s["bias"],
+                           d_logp=s["logp"], d_lens=s["lens"], **how)
+        return {k: s[k] for k in ("bytes", "logp")}
+    if path == "norm_train":
+        codec.rms_norm(s["x"], s["out"], d_weight=s["weight"], d_residual=s["residual"],
+                       d_sum=s["sum"], eps=_EPS, d_lens=s["lens"])
+        codec.rms_norm_grad(s["sum"], s["dout"], s["dx"], s["work"], d_weight=s["weight"],
+                            d_dsum=s["dsum"], d_dweight=s["dweight"], eps=_EPS, d_lens=s["lens"])
+        return {k: s[k] for k in ("sum", "out", "dx", "dweight")}
+    if path == "project":
+        codec.rms_norm(s["x"], d_weight=s["weight"], d_residual=s["residual"], d_sum=s["sum"],
+                       d_out8=s["x8"], d_scale8=s["scale8"], eps=_EPS, d_lens=s["lens"])
+        codec.int8_matmul(s["x8"], s["scale8"], s["packed"], s["wscale"], s["out"],
+                          d_bias=s["bias"], d_lens=s["lens"])
+        return {k: s[k] for k in ("sum", "scale8", "out")}
+    args = [s[k] for k in ("q", "k", "v", "g", "beta")]
+    heads = _MODELS[s["case"]["model"]][1]
+    codec.delta_rule(*args, s["out"], s["work"], heads=heads, scale=s["scale"], unit_qk=True,
+                     d_state_in=s["state_in"], d_state_out=s["state_out"], d_lens=s["lens"],
+                     d_saved=s.get("saved"))
+    names = ["out", "state_out"]
+    if path == "delta_train":
+        grads = ["dq", "dk", "dv", "dg", "dbeta"]
+        codec.delta_rule_grad(*args, s["saved"], s["dout"], *[s[k] for k in grads], s["work"],
+                              heads=heads, scale=s["scale"], unit_qk=True,
+                              d_state_in=s["state_in"], d_dstate_out=s["dstate_out"],
+                              d_dstate_in=s["dstate_in"], d_lens=s["lens"])
+        names += grads + ["dstate_in"]
+    return {k: s[k] for k in names}
+
+
+# ------------------------------------------------- the operators' plain form
+def _mask(s):
+    """[lanes, T, 1]: 1 where a row lies within its lane's length."""
+    case = s["case"]
+    if s["lens"] is None:
+        return torch.ones((case["lanes"], case["T"], 1), device="cuda")
+    return (torch.arange(case["T"], device="cuda") < s["lens"][:, None]).float()[..., None]
+
+
+def _norm(s):
+    h = s["x"].float() + s["residual"].float()
+    return h, torch.rsqrt((h * h).mean(-1, keepdim=True) + _EPS)
+
+
+def _norm_train(s):
+    on, dt = _mask(s), s["x"].dtype
+    h, r = _norm(s)
+    total = (h * on).to(dt)
+    got = {"sum": total, "out": (h * r * s["weight"] * on).to(dt)}
+    h = total.float()  # the gradient starts from the sum as it was stored
+    r = torch.rsqrt((h * h).mean(-1, keepdim=True) + _EPS)
+    dy, n = s["dout"].float() * on, h * r
+    wdy = s["weight"] * dy
+    dx = r * (wdy - n * (n * wdy).mean(-1, keepdim=True)) + s["dsum"].float()
+    got.update(dx=(dx * on).to(dt), dweight=(dy * n).double().sum((0, 1)).float())
+    return got
+
+
+def _project(s):
+    on, dt = _mask(s), s["x"].dtype
+    # in 64 bits: a value may lie next to the border of two steps of 1 / 127
+    h = s["x"].double() + s["residual"].double()
+    r = torch.rsqrt((h * h).mean(-1, keepdim=True) + _EPS)
+    t = h * s["weight"]
+    top = t.abs().amax(-1, keepdim=True)
+    x8 = torch.round(t * (127 / top)).float()
+    scale8 = (top * r / 127).float()
+    acc = 0.0
+    w = s["w8"].float()
+    for k in range(0, w.shape[1], 1024):  # sums that 32 bits hold exactly
+        acc = acc + torch.matmul(x8[..., k:k + 1024], w[:, k:k + 1024].t().contiguous())
+    out = acc * scale8 * s["wscale"] + s["bias"]
+    return {"sum": (h * on).to(dt), "scale8": (scale8 * on)[..., 0], "out": (out * on).to(dt)}
+
+
+def _sample(s):
+    # in 64 bits: a random number may lie next to the border of two bytes
+    on = _mask(s)[..., 0]
+    x = s["logits"].double() + s["bias"].double()
+    x = x - x.amax(-1, keepdim=True)
+    temp, top_k, top_p, min_p = (s["params"][:, i].double()[:, None, None] for i in range(4))
+    greedy = temp <= 0
+    w = torch.exp(x / torch.where(greedy, torch.ones_like(temp), temp))
+    order = torch.sort(x, dim=-1, descending=True, stable=True)[1]
+    sorted_w = w.gather(-1, order)
+    rank = torch.arange(256, device="cuda")
+    keep = (rank < top_k) | (top_k < 1)
+    sorted_w = sorted_w * keep
+    before = torch.cumsum(sorted_w, -1) - sorted_w
+    keep = (before < top_p * sorted_w.sum(-1, keepdim=True)) | (top_p >= 1)
+    keep = (keep & (sorted_w >= min_p) & ~greedy) | (rank == 0)
+    kept = torch.zeros_like(w).scatter_(-1, order, sorted_w * keep)
+    total = torch.cumsum(kept, -1)
+    u = s["uniform"].double()[..., None] * total[..., -1:]
+    byte = (total <= u).sum(-1, keepdim=True).clamp_(max=255)
+    logp = torch.log(kept.gather(-1, byte) / total[..., -1:])[..., 0]
+    return {"bytes": (byte[..., 0] * on.long()).to(torch.uint8),
+            "logp": torch.where(on > 0, logp, torch.zeros_like(logp)).float()}
+
+
+_CHUNK = 64
+
+
+def _chunks(t, heads, group=1):
+    """[lanes, T, heads * d] -> [lanes, heads * group, chunks, 64, d] in fp32,
+    zero behind the last position."""
+    lanes, T, width = t.shape
+    n = (T + _CHUNK - 1) // _CHUNK
+    p = torch.zeros((lanes, n * _CHUNK, width), device="cuda")
+    p[:, :T] = t
+    p = p.view(lanes, n, _CHUNK, heads, width // heads).permute(0, 3, 1, 2, 4)
+    return p.repeat_interleave(group, 1).contiguous()
+
+
+def _rows(t, T):
+    """The inverse of _chunks, without its groups."""
+    lanes, heads, n, c, d = t.shape
+    return t.permute(0, 2, 3, 1, 4).reshape(lanes, n * c, heads * d)[:, :T]
+
+
+def _t(x):
+    return x.transpose(-1, -2).contiguous()
+
+
+def _delta(s):
+    case, dt = s["case"], s["q"].dtype
+    _, h, hv, dk, dv = _MODELS[case["model"]]
+    group, T, on = hv // h, case["T"], _mask(s)
+    live = _chunks(on, 1)
+    q, k = _chunks(s["q"].float() * on, h, group), _chunks(s["k"].float() * on, h, group)
+    rq = torch.rsqrt((q * q).sum(-1, keepdim=True) + _EPS)
+    rk = torch.rsqrt((k * k).sum(-1, keepdim=True) + _EPS)
+    q, k = q * rq, k * rk * live
+    v = _chunks(s["v"].float() * on, hv)
+    beta = _chunks(s["beta"] * on, hv)
+    # sums of log decays in 64 bits: their differences are exponents
+    sums = torch.cumsum(_chunks(s["g"] * on, hv).double(), 3)
+    n = q.shape[2]
+    low = torch.ones((_CHUNK, _CHUNK), device="cuda").tril()
+    between = torch.exp(torch.where(low > 0, sums - sums.transpose(-1, -2),
+                                    torch.zeros_like(sums))).float() * low
+    since = torch.exp(sums).float()
+    left = torch.exp(sums[:, :, :, -1:] - sums).float()
+    kk = torch.matmul(k, _t(k)) * between * low.tril(-1)
+    a = kk * beta
+    p = torch.matmul(q, _t(k)) * between * s["scale"]
+    inv = torch.zeros_like(a)  # of 1 + a, row by row
+    for i in range(_CHUNK):
+        inv[:, :, :, i] = -torch.matmul(a[:, :, :, i:i + 1], inv)[:, :, :, 0]
+        inv[:, :, :, i, i] = 1
+    w, u = torch.matmul(inv, k * beta * since), torch.matmul(inv, v * beta)
+    k_left, k_left_t = k * left, _t(k * left)
+    S, states, new = s["state_in"], [], []
+    for c in range(n):
+        states.append(S)
+        new.append(u[:, :, c] - torch.matmul(w[:, :, c], S))
+        S = S * since[:, :, c, -1:] + torch.matmul(k_left_t[:, :, c], new[-1])
+    state, new = torch.stack(states, 2), torch.stack(new, 2)
+    got = {"state_out": S}
+    q_since = q * since * s["scale"]
+    out = torch.matmul(q_since, state) + torch.matmul(p, new)
+    got["out"] = (_rows(out, T) * on).to(dt)
+    if case["path"] == "delta":
+        return got
+    dout = _chunks(s["dout"].float() * on, hv)
+    dnew, q_since_t, w_t = torch.matmul(_t(p), dout), _t(q_since), _t(w)
+    dS, dstates = s["dstate_out"], []
+    for c in reversed(range(n)):
+        dstates.append(dS)
+        dnew[:, :, c] += torch.matmul(k_left[:, :, c], dS)
+        dS = (dS * since[:, :, c, -1:] + torch.matmul(q_since_t[:, :, c], dout[:, :, c])
+              - torch.matmul(w_t[:, :, c], dnew[:, :, c]))
+    got["dstate_in"] = dS
+    dstate = torch.stack(dstates[::-1], 2)
+    dr = torch.matmul(_t(inv), dnew)
+    da = -torch.matmul(dr, _t(new)) * low.tril(-1)
+    dp = torch.matmul(dout, _t(new)) * low
+    state_t = _t(state)
+    out_state, new_state = torch.matmul(dout, state_t), torch.matmul(new, _t(dstate))
+    dr_state, seen = torch.matmul(dr, state_t), torch.matmul(k, state)
+    da_b, dp_b = da * between * beta, dp * between * s["scale"]
+    dq = out_state * since * s["scale"] + torch.matmul(dp_b, k)
+    dkey = (torch.matmul(_t(dp_b), q) + torch.matmul(da_b + _t(da_b), k) + new_state * left
+            - dr_state * since * beta)
+    dbeta = (dr * (v - seen * since)).sum(-1, keepdim=True) + (da * kk).sum(-1, keepdim=True)
+    m = da * a + dp * p
+    last = (new_state * k_left).sum(-1, keepdim=True)
+    dsum = (m.sum(-1, keepdim=True) - m.sum(-2)[..., None] - last
+            + (out_state * q_since).sum(-1, keepdim=True)
+            - (dr * seen).sum(-1, keepdim=True) * beta * since)
+    dsum[:, :, :, -1:] += (last.sum(3, keepdim=True) + since[:, :, :, -1:]
+                           * (dstate * state).sum((-1, -2))[..., None, None])
+    dg = dsum.flip(3).double().cumsum(3).float().flip(3)
+
+    def shared(x):  # of the value heads that share a head, and through its length
+        lanes = x.shape[0]
+        return x.view(lanes, h, group, n, _CHUNK, dk).sum(2)
+
+    q, k, rq, rk = q[:, ::group], k[:, ::group], rq[:, ::group], rk[:, ::group]
+    dq, dkey = shared(dq), shared(dkey)
+    dq = rq * (dq - q * (q * dq).sum(-1, keepdim=True))
+    dkey = rk * (dkey - k * (k * dkey).sum(-1, keepdim=True))
+    got.update(dq=(_rows(dq, T) * on).to(dt), dk=(_rows(dkey, T) * on).to(dt),
+               dv=(_rows(dr * beta, T) * on).to(dt), dg=_rows(dg, T) * on,
+               dbeta=_rows(dbeta, T) * on)
+    return got
+
+
+# ----------------------------------------------------------- what it needs
+def work(case):
+    """Each input read and each output written once; multiplications and
+    additions (and an exponential as one operation) of the formulas."""
+    width, h, hv, dk, dv = _MODELS[case["model"]]
+    lanes, rows, path = case["lanes"], case["lanes"] * case["T"], case["path"]
+    size = 2 if case["precision"] == "bf16" else 4
+    if path == "sample":
+        return {"bytes": rows * (256 * size + 4 + 1 + 4) + 1024, "flops": rows * 256 * 8}
+    if path == "norm_train":
+        return {"bytes": rows * width * size * 7 + 8 * width, "flops": rows * width * 16}
+    if path == "project":
+        n = _columns(case)
+        return {"bytes": rows * (width * size * 3 + n * size + 4) + n * (width + 8) + 4 * width,
+                "flops": rows * (2 * width * n + 8 * width)}
+    states = 4 * lanes * hv * dk * dv
+    moved = rows * (size * (2 * h * dk + 2 * hv * dv) + 8 * hv) + 2 * states
+    flops = rows * hv * 7 * dk * dv
+    if path == "delta_train":
+        moved += rows * (size * (2 * h * dk + 2 * hv * dv) + 8 * hv) + 2 * states
+        flops += rows * hv * 16 * dk * dv
+    return {"bytes": moved, "flops": flops}
+
+
+# -------------------------------------------------------------- in 64 bits
+def exact(case, seed):
+    s = prepare(case, seed)
+    lanes, T, path = case["lanes"], case["T"], case["path"]
+    lens = [T] * lanes if s["lens"] is None else s["lens"].tolist()
+    valid = torch.zeros((lanes, T), dtype=torch.bool, device="cuda")
+    for i, n in enumerate(lens):
+        valid[i, :n] = True
+    if path == "sample":
+        return _exact_sample(s, valid)
+    if path in ("delta", "delta_train"):
+        return _exact_delta(s, valid)
+    dt, on = s["x"].dtype, valid[..., None].double()
+    total, weight = s["x"].double() + s["residual"].double(), s["weight"].double()
+    length = torch.sqrt((total ** 2).mean(-1, keepdim=True) + _EPS)
+    if path == "project":
+        y = total / length * weight
+        scale8 = y.abs().amax(-1, keepdim=True) / 127
+        values = torch.round(y / scale8) * scale8
+        out = torch.matmul(values, (s["w8"].double() * s["wscale"].double()[:, None]).t())
+        return {"sum": total * on, "scale8": (scale8 * on)[..., 0],
+                "out": (out + s["bias"].double()) * on}
+    got = {"sum": total * on, "out": total / length * weight * on}
+    h = total.to(dt).double().requires_grad_()  # as it was stored
+    weight.requires_grad_()
+    out = h / torch.sqrt((h ** 2).mean(-1, keepdim=True) + _EPS) * weight
+    ((out * s["dout"].double() + h * s["dsum"].double()) * on).sum().backward()
+    got.update(dx=h.grad, dweight=weight.grad)
+    return got
+
+
+def _exact_sample(s, valid):
+    x = s["logits"].double() + s["bias"].double()
+    lanes, T, _ = x.shape
+    p = s["params"].double()
+    ids = torch.arange(256, device="cuda")
+    byte = torch.zeros((lanes, T), dtype=torch.uint8, device="cuda")
+    logp = torch.zeros((lanes, T), dtype=torch.float64, device="cuda")
+    for i in range(0, lanes, 16):
+        xs = x[i:i + 16]
+        temp, top_k, top_p, min_p = (p[i:i + 16, j, None, None] for j in range(4))
+        # a byte's rank: how many stand before it
+        ahead = ((xs[..., None, :] > xs[..., :, None])
+                 | ((xs[..., None, :] == xs[..., :, None]) & (ids[None, :] < ids[:, None])))
+        rank = ahead.sum(-1)
+        prob = torch.softmax(xs / torch.where(temp > 0, temp, torch.ones_like(temp)), -1)
+        alive = torch.where(top_k >= 1, rank < top_k, torch.ones_like(rank, dtype=torch.bool))
+        prob = prob * alive
+        prob = prob / prob.sum(-1, keepdim=True)
+        mass = torch.matmul(ahead.double(), prob[..., None])[..., 0]  # of those before it
+        alive &= (mass < top_p) | (top_p >= 1)
+        alive &= prob >= min_p * prob.amax(-1, keepdim=True)
+        alive = torch.where(temp > 0, alive, torch.zeros_like(alive)) | (rank == 0)
+        prob = prob * alive
+        prob = prob / prob.sum(-1, keepdim=True)
+        edge = torch.cumsum(prob, -1)
+        pick = torch.argmax((edge > s["uniform"][i:i + 16].double()[..., None]).int(), -1)
+        byte[i:i + 16] = pick.to(torch.uint8)
+        logp[i:i + 16] = torch.log(prob.gather(-1, pick[..., None])[..., 0])
+    return {"bytes": byte * valid, "logp": torch.where(valid, logp, torch.zeros_like(logp))}
+
+
+def _exact_delta(s, valid):
+    case = s["case"]
+    _, h, hv, dk, dv = _MODELS[case["model"]]
+    lanes, T = case["lanes"], case["T"]
+
+    def heads(t, count):
+        t = t.double().view(lanes, T, count, -1)
+        return t.repeat_interleave(hv // count, 2)
+
+    length = [torch.sqrt((heads(s[n], h) ** 2).sum(-1, keepdim=True) + _EPS) for n in ("q", "k")]
+    q, k = heads(s["q"], h) / length[0], heads(s["k"], h) / length[1]
+    v, beta = heads(s["v"], hv), s["beta"].double()
+    decay = torch.exp(s["g"].double())
+    train = case["path"] == "delta_train"
+    S, outs, states, errors = s["state_in"].double(), [], [], []
+    for t in range(T):
+        here = valid[:, t, None, None, None]
+        kept = S * decay[:, t, :, None, None]
+        error = v[:, t] - torch.matmul(k[:, t, :, None], kept)[..., 0, :]
+        new = kept + (beta[:, t, :, None] * k[:, t])[..., None] * error[..., None, :]
+        if train:
+            states.append(S)
+            errors.append(error)
+        S = torch.where(here, new, S)
+        outs.append(torch.matmul(q[:, t, :, None], S)[..., 0, :])
+    on = valid[..., None].double()
+    got = {"out": torch.stack(outs, 1).flatten(2) * s["scale"] * on, "state_out": S}
+    if not train:
+        return got
+    dout = s["dout"].double().view(lanes, T, hv, dv) * s["scale"]
+    dS, rows = s["dstate_out"].double(), {n: [] for n in ("dq", "dk", "dv", "dg", "dbeta")}
+    for t in reversed(range(T)):
+        here = valid[:, t, None, None, None]
+        kept = states[t] * decay[:, t, :, None, None]
+        after = states[t + 1] if t + 1 < T else S
+        full = dS + q[:, t, :, :, None] * dout[:, t, :, None]
+        through = torch.matmul(k[:, t, :, None], full)[..., 0, :]  # into k's row of the state
+        derror = beta[:, t, :, None] * through
+        back = full - k[:, t, :, :, None] * derror[..., None, :]
+        rows["dq"].append(torch.matmul(after, dout[:, t, :, :, None])[..., 0])
+        rows["dv"].append(derror)
+        rows["dbeta"].append((through * errors[t]).sum(-1))
+        rows["dk"].append(beta[:, t, :, None] * torch.matmul(full, errors[t][..., None])[..., 0]
+                          - torch.matmul(kept, derror[..., None])[..., 0])
+        rows["dg"].append((back * kept).sum((-1, -2)))
+        dS = torch.where(here, back * decay[:, t, :, None, None], dS)
+    rows = {n: torch.stack(x[::-1], 1) for n, x in rows.items()}
+    for name, unit, size in (("dq", q, length[0]), ("dk", k, length[1])):
+        # through the division by the length, then over the heads that share a row
+        d = (rows[name] - unit * (unit * rows[name]).sum(-1, keepdim=True)) / size
+        rows[name] = d.view(lanes, T, h, hv // h, dk).sum(3)
+    for name, d in rows.items():
+        got[name] = (d.flatten(2) if d.dim() == 4 else d) * on
+    got["dstate_in"] = dS
+    return got

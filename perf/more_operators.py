@@ -121,9 +121,9 @@ def _type(case):
 
 
 def _columns(case):
-    """Channels of the block's opening product: q, k, v and a gate beside v."""
+    """Channels of the block's opening product: q, k, v and a log decay and beta a head of v."""
     _, h, hv, dk, dv = _MODELS[case["model"]]
-    return 2 * h * dk + 2 * hv * dv
+    return 2 * h * dk + hv * dv + 2 * hv
 
 
 def prepare(case, seed):

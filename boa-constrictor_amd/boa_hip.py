@@ -63,6 +63,27 @@ class ScanGrads(C.Structure):
                 ("d_dstate_in", C.c_void_p)]
 
 
+class Delta(C.Structure):
+    """boa_delta: the inputs of the gated delta rule."""
+    _fields_ = [("lanes", C.c_int32), ("T", C.c_int32), ("heads", C.c_int32),
+                ("v_heads", C.c_int32), ("d_k", C.c_int32), ("d_v", C.c_int32),
+                ("precision", C.c_int32), ("unit_qk", C.c_int32), ("scale", C.c_float),
+                ("d_lens", C.c_void_p), ("q", Rows), ("k", Rows), ("v", Rows), ("g", Rows),
+                ("beta", Rows), ("d_state_in", C.c_void_p)]
+
+
+class DeltaGrads(C.Structure):
+    """boa_delta_grads: the outputs of the gated delta rule's gradient."""
+    _fields_ = [("dq", Rows), ("dk", Rows), ("dv", Rows), ("dg", Rows), ("dbeta", Rows),
+                ("d_dstate_in", C.c_void_p)]
+
+
+class Sampling(C.Structure):
+    """boa_sampling: how a byte is chosen."""
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_float), ("top_p", C.c_float),
+                ("min_p", C.c_float)]
+
+
 def build(clean: bool = False) -> str:
     """Compile libboa_hip.so and the boa CLI for gfx950 (hipcc)."""
     if clean:
@@ -122,6 +143,26 @@ def lib():
             "boa_next_byte_loss": (C.c_int, [P, C.POINTER(Rows), P, P, i64, P, i32, i32, i32, f32,
                                              P, P, C.POINTER(Rows), P, P, i64]),
             "boa_next_byte_loss_work_bytes": (i64, [i32, i32]),
+            "boa_rms_norm": (C.c_int, [P, C.POINTER(Rows), C.POINTER(Rows), P, P, i32, i32, i32,
+                                       i32, f32, C.POINTER(Rows), C.POINTER(Rows),
+                                       C.POINTER(Rows), P]),
+            "boa_rms_norm_grad": (C.c_int, [P, C.POINTER(Rows), P, P, i32, i32, i32, i32, f32,
+                                            C.POINTER(Rows), C.POINTER(Rows), C.POINTER(Rows), P,
+                                            P, i64]),
+            "boa_rms_norm_grad_work_bytes": (i64, [i32, i32, i32]),
+            "boa_int8_rows": (C.c_int, [P, C.POINTER(Rows), P, i32, i32, i32, i32,
+                                        C.POINTER(Rows), P]),
+            "boa_int8_pack": (C.c_int, [P, P, i32, i32, P]),
+            "boa_int8_pack_bytes": (i64, [i32, i32]),
+            "boa_int8_matmul": (C.c_int, [P, C.POINTER(Rows), P, P, i32, i32, i32, P, P, i32, P,
+                                          i32, C.POINTER(Rows)]),
+            "boa_delta_rule": (C.c_int, [P, C.POINTER(Delta), C.POINTER(Rows), P, P, P, i64]),
+            "boa_delta_rule_grad": (C.c_int, [P, C.POINTER(Delta), P, C.POINTER(Rows), P,
+                                              C.POINTER(DeltaGrads), P, i64]),
+            "boa_delta_rule_saved_floats": (i64, [i32, i32, i32, i32, i32, i32]),
+            "boa_delta_rule_work_bytes": (i64, [i32, i32, i32, i32, i32, i32, i32]),
+            "boa_sample_bytes": (C.c_int, [P, C.POINTER(Rows), P, P, P, i32, i32, i32,
+                                           C.POINTER(Sampling), P, P, i64, P]),
             "boa_cdf_from_logits": (C.c_int, [P, P, P, i32, P]),
             "boa_cdf_from_probs": (C.c_int, [P, P, i32, i32, P]),
             "boa_rc_encode_cdf": (C.c_int, [P, P, P, i32, i32, P, i64, P]),
@@ -251,6 +292,24 @@ def selective_scan_work_bytes(lanes, T, channels, d_state, grad=False):
 
 def next_byte_loss_work_bytes(lanes, T):
     return _size(lib().boa_next_byte_loss_work_bytes(*_int32(lanes, T)), "next_byte_loss")
+
+
+def rms_norm_grad_work_bytes(lanes, T, width):
+    return _size(lib().boa_rms_norm_grad_work_bytes(*_int32(lanes, T, width)), "rms_norm_grad")
+
+
+def int8_pack_bytes(n, k):
+    return _size(lib().boa_int8_pack_bytes(*_int32(n, k)), "int8_pack")
+
+
+def delta_rule_saved_floats(lanes, T, heads, v_heads, d_k, d_v):
+    return _size(lib().boa_delta_rule_saved_floats(*_int32(lanes, T, heads, v_heads, d_k, d_v)),
+                 "delta_rule")
+
+
+def delta_rule_work_bytes(lanes, T, heads, v_heads, d_k, d_v, grad=False):
+    return _size(lib().boa_delta_rule_work_bytes(*_int32(lanes, T, heads, v_heads, d_k, d_v),
+                                                 int(grad)), "delta_rule")
 
 
 class Codec:
@@ -429,6 +488,178 @@ class Codec:
             _tensor(d_loss, "loss", (lanes, T), f32, dev), _tensor(d_total, "total", (1,), f32, dev),
             dx, _tensor(d_dbias, "dbias", (256,), f32, dev), *_work(d_work, dev)),
             "next_byte_loss")
+
+    # ---- a gated-delta-rule predictor's operators (boa_rms_norm and the calls
+    # after it in boa_hip.h): tensors and rows as for the training operators
+    def rms_norm(self, d_x, d_out=None, d_weight=None, d_residual=None, d_sum=None, d_out8=None,
+                 d_scale8=None, eps=1e-6, d_lens=None):
+        """sum = x + residual, out = weight sum / its root mean square, and the
+        same in 8 bits: out8 int8 [lanes, T, width], scale8 float32 [lanes, T]."""
+        torch = sys.modules["torch"]
+        dev, f32, dt, prec = self.device, torch.float32, d_x.dtype, _precision(d_x, "x")
+        lanes, T, width = d_x.shape
+        if (lanes | T | width) >> 31:
+            _int32(lanes, T, width)
+
+        def rows(t, name, dtype=dt):
+            return None if t is None else C.byref(_rows(t, name, lanes, T, width, dtype, dev))
+
+        self._check(lib().boa_rms_norm(
+            self.h, rows(d_x, "x"), rows(d_residual, "residual"),
+            _tensor(d_weight, "weight", (width,), f32, dev),
+            _tensor(d_lens, "lens", (lanes,), torch.int32, dev), lanes, T, width, prec, eps,
+            rows(d_sum, "sum"), rows(d_out, "out"), rows(d_out8, "out8", torch.int8),
+            _tensor(d_scale8, "scale8", (lanes, T), f32, dev)), "rms_norm")
+
+    def rms_norm_grad(self, d_h, d_dout, d_dx, d_work=None, d_weight=None, d_dsum=None,
+                      d_dweight=None, eps=1e-6, d_lens=None):
+        """dx (of x and of residual) and dweight from h (the sum) and the
+        gradients of out and of sum; dx may be dout or dsum."""
+        torch = sys.modules["torch"]
+        dev, f32, dt, prec = self.device, torch.float32, d_h.dtype, _precision(d_h, "h")
+        lanes, T, width = d_h.shape
+        if (lanes | T | width) >> 31:
+            _int32(lanes, T, width)
+
+        def rows(t, name):
+            return None if t is None else C.byref(_rows(t, name, lanes, T, width, dt, dev))
+
+        self._check(lib().boa_rms_norm_grad(
+            self.h, rows(d_h, "h"), _tensor(d_weight, "weight", (width,), f32, dev),
+            _tensor(d_lens, "lens", (lanes,), torch.int32, dev), lanes, T, width, prec, eps,
+            rows(d_dout, "dout"), rows(d_dsum, "dsum"), rows(d_dx, "dx"),
+            _tensor(d_dweight, "dweight", (width,), f32, dev), *_work(d_work, dev)),
+            "rms_norm_grad")
+
+    def int8_rows(self, d_x, d_out8, d_scale8, d_lens=None):
+        """x's rows in 8 bits (int8 [lanes, T, width]) with a scale each."""
+        torch = sys.modules["torch"]
+        dev, dt, prec = self.device, d_x.dtype, _precision(d_x, "x")
+        lanes, T, width = d_x.shape
+        if (lanes | T | width) >> 31:
+            _int32(lanes, T, width)
+        self._check(lib().boa_int8_rows(
+            self.h, C.byref(_rows(d_x, "x", lanes, T, width, dt, dev)),
+            _tensor(d_lens, "lens", (lanes,), torch.int32, dev), lanes, T, width, prec,
+            C.byref(_rows(d_out8, "out8", lanes, T, width, torch.int8, dev)),
+            _tensor(d_scale8, "scale8", (lanes, T), torch.float32, dev)), "int8_rows")
+
+    def int8_pack(self, d_w8, d_packed):
+        """int8 weights [n, k] as int8_matmul reads them (int8_pack_bytes(n, k)
+        bytes of any type)."""
+        torch = sys.modules["torch"]
+        if d_w8.dim() != 2:
+            raise ValueError(f"w8: want int8 [n, k], got {tuple(d_w8.shape)}")
+        n, k = _int32(*d_w8.shape)
+        self._packed(d_packed, n, k)
+        self._check(lib().boa_int8_pack(self.h, _tensor(d_w8, "w8", (n, k), torch.int8, self.device),
+                                        n, k, d_packed.data_ptr()), "int8_pack")
+
+    def _packed(self, t, n, k):
+        need = lib().boa_int8_pack_bytes(n, k)
+        if t.nbytes < need or t.get_device() != self.device or not t.is_contiguous():
+            raise ValueError(f"packed: want {need} contiguous bytes on cuda:{self.device}")
+        return t.data_ptr()
+
+    def int8_matmul(self, d_x8, d_scale8, d_packed, d_wscale, d_out, d_bias=None, d_lens=None):
+        """out [lanes, T, n] = scale8 wscale (x8 . packed weights) + bias."""
+        torch = sys.modules["torch"]
+        dev, f32, dt, prec = self.device, torch.float32, d_out.dtype, _precision(d_out, "out")
+        lanes, T, n = d_out.shape
+        if d_x8.dim() != 3:
+            raise ValueError(f"x8: want int8 [lanes, T, k], got {tuple(d_x8.shape)}")
+        k = d_x8.shape[2]
+        if (lanes | T | n | k) >> 31:
+            _int32(lanes, T, n, k)
+        self._check(lib().boa_int8_matmul(
+            self.h, C.byref(_rows(d_x8, "x8", lanes, T, k, torch.int8, dev)),
+            _tensor(d_scale8, "scale8", (lanes, T), f32, dev),
+            _tensor(d_lens, "lens", (lanes,), torch.int32, dev), lanes, T, k,
+            self._packed(d_packed, n, k), _tensor(d_wscale, "wscale", (n,), f32, dev), n,
+            _tensor(d_bias, "bias", (n,), f32, dev), prec,
+            C.byref(_rows(d_out, "out", lanes, T, n, dt, dev))), "int8_matmul")
+
+    def _delta_args(self, q, k, v, g, beta, heads, scale, unit_qk, state_in, lens):
+        torch = sys.modules["torch"]
+        dev, f32, prec, dt = self.device, torch.float32, _precision(q, "q"), q.dtype
+        if g.dim() != 3 or v.dim() != 3:
+            raise ValueError("v and g: want [lanes, T, width]")
+        (lanes, T, qw), hv, vw = q.shape, g.shape[2], v.shape[2]
+        if heads < 1 or hv < 1 or qw % heads or vw % hv:
+            raise ValueError(f"q of {qw} columns in {heads} heads, v of {vw} in {hv}")
+        dk, dv = qw // heads, vw // hv
+        if (lanes | T | heads | hv | dk | dv) >> 31:
+            _int32(lanes, T, heads, hv, dk, dv)
+        return Delta(lanes, T, heads, hv, dk, dv, prec, int(unit_qk), scale,
+                     _tensor(lens, "lens", (lanes,), torch.int32, dev),
+                     _rows(q, "q", lanes, T, qw, dt, dev), _rows(k, "k", lanes, T, qw, dt, dev),
+                     _rows(v, "v", lanes, T, vw, dt, dev), _rows(g, "g", lanes, T, hv, f32, dev),
+                     _rows(beta, "beta", lanes, T, hv, f32, dev),
+                     _tensor(state_in, "state_in", (lanes, hv, dk, dv), f32, dev))
+
+    def _delta_saved(self, t, d, dev):
+        if t is None:
+            return None
+        torch = sys.modules["torch"]
+        n = lib().boa_delta_rule_saved_floats(d.lanes, d.T, d.heads, d.v_heads, d.d_k, d.d_v)
+        if t.numel() < n:
+            raise ValueError(f"saved: want {n} floats, got {t.numel()}")
+        return _tensor(t, "saved", t.shape, torch.float32, dev)
+
+    def delta_rule(self, d_q, d_k, d_v, d_g, d_beta, d_out, d_work=None, heads=1, scale=1.0,
+                   unit_qk=True, d_state_in=None, d_state_out=None, d_lens=None, d_saved=None):
+        """The gated delta rule: q and k [lanes, T, heads * d_k], v and out
+        [lanes, T, v_heads * d_v], g and beta float32 [lanes, T, v_heads],
+        states float32 [lanes, v_heads, d_k, d_v]; d_saved
+        (delta_rule_saved_floats floats) keeps what its gradient starts from."""
+        d, dev = self._delta_args(d_q, d_k, d_v, d_g, d_beta, heads, scale, unit_qk, d_state_in,
+                                  d_lens), self.device
+        out = _rows(d_out, "out", d.lanes, d.T, d.v_heads * d.d_v, d_q.dtype, dev)
+        state = (d.lanes, d.v_heads, d.d_k, d.d_v)
+        self._check(lib().boa_delta_rule(
+            self.h, C.byref(d), C.byref(out),
+            _tensor(d_state_out, "state_out", state, d_g.dtype, dev),
+            self._delta_saved(d_saved, d, dev), *_work(d_work, dev)), "delta_rule")
+
+    def delta_rule_grad(self, d_q, d_k, d_v, d_g, d_beta, d_saved, d_dout, d_dq, d_dk, d_dv, d_dg,
+                        d_dbeta, d_work=None, heads=1, scale=1.0, unit_qk=True, d_state_in=None,
+                        d_dstate_out=None, d_dstate_in=None, d_lens=None):
+        """Gradients of delta_rule, from its inputs, its d_saved and the
+        gradients of its outputs (d_dstate_out None: zero)."""
+        d, dev = self._delta_args(d_q, d_k, d_v, d_g, d_beta, heads, scale, unit_qk, d_state_in,
+                                  d_lens), self.device
+        f32, dt, lanes, T, hv = d_g.dtype, d_q.dtype, d.lanes, d.T, d.v_heads
+        qw, vw, state = heads * d.d_k, hv * d.d_v, (lanes, hv, d.d_k, d.d_v)
+        dout = _rows(d_dout, "dout", lanes, T, vw, dt, dev)
+        grads = DeltaGrads(_rows(d_dq, "dq", lanes, T, qw, dt, dev),
+                           _rows(d_dk, "dk", lanes, T, qw, dt, dev),
+                           _rows(d_dv, "dv", lanes, T, vw, dt, dev),
+                           _rows(d_dg, "dg", lanes, T, hv, f32, dev),
+                           _rows(d_dbeta, "dbeta", lanes, T, hv, f32, dev),
+                           _tensor(d_dstate_in, "dstate_in", state, f32, dev))
+        self._check(lib().boa_delta_rule_grad(
+            self.h, C.byref(d), self._delta_saved(d_saved, d, dev), C.byref(dout),
+            _tensor(d_dstate_out, "dstate_out", state, f32, dev), C.byref(grads),
+            *_work(d_work, dev)), "delta_rule_grad")
+
+    def sample_bytes(self, d_logits, d_uniform, d_bytes, d_bias=None, d_logp=None,
+                     temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, d_params=None, d_lens=None):
+        """A byte (uint8 [lanes, T]) for every row of logits [lanes, T, 256] by
+        the random numbers uniform [lanes, T]; d_params float32 [lanes, 4]:
+        temperature, top_k, top_p and min_p of each lane."""
+        torch = sys.modules["torch"]
+        dev, f32, prec = self.device, torch.float32, _precision(d_logits, "logits")
+        out, stride, lanes, T = _bytes(d_bytes, "bytes", dev)
+        how = None
+        if d_params is None:
+            how = C.byref(Sampling(temperature, top_k, top_p, min_p))
+        self._check(lib().boa_sample_bytes(
+            self.h, C.byref(_rows(d_logits, "logits", lanes, T, 256, d_logits.dtype, dev)),
+            _tensor(d_bias, "bias", (256,), f32, dev),
+            _tensor(d_uniform, "uniform", (lanes, T), f32, dev),
+            _tensor(d_lens, "lens", (lanes,), torch.int32, dev), lanes, T, prec, how,
+            _tensor(d_params, "params", (lanes, 4), f32, dev), out, stride,
+            _tensor(d_logp, "logp", (lanes, T), f32, dev)), "sample_bytes")
 
     def compress_device(self, d_data, n, chunk_size, d_payload, cap_words, max_chunks=0):
         import numpy as np

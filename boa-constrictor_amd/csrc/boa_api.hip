@@ -23,6 +23,7 @@
 #include "../../include/boa_hip.h"
 #include "boa_kernels.h"
 #include "container.h"
+#include "predictor_ops.h"
 #include "train_kernels.h"
 
 using namespace boa;
@@ -1054,6 +1055,16 @@ bool scan_sizes_ok(int64_t lanes, int64_t T, int64_t channels, int64_t ds) {
   return seqs_ok(lanes, T) && channels >= 1 && channels <= 4096 && (ds == 16 || ds == 32);
 }
 
+bool norm_sizes_ok(int64_t lanes, int64_t T, int64_t width) {
+  return seqs_ok(lanes, T) && width >= 1 && width <= 8192;
+}
+bool int8_sizes_ok(int64_t n, int64_t k) { return n >= 1 && n <= 65536 && k >= 1 && k <= 16384; }
+bool delta_sizes_ok(int64_t lanes, int64_t T, int64_t heads, int64_t v_heads, int64_t dk,
+                    int64_t dv) {
+  return seqs_ok(lanes, T) && heads >= 1 && v_heads >= heads && v_heads <= 1024 &&
+         v_heads % heads == 0 && dk >= 1 && dk <= 128 && dv >= 1 && dv <= 128;
+}
+
 // Collects the first thing that is wrong with a call's arguments.
 struct TrainCheck {
   const char* bad = nullptr;   // what is wrong
@@ -1143,6 +1154,57 @@ struct TrainCheck {
   static bool scan_input(const boa_scan& s, const void* p) {
     return p == s.u.d || p == s.delta.d || p == s.z.d || p == s.b.d || p == s.c.d || p == s.d_A ||
            p == s.d_D || p == s.d_delta_bias || p == s.d_state_in;
+  }
+  // int8 rows
+  void rows8(const boa_rows* r, int64_t width, bool written, const char* what) {
+    const int keep = size;
+    size = 1;
+    if (written) out(r, width, what);
+    else in(r, what);
+    near(r, what);
+    size = keep;
+  }
+  // an output that may be an input only with the same strides
+  void same_or_other(const boa_rows* o, const boa_rows* i, const char* what) {
+    that(bad || !o || !i || o->d != i->d ||
+             (o->lane_stride == i->lane_stride && o->row_stride == i->row_stride),
+         "an output is an input with other strides: ", what);
+  }
+  void delta(const boa_delta* s, DeltaArgs& a) {
+    that(s != nullptr, "delta is NULL");
+    if (bad) return;
+    sizes(s->lanes, s->T, s->precision);
+    that(delta_sizes_ok(s->lanes, s->T, s->heads, s->v_heads, s->d_k, s->d_v),
+         "v_heads has to be a multiple of heads, 1 .. 1024, d_k and d_v 1 .. 128");
+    floats(s->d_lens, 4, true, "lens");
+    in(&s->q, "q"), near(&s->q, "q");
+    in(&s->k, "k"), near(&s->k, "k");
+    in(&s->v, "v"), near(&s->v, "v");
+    const int keep = size;
+    size = 4;
+    in(&s->g, "g"), near(&s->g, "g");
+    in(&s->beta, "beta"), near(&s->beta, "beta");
+    size = keep;
+    floats(s->d_state_in, 16, true, "state_in");
+    a = DeltaArgs{};
+    a.q = Seqs{s->lanes, s->T, s->d_lens};
+    a.H = s->heads;
+    a.HV = s->v_heads;
+    a.dk = s->d_k;
+    a.dv = s->d_v;
+    a.scale = s->scale;
+    a.unit = s->unit_qk != 0;
+    a.bf16 = s->precision == 1;
+    a.qr = from(s->q);
+    a.k = from(s->k);
+    a.v = from(s->v);
+    a.g = from(s->g);
+    a.beta = from(s->beta);
+    a.state_in = s->d_state_in;
+  }
+  static bool delta_input(const boa_delta& s, const void* p) {
+    return p == s.q.d || p == s.k.d || p == s.v.d || p == s.g.d || p == s.beta.d ||
+           p == s.d_state_in;
   }
 };
 
@@ -1831,6 +1893,280 @@ int boa_next_byte_loss(boa_ctx* c, const boa_rows* logits, const float* d_bias,
     return launch_loss({Seqs{lanes, T, d_lens}, k.from(*logits), d_targets, target_stride, d_bias,
                         scale, d_loss, d_total, dlogits ? k.to(*dlogits) : RowsOut{nullptr, 0, 0},
                         d_dbias, d_work, precision == 1}, c->stream);
+  });
+}
+
+// ---- a gated-delta-rule predictor's operators -------------------------------
+
+int64_t boa_rms_norm_grad_work_bytes(int32_t lanes, int32_t T, int32_t width) {
+  if (!norm_sizes_ok(lanes, T, width)) return -1;
+  return (int64_t)norm_grad_work((int64_t)lanes * T, width);
+}
+
+int64_t boa_int8_pack_bytes(int32_t n, int32_t k) {
+  return int8_sizes_ok(n, k) ? int8_packed_bytes(n, k) : -1;
+}
+
+int64_t boa_delta_rule_saved_floats(int32_t lanes, int32_t T, int32_t heads, int32_t v_heads,
+                                    int32_t d_k, int32_t d_v) {
+  if (!delta_sizes_ok(lanes, T, heads, v_heads, d_k, d_v)) return -1;
+  return delta_saved_floats(lanes, T, heads, v_heads, d_k, d_v);
+}
+
+int64_t boa_delta_rule_work_bytes(int32_t lanes, int32_t T, int32_t heads, int32_t v_heads,
+                                  int32_t d_k, int32_t d_v, int32_t grad) {
+  if (!delta_sizes_ok(lanes, T, heads, v_heads, d_k, d_v)) return -1;
+  return delta_work_bytes(lanes, T, heads, v_heads, d_k, d_v, grad != 0);
+}
+
+int boa_rms_norm(boa_ctx* c, const boa_rows* x, const boa_rows* residual, const float* d_weight,
+                 const int32_t* d_lens, int32_t lanes, int32_t T, int32_t width, int32_t precision,
+                 float eps, const boa_rows* sum, const boa_rows* out, const boa_rows* out8,
+                 float* d_scale8) {
+  return train_call(c, "boa_rms_norm", [&](TrainCheck& k) {
+    k.sizes(lanes, T, precision);
+    k.that(width >= 1 && width <= 8192, "width has to be 1 .. 8192");
+    k.that(eps >= 0.0f && eps < HUGE_VALF, "eps has to be 0 or more");
+    k.in(x, "x"), k.near(x, "x");
+    if (residual) k.in(residual, "residual"), k.near(residual, "residual");
+    k.floats(d_weight, 4, true, "weight");
+    k.floats(d_lens, 4, true, "lens");
+    k.that(sum || out || out8, "no output is wanted");
+    if (sum) {
+      k.out(sum, width, "sum"), k.near(sum, "sum");
+      k.same_or_other(sum, x, "sum"), k.same_or_other(sum, residual, "sum");
+    }
+    if (out) {
+      k.out(out, width, "out"), k.near(out, "out");
+      k.that(k.bad || (out->d != x->d && (!residual || out->d != residual->d) &&
+                       (!sum || out->d != sum->d)), "out is an input or another output");
+    }
+    if (out8) {
+      k.rows8(out8, width, true, "out8");
+      k.floats(d_scale8, 4, false, "scale8");
+      k.that(k.bad || (out8->d != x->d && (!residual || out8->d != residual->d) &&
+                       (!sum || out8->d != sum->d) && (!out || out8->d != out->d)),
+             "out8 is an input or another output");
+    }
+    if (k.bad) return hipSuccess;
+    NormArgs a{};
+    a.q = Seqs{lanes, T, d_lens};
+    a.width = width;
+    a.eps = eps;
+    a.norm = true;
+    a.bf16 = precision == 1;
+    a.x = k.from(*x);
+    if (residual) a.res = k.from(*residual);
+    a.weight = d_weight;
+    if (sum) a.sum = k.to(*sum);
+    if (out) a.out = k.to(*out);
+    if (out8) a.out8 = k.to(*out8);
+    a.scale8 = d_scale8;
+    return launch_norm(a, c->stream);
+  });
+}
+
+int boa_rms_norm_grad(boa_ctx* c, const boa_rows* h, const float* d_weight, const int32_t* d_lens,
+                      int32_t lanes, int32_t T, int32_t width, int32_t precision, float eps,
+                      const boa_rows* dout, const boa_rows* dsum, const boa_rows* dx,
+                      float* d_dweight, void* d_work, int64_t work_bytes) {
+  return train_call(c, "boa_rms_norm_grad", [&](TrainCheck& k) {
+    k.sizes(lanes, T, precision);
+    k.that(width >= 1 && width <= 8192, "width has to be 1 .. 8192");
+    k.that(eps >= 0.0f && eps < HUGE_VALF, "eps has to be 0 or more");
+    k.in(h, "h"), k.near(h, "h");
+    k.floats(d_weight, 4, true, "weight");
+    k.floats(d_lens, 4, true, "lens");
+    k.in(dout, "dout"), k.near(dout, "dout");
+    if (dsum) k.in(dsum, "dsum"), k.near(dsum, "dsum");
+    k.out(dx, width, "dx"), k.near(dx, "dx");
+    k.that(k.bad || dx->d != h->d, "dx is an input");
+    k.same_or_other(dx, dout, "dx"), k.same_or_other(dx, dsum, "dx");
+    k.floats(d_dweight, 4, true, "dweight");
+    k.that(k.bad || !d_dweight || d_dweight != d_weight, "dweight is an input");
+    if (d_dweight) k.work(d_work, work_bytes, boa_rms_norm_grad_work_bytes(lanes, T, width));
+    if (k.bad) return hipSuccess;
+    NormGradArgs a{};
+    a.q = Seqs{lanes, T, d_lens};
+    a.width = width;
+    a.eps = eps;
+    a.bf16 = precision == 1;
+    a.h = k.from(*h);
+    a.dout = k.from(*dout);
+    if (dsum) a.dsum = k.from(*dsum);
+    a.weight = d_weight;
+    a.dx = k.to(*dx);
+    a.dweight = d_dweight;
+    a.work = d_work;
+    return launch_norm_grad(a, c->stream);
+  });
+}
+
+int boa_int8_rows(boa_ctx* c, const boa_rows* x, const int32_t* d_lens, int32_t lanes, int32_t T,
+                  int32_t width, int32_t precision, const boa_rows* out8, float* d_scale8) {
+  return train_call(c, "boa_int8_rows", [&](TrainCheck& k) {
+    k.sizes(lanes, T, precision);
+    k.that(width >= 1 && width <= 8192, "width has to be 1 .. 8192");
+    k.in(x, "x"), k.near(x, "x");
+    k.floats(d_lens, 4, true, "lens");
+    k.rows8(out8, width, true, "out8");
+    k.floats(d_scale8, 4, false, "scale8");
+    k.that(k.bad || out8->d != x->d, "out8 is an input");
+    if (k.bad) return hipSuccess;
+    NormArgs a{};
+    a.q = Seqs{lanes, T, d_lens};
+    a.width = width;
+    a.bf16 = precision == 1;
+    a.x = k.from(*x);
+    a.out8 = k.to(*out8);
+    a.scale8 = d_scale8;
+    return launch_norm(a, c->stream);
+  });
+}
+
+int boa_int8_pack(boa_ctx* c, const int8_t* d_w, int32_t n, int32_t kk, void* d_packed) {
+  return train_call(c, "boa_int8_pack", [&](TrainCheck& k) {
+    k.that(int8_sizes_ok(n, kk), "n has to be 1 .. 65536, k 1 .. 16384");
+    k.floats(d_w, 1, false, "w");
+    k.floats(d_packed, 16, false, "packed");
+    k.that(k.bad || d_w != d_packed, "packed is an input");
+    if (k.bad) return hipSuccess;
+    return launch_int8_pack(d_w, n, kk, d_packed, c->stream);
+  });
+}
+
+int boa_int8_matmul(boa_ctx* c, const boa_rows* x8, const float* d_scale8, const int32_t* d_lens,
+                    int32_t lanes, int32_t T, int32_t kk, const void* d_packed,
+                    const float* d_wscale, int32_t n, const float* d_bias, int32_t precision,
+                    const boa_rows* out) {
+  return train_call(c, "boa_int8_matmul", [&](TrainCheck& k) {
+    k.sizes(lanes, T, precision);
+    k.that(int8_sizes_ok(n, kk), "n has to be 1 .. 65536, k 1 .. 16384");
+    k.rows8(x8, kk, false, "x8");
+    k.floats(d_scale8, 4, false, "scale8");
+    k.floats(d_lens, 4, true, "lens");
+    k.floats(d_packed, 16, false, "packed");
+    k.floats(d_wscale, 4, false, "wscale");
+    k.floats(d_bias, 4, true, "bias");
+    k.out(out, n, "out"), k.near(out, "out");
+    k.that(k.bad || (out->d != x8->d && out->d != d_packed && out->d != d_scale8 &&
+                     out->d != d_wscale && out->d != d_bias), "out is an input");
+    if (k.bad) return hipSuccess;
+    Int8Args a{};
+    a.q = Seqs{lanes, T, d_lens};
+    a.N = n;
+    a.K = kk;
+    a.x = k.from(*x8);
+    a.xscale = d_scale8;
+    a.packed = d_packed;
+    a.wscale = d_wscale;
+    a.bias = d_bias;
+    a.out = k.to(*out);
+    a.bf16 = precision == 1;
+    return launch_int8(a, c->stream);
+  });
+}
+
+int boa_delta_rule(boa_ctx* c, const boa_delta* d, const boa_rows* out, float* d_state_out,
+                   float* d_saved, void* d_work, int64_t work_bytes) {
+  return train_call(c, "boa_delta_rule", [&](TrainCheck& k) {
+    DeltaArgs a{};
+    k.delta(d, a);
+    if (k.bad) return hipSuccess;
+    k.out(out, (int64_t)d->v_heads * d->d_v, "out"), k.near(out, "out");
+    k.floats(d_state_out, 16, true, "state_out");
+    k.floats(d_saved, 16, true, "saved");
+    k.that(k.bad || !k.delta_input(*d, out->d), "out is an input");
+    if (!d_saved)
+      k.work(d_work, work_bytes, boa_delta_rule_work_bytes(d->lanes, d->T, d->heads, d->v_heads,
+                                                           d->d_k, d->d_v, 0));
+    if (k.bad) return hipSuccess;
+    a.out = k.to(*out);
+    a.state_out = d_state_out;
+    a.saved = d_saved;
+    a.work = d_work;
+    return launch_delta(a, c->stream);
+  });
+}
+
+int boa_delta_rule_grad(boa_ctx* c, const boa_delta* d, const float* d_saved, const boa_rows* dout,
+                        const float* d_dstate_out, const boa_delta_grads* g, void* d_work,
+                        int64_t work_bytes) {
+  return train_call(c, "boa_delta_rule_grad", [&](TrainCheck& k) {
+    DeltaGradArgs a{};
+    k.delta(d, a.f);
+    k.that(g != nullptr, "grads is NULL");
+    if (k.bad) return hipSuccess;
+    const int64_t qk = (int64_t)d->heads * d->d_k;
+    k.floats(d_saved, 16, false, "saved");
+    k.in(dout, "dout"), k.near(dout, "dout");
+    k.floats(d_dstate_out, 4, true, "dstate_out");
+    k.out(&g->dq, qk, "dq"), k.near(&g->dq, "dq");
+    k.out(&g->dk, qk, "dk"), k.near(&g->dk, "dk");
+    k.out(&g->dv, (int64_t)d->v_heads * d->d_v, "dv"), k.near(&g->dv, "dv");
+    const int keep = k.size;
+    k.size = 4;
+    k.out(&g->dg, d->v_heads, "dg"), k.near(&g->dg, "dg");
+    k.out(&g->dbeta, d->v_heads, "dbeta"), k.near(&g->dbeta, "dbeta");
+    k.size = keep;
+    k.floats(g->d_dstate_in, 4, true, "dstate_in");
+    for (const void* p : {(const void*)g->dq.d, (const void*)g->dk.d, (const void*)g->dv.d,
+                          (const void*)g->dg.d, (const void*)g->dbeta.d})
+      k.that(k.bad || (!k.delta_input(*d, p) && p != dout->d && p != d_saved),
+             "a gradient is an input");
+    k.work(d_work, work_bytes, boa_delta_rule_work_bytes(d->lanes, d->T, d->heads, d->v_heads,
+                                                         d->d_k, d->d_v, 1));
+    if (k.bad) return hipSuccess;
+    a.f.saved = const_cast<float*>(d_saved);
+    a.f.work = d_work;
+    a.dout = k.from(*dout);
+    a.dstate_out = d_dstate_out;
+    a.dq = k.to(g->dq);
+    a.dk = k.to(g->dk);
+    a.dv = k.to(g->dv);
+    a.dg = k.to(g->dg);
+    a.dbeta = k.to(g->dbeta);
+    a.dstate_in = g->d_dstate_in;
+    return launch_delta_grad(a, c->stream);
+  });
+}
+
+int boa_sample_bytes(boa_ctx* c, const boa_rows* logits, const float* d_bias,
+                     const float* d_uniform, const int32_t* d_lens, int32_t lanes, int32_t T,
+                     int32_t precision, const boa_sampling* params, const boa_sampling* d_params,
+                     uint8_t* d_bytes, int64_t byte_stride, float* d_logp) {
+  return train_call(c, "boa_sample_bytes", [&](TrainCheck& k) {
+    k.sizes(lanes, T, precision);
+    k.in(logits, "logits"), k.near(logits, "logits");
+    k.floats(d_bias, 4, true, "bias");
+    k.floats(d_uniform, 4, false, "uniform");
+    k.floats(d_lens, 4, true, "lens");
+    k.that(params || d_params, "params and d_params are both NULL");
+    k.floats(d_params, 4, true, "params");
+    k.that(!params || d_params || (params->temperature == params->temperature &&
+                                   params->top_k == params->top_k &&
+                                   params->top_p == params->top_p &&
+                                   params->min_p == params->min_p), "a setting is NaN");
+    k.bytes(d_bytes, byte_stride, "bytes");
+    k.that(lanes == 1 || byte_stride >= T, "rows overlap: ", "bytes");
+    k.floats(d_logp, 4, true, "logp");
+    k.that(k.bad || ((const void*)d_bytes != logits->d && (const void*)d_bytes != d_uniform &&
+                     (const void*)d_logp != logits->d && (!d_logp || d_logp != d_uniform)),
+           "an output is an input");
+    if (k.bad) return hipSuccess;
+    SampleArgs a{};
+    a.q = Seqs{lanes, T, d_lens};
+    a.logits = k.from(*logits);
+    a.bias = d_bias;
+    a.uniform = d_uniform;
+    if (!d_params) a.how = SampleHow{params->temperature, params->top_k, params->top_p,
+                                     params->min_p};
+    a.each = reinterpret_cast<const SampleHow*>(d_params);
+    a.bytes = d_bytes;
+    a.stride = byte_stride;
+    a.logp = d_logp;
+    a.bf16 = precision == 1;
+    return launch_sample(a, c->stream);
   });
 }
 

@@ -250,6 +250,115 @@ int boa_next_byte_loss(boa_ctx* ctx, const boa_rows* logits, const float* d_bias
                        int64_t work_bytes);
 int64_t boa_next_byte_loss_work_bytes(int32_t lanes, int32_t T);
 
+/* ---- a gated-delta-rule predictor's operators (device pointers) ------------ */
+/* The recurrence of predictors that keep a matrix of associations instead of
+ * the scan's vector, what stands around it in a block, and the choice of a
+ * byte.  Rows, lane lengths, strides, types, workspaces, streams and capture
+ * are as for the training operators above; row strides are at most 2^25. */
+
+/* Root-mean-square norm of x + residual:
+ *   h = x + residual    r = 1 / sqrt(mean h^2 + eps)    out = h r weight
+ * rows `width` (1 .. 8192) wide; d_weight [width] fp32, NULL: ones; residual
+ * NULL: none.  Outputs, each may be NULL: sum (h; it may be x or residual
+ * itself, with the same strides) and out, rows of the type `precision`; out8
+ * with d_scale8 [lanes][T], the out rows in 8 bits: of t = h weight,
+ * out8 = rint(127 t / max |t|) and scale8 = max |t| r / 127, so that out8
+ * scale8 is out within half a step.  A boa_rows of int8 has strides in bytes.
+ * A row of zeros has scale 0, one with a value that is not finite scale NaN or
+ * infinity. */
+int boa_rms_norm(boa_ctx* ctx, const boa_rows* x, const boa_rows* residual, const float* d_weight,
+                 const int32_t* d_lens, int32_t lanes, int32_t T, int32_t width, int32_t precision,
+                 float eps, const boa_rows* sum, const boa_rows* out, const boa_rows* out8,
+                 float* d_scale8);
+/* The gradient from h (the sum rows, or x where there is no residual), that of
+ * out and (NULL: zero) that of sum: dx rows, which are those of x and of
+ * residual alike and may be dout or dsum itself (same strides), and d_dweight
+ * [width] (NULL: not wanted, and no workspace needed). */
+int boa_rms_norm_grad(boa_ctx* ctx, const boa_rows* h, const float* d_weight,
+                      const int32_t* d_lens, int32_t lanes, int32_t T, int32_t width,
+                      int32_t precision, float eps, const boa_rows* dout, const boa_rows* dsum,
+                      const boa_rows* dx, float* d_dweight, void* d_work, int64_t work_bytes);
+int64_t boa_rms_norm_grad_work_bytes(int32_t lanes, int32_t T, int32_t width);
+
+/* Rows in 8 bits: out8 = rint(127 x / max |x|), scale8 = max |x| / 127. */
+int boa_int8_rows(boa_ctx* ctx, const boa_rows* x, const int32_t* d_lens, int32_t lanes, int32_t T,
+                  int32_t width, int32_t precision, const boa_rows* out8, float* d_scale8);
+/* Weights [n][k] int8 (n 1 .. 65536 output channels, k 1 .. 16384), laid out
+ * once as the product reads them: boa_int8_pack_bytes bytes at d_packed, 16-byte
+ * aligned. */
+int boa_int8_pack(boa_ctx* ctx, const int8_t* d_w, int32_t n, int32_t k, void* d_packed);
+int64_t boa_int8_pack_bytes(int32_t n, int32_t k);
+/* out = scale8 wscale sum_k x8 w + bias: int8 rows x8 (k wide) with a scale
+ * each, packed weights with a scale for each channel, d_bias [n] or NULL; out
+ * rows (n wide) of the type `precision`.  The sums are exact, so a lane's
+ * results do not depend on the other lanes or their number. */
+int boa_int8_matmul(boa_ctx* ctx, const boa_rows* x8, const float* d_scale8, const int32_t* d_lens,
+                    int32_t lanes, int32_t T, int32_t k, const void* d_packed,
+                    const float* d_wscale, int32_t n, const float* d_bias, int32_t precision,
+                    const boa_rows* out);
+
+/* The gated delta rule.  For each of v_heads states S [d_k][d_v]:
+ *   S = e^g S;   e = v - S^T k;   S = S + beta k e^T;   out = scale S^T q
+ * q and k rows hold `heads` heads of d_k (1 .. 128), v and out rows v_heads
+ * (a multiple of heads, at most 1024) of d_v (1 .. 128); v_heads / heads
+ * neighbouring heads of v share one of q and k.  g (log decays) and beta are
+ * fp32 rows v_heads wide, whatever `precision` is.  unit_qk: q and k are
+ * divided by their lengths sqrt(sum of squares + 1e-6) first.  A log decay
+ * below -1e4 (-inf too) forgets the state.  States [lanes][v_heads][d_k][d_v]
+ * fp32; d_state_in NULL is zero.  With T = 1 this is a decode step.  Positions
+ * are taken 64 at a time: a value that is not finite spoils the results of its
+ * lane and head from the first of its 64 on, and none of other lanes. */
+typedef struct {
+    int32_t lanes, T, heads, v_heads, d_k, d_v, precision, unit_qk;
+    float scale;
+    const int32_t* d_lens;
+    boa_rows q, k, v, g, beta;
+    const float* d_state_in;
+} boa_delta;
+/* Gradients: rows as their inputs' (g and beta fp32); dstate_in NULL: not
+ * wanted; it may be the gradient of state_out itself. */
+typedef struct {
+    boa_rows dq, dk, dv, dg, dbeta;
+    float* d_dstate_in;
+} boa_delta_grads;
+/* d_state_out (may be NULL, may be d_state_in itself): the states after each
+ * lane's last position; a lane of length 0 passes its state on.  d_saved: NULL,
+ * or where what the gradient starts from is kept (boa_delta_rule_saved_floats
+ * floats).  Both, and d_state_in, 16-byte aligned. */
+int boa_delta_rule(boa_ctx* ctx, const boa_delta* d, const boa_rows* out, float* d_state_out,
+                   float* d_saved, void* d_work, int64_t work_bytes);
+/* The gradient of that call, given its inputs, its d_saved, the gradient of
+ * out and (NULL: zero) of state_out. */
+int boa_delta_rule_grad(boa_ctx* ctx, const boa_delta* d, const float* d_saved,
+                        const boa_rows* dout, const float* d_dstate_out,
+                        const boa_delta_grads* grads, void* d_work, int64_t work_bytes);
+int64_t boa_delta_rule_saved_floats(int32_t lanes, int32_t T, int32_t heads, int32_t v_heads,
+                                    int32_t d_k, int32_t d_v);
+int64_t boa_delta_rule_work_bytes(int32_t lanes, int32_t T, int32_t heads, int32_t v_heads,
+                                  int32_t d_k, int32_t d_v, int32_t grad);
+
+/* A byte for every row of logits (256 wide), as boa_step_batch leaves them, by
+ * a given random number in [0, 1) [lanes][T]: x = logits + bias (NULL: none),
+ * weight exp((x - max x) / temperature), ranked by x, the lowest byte first
+ * among equals; kept are the first top_k, of those the shortest prefix of at
+ * least top_p of their weight, of those the bytes of at least min_p times the
+ * first one's weight; the byte is the first, in order of its value, up to which
+ * the kept weights sum to more than the number's share of their sum.
+ * temperature 0 or less: the first in rank.  top_k below 1, top_p from 1 on and
+ * min_p of 0 or less leave nothing out; the first in rank always stays.
+ * d_params (device, may be NULL): {temperature, top_k, top_p, min_p} of each
+ * lane, in place of `params`.  All of it in 64 bits.  d_bytes: byte t of lane l
+ * at l byte_stride + t; d_logp [lanes][T] (may be NULL): log of the byte's
+ * share of the kept weights.  Logits of -inf are bytes ruled out; a row with
+ * NaN, +inf or nothing else than -inf gives byte 0 and logp NaN. */
+typedef struct {
+    float temperature, top_k, top_p, min_p;
+} boa_sampling;
+int boa_sample_bytes(boa_ctx* ctx, const boa_rows* logits, const float* d_bias,
+                     const float* d_uniform, const int32_t* d_lens, int32_t lanes, int32_t T,
+                     int32_t precision, const boa_sampling* params, const boa_sampling* d_params,
+                     uint8_t* d_bytes, int64_t byte_stride, float* d_logp);
+
 /* ---- CDF and coder level (device pointers) ------------------------------ */
 /* Integer CDFs of logits rows: d_qcdf [rows][257] with low_k in column k and
  * 2^24 in column 256; d_bias (may be NULL) is added first.  This is the CDF

@@ -51,10 +51,28 @@ __device__ __forceinline__ void store_row(T* p, const float (&v)[V]) {
   }
 }
 
-// sums and greatest values over the G threads of a row, in every one of them;
-// rows of a block's 256 threads pass through `part`
-template <int G, typename F, typename X>
-__device__ __forceinline__ X row_all(X x, F f, X* part) {
+// where thread g's u-th vector of a row is read
+template <int V, int G>
+__device__ __forceinline__ int column(int u, int g, int width) {
+  const int i = (u * G + g) * V;
+  return i < width ? i : 0;
+}
+
+// x over the G threads of a row, in every one of them; a row of a block's 256
+// threads passes through `part`
+template <int G, typename F>
+__device__ __forceinline__ float row_all(float x, F f, float* part) {
+  x = G == 16 ? over16(x, f) : over64(x, f);
+  if constexpr (G == 256) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = f(f(part[0], part[1]), f(part[2], part[3]));
+  }
+  return x;
+}
+template <int G, typename F>
+__device__ __forceinline__ double row_all64(double x, F f, double* part) {
 #pragma unroll
   for (int m = 1; m < (G < 64 ? G : 64); m *= 2) x = f(x, __shfl_xor(x, m));
   if constexpr (G == 256) {
@@ -65,14 +83,24 @@ __device__ __forceinline__ X row_all(X x, F f, X* part) {
   }
   return x;
 }
-struct Add {
-  template <typename X> __device__ X operator()(X a, X b) const { return a + b; }
-};
 struct Most {  // NaN wins
-  __device__ double operator()(double a, double b) const {
-    return a != a ? a : (b > a || b != b ? b : a);
-  }
+  template <typename X>
+  __device__ X operator()(X a, X b) const { return a != a ? a : (b > a || b != b ? b : a); }
 };
+
+// 127 t / top to the nearest whole number.  f is the quotient in fp32, off by
+// under 5e-5 (h, t, the step and the product are rounded, 127 being the most);
+// where that leaves the number open, t and the product are taken in 64 bits, and
+// next to a border the quotient itself.
+__device__ __forceinline__ int step_of(float f, float x, float res, float w, double top,
+                                       double step) {
+  const float r = __builtin_rintf(f);
+  if (__builtin_fabsf(f - r) <= 0.5f - 1e-4f) return (int)r;
+  const double t = ((double)x + (double)res) * (double)w;
+  double q = t * step;
+  if (__builtin_fabs(q - __builtin_rint(q)) > 0.5 - 1e-9) q = t * 127.0 / top;
+  return (int)__builtin_rint(q);
+}
 
 template <typename T, int V, int G, int U, bool OUT8>
 __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a, uint32_t rows) {
@@ -80,6 +108,14 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a, uint32_t ro
   constexpr int R = 256 / G;  // rows of a block
   const int g = threadIdx.x % G;
   const uint32_t len = a.q.T;
+  float w[U][V];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int i = (u * G + g) * V + j;
+      w[u][j] = i < a.width ? (a.weight ? a.weight[i] : 1.0f) : 0.0f;
+    }
   for (uint64_t b = (uint64_t)blockIdx.x * R; b < rows; b += (uint64_t)gridDim.x * R) {
     const uint64_t r = b + threadIdx.x / G;
     const uint32_t l = r < rows ? (uint32_t)r / len : 0, t = r < rows ? (uint32_t)r - l * len : 0;
@@ -87,28 +123,38 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a, uint32_t ro
     const T* x = (const T*)a.x.d + l * a.x.lane + t * a.x.row;
     const T* res = a.res.d ? (const T*)a.res.d + l * a.res.lane + t * a.res.row : nullptr;
     float h[U][V], hr[U][V];
+    // no branch between a row's loads, each of which would wait for the last:
+    // threads past its end read its first elements
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = (u * G + g) * V;
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int j = 0; j < V; ++j) h[u][j] = hr[u][j] = 0.0f;
-      if (live && i < a.width) {
-        load_row<V>(x + i, h[u]);
-        if (res) load_row<V>(res + i, hr[u]);
+    if (live) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) load_row<V>(x + column<V, G>(u, g, a.width), h[u]);
+      if (res)
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_row<V>(res + column<V, G>(u, g, a.width), hr[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if ((u * G + g) * V >= a.width) h[u][j] = hr[u][j] = 0.0f;
+    float ss = 0.0f, most = 0.0f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float s = h[u][j] + hr[u][j];
+        ss += s * s;
+        if constexpr (OUT8) most = Most()(most, __builtin_fabsf(s * w[u][j]));
       }
-    }
-    float ss = 0.0f;
+    float rn = 1.0f;
     if (a.norm) {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float s = h[u][j] + hr[u][j];
-          ss += s * s;
-        }
-      ss = row_all<G>(ss, Add(), (float*)part);
+      ss = row_all<G>(ss, Sum(), (float*)part);
+      rn = 1.0f / __builtin_sqrtf(ss / (float)a.width + a.eps);
     }
-    const float rn = a.norm ? 1.0f / __builtin_sqrtf(ss / (float)a.width + a.eps) : 1.0f;
     if (a.sum.d && live) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -126,56 +172,46 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a, uint32_t ro
         if (i < a.width) {
           float y[V];
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            y[j] = (h[u][j] + hr[u][j]) * rn;
-            if (a.weight) y[j] *= a.weight[i + j];
-          }
+          for (int j = 0; j < V; ++j) y[j] = (h[u][j] + hr[u][j]) * rn * w[u][j];
           store_row<V>((T*)a.out.d + l * a.out.lane + t * a.out.row + i, y);
         }
       }
     }
     if constexpr (OUT8) {
+      most = row_all<G>(most, Most(), (float*)part);
+      // the greatest in 64 bits is among those next to the greatest in fp32
+      // (all of them, where fp32 has few digits left or none)
+      const float near = most < 1e-30f || !(most < __builtin_inff()) ? 0.0f : most * (1.0f - 0x1p-21f);
       double top = 0.0;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = (u * G + g) * V;
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          double v = (double)h[u][j] + (double)hr[u][j];
-          if (a.weight && i < a.width) v *= (double)a.weight[i + j];
-          top = Most()(top, __builtin_fabs(v));
-        }
-      }
-      top = row_all<G>(top, Most(), part);
+        for (int j = 0; j < V; ++j)
+          if (!(__builtin_fabsf((h[u][j] + hr[u][j]) * w[u][j]) < near))
+            top = Most()(top, __builtin_fabs(((double)h[u][j] + (double)hr[u][j]) * (double)w[u][j]));
+      top = row_all64<G>(top, Most(), part);
       const double step = top > 0.0 ? 127.0 / top : 0.0;
+      const float step32 = near > 0.0f ? (float)step : __builtin_nanf("");  // NaN: all in 64 bits
       if (live) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int i = (u * G + g) * V;
           if (i < a.width) {
-            int8_t q[V];
+            int q[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-              double v = (double)h[u][j] + (double)hr[u][j];
-              if (a.weight) v *= (double)a.weight[i + j];
-              // (where the product may be on the other side of a border, the quotient)
-              double f = v * step;
-              if (__builtin_fabs(f - __builtin_rint(f)) > 0.5 - 1e-9) f = v * 127.0 / top;
-              q[j] = (int8_t)(int)__builtin_rint(f);
-            }
+            for (int j = 0; j < V; ++j)
+              q[j] = top > 0.0 ? step_of((h[u][j] + hr[u][j]) * w[u][j] * step32, h[u][j], hr[u][j],
+                                         w[u][j], top, step)
+                               : 0;
             int8_t* o = (int8_t*)a.out8.d + l * a.out8.lane + t * a.out8.row + i;
-            if constexpr (V == 4) {
-              uint32_t w = 0;
+            if constexpr (V >= 4) {
+              uint32_t p[V / 4] = {};
 #pragma unroll
-              for (int j = 0; j < 4; ++j) w |= (uint32_t)(uint8_t)q[j] << (8 * j);
-              *reinterpret_cast<uint32_t*>(o) = w;
-            } else if constexpr (V == 8) {
-              uint32_t w[2] = {0, 0};
-#pragma unroll
-              for (int j = 0; j < 8; ++j) w[j / 4] |= (uint32_t)(uint8_t)q[j] << (8 * (j % 4));
-              *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1]);
+              for (int j = 0; j < V; ++j) p[j / 4] |= (uint32_t)(q[j] & 255) << (8 * (j % 4));
+              if constexpr (V == 4) *reinterpret_cast<uint32_t*>(o) = p[0];
+              else *reinterpret_cast<uint2*>(o) = make_uint2(p[0], p[1]);
             } else {
-              o[0] = q[0];
+              o[0] = (int8_t)q[0];
             }
           }
         }
@@ -188,6 +224,7 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a, uint32_t ro
 template <typename T, int V, int G, int U>
 __global__ __launch_bounds__(256) void norm_grad_kernel(const NormGradArgs a, uint32_t rows) {
   __shared__ float part[4];
+  __shared__ float group[U * V * 256];  // partial sums of the block's row groups
   constexpr int R = 256 / G;
   const int g = threadIdx.x % G;
   const uint32_t len = a.q.T;
@@ -211,16 +248,24 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(const NormGradArgs a, ui
     const T* sp = a.dsum.d ? (const T*)a.dsum.d + l * a.dsum.lane + t * a.dsum.row : nullptr;
     float ss = 0.0f, c = 0.0f;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = (u * G + g) * V;
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int j = 0; j < V; ++j) h[u][j] = dy[u][j] = ds[u][j] = 0.0f;
-      if (live && i < a.width) {
-        load_row<V>(hp + i, h[u]);
-        load_row<V>(dp + i, dy[u]);
-        if (sp) load_row<V>(sp + i, ds[u]);
+    if (live) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        load_row<V>(hp + column<V, G>(u, g, a.width), h[u]);
+        load_row<V>(dp + column<V, G>(u, g, a.width), dy[u]);
       }
+      if (sp)
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_row<V>(sp + column<V, G>(u, g, a.width), ds[u]);
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if ((u * G + g) * V >= a.width) h[u][j] = dy[u][j] = 0.0f;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -228,8 +273,8 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(const NormGradArgs a, ui
         ss += h[u][j] * h[u][j];
         c += h[u][j] * (w[u][j] * dy[u][j]);
       }
-    ss = row_all<G>(ss, Add(), part);
-    c = row_all<G>(c, Add(), part);
+    ss = row_all<G>(ss, Sum(), part);
+    c = row_all<G>(c, Sum(), part);
     const float rn = 1.0f / __builtin_sqrtf(ss / (float)a.width + a.eps);
     const float m = c * rn / (float)a.width;  // mean of n w dy
     if (there) {
@@ -248,32 +293,40 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(const NormGradArgs a, ui
     }
   }
   if (!a.dweight) return;
-  // the block's rows of partial sums, one for each of its R row groups
-  float* out = (float*)a.work + ((size_t)blockIdx.x * R + threadIdx.x / G) * a.width;
+  // the block's sums: of its R row groups, in order
+  float* out = (float*)a.work + (size_t)blockIdx.x * a.width;
+  constexpr int N = U * V * G;  // elements of a row, padded
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int i = (u * G + g) * V + j;
-      if (i < a.width) out[i] = dw[u][j];
-    }
+    for (int j = 0; j < V; ++j) group[threadIdx.x / G * N + (u * G + g) * V + j] = dw[u][j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.width; i += 256) {
+    float s = group[i];
+    for (int k = 1; k < R; ++k) s += group[k * N + i];
+    out[i] = s;
+  }
 }
 
-// dweight[i] = sum of n partial rows, in an order that the sizes decide
+// dweight[i] = sum of n partial rows in 64 bits, in an order that the sizes
+// decide: eight columns a block, so that few blocks do not sum it all
 __global__ __launch_bounds__(1024) void norm_dweight_kernel(const float* part, int n, int width,
                                                             float* dweight) {
-  __shared__ float sum[32][33];
-  const int col = blockIdx.x * 32 + threadIdx.x % 32, first = threadIdx.x / 32;
-  float s = 0.0f;
-  if (col < width)
-    for (int k = first; k < n; k += 32) s += part[(size_t)k * width + col];
-  sum[first][threadIdx.x % 32] = s;
-  __syncthreads();
-  if (threadIdx.x < 32 && col < width) {
-    s = 0.0f;
-    for (int k = 0; k < 32; ++k) s += sum[k][threadIdx.x];
-    dweight[col] = s;
+  __shared__ double sum[128][9];
+  const int c = threadIdx.x % 8, col = blockIdx.x * 8 + c, first = threadIdx.x / 8;
+  double s = 0.0;
+  if (col < width) {
+#pragma unroll 8
+    for (int k = first; k < n; k += 128) s += (double)part[(size_t)k * width + col];
   }
+  sum[first][c] = s;
+  __syncthreads();
+#pragma unroll
+  for (int m = 64; m; m /= 2) {
+    if (first < m) sum[first][c] += sum[first + m][c];
+    __syncthreads();
+  }
+  if (threadIdx.x < 8 && col < width) dweight[col] = (float)sum[0][c];
 }
 
 // Threads and vectors of a row: a row of nv vectors takes 16 threads up to 32
@@ -310,7 +363,8 @@ template <typename T, int V>
 hipError_t norm_of(const NormArgs& a, hipStream_t s) {
   const uint32_t rows = (uint32_t)a.q.lanes * (uint32_t)a.q.T;
   auto go = [&](auto G, auto U) {
-    const uint32_t blocks = std::min<uint32_t>(((uint64_t)rows * G + 255) / 256, MAX_BLOCKS);
+    // eight blocks a CU, which keep the weight in registers from row to row
+    const uint32_t blocks = std::min<uint32_t>(((uint64_t)rows * G + 255) / 256, 2048);
     if (a.out8.d)
       BOA_LAUNCH((norm_kernel<T, V, G, U, true>), blocks, 256, 0, s, a, rows);
     else
@@ -352,8 +406,8 @@ hipError_t norm_grad_of(const NormGradArgs& a, hipStream_t s) {
   if (!done) for_shape(sh, go);
   hipError_t e = hipGetLastError();
   if (e || !a.dweight) return e;
-  BOA_LAUNCH(norm_dweight_kernel, (a.width + 31) / 32, 1024, 0, s, (const float*)a.work,
-             (int)(blocks * (256 / sh.G)), a.width, a.dweight);
+  BOA_LAUNCH(norm_dweight_kernel, (a.width + 7) / 8, 1024, 0, s, (const float*)a.work,
+             (int)blocks, a.width, a.dweight);
   return hipGetLastError();
 }
 
@@ -381,7 +435,7 @@ size_t norm_grad_work(int64_t rows, int width) {
   int64_t n = 0;
   for (int v : {1, 4, 8}) {
     const Shape sh = shape_of((width + v - 1) / v);
-    n = std::max<int64_t>(n, (int64_t)grad_blocks(rows, sh.G) * (256 / sh.G));
+    n = std::max<int64_t>(n, grad_blocks(rows, sh.G));
   }
   return (size_t)n * width * 4;
 }

@@ -13,6 +13,26 @@ inline bool rows_by_16(const void* d, int64_t lane, int64_t row, int width, int 
   return ((uintptr_t)d & 15) == 0 && lane % v == 0 && row % v == 0 && width % v == 0;
 }
 
+// x with f applied over the 16 lanes of a row of lanes, and over all 64
+template <typename F>
+__device__ __forceinline__ float over16(float x, F f) {
+  x = f(x, dpp_move<DPP_XOR1>(x));
+  x = f(x, dpp_move<DPP_XOR2>(x));
+  x = f(x, dpp_move<DPP_HALF_MIRROR>(x));
+  return f(x, dpp_move<DPP_MIRROR>(x));
+}
+template <typename F>
+__device__ __forceinline__ float over64(float x, F f) {
+  x = over16(x, f);
+  const auto a = __builtin_amdgcn_permlane16_swap(f2u(x), f2u(x), false, false);
+  x = f(u2f(a[0]), u2f(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
+  return f(u2f(b[0]), u2f(b[1]));
+}
+struct Sum {
+  __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+
 // ---- norm and rows in 8 bits (norm.hip) ------------------------------------
 struct NormArgs {
   Seqs q;

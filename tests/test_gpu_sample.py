@@ -43,7 +43,7 @@ def choose(x, u, temp, k, p, m):
 
 HOW = [(1.0, 0, 1.0, 0.0), (0.7, 40, 0.9, 0.02), (0.0, 5, 0.5, 0.0), (2.5, 1, 1.0, 0.0),
        (1.3, 0, 0.3, 0.0), (1.0, 0, 0.0, 0.0), (0.9, 0, 1.0, 0.3), (0.1, 256, 0.99, 1.0),
-       (5.0, 3.5, 2.0, -1.0), (1.0, 1000, 1.5, 0.0)]
+       (5.0, 3.5, 2.0, -1.0), (1.0, 1000, 1.5, 0.0), (1.0, 0, 1.0, 1.5), (3.0, 200, 0.999, 1e-3)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

@@ -6,25 +6,30 @@
 // (delta_step_kernel).  Many are taken in chunks of 64: with sums G of the log
 // decays within the chunk, D_ij = e^(G_i - G_j) and the chunk's first state S,
 //   A_ij = beta_i D_ij k_i.k_j (j < i)       T = (1 + A)^-1
-//   W = T diag(beta e^G) K      U = T diag(beta) V      N = U - W S      (the e, times beta)
-//   P_ij = scale D_ij q_i.k_j (j <= i)       O = scale diag(e^G) Q S + P N
-//   S' = e^G_64 S + sum_j e^(G_64 - G_j) k_j N_j^T
-// W, U and T belong to the chunk alone (prep kernel, all chunks at once); the
-// states follow one from the other, two products a chunk (chain kernel, the
-// columns of S shared out); then O, all chunks at once (out kernel).
+//   P_ij = scale D_ij q_i.k_j (j <= i)
+//   R = diag(beta) (V - diag(e^G) K S)       N = T R      (the e, times beta)
+//   O = scale diag(e^G) Q S + P N            S' = e^G_64 S + sum_j e^(G_64 - G_j) k_j N_j^T
+// T and P belong to the chunk alone (prep kernel, all chunks at once).  The rest
+// follows the states from chunk to chunk (chain kernel), but no column of S, N
+// and O needs another: a wave takes 16 columns and keeps them in registers from
+// product to product.
 // The gradient, with dO and the gradient dS of the chunk's last state:
 //   dN = P^T dO + diag(e^(G_64 - G)) K dS                   dR = T^T dN
-//   dS_before = e^G_64 dS + scale (diag(e^G) Q)^T dO - W^T dN
+//   dS_before = e^G_64 dS + scale Q^T diag(e^G) dO - K^T diag(beta e^G) dR
+// is a chain of the same kind, backwards, and
 //   dV = diag(beta) dR      dA = -dR N^T (j < i)      dP = dO N^T (j <= i)
-// and dQ, dK, dbeta, dG from these, the products dO S^T, dR S^T, N dS^T and
-// the elementwise rules.  Again what belongs to one chunk alone runs for all
-// chunks at once, around a chain for dS.
+// and dQ, dK, dbeta, dG, from these, the products dO S^T, dR S^T, N dS^T and the
+// elementwise rules, again belong to one chunk (last kernel).
 //
 // T comes from substitution within blocks of 16 and products between them, so
 // keys that are equal or nearly so (the same byte again and again) do not
 // spoil it.  Sums of log decays and their differences are held in 64 bits: a
 // decay of -1e4 forgets all that is before it and leaves what is after it
-// exact.  All else is fp32: products on the fp32 MFMA.
+// exact.  All else has fp32's precision.  For fp32 rows the products are on the
+// fp32 MFMA; for bf16 rows on the bf16 MFMA, sixteen times as fast, where an
+// fp32 operand is the sum of three bf16 ones (24 bits) and products of parts
+// below 2^-24 are left out: three products against rows, which are exact, six
+// between fp32 operands.
 #include <algorithm>
 
 #include "predictor_ops.h"
@@ -34,9 +39,12 @@ namespace boa {
 namespace {
 
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr int C = 64;          // positions of a chunk
-constexpr int CP = C + 4;      // pitch of a [64][64] tile in LDS
+constexpr int CP = C + 4;      // pitch of a [64][64] tile of floats in LDS
 constexpr float EPS = 1e-6f;   // under the root of a row's length
+constexpr f4 ZERO = {0.0f, 0.0f, 0.0f, 0.0f};
 
 // e^x for x in 64 bits, to an fp32's precision whatever its size
 __device__ __forceinline__ float exp_of(double x) {
@@ -62,135 +70,240 @@ __device__ __forceinline__ void st1(T* p, float x) {
   if constexpr (sizeof(T) == 4) *p = x;
   else *p = f32_to_bf16(x);
 }
-// four elements from column c on of a row of d, zero past d; wide: in one piece
+// four elements from column c on of a row of d, zero past d; wide: in one piece.
+// No branch (a load in one would wait for those before it): what is past d reads
+// the row's first or last element.
 template <typename T>
 __device__ __forceinline__ f4 ld4(const T* row, int c, int d, bool wide) {
-  f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  f4 v;
   if (wide) {
-    if (c < d) {
-      if constexpr (sizeof(T) == 4) {
-        v = *reinterpret_cast<const f4*>(row + c);
-      } else {
-        const uint2 w = *reinterpret_cast<const uint2*>(row + c);
-        v = f4{u2f(w.x << 16), u2f(w.x & 0xFFFF0000u), u2f(w.y << 16), u2f(w.y & 0xFFFF0000u)};
-      }
+    const T* p = row + (c < d ? c : 0);
+    if constexpr (sizeof(T) == 4) {
+      v = *reinterpret_cast<const f4*>(p);
+    } else {
+      const u2 w = *reinterpret_cast<const u2*>(p);
+      v = f4{u2f(w[0] << 16), u2f(w[0] & 0xFFFF0000u), u2f(w[1] << 16), u2f(w[1] & 0xFFFF0000u)};
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (c + i < d) v[i] = ld1(row + c + i);
+    for (int i = 0; i < 4; ++i) v[i] = ld1(row + min(c + i, d - 1));
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = c + i < d ? v[i] : 0.0f;
   return v;
 }
-
-// sum over the 16 lanes of a row of lanes, in each of them
-__device__ __forceinline__ float sum16(float x) {
-  x = dpp_add<DPP_XOR1>(x);
-  x = dpp_add<DPP_XOR2>(x);
-  x = dpp_add<DPP_HALF_MIRROR>(x);
-  return dpp_add<DPP_MIRROR>(x);
+template <typename T>
+__device__ __forceinline__ void st4(T* row, int c, int d, bool wide, f4 v) {
+  if (wide) {
+    if (c >= d) return;
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<f4*>(row + c) = v;
+    else *reinterpret_cast<u2*>(row + c) = u2{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i < d) st1(row + c + i, v[i]);
+  }
 }
 
-// ---- products of tiles on v_mfma_f32_16x16x4f32 ----------------------------
-// Lane (i = lane % 16, g = lane / 16) holds of A row i, of B column i and of
-// the result rows 4 g + r of column i.  Of every 16 of k the MFMA's step j
-// takes k = 4 g + j, so an operand with k along its rows is read four at once.
-// a(kk) and b(kk, n) give those four of the kk-th 16.
-template <int NT, int K, typename A, typename B>
-__device__ __forceinline__ void mma(f4 (&acc)[NT], A a, B b) {
+// ---- products --------------------------------------------------------------
+// Lane (i = lane % 16, g = lane / 16) holds of a left operand row i, of a right
+// one column i, of a 16 x 16 result rows 4 g .. 4 g + 3 of column i.  Of every 32
+// of k it holds eight, 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3: then two
+// results, one under the other, are the right operand of the next product as
+// they lie.  (Which k a slot stands for matters to neither MFMA, as long as both
+// operands agree.)
+//
+// An operand's eight values are P pieces of 16 bytes.  bf16 rows: one piece,
+// exact; fp32 values beside them: three, x = hi + mid + lo in bf16.  fp32 rows
+// and values beside them: two pieces of four floats.
+template <int P>
+struct Frag {
+  u4 p[P];
+};
+template <typename T>
+struct Mode;
+template <>
+struct Mode<uint16_t> {
+  static constexpr int ROWS = 1, FULL = 3;
+};
+template <>
+struct Mode<float> {
+  static constexpr int ROWS = 2, FULL = 2;
+};
+
+// one of three parts of a pair of floats; x and y keep the rest
+__device__ __forceinline__ uint32_t part_of(float& x, float& y) {
+  const uint32_t h = bf16_pair(x, y);
+  x -= u2f(h << 16);
+  y -= u2f(h & 0xFFFF0000u);
+  return h;
+}
+template <typename T>
+__device__ __forceinline__ Frag<Mode<T>::FULL> full(f4 a, f4 b) {
+  Frag<Mode<T>::FULL> r;
+  if constexpr (sizeof(T) == 4) {
+    r.p[0] = __builtin_bit_cast(u4, a);
+    r.p[1] = __builtin_bit_cast(u4, b);
+  } else {
 #pragma unroll
-  for (int kk = 0; kk < K / 16; ++kk) {
-    const f4 x = a(kk);
+    for (int p = 0; p < 3; ++p) {
+      float x0 = a[0], x1 = a[1], x2 = a[2], x3 = a[3], y0 = b[0], y1 = b[1], y2 = b[2], y3 = b[3];
+      r.p[p] = u4{part_of(x0, x1), part_of(x2, x3), part_of(y0, y1), part_of(y2, y3)};
+      a = f4{x0, x1, x2, x3};
+      b = f4{y0, y1, y2, y3};
+    }
+  }
+  return r;
+}
+// of values that rows hold exactly
+template <typename T>
+__device__ __forceinline__ Frag<Mode<T>::ROWS> rows_of(f4 a, f4 b) {
+  Frag<Mode<T>::ROWS> r;
+  if constexpr (sizeof(T) == 4) {
+    r.p[0] = __builtin_bit_cast(u4, a);
+    r.p[1] = __builtin_bit_cast(u4, b);
+  } else {
+    r.p[0] = u4{bf16_pair(a[0], a[1]), bf16_pair(a[2], a[3]), bf16_pair(b[0], b[1]),
+                bf16_pair(b[2], b[3])};
+  }
+  return r;
+}
+template <typename T, int PA, int PB>
+__device__ __forceinline__ void mma(f4& acc, const Frag<PA>& a, const Frag<PB>& b) {
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const f4 y = b(kk, n);
+    for (int h = 0; h < 2; ++h) {
+      const f4 x = __builtin_bit_cast(f4, a.p[h]), y = __builtin_bit_cast(f4, b.p[h]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], acc[n], 0, 0, 0);
+      for (int e = 0; e < 4; ++e)
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], acc, 0, 0, 0);
+    }
+  } else {
+    typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+    // the small parts first
+#pragma unroll
+    for (int s = 2; s >= 0; --s)
+#pragma unroll
+      for (int i = 0; i < PA; ++i)
+        if (s - i >= 0 && s - i < PB)
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a.p[i]),
+                                                        __builtin_bit_cast(b8, b.p[s - i]), acc, 0,
+                                                        0, 0);
+  }
+}
+
+// ---- operands in LDS -------------------------------------------------------
+// A block is 16 rows x 32 of k as the lanes hold it, piece by piece, 16 bytes a
+// lane; a tile of U blocks across.  The lanes of g are turned by 4 g, so that
+// writes of neighbouring k fall into different banks.
+__device__ __forceinline__ int slot_of(int i, int g) { return (i ^ (g << 2)) + 16 * g; }
+template <int P>
+__device__ __forceinline__ Frag<P> get(const u4* tile, int block, int slot) {
+  Frag<P> r;
+#pragma unroll
+  for (int p = 0; p < P; ++p) r.p[p] = tile[(block * P + p) * 64 + slot];
+  return r;
+}
+// four values of one row, k .. k + 3 (k a multiple of 4)
+template <typename T, int P>
+__device__ __forceinline__ void put(u4* tile, int U, int row, int k, f4 v) {
+  const int block = row / 16 * U + k / 32, h = k / 16 % 2, slot = slot_of(row % 16, k / 4 % 4);
+  if constexpr (sizeof(T) == 4) {
+    tile[(block * 2 + h) * 64 + slot] = __builtin_bit_cast(u4, v);
+  } else {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      float a = v[0], b = v[1], c = v[2], d = v[3];
+      const u2 w = {part_of(a, b), part_of(c, d)};
+      reinterpret_cast<u2*>(tile + (block * P + p) * 64 + slot)[h] = w;
+      v = f4{a, b, c, d};
     }
   }
 }
-// of a tile with k along its rows: rows i0 + i, k from 16 kk + 4 g
-__device__ __forceinline__ f4 along(const float* t, int pitch, int i0, int kk, int lane) {
-  return *reinterpret_cast<const f4*>(t + (i0 + lane % 16) * pitch + kk * 16 + lane / 16 * 4);
-}
-// of a tile with k across its rows: column i0 + i of rows 16 kk + 4 g ..
-__device__ __forceinline__ f4 across(const float* t, int pitch, int i0, int kk, int lane) {
-  const float* p = t + (kk * 16 + lane / 16 * 4) * pitch + i0 + lane % 16;
-  return f4{p[0], p[pitch], p[2 * pitch], p[3 * pitch]};
-}
 
-// ---- what belongs to a (lane, value head, chunk) ---------------------------
-// Everything that passes between the kernels lies in one record per chunk,
-// chunks of a (lane, value head) one after the other: S [DK][DV], N [64][DV]
-// (U at first), W [64][DK], T [64][64].
-template <int DK, int DV>
-struct Record {
-  static constexpr int S = 0, N = DK * DV, W = N + C * DV, T = W + C * DK, SIZE = T + C * C;
+// Four rows x four columns of a chunk's rows at a time, a thread: taken from
+// memory, and put as rows (k along them) or across (k over the positions).
+struct Four {
+  f4 v[4];  // v[e]: row 4 pg + e
 };
-// and of the gradient: dS [DK][DV], dN [64][DV]
-template <int DK, int DV>
-struct GradRecord {
-  static constexpr int S = 0, N = DK * DV, SIZE = N + C * DV;
-};
+__device__ __forceinline__ Four turned(const Four& x) {
+  Four t;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) t.v[c] = f4{x.v[0][c], x.v[1][c], x.v[2][c], x.v[3][c]};
+  return t;
+}
+template <typename T, int P>
+__device__ __forceinline__ void put_rows(u4* tile, int U, int row, int k, const Four& x) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) put<T, P>(tile, U, row + e, k, x.v[e]);
+}
 
 struct Place {
-  int l, h, c;     // lane, value head, chunk
+  int l, h, c;     // lane, head, chunk
   int n;           // positions of the chunk within the lane's length
 };
-__device__ __forceinline__ Place place_of(const DeltaArgs& a, uint64_t b, int heads, int chunks) {
-  Place p;
-  p.c = (int)(b % chunks);
-  const uint64_t lh = b / chunks;
-  p.h = (int)(lh % heads);
-  p.l = (int)(lh / heads);
-  const int left = seq_len(a.q, p.l) - p.c * C;
-  p.n = left < 0 ? 0 : (left < C ? left : C);
-  return p;
+__device__ __forceinline__ int within(int len, int c) {
+  const int left = len - c * C;
+  return left < 0 ? 0 : (left < C ? left : C);
+}
+// the first element of a chunk's row for a head of d columns
+template <typename T>
+__device__ __forceinline__ T* row_at(const RowsIn& r, const Place& p, int h, int d, int row) {
+  return (T*)r.d + p.l * r.lane + (int64_t)(p.c * C + row) * r.row + (int64_t)h * d;
+}
+template <typename T>
+__device__ __forceinline__ T* row_at(const RowsOut& r, const Place& p, int h, int d, int row) {
+  return (T*)r.d + p.l * r.lane + (int64_t)(p.c * C + row) * r.row + (int64_t)h * d;
+}
+// rows pos .. pos + 3, columns col .. col + 3; zero past the chunk's positions
+// (p.n of them, one at least) and past d
+template <typename T>
+__device__ __forceinline__ Four four_of(const RowsIn& r, const Place& p, int h, int d, bool wide,
+                                        int pos, int col) {
+  Four x;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    x.v[e] = ld4(row_at<const T>(r, p, h, d, min(pos + e, p.n - 1)), col, d, wide);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (pos + e >= p.n) x.v[e] = ZERO;
+  return x;
 }
 
-// a tile of the chunk's rows, heads d wide at head h, into LDS; zero elsewhere
-template <typename T, int D>
-__device__ __forceinline__ void bring(float* t, const RowsIn& r, const Place& p, int h, int d,
-                                      bool wide) {
-  constexpr int PITCH = D + 4;
-  for (int i = threadIdx.x; i < C * D / 4; i += blockDim.x) {
-    const int row = i / (D / 4), col = i % (D / 4) * 4;
-    f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (row < p.n)
-      v = ld4((const T*)r.d + p.l * r.lane + (int64_t)(p.c * C + row) * r.row + (int64_t)h * d,
-              col, d, wide);
-    *reinterpret_cast<f4*>(t + row * PITCH + col) = v;
-  }
+// ---- what passes between the kernels, of a (lane, value head, chunk) -------
+// T and P, lower triangles of 64 x 64, as operands: six blocks each (row tile t,
+// 32 of k u: t = 0, 1: u = 0; t = 2, 3: u = 0, 1), transposed for the gradient
+// (t = 0, 1: u = 0, 1; t = 2, 3: u = 1).
+constexpr int TRI = 6;
+template <bool TRANS>
+__device__ __forceinline__ constexpr int tri_block(int t, int u) {
+  return TRANS ? (t < 2 ? 2 * t + u : t + 2) : (t < 2 ? t : 2 * t - 2 + u);
 }
-// ... of floats [64][D] that lie one after the other
-template <int D>
-__device__ __forceinline__ void bring_dense(float* t, const float* from) {
-  constexpr int PITCH = D + 4;
-  for (int i = threadIdx.x; i < C * D / 4; i += blockDim.x)
-    *reinterpret_cast<f4*>(t + i / (D / 4) * PITCH + i % (D / 4) * 4) =
-        *reinterpret_cast<const f4*>(from + i * 4);
+template <bool TRANS>
+__device__ __forceinline__ constexpr bool tri_has(int t, int u) {
+  return TRANS ? (t < 2 || u == 1) : (t >= 2 || u == 0);
 }
+// Coefficients of the rows, floats: beta; beta e^G / |k|; e^(G_64 - G) / |k|;
+// scale e^G / |q|; then e^G_64.
+constexpr int COEF = 4 * C + 4;
+template <typename T>
+constexpr int IMAGE = 2 * TRI * Mode<T>::FULL * 64;  // 16-byte pieces of T and P
+constexpr int64_t PREP_BYTES = 2 * TRI * 3 * 1024 + COEF * 4;  // the larger of the types'
 
-// the chunk's coefficients, by the block's first wave
-struct Coef {
-  double sum[C];   // G
+// the block's sums of log decays and betas, by its first wave
+struct Decays {
+  double sum[C];  // G
   float beta[C];
   float since[C];  // e^G
   float left[C];   // e^(G_64 - G)
-  float rk[C];     // 1 / length of k (1 where rows are taken raw)
-  float rq[C];     // scale / length of q
 };
-__device__ __forceinline__ void decays_of(Coef& s, const DeltaArgs& a, const Place& p) {
+__device__ __forceinline__ void decays_of(Decays& s, const DeltaArgs& a, const Place& p) {
   const int i = threadIdx.x;
   if (i >= C) return;
-  double g = 0.0;
-  float beta = 0.0f;
-  if (i < p.n) {
-    const int64_t t = p.c * C + i;
-    g = log_decay(*((const float*)a.g.d + p.l * a.g.lane + t * a.g.row + p.h));
-    beta = *((const float*)a.beta.d + p.l * a.beta.lane + t * a.beta.row + p.h);
-  }
+  const int64_t t = p.c * C + min(i, p.n - 1);
+  double g = log_decay(*((const float*)a.g.d + p.l * a.g.lane + t * a.g.row + p.h));
+  float beta = *((const float*)a.beta.d + p.l * a.beta.lane + t * a.beta.row + p.h);
+  if (i >= p.n) g = 0.0, beta = 0.0f;
 #pragma unroll
   for (int m = 1; m < C; m *= 2) {
     const double y = __shfl_up(g, m);
@@ -202,63 +315,94 @@ __device__ __forceinline__ void decays_of(Coef& s, const DeltaArgs& a, const Pla
   s.since[i] = exp_of(g);
   s.left[i] = exp_of(all - g);
 }
-// 1 / length of the tile's 64 rows, four threads a row; needs 256 threads
-template <int D>
-__device__ __forceinline__ void lengths_of(float* r, const float* t, bool unit, float scale) {
-  constexpr int PITCH = D + 4;
-  const int row = threadIdx.x / 4, part = threadIdx.x % 4;
-  float s = 0.0f;
-  if (unit) {
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      const f4 v = *reinterpret_cast<const f4*>(t + row * PITCH + (i * 4 + part) * 4);
-      s += v[0] * v[0] + v[1] * v[1] + v[2] * v[2] + v[3] * v[3];
-    }
-    s = dpp_add<DPP_XOR1>(s);
-    s = dpp_add<DPP_XOR2>(s);
-    s = scale / __builtin_sqrtf(s + EPS);
-  } else {
-    s = scale;
-  }
-  if (part == 0) r[row] = s;
+
+// ---- prep ------------------------------------------------------------------
+// products of [64][64] tiles of floats on the fp32 MFMA, for T alone: rows i0 +
+// i, k from 16 kk + 4 g along the rows or across them
+__device__ __forceinline__ f4 along(const float* t, int i0, int kk, int lane) {
+  return *reinterpret_cast<const f4*>(t + (i0 + lane % 16) * CP + kk * 16 + lane / 16 * 4);
 }
-__device__ __forceinline__ float between(const Coef& s, int i, int j) {
-  return exp_of(s.sum[i] - s.sum[j]);
+__device__ __forceinline__ f4 across(const float* t, int i0, int kk, int lane) {
+  const float* p = t + (kk * 16 + lane / 16 * 4) * CP + i0 + lane % 16;
+  return f4{p[0], p[CP], p[2 * CP], p[3 * CP]};
+}
+__device__ __forceinline__ void mma16(f4& acc, f4 x, f4 y) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], acc, 0, 0, 0);
 }
 
-// ---- prep: W, U and T of every chunk ---------------------------------------
-template <typename T, int DK, int DV>
-__global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a, float* rec, int chunks,
-                                                         uint64_t blocks, bool wide) {
-  using R = Record<DK, DV>;
-  constexpr int D = DK > DV ? DK : DV;
-  __shared__ __align__(16) float x[C * (D + 4)];
+// A block per (lane, value head, chunk): T and P as the chain reads them, and
+// the coefficients.
+template <typename T, int DK, bool TRANS>
+__global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a, unsigned char* prep,
+                                                         int chunks, uint64_t blocks, bool wide) {
+  using M = Mode<T>;
+  constexpr int U = DK / 32, P = M::ROWS;
+  __shared__ u4 ka[4 * U * P * 64], qa[4 * U * P * 64];
   __shared__ __align__(16) float am[C * CP], tm[C * CP];
-  __shared__ Coef s;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane % 16, g4 = lane / 16 * 4;
+  __shared__ float ssk[C], ssq[C], rk[C], rq[C];
+  __shared__ Decays s;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i16 = lane % 16, g = lane / 16, g4 = 4 * g, sl = slot_of(i16, g);
   for (uint64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const Place p = place_of(a, b, a.HV, chunks);
+    Place p;
+    p.c = (int)(b % chunks);
+    p.h = (int)(b / chunks % a.HV);
+    p.l = (int)(b / chunks / a.HV);
+    p.n = within(seq_len(a.q, p.l), p.c);
     if (!p.n) continue;
+    const int kh = p.h / (a.HV / a.H);
+    Four k[DK / 64], q[DK / 64];
+#pragma unroll
+    for (int i = 0; i < DK / 64; ++i) {
+      k[i] = four_of<T>(a.k, p, kh, a.dk, wide, tid / 16 * 4, i * 64 + tid % 16 * 4);
+      q[i] = four_of<T>(a.qr, p, kh, a.dk, wide, tid / 16 * 4, i * 64 + tid % 16 * 4);
+    }
     __syncthreads();
-    bring<T, DK>(x, a.k, p, p.h / (a.HV / a.H), a.dk, wide);
     decays_of(s, a, p);
+#pragma unroll
+    for (int i = 0; i < DK / 64; ++i) {
+      put_rows<T, P>(ka, U, tid / 16 * 4, i * 64 + tid % 16 * 4, k[i]);
+      put_rows<T, P>(qa, U, tid / 16 * 4, i * 64 + tid % 16 * 4, q[i]);
+    }
+    for (int i = tid; i < C * CP; i += 256) tm[i] = 0.0f;
     __syncthreads();
-    lengths_of<DK>(s.rk, x, a.unit, 1.0f);
-    for (int i = threadIdx.x; i < C * C; i += 256) tm[i / C * CP + i % C] = 0.0f;
-    __syncthreads();
-    {
-      f4 acc[4] = {};
-      mma<4, DK>(acc, [&](int kk) { return along(x, DK + 4, wave * 16, kk, lane); },
-                 [&](int kk, int n) { return along(x, DK + 4, n * 16, kk, lane); });
+    // this wave's 16 rows of K K^T and Q K^T up to the diagonal; Q Q^T for the
+    // lengths, as K K^T's diagonal has those of k
+    f4 kk[4] = {}, qk[4] = {}, qq = ZERO;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const Frag<P> x = get<P>(ka, wave * U + u, sl), y = get<P>(qa, wave * U + u, sl);
+      mma<T>(qq, y, y);
 #pragma unroll
       for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = wave * 16 + g4 + r, j = n * 16 + i16;
-          am[i * CP + j] =
-              j < i ? acc[n][r] * (s.beta[i] * s.rk[i] * s.rk[j] * between(s, i, j)) : 0.0f;
+        if (n <= wave) {
+          const Frag<P> z = get<P>(ka, n * U + u, sl);
+          mma<T>(kk[n], x, z);
+          mma<T>(qk[n], y, z);
         }
     }
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (n == wave && g4 + r == i16) ssk[wave * 16 + i16] = kk[n][r], ssq[wave * 16 + i16] = qq[r];
+    __syncthreads();
+    if (tid < C) {
+      rk[tid] = a.unit ? 1.0f / __builtin_sqrtf(ssk[tid] + EPS) : 1.0f;
+      rq[tid] = a.unit ? a.scale / __builtin_sqrtf(ssq[tid] + EPS) : a.scale;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = wave * 16 + g4 + r, j = n * 16 + i16;
+        float d = 0.0f;
+        if (n <= wave && j <= i) d = exp_of(s.sum[i] - s.sum[j]);
+        am[i * CP + j] = n <= wave && j < i ? kk[n][r] * (s.beta[i] * rk[i] * rk[j] * d) : 0.0f;
+        qk[n][r] = n <= wave && j <= i ? qk[n][r] * (rq[i] * rk[j] * d) : 0.0f;
+      }
     __syncthreads();
     // the diagonal blocks of T by substitution, a column in each of 16 lanes
     if (lane < 16) {
@@ -278,612 +422,686 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a, floa
     // product's result lies as the next one's right operand
     if (wave < 2) {
       const int o = wave * 32;
-      f4 at[1] = {}, t21[1] = {};
-      mma<1, 16>(at, [&](int kk) { return along(am + o, CP, o + 16, kk, lane); },
-                 [&](int kk, int) { return across(tm + o * CP + o, CP, 0, kk, lane); });
-      mma<1, 16>(t21, [&](int kk) { return along(tm + o + 16, CP, o + 16, kk, lane); },
-                 [&](int, int) { return at[0]; });
+      f4 at = ZERO, t21 = ZERO;
+      mma16(at, along(am + o, o + 16, 0, lane), across(tm + o * CP + o, 0, 0, lane));
+      mma16(t21, along(tm + o + 16, o + 16, 0, lane), at);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) tm[(o + 16 + g4 + r) * CP + o + i16] = -t21[0][r];
+      for (int r = 0; r < 4; ++r) tm[(o + 16 + g4 + r) * CP + o + i16] = -t21[r];
     }
     __syncthreads();
     {
       const int ri = 32 + wave / 2 * 16, cj = wave % 2 * 16;
-      f4 at[2][1] = {}, t21[1] = {};
+      f4 t21 = ZERO;
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
-        mma<1, 32>(at[m], [&](int kk) { return along(am, CP, 32 + m * 16, kk, lane); },
-                   [&](int kk, int) { return across(tm, CP, cj, kk, lane); });
-      mma<1, 32>(t21, [&](int kk) { return along(tm + 32, CP, ri, kk, lane); },
-                 [&](int kk, int) { return at[kk][0]; });
+      for (int m = 0; m < 2; ++m) {
+        f4 at = ZERO;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) tm[(ri + g4 + r) * CP + cj + i16] = -t21[0][r];
+        for (int kk2 = 0; kk2 < 2; ++kk2)
+          mma16(at, along(am, 32 + m * 16, kk2, lane), across(tm, cj, kk2, lane));
+        mma16(t21, along(tm + 32, ri, m, lane), at);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) tm[(ri + g4 + r) * CP + cj + i16] = -t21[r];
     }
+    __syncthreads();  // am has been read: P takes its place
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) am[(wave * 16 + g4 + r) * CP + n * 16 + i16] = qk[n][r];
     __syncthreads();
-    float* out = rec + b * R::SIZE;
-    if (a.saved)
-      for (int i = threadIdx.x; i < C * C / 4; i += 256)
-        *reinterpret_cast<f4*>(out + R::T + i * 4) =
-            *reinterpret_cast<const f4*>(tm + i / (C / 4) * CP + i % (C / 4) * 4);
-    {
-      f4 acc[DK / 16] = {};
-      mma<DK / 16, C>(
-          acc,
-          [&](int kk) {
-            f4 v = along(tm, CP, wave * 16, kk, lane);
+    unsigned char* at = prep + b * PREP_BYTES;
+    u4* image = reinterpret_cast<u4*>(at);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int m = kk * 16 + g4 + j;
-              v[j] *= s.beta[m] * s.since[m] * s.rk[m];
-            }
-            return v;
-          },
-          [&](int kk, int n) { return across(x, DK + 4, n * 16, kk, lane); });
+    for (int it = 0; it < 3; ++it) {
+      const int job = it * 4 + wave;  // of T's and P's six blocks
+      const int block = job % TRI;
+      const float* m = job < TRI ? tm : am;
+      int t, u;
+      if (TRANS) t = block < 4 ? block / 2 : block - 2, u = block < 4 ? block % 2 : 1;
+      else t = block < 2 ? block : block / 2 + 1, u = block < 2 ? 0 : block % 2;
+      f4 lo, hi;
+      if (TRANS) {
+        lo = across(m, t * 16, 2 * u, lane);
+        hi = across(m, t * 16, 2 * u + 1, lane);
+      } else {
+        lo = along(m, t * 16, 2 * u, lane);
+        hi = along(m, t * 16, 2 * u + 1, lane);
+      }
+      const Frag<M::FULL> f = full<T>(lo, hi);
 #pragma unroll
-      for (int n = 0; n < DK / 16; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          out[R::W + (wave * 16 + g4 + r) * DK + n * 16 + i16] = acc[n][r];
+      for (int i = 0; i < M::FULL; ++i) image[(job * M::FULL + i) * 64 + sl] = f.p[i];
     }
-    __syncthreads();
-    bring<T, DV>(x, a.v, p, p.h, a.dv, wide);
-    __syncthreads();
-    {
-      f4 acc[DV / 16] = {};
-      mma<DV / 16, C>(
-          acc,
-          [&](int kk) {
-            f4 v = along(tm, CP, wave * 16, kk, lane);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] *= s.beta[kk * 16 + g4 + j];
-            return v;
-          },
-          [&](int kk, int n) { return across(x, DV + 4, n * 16, kk, lane); });
-#pragma unroll
-      for (int n = 0; n < DV / 16; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          out[R::N + (wave * 16 + g4 + r) * DV + n * 16 + i16] = acc[n][r];
+    float* coef = reinterpret_cast<float*>(at + PREP_BYTES - COEF * 4);
+    if (tid < C) {
+      coef[tid] = s.beta[tid];
+      coef[C + tid] = s.beta[tid] * s.since[tid] * rk[tid];
+      coef[2 * C + tid] = s.left[tid] * rk[tid];
+      coef[3 * C + tid] = rq[tid] * s.since[tid];
+      if (tid == C - 1) coef[4 * C] = s.since[tid];
     }
   }
 }
 
-// ---- chain: the states of a (lane, value head), BV columns a block ---------
-constexpr int BV = 32;
-template <typename T, int DK, int DV>
-__global__ __launch_bounds__(256) void delta_chain_kernel(const DeltaArgs a, float* rec, int chunks,
-                                                          uint64_t blocks, bool wide) {
-  using R = Record<DK, DV>;
-  constexpr int SP = BV + 4, ST = DK / 64;  // row tiles of S a wave
-  __shared__ __align__(16) float kt[C * (DK + 4)], sm[DK * SP], nm[C * SP];
-  __shared__ Coef s;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane % 16, g4 = lane / 16 * 4;
+// ---- chain -----------------------------------------------------------------
+// A block per (lane, value head, 64 columns), a wave 16 of them.  Of a chunk the
+// block's LDS holds K as rows and across, Q as rows (the gradient's chain: across),
+// T and P (there: transposed) and the coefficients; the next chunk's are under
+// way in registers.  The state, 16 columns of it, stays in the wave's registers.
+template <typename T, int DK, bool TRANS>
+struct ChainLds {
+  u4 ka[4 * (DK / 32) * Mode<T>::ROWS * 64], kt[DK / 16 * 2 * Mode<T>::ROWS * 64];
+  u4 q[4 * (DK / 32) * Mode<T>::ROWS * 64];  // rows, or across: as many blocks
+  u4 tri[IMAGE<T>];
+  float coef[COEF];
+};
+template <typename T, int DK>
+struct ChainNext {
+  static constexpr int IMG = (IMAGE<T> + 255) / 256;
+  Four k[DK / 64], q[DK / 64];
+  u4 img[IMG];
+  float coef[2];
+  __device__ __forceinline__ void load(const DeltaArgs& a, const unsigned char* prep, const Place& p,
+                                       int kh, bool wide) {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < IMG; ++i)
+      img[i] = reinterpret_cast<const u4*>(prep)[min(tid + 256 * i, IMAGE<T> - 1)];
+    const float* c = reinterpret_cast<const float*>(prep + PREP_BYTES - COEF * 4);
+    coef[0] = c[tid];
+    coef[1] = c[4 * C];
+#pragma unroll
+    for (int i = 0; i < DK / 64; ++i) {
+      k[i] = four_of<T>(a.k, p, kh, a.dk, wide, tid / 16 * 4, i * 64 + tid % 16 * 4);
+      q[i] = four_of<T>(a.qr, p, kh, a.dk, wide, tid / 16 * 4, i * 64 + tid % 16 * 4);
+    }
+  }
+  template <bool TRANS>
+  __device__ __forceinline__ void store(ChainLds<T, DK, TRANS>& s) const {
+    const int tid = threadIdx.x, pos = tid / 16 * 4;
+    constexpr int P = Mode<T>::ROWS;
+#pragma unroll
+    for (int i = 0; i < DK / 64; ++i) {
+      const int col = i * 64 + tid % 16 * 4;
+      put_rows<T, P>(s.ka, DK / 32, pos, col, k[i]);
+      put_rows<T, P>(s.kt, 2, col, pos, turned(k[i]));
+      if (TRANS) put_rows<T, P>(s.q, 2, col, pos, turned(q[i]));
+      else put_rows<T, P>(s.q, DK / 32, pos, col, q[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < IMG; ++i)
+      if (tid + 256 * i < IMAGE<T>) s.tri[tid + 256 * i] = img[i];
+    s.coef[tid] = coef[0];
+    if (tid == 0) s.coef[4 * C] = coef[1];
+  }
+};
+
+// rows 4 g .. of tile t of a [64] array
+__device__ __forceinline__ f4 four_rows(const float* c, int t, int g) {
+  return *reinterpret_cast<const f4*>(c + t * 16 + 4 * g);
+}
+
+template <typename T, int DK>
+__global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_chain_kernel(
+    const DeltaArgs a, const unsigned char* prep, float* rec, int chunks, int tiles,
+    uint64_t blocks, bool wide) {
+  using M = Mode<T>;
+  constexpr int U = DK / 32, MT = DK / 16, FULL = M::FULL, P = M::ROWS;
+  extern __shared__ __align__(16) unsigned char lds[];
+  ChainLds<T, DK, false>& s = *reinterpret_cast<ChainLds<T, DK, false>*>(lds);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i16 = lane % 16, g = lane / 16, sl = slot_of(i16, g);
   for (uint64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const int v0 = (int)(b % (DV / BV)) * BV;
-    const uint64_t lh = b / (DV / BV);
+    const uint64_t lh = b / tiles;
     Place p;
     p.h = (int)(lh % a.HV);
     p.l = (int)(lh / a.HV);
-    const int len = seq_len(a.q, p.l);
-    f4 st[ST][2];
+    const int kh = p.h / (a.HV / a.H), len = seq_len(a.q, p.l), last = (len + C - 1) / C;
+    const int v0 = (int)(b % tiles) * 64 + wave * 16, col = v0 + i16;
+    const bool mine = col < a.dv;
     const int64_t state = (int64_t)lh * a.dk * a.dv;
+    f4 st[MT];
 #pragma unroll
-    for (int m = 0; m < ST; ++m)
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = wave * (DK / 4) + m * 16 + g4 + r, j = v0 + n * 16 + i16;
-          st[m][n][r] = a.state_in && i < a.dk && j < a.dv
-                            ? a.state_in[state + (int64_t)i * a.dv + j] : 0.0f;
-        }
-    for (p.c = 0; p.c * C < len; ++p.c) {
-      p.n = min(C, len - p.c * C);
-      float* at = rec + (lh * chunks + p.c) * R::SIZE;
-      __syncthreads();
-      bring<T, DK>(kt, a.k, p, p.h / (a.HV / a.H), a.dk, wide);
-      decays_of(s, a, p);
-#pragma unroll
-      for (int m = 0; m < ST; ++m)
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int i = wave * (DK / 4) + m * 16 + g4 + r, j = n * 16 + i16;
-            sm[i * SP + j] = st[m][n][r];
-            at[R::S + i * DV + v0 + j] = st[m][n][r];
-          }
-      __syncthreads();
-      lengths_of<DK>(s.rk, kt, a.unit, 1.0f);
-      f4 acc[2];
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
+    for (int m = 0; m < MT; ++m) {
+      st[m] = ZERO;
+      if (a.state_in && mine)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          acc[n][r] = -at[R::N + (wave * 16 + g4 + r) * DV + v0 + n * 16 + i16];
-      mma<2, DK>(acc,
-                 [&](int kk) {
-                   return *reinterpret_cast<const f4*>(at + R::W + (wave * 16 + i16) * DK +
-                                                       kk * 16 + g4);
-                 },
-                 [&](int kk, int n) { return across(sm, SP, n * 16, kk, lane); });
-      __syncthreads();
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = wave * 16 + g4 + r, j = n * 16 + i16;
-          at[R::N + i * DV + v0 + j] = -acc[n][r];
-          nm[i * SP + j] = -acc[n][r] * (s.left[i] * s.rk[i]);
-        }
-      __syncthreads();
-      const float all = s.since[C - 1];
-#pragma unroll
-      for (int m = 0; m < ST; ++m) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n) st[m][n] *= all;
-        mma<2, C>(st[m],
-                  [&](int kk) {
-                    return across(kt, DK + 4, wave * (DK / 4) + m * 16, kk, lane);
-                  },
-                  [&](int kk, int n) { return across(nm, SP, n * 16, kk, lane); });
-      }
+          if (m * 16 + 4 * g + r < a.dk)
+            st[m][r] = a.state_in[state + (int64_t)(m * 16 + 4 * g + r) * a.dv + col];
     }
-    if (a.state_out) {
+    ChainNext<T, DK> next;
+    f4 v[4];
+    auto bring = [&](int c) {
+      p.c = c;
+      p.n = within(len, c);
+      next.load(a, prep + (lh * chunks + c) * PREP_BYTES, p, kh, wide);
 #pragma unroll
-      for (int m = 0; m < ST; ++m)
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int r = 0; r < 4; ++r)
+          v[t][r] = ld1(row_at<const T>(a.v, p, p.h, a.dv, min(t * 16 + 4 * g + r, p.n - 1)) +
+                        min(col, a.dv - 1));
+    };
+    if (last > 0) bring(0);
+    for (int c = 0; c < last; ++c) {
+      __syncthreads();
+      next.store(s);
+      f4 vc[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) vc[t][r] = mine ? v[t][r] : 0.0f;
+      const int n = p.n;
+      __syncthreads();
+      if (c + 1 < last) bring(c + 1);
+      if (v0 >= a.dv) continue;
+      float* at = rec ? rec + (lh * chunks + c) * (int64_t)(a.dv * (DK + C)) : nullptr;
+      if (rec && mine) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          *reinterpret_cast<f4*>(at + (int64_t)col * DK + m * 16 + 4 * g) = st[m];
+      }
+      f4 o[4], x[4];
+      {
+        Frag<FULL> sf[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) sf[u] = full<T>(st[2 * u], st[2 * u + 1]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          x[t] = o[t] = ZERO;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            mma<T>(x[t], get<P>(s.ka, t * U + u, sl), sf[u]);
+            mma<T>(o[t], get<P>(s.q, t * U + u, sl), sf[u]);
+          }
+        }
+      }
+      f4 nn[4];
+      {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          x[t] = four_rows(s.coef, t, g) * vc[t] - four_rows(s.coef + C, t, g) * x[t];
+        Frag<FULL> rf[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) rf[u] = full<T>(x[2 * u], x[2 * u + 1]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          nn[t] = ZERO;
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            if (tri_has<false>(t, u)) mma<T>(nn[t], get<FULL>(s.tri, tri_block<false>(t, u), sl), rf[u]);
+        }
+      }
+      if (rec && mine) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          *reinterpret_cast<f4*>(at + a.dv * DK + (int64_t)col * C + t * 16 + 4 * g) = nn[t];
+      }
+      {
+        Frag<FULL> nf[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) nf[u] = full<T>(nn[2 * u], nn[2 * u + 1]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          o[t] *= four_rows(s.coef + 3 * C, t, g);
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            if (tri_has<false>(t, u))
+              mma<T>(o[t], get<FULL>(s.tri, TRI + tri_block<false>(t, u), sl), nf[u]);
+        }
+        Place here = p;
+        here.c = c;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int i = wave * (DK / 4) + m * 16 + g4 + r, j = v0 + n * 16 + i16;
-            if (i < a.dk && j < a.dv) a.state_out[state + (int64_t)i * a.dv + j] = st[m][n][r];
+            const int row = t * 16 + 4 * g + r;
+            if (row < n && mine) st1(row_at<T>(a.out, here, p.h, a.dv, row) + col, o[t][r]);
           }
-    }
-  }
-}
-
-// P [64][64] into pm from the tiles of q and k
-template <int DK>
-__device__ __forceinline__ void scores(float* pm, const float* qt, const float* kt, const Coef& s,
-                                       int wave, int lane) {
-  f4 acc[4] = {};
-  mma<4, DK>(acc, [&](int kk) { return along(qt, DK + 4, wave * 16, kk, lane); },
-             [&](int kk, int n) { return along(kt, DK + 4, n * 16, kk, lane); });
-#pragma unroll
-  for (int n = 0; n < 4; ++n)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = wave * 16 + lane / 16 * 4 + r, j = n * 16 + lane % 16;
-      pm[i * CP + j] = j <= i ? acc[n][r] * (s.rq[i] * s.rk[j] * between(s, i, j)) : 0.0f;
-    }
-}
-
-// ---- out: O of every chunk ---------------------------------------------------
-template <typename T, int DK, int DV>
-__global__ __launch_bounds__(256) void delta_out_kernel(const DeltaArgs a, const float* rec,
-                                                        int chunks, uint64_t blocks, bool wide) {
-  using R = Record<DK, DV>;
-  constexpr int D = DK > DV ? DK : DV;
-  extern __shared__ __align__(16) float lds[];
-  float* qt = lds;                    // [64][DK + 4]
-  float* x = qt + C * (DK + 4);       // [64][D + 4]: k, then N, then 64 rows of S at a time
-  float* pm = x + C * (D + 4);        // [64][CP]
-  Coef& s = *reinterpret_cast<Coef*>(pm + C * CP);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane % 16, g4 = lane / 16 * 4;
-  for (uint64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const Place p = place_of(a, b, a.HV, chunks);
-    if (!p.n) continue;
-    const float* at = rec + b * R::SIZE;
-    const int kh = p.h / (a.HV / a.H);
-    __syncthreads();
-    bring<T, DK>(qt, a.qr, p, kh, a.dk, wide);
-    bring<T, DK>(x, a.k, p, kh, a.dk, wide);
-    decays_of(s, a, p);
-    __syncthreads();
-    lengths_of<DK>(s.rk, x, a.unit, 1.0f);
-    lengths_of<DK>(s.rq, qt, a.unit, a.scale);
-    __syncthreads();
-    scores<DK>(pm, qt, x, s, wave, lane);
-    __syncthreads();
-    f4 acc[DV / 16] = {};
-#pragma unroll
-    for (int part = 0; part < DK / 64; ++part) {
-      bring_dense<DV>(x, at + R::S + part * 64 * DV);
-      __syncthreads();
-      mma<DV / 16, 64>(acc,
-                       [&](int kk) { return along(qt + part * 64, DK + 4, wave * 16, kk, lane); },
-                       [&](int kk, int n) { return across(x, DV + 4, n * 16, kk, lane); });
-      __syncthreads();
-    }
-#pragma unroll
-    for (int n = 0; n < DV / 16; ++n)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = wave * 16 + g4 + r;
-        acc[n][r] *= s.rq[i] * s.since[i];
       }
-    bring_dense<DV>(x, at + R::N);
-    __syncthreads();
-    mma<DV / 16, C>(acc, [&](int kk) { return along(pm, CP, wave * 16, kk, lane); },
-                    [&](int kk, int n) { return across(x, DV + 4, n * 16, kk, lane); });
+      {
+        Frag<FULL> nf[2];
 #pragma unroll
-    for (int n = 0; n < DV / 16; ++n)
+        for (int u = 0; u < 2; ++u)
+          nf[u] = full<T>(nn[2 * u] * four_rows(s.coef + 2 * C, 2 * u, g),
+                          nn[2 * u + 1] * four_rows(s.coef + 2 * C, 2 * u + 1, g));
+        const float all = s.coef[4 * C];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = wave * 16 + g4 + r, j = n * 16 + i16;
-        if (i < p.n && j < a.dv)
-          st1((T*)a.out.d + p.l * a.out.lane + (int64_t)(p.c * C + i) * a.out.row +
-                  (int64_t)p.h * a.dv + j, acc[n][r]);
+        for (int m = 0; m < MT; ++m) {
+          st[m] *= all;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) mma<T>(st[m], get<P>(s.kt, m * 2 + u, sl), nf[u]);
+        }
       }
+    }
+    if (a.state_out && mine) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (m * 16 + 4 * g + r < a.dk)
+            a.state_out[state + (int64_t)(m * 16 + 4 * g + r) * a.dv + col] = st[m][r];
+    }
+    __syncthreads();
   }
 }
 
-// ---- the gradient's first part: P^T dO of every chunk ----------------------
-template <typename T, int DK, int DV>
-__global__ __launch_bounds__(256) void delta_grad_first_kernel(const DeltaGradArgs ga, float* grec,
-                                                               int chunks, uint64_t blocks,
-                                                               bool wide) {
-  using GR = GradRecord<DK, DV>;
-  constexpr int D = DK > DV ? DK : DV;
-  extern __shared__ __align__(16) float lds[];
+// The gradient's chain, from the last chunk to the first: dS and dR of every
+// chunk, both with a column of d_v after the other, as S and N are kept.
+template <typename T, int DK>
+__global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_chain_kernel(
+    const DeltaGradArgs ga, const unsigned char* prep, float* grec, int chunks, int tiles,
+    uint64_t blocks, bool wide) {
+  using M = Mode<T>;
+  constexpr int U = DK / 32, MT = DK / 16, FULL = M::FULL, P = M::ROWS;
+  extern __shared__ __align__(16) unsigned char lds[];
   const DeltaArgs& a = ga.f;
-  float* qt = lds;
-  float* x = qt + C * (DK + 4);
-  float* pm = x + C * (D + 4);
-  Coef& s = *reinterpret_cast<Coef*>(pm + C * CP);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane % 16, g4 = lane / 16 * 4;
+  ChainLds<T, DK, true>& s = *reinterpret_cast<ChainLds<T, DK, true>*>(lds);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i16 = lane % 16, g = lane / 16, sl = slot_of(i16, g);
   for (uint64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const Place p = place_of(a, b, a.HV, chunks);
-    if (!p.n) continue;
-    float* at = grec + b * GR::SIZE;
-    const int kh = p.h / (a.HV / a.H);
-    __syncthreads();
-    bring<T, DK>(qt, a.qr, p, kh, a.dk, wide);
-    bring<T, DK>(x, a.k, p, kh, a.dk, wide);
-    decays_of(s, a, p);
-    __syncthreads();
-    lengths_of<DK>(s.rk, x, a.unit, 1.0f);
-    lengths_of<DK>(s.rq, qt, a.unit, a.scale);
-    __syncthreads();
-    scores<DK>(pm, qt, x, s, wave, lane);
-    __syncthreads();
-    bring<T, DV>(x, ga.dout, p, p.h, a.dv, wide);
-    __syncthreads();
-    f4 acc[DV / 16] = {};
-    mma<DV / 16, C>(acc, [&](int kk) { return across(pm, CP, wave * 16, kk, lane); },
-                    [&](int kk, int n) { return across(x, DV + 4, n * 16, kk, lane); });
-#pragma unroll
-    for (int n = 0; n < DV / 16; ++n)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        at[GR::N + (wave * 16 + g4 + r) * DV + n * 16 + i16] = acc[n][r];
-  }
-}
-
-// ---- the gradient's chain: dS from the last chunk to the first -------------
-template <typename T, int DK, int DV>
-__global__ __launch_bounds__(256) void delta_grad_chain_kernel(const DeltaGradArgs ga,
-                                                               const float* rec, float* grec,
-                                                               int chunks, uint64_t blocks,
-                                                               bool wide) {
-  using R = Record<DK, DV>;
-  using GR = GradRecord<DK, DV>;
-  constexpr int SP = BV + 4, ST = DK / 64;
-  extern __shared__ __align__(16) float lds[];
-  const DeltaArgs& a = ga.f;
-  float* kt = lds;                    // [64][DK + 4]: k, then W
-  float* qt = kt + C * (DK + 4);      // [64][DK + 4]
-  float* sm = qt + C * (DK + 4);      // [DK][SP]: dS
-  float* om = sm + DK * SP;           // [64][SP]: dO
-  float* nm = om + C * SP;            // [64][SP]: dN
-  Coef& s = *reinterpret_cast<Coef*>(nm + C * SP);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane % 16, g4 = lane / 16 * 4;
-  for (uint64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const int v0 = (int)(b % (DV / BV)) * BV;
-    const uint64_t lh = b / (DV / BV);
+    const uint64_t lh = b / tiles;
     Place p;
     p.h = (int)(lh % a.HV);
     p.l = (int)(lh / a.HV);
-    const int kh = p.h / (a.HV / a.H);
-    const int len = seq_len(a.q, p.l);
-    f4 st[ST][2];
+    const int kh = p.h / (a.HV / a.H), len = seq_len(a.q, p.l), last = (len + C - 1) / C;
+    const int v0 = (int)(b % tiles) * 64 + wave * 16, col = v0 + i16;
+    const bool mine = col < a.dv;
     const int64_t state = (int64_t)lh * a.dk * a.dv;
+    f4 st[MT];
 #pragma unroll
-    for (int m = 0; m < ST; ++m)
+    for (int m = 0; m < MT; ++m) {
+      st[m] = ZERO;
+      if (ga.dstate_out && mine)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+        for (int r = 0; r < 4; ++r)
+          if (m * 16 + 4 * g + r < a.dk)
+            st[m][r] = ga.dstate_out[state + (int64_t)(m * 16 + 4 * g + r) * a.dv + col];
+    }
+    ChainNext<T, DK> next;
+    f4 o[4];
+    auto bring = [&](int c) {
+      p.c = c;
+      p.n = within(len, c);
+      next.load(a, prep + (lh * chunks + c) * PREP_BYTES, p, kh, wide);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = wave * (DK / 4) + m * 16 + g4 + r, j = v0 + n * 16 + i16;
-          st[m][n][r] = ga.dstate_out && i < a.dk && j < a.dv
-                            ? ga.dstate_out[state + (int64_t)i * a.dv + j] : 0.0f;
-        }
-    for (p.c = (len + C - 1) / C - 1; p.c >= 0; --p.c) {
-      p.n = min(C, len - p.c * C);
-      const float* at = rec + (lh * chunks + p.c) * R::SIZE;
-      float* gat = grec + (lh * chunks + p.c) * GR::SIZE;
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          o[t][r] = ld1(row_at<const T>(ga.dout, p, p.h, a.dv, min(t * 16 + 4 * g + r, p.n - 1)) +
+                        min(col, a.dv - 1));
+    };
+    if (last > 0) bring(last - 1);
+    for (int c = last - 1; c >= 0; --c) {
       __syncthreads();
-      bring<T, DK>(kt, a.k, p, kh, a.dk, wide);
-      bring<T, DK>(qt, a.qr, p, kh, a.dk, wide);
-      decays_of(s, a, p);
+      next.store(s);
+      f4 dout[4];
 #pragma unroll
-      for (int m = 0; m < ST; ++m)
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int i = wave * (DK / 4) + m * 16 + g4 + r, j = n * 16 + i16;
-            sm[i * SP + j] = st[m][n][r];
-            gat[GR::S + i * DV + v0 + j] = st[m][n][r];
-          }
+        for (int r = 0; r < 4; ++r)
+          dout[t][r] = mine && t * 16 + 4 * g + r < p.n ? o[t][r] : 0.0f;
       __syncthreads();
-      lengths_of<DK>(s.rk, kt, a.unit, 1.0f);
-      lengths_of<DK>(s.rq, qt, a.unit, a.scale);
-      __syncthreads();
-      for (int i = threadIdx.x; i < C * BV; i += 256) {
-        const int row = i / BV, col = v0 + i % BV;
-        float v = 0.0f;
-        if (row < p.n && col < a.dv)
-          v = ld1((const T*)ga.dout.d + p.l * ga.dout.lane +
-                  (int64_t)(p.c * C + row) * ga.dout.row + (int64_t)p.h * a.dv + col);
-        om[row * SP + i % BV] = v * (s.rq[row] * s.since[row]);
+      if (c > 0) bring(c - 1);
+      if (v0 >= a.dv) continue;
+      float* at = grec + (lh * chunks + c) * (int64_t)(a.dv * (DK + C));
+      if (mine) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          *reinterpret_cast<f4*>(at + (int64_t)col * DK + m * 16 + 4 * g) = st[m];
       }
-      f4 acc[2] = {};
-      mma<2, DK>(acc, [&](int kk) { return along(kt, DK + 4, wave * 16, kk, lane); },
-                 [&](int kk, int n) { return across(sm, SP, n * 16, kk, lane); });
+      f4 dn[4];
+      {
+        Frag<FULL> sf[U];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+        for (int u = 0; u < U; ++u) sf[u] = full<T>(st[2 * u], st[2 * u + 1]);
+        Frag<P> of[2];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = wave * 16 + g4 + r, j = n * 16 + i16;
-          float* d = gat + GR::N + i * DV + v0 + j;
-          const float v = *d + acc[n][r] * (s.left[i] * s.rk[i]);
-          *d = v;
-          nm[i * SP + j] = -v;
+        for (int u = 0; u < 2; ++u) of[u] = rows_of<T>(dout[2 * u], dout[2 * u + 1]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          dn[t] = ZERO;
+#pragma unroll
+          for (int u = 0; u < U; ++u) mma<T>(dn[t], get<P>(s.ka, t * U + u, sl), sf[u]);
+          dn[t] *= four_rows(s.coef + 2 * C, t, g);
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            if (tri_has<true>(t, u))
+              mma<T>(dn[t], get<FULL>(s.tri, TRI + tri_block<true>(t, u), sl), of[u]);
         }
-      __syncthreads();
-      bring_dense<DK>(kt, at + R::W);
-      __syncthreads();
-      const float all = s.since[C - 1];
+      }
+      f4 dr[4];
+      {
+        Frag<FULL> nf[2];
 #pragma unroll
-      for (int m = 0; m < ST; ++m) {
-        const int i0 = wave * (DK / 4) + m * 16;
+        for (int u = 0; u < 2; ++u) nf[u] = full<T>(dn[2 * u], dn[2 * u + 1]);
 #pragma unroll
-        for (int n = 0; n < 2; ++n) st[m][n] *= all;
-        mma<2, C>(st[m], [&](int kk) { return across(qt, DK + 4, i0, kk, lane); },
-                  [&](int kk, int n) { return across(om, SP, n * 16, kk, lane); });
-        mma<2, C>(st[m], [&](int kk) { return across(kt, DK + 4, i0, kk, lane); },
-                  [&](int kk, int n) { return across(nm, SP, n * 16, kk, lane); });
+        for (int t = 0; t < 4; ++t) {
+          dr[t] = ZERO;
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            if (tri_has<true>(t, u)) mma<T>(dr[t], get<FULL>(s.tri, tri_block<true>(t, u), sl), nf[u]);
+        }
+      }
+      if (mine) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          *reinterpret_cast<f4*>(at + a.dv * DK + (int64_t)col * C + t * 16 + 4 * g) = dr[t];
+      }
+      {
+        Frag<FULL> of[2], rf[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          of[u] = full<T>(dout[2 * u] * four_rows(s.coef + 3 * C, 2 * u, g),
+                          dout[2 * u + 1] * four_rows(s.coef + 3 * C, 2 * u + 1, g));
+          rf[u] = full<T>(dr[2 * u] * -four_rows(s.coef + C, 2 * u, g),
+                          dr[2 * u + 1] * -four_rows(s.coef + C, 2 * u + 1, g));
+        }
+        const float all = s.coef[4 * C];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          st[m] *= all;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            mma<T>(st[m], get<P>(s.q, m * 2 + u, sl), of[u]);
+            mma<T>(st[m], get<P>(s.kt, m * 2 + u, sl), rf[u]);
+          }
+        }
       }
     }
-    if (ga.dstate_in) {
+    if (ga.dstate_in && mine) {
 #pragma unroll
-      for (int m = 0; m < ST; ++m)
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int i = wave * (DK / 4) + m * 16 + g4 + r, j = v0 + n * 16 + i16;
-            if (i < a.dk && j < a.dv) ga.dstate_in[state + (int64_t)i * a.dv + j] = st[m][n][r];
-          }
+        for (int r = 0; r < 4; ++r)
+          if (m * 16 + 4 * g + r < a.dk)
+            ga.dstate_in[state + (int64_t)(m * 16 + 4 * g + r) * a.dv + col] = st[m][r];
     }
+    __syncthreads();
   }
 }
 
-// ---- the gradient's last part: the rows' gradients of every chunk ----------
-// A block takes a chunk of a head of k and all value heads that share it, so
-// that their gradients of q and k are summed in registers, in one order.
-template <typename T, int DK, int DV>
-__global__ __launch_bounds__(256) void delta_grad_last_kernel(const DeltaGradArgs ga,
-                                                              const float* rec, const float* grec,
-                                                              int chunks, uint64_t blocks,
-                                                              bool wide) {
-  using R = Record<DK, DV>;
-  using GR = GradRecord<DK, DV>;
-  constexpr int NK = DK / 16, NV = DV / 16;
-  extern __shared__ __align__(16) float lds[];
+// ---- the rows' gradients of a chunk ----------------------------------------
+// A block per (lane, head of k, chunk) takes all value heads that share the head,
+// a wave 16 of the positions, "own".  Products over d_v come 32 columns at a
+// time, N, dR, dO, S and dS as left operands in LDS and this wave's own rows of
+// them (the same pieces) as right ones:
+//   m < w:  dP^T, dA^T (rows j of tile m, column i own)      m > w:  dP, dA (rows i of tile m, column j own)
+// and both for the wave's own tile w; so sums over rows and over columns of dP P
+// and dA A stay within the wave, and what K and Q are multiplied with lies as the
+// right operand.  dQ^T and dK^T [d_k][own] leave as four neighbouring columns a lane.
+template <typename T, int DK>
+struct LastLds {
+  static constexpr int P = Mode<T>::ROWS, FULL = Mode<T>::FULL;
+  union {
+    struct {
+      u4 a[4 * (DK / 32) * P * 64], b[4 * (DK / 32) * P * 64];  // K, Q: rows; then across
+    } k;
+    struct {
+      u4 n[4 * FULL * 64], r[4 * FULL * 64], o[4 * P * 64];
+      u4 s[DK / 16 * FULL * 64], d[DK / 16 * FULL * 64];
+    } v;
+  };
+  float dot[8][C];  // dR . v, by groups of four columns
+  float ssk[C], ssq[C], rk[C], rq[C], dsum[C];
+  float tail[8];
+  Decays dec;
+};
+template <typename T, int DK>
+__global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_last_kernel(
+    const DeltaGradArgs ga, const float* rec, const float* grec, int chunks, uint64_t blocks,
+    bool wide, bool wide_out) {
+  constexpr int U = DK / 32, MT = DK / 16, FULL = Mode<T>::FULL, P = Mode<T>::ROWS;
+  extern __shared__ __align__(16) unsigned char lds[];
   const DeltaArgs& a = ga.f;
-  float* kt = lds;                    // [64][DK + 4]
-  float* qt = kt + C * (DK + 4);      // [64][DK + 4]
-  float* dr = qt + C * (DK + 4);      // [64][DV + 4]
-  float* e1 = dr + C * (DV + 4);      // [64][CP]: dP scale D
-  float* e2 = e1 + C * CP;            // [64][CP]: dA beta D
-  float* col = e2 + C * CP;           // [4][64]: a wave's column sums
-  float* dsum = col + 4 * C;          // [64]: gradient of G
-  float* tail = dsum + C;             // [4]: a wave's part of <dS, S>
-  Coef& s = *reinterpret_cast<Coef*>(tail + 4);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane % 16, g4 = lane / 16 * 4;
-  const int group = a.HV / a.H, r0 = wave * 16 + g4;  // this lane's rows of results: r0 ..
+  LastLds<T, DK>& s = *reinterpret_cast<LastLds<T, DK>*>(lds);
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i16 = lane % 16, g = lane / 16, g4 = 4 * g, sl = slot_of(i16, g);
+  const int group = a.HV / a.H, own = w * 16 + i16;
   for (uint64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-    Place p = place_of(a, b, a.H, chunks);
-    const int kh = p.h, rows = min(C, a.q.T - p.c * C);
-    f4 dq[NK] = {}, dk[NK] = {};
-    __syncthreads();
-    if (p.n) {
-      bring<T, DK>(kt, a.k, p, kh, a.dk, wide);
-      bring<T, DK>(qt, a.qr, p, kh, a.dk, wide);
-      __syncthreads();
-      lengths_of<DK>(s.rk, kt, a.unit, 1.0f);
-      lengths_of<DK>(s.rq, qt, a.unit, a.scale);
+    Place p;
+    p.c = (int)(b % chunks);
+    const int kh = (int)(b / chunks % a.H);
+    p.l = (int)(b / chunks / a.H);
+    p.n = within(seq_len(a.q, p.l), p.c);
+    const int rows = min(C, a.q.T - p.c * C);
+    if (!p.n) {  // past the lane's length: zero
+      for (int i = tid; i < rows * group; i += 256) {
+        const int64_t t = p.c * C + i / group, h = kh * group + i % group;
+        ((float*)ga.dg.d)[p.l * ga.dg.lane + t * ga.dg.row + h] = 0.0f;
+        ((float*)ga.dbeta.d)[p.l * ga.dbeta.lane + t * ga.dbeta.row + h] = 0.0f;
+      }
+      const int wv = group * a.dv;
+      for (int i = tid; i < rows * wv; i += 256)
+        st1(row_at<T>(ga.dv, p, kh, wv, i / wv) + i % wv, 0.0f);
+      for (int i = tid; i < rows * a.dk; i += 256) {
+        st1(row_at<T>(ga.dq, p, kh, a.dk, i / a.dk) + i % a.dk, 0.0f);
+        st1(row_at<T>(ga.dk, p, kh, a.dk, i / a.dk) + i % a.dk, 0.0f);
+      }
+      continue;
     }
+    // K and Q as rows: their products, the lengths
+    auto bring_kq = [&](bool across_) {
+      Four k[DK / 64], q[DK / 64];
+#pragma unroll
+      for (int i = 0; i < DK / 64; ++i) {
+        k[i] = four_of<T>(a.k, p, kh, a.dk, wide, tid / 16 * 4, i * 64 + tid % 16 * 4);
+        q[i] = four_of<T>(a.qr, p, kh, a.dk, wide, tid / 16 * 4, i * 64 + tid % 16 * 4);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < DK / 64; ++i) {
+        const int pos = tid / 16 * 4, col = i * 64 + tid % 16 * 4;
+        if (across_) {
+          put_rows<T, P>(s.k.a, 2, col, pos, turned(k[i]));
+          put_rows<T, P>(s.k.b, 2, col, pos, turned(q[i]));
+        } else {
+          put_rows<T, P>(s.k.a, U, pos, col, k[i]);
+          put_rows<T, P>(s.k.b, U, pos, col, q[i]);
+        }
+      }
+      __syncthreads();
+    };
+    bring_kq(false);
+    // kk: rows of tile m, column own; qk: m < w: q of own, k of tile m; m > w: q
+    // of tile m, k of own; the wave's own tile has both (mid: the second)
+    f4 kk[4] = {}, qk[4] = {}, mid_qk = ZERO;
+    {
+      f4 qq = ZERO;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const Frag<P> ko = get<P>(s.k.a, w * U + u, sl), qo = get<P>(s.k.b, w * U + u, sl);
+        mma<T>(qq, qo, qo);
+        mma<T>(mid_qk, qo, ko);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const Frag<P> km = get<P>(s.k.a, m * U + u, sl);
+          mma<T>(kk[m], km, ko);
+          if (m <= w) mma<T>(qk[m], km, qo);
+          else mma<T>(qk[m], get<P>(s.k.b, m * U + u, sl), ko);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (m == w && g4 + r == i16) s.ssk[own] = kk[m][r], s.ssq[own] = qq[r];
+    }
+    __syncthreads();
+    if (tid < C) {
+      s.rk[tid] = a.unit ? 1.0f / __builtin_sqrtf(s.ssk[tid] + EPS) : 1.0f;
+      s.rq[tid] = a.unit ? a.scale / __builtin_sqrtf(s.ssq[tid] + EPS) : a.scale;
+    }
+    // this lane's columns of its own rows of q and k
+    f4 qo[MT], ko[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      qo[m] = ld4(row_at<const T>(a.qr, p, kh, a.dk, min(own, p.n - 1)), m * 16 + g4, a.dk, wide);
+      ko[m] = ld4(row_at<const T>(a.k, p, kh, a.dk, min(own, p.n - 1)), m * 16 + g4, a.dk, wide);
+    }
+    // what K and Q are multiplied with, and what comes from the states
+    f4 e[4] = {}, mid_e = ZERO, f[4] = {}, dq[MT] = {}, dk[MT] = {};
     for (int vh = kh * group; vh < (kh + 1) * group; ++vh) {
       p.h = vh;
-      if (!p.n) {  // rows past the length: zero
-        for (int i = threadIdx.x; i < rows; i += 256) {
-          const int64_t t = p.c * C + i;
-          ((float*)ga.dg.d)[p.l * ga.dg.lane + t * ga.dg.row + vh] = 0.0f;
-          ((float*)ga.dbeta.d)[p.l * ga.dbeta.lane + t * ga.dbeta.row + vh] = 0.0f;
+      const int64_t at = (((int64_t)p.l * a.HV + vh) * chunks + p.c) * (a.dv * (DK + C));
+      const float *S = rec + at, *N = S + a.dv * DK, *dS = grec + at, *dR = dS + a.dv * DK;
+      __syncthreads();
+      decays_of(s.dec, a, p);
+      f4 pp[4] = {}, aa[4] = {}, mid_p = ZERO, mid_a = ZERO, os[MT] = {}, rs[MT] = {}, ns[MT] = {};
+      float dots[4] = {}, tail = 0.0f;
+      for (int v0 = 0; v0 < a.dv; v0 += 32) {
+        // N and dR: 8 x 16 pieces of 4 columns x 4 positions; dO as many; S and dS
+        // 8 x DK / 4
+        const int half = tid / 128, pg = tid % 16, vg = tid / 16 % 8, v4 = v0 + vg * 4;
+        Four x, od, sx[DK / 64], dx[DK / 64];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x.v[i] = *reinterpret_cast<const f4*>((half ? dR : N) +
+                                                (int64_t)min(v4 + i, a.dv - 1) * C + pg * 4);
+        od = four_of<T>(half ? a.v : ga.dout, p, vh, a.dv, wide, pg * 4, v4);
+#pragma unroll
+        for (int i = 0; i < DK / 64; ++i) {
+          const int d4 = (i * 16 + tid % 16) * 4;
+          const int sv = v0 + (tid / 16 % 8) * 4;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            sx[i].v[j] = *reinterpret_cast<const f4*>((half ? dS : S) +
+                                                      (int64_t)min(sv + j, a.dv - 1) * DK + d4);
         }
-        for (int i = threadIdx.x; i < rows * a.dv; i += 256)
-          st1((T*)ga.dv.d + p.l * ga.dv.lane + (int64_t)(p.c * C + i / a.dv) * ga.dv.row +
-                  (int64_t)vh * a.dv + i % a.dv, 0.0f);
-        continue;
+        (void)dx;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (v4 + i >= a.dv) {
+            x.v[i] = ZERO;
+#pragma unroll
+            for (int j = 0; j < DK / 64; ++j) sx[j].v[i] = ZERO;
+          }
+        __syncthreads();
+        const Four xt = turned(x);  // rows: positions
+        put_rows<T, FULL>(half ? s.v.r : s.v.n, 1, pg * 4, vg * 4, xt);
+        if (half) {
+          // dV, and dR . v
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f4 d = xt.v[i] * od.v[i];
+            dots[i] += d[0] + d[1] + d[2] + d[3];
+            const int pos = pg * 4 + i;
+            if (pos < rows)
+              st4(row_at<T>(ga.dv, p, vh, a.dv, pos), v4, a.dv, wide_out,
+                  pos < p.n ? xt.v[i] * s.dec.beta[pos] : ZERO);
+          }
+        } else {
+          put_rows<T, P>(s.v.o, 1, pg * 4, vg * 4, od);
+        }
+#pragma unroll
+        for (int i = 0; i < DK / 64; ++i)
+          put_rows<T, FULL>(half ? s.v.d : s.v.s, 1, (i * 16 + tid % 16) * 4, vg * 4, turned(sx[i]));
+        __syncthreads();
+        const Frag<FULL> no = get<FULL>(s.v.n, w, sl), ro = get<FULL>(s.v.r, w, sl);
+        const Frag<P> oo = get<P>(s.v.o, w, sl);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          if (m <= w) {
+            const Frag<FULL> nm = get<FULL>(s.v.n, m, sl);
+            mma<T>(pp[m], nm, oo);
+            mma<T>(aa[m], nm, ro);
+          } else {
+            mma<T>(pp[m], get<P>(s.v.o, m, sl), no);
+            mma<T>(aa[m], get<FULL>(s.v.r, m, sl), no);
+          }
+        }
+        mma<T>(mid_p, oo, no);
+        mma<T>(mid_a, ro, no);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const Frag<FULL> sm = get<FULL>(s.v.s, m, sl);
+          mma<T>(os[m], sm, oo);
+          mma<T>(rs[m], sm, ro);
+          mma<T>(ns[m], get<FULL>(s.v.d, m, sl), no);
+        }
       }
-      const uint64_t at = ((uint64_t)p.l * a.HV + vh) * chunks + p.c;
-      const float *S = rec + at * R::SIZE + R::S, *N = rec + at * R::SIZE + R::N,
-                  *tm = rec + at * R::SIZE + R::T, *dS = grec + at * GR::SIZE + GR::S,
-                  *dN = grec + at * GR::SIZE + GR::N;
-      __syncthreads();
-      decays_of(s, a, p);
-      __syncthreads();
-      float dbeta[4] = {}, dg[4] = {};
-      {
-        // dR = T^T dN; dV; dR . v into dbeta
-        f4 acc[NV] = {};
-        mma<NV, C>(acc, [&](int kk) { return across(tm, C, wave * 16, kk, lane); },
-                   [&](int kk, int n) { return across(dN, DV, n * 16, kk, lane); });
+      // <dS, S>: the two halves of the block hold one each, so from memory
+      for (int i = tid; i < a.dv * DK / 4; i += 256) {
+        const f4 u = *reinterpret_cast<const f4*>(S + i * 4);
+        const f4 d = *reinterpret_cast<const f4*>(dS + i * 4);
+        tail += u[0] * d[0] + u[1] * d[1] + u[2] * d[2] + u[3] * d[3];
+      }
+      tail = over64(tail, Sum());
+      if (tid >= 128) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s.dot[tid / 16 % 8][tid % 16 * 4 + i] = dots[i];
+      }
+      const double G = s.dec.sum[own];
+      const float beta = s.dec.beta[own], rk = s.rk[own], rq = s.rq[own];
+      // sums over a row of dP P and dA A, over a column, and of dA k.k D
+      float over = 0.0f, down = 0.0f, with_beta = 0.0f;
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int i = r0 + r;
-          const int64_t t = p.c * C + i;
-          const T* v = (const T*)a.v.d + p.l * a.v.lane + t * a.v.row + (int64_t)vh * a.dv;
-          T* o = (T*)ga.dv.d + p.l * ga.dv.lane + t * ga.dv.row + (int64_t)vh * a.dv;
-          float dot = 0.0f;
-#pragma unroll
-          for (int n = 0; n < NV; ++n) {
-            const int j = n * 16 + i16;
-            dr[i * (DV + 4) + j] = acc[n][r];
-            if (j < a.dv && i < rows) {
-              if (i < p.n) dot += acc[n][r] * ld1(v + j);
-              st1(o + j, i < p.n ? acc[n][r] * s.beta[i] : 0.0f);
-            }
+          const int o = m * 16 + g4 + r;
+          const double dG = s.dec.sum[o] - G;
+          const float d = exp_of(o < own ? -dG : dG), rko = s.rk[o], rqo = s.rq[o];
+          const float ukk = kk[m][r] * rk * rko;
+          if (m <= w) {  // own is the row, o the column
+            const float dP = o <= own ? pp[m][r] * d : 0.0f;
+            const float dA = o < own ? -aa[m][r] * d : 0.0f;
+            over += dP * (qk[m][r] * (rq * rko)) + dA * (beta * ukk);
+            with_beta += dA * ukk;
+            e[m][r] += dP * (rko * a.scale);
+            f[m][r] += dA * (beta * rko);
           }
-          dbeta[r] += sum16(dot);
+          if (m >= w) {  // o is the row, own the column
+            const float p0 = m == w ? mid_p[r] : pp[m][r], a0 = m == w ? mid_a[r] : aa[m][r];
+            const float q0 = m == w ? mid_qk[r] : qk[m][r], bo = s.dec.beta[o];
+            const float dP = o >= own ? p0 * d : 0.0f;
+            const float dA = o > own ? -a0 * d : 0.0f;
+            down += dP * (q0 * (rqo * rk)) + dA * (bo * ukk);
+            if (m == w) mid_e[r] += dP * rqo;
+            else e[m][r] += dP * rqo;
+            f[m][r] += dA * (bo * rko);
+          }
         }
+      // from the states
+      float oq = 0.0f, rsk = 0.0f, nsk = 0.0f;
+      const float since = s.dec.since[own], left = s.dec.left[own];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          oq += os[m][r] * qo[m][r];
+          rsk += rs[m][r] * ko[m][r];
+          nsk += ns[m][r] * ko[m][r];
+        }
+        dq[m] += os[m] * (since * a.scale);
+        dk[m] += ns[m] * left - rs[m] * (since * beta);
       }
-      __syncthreads();
-      // this lane's row of dO as an operand: k along the row
-      const int oi = wave * 16 + i16;
-      const T* drow = (const T*)ga.dout.d + p.l * ga.dout.lane +
-                      (int64_t)(p.c * C + oi) * ga.dout.row + (int64_t)vh * a.dv;
-      auto dout = [&](int kk) {
-        return oi < p.n ? ld4(drow, kk * 16 + g4, a.dv, wide) : f4{0.0f, 0.0f, 0.0f, 0.0f};
+      auto across_g = [&](float x) {
+        x = fold16(x, x);
+        return fold32(x, x);
       };
-      auto drop = [&](int kk) { return along(dr, DV + 4, wave * 16, kk, lane); };
-      auto dense = [&](const float* m, int pitch, int n, int kk) {
-        return *reinterpret_cast<const f4*>(m + (n * 16 + i16) * pitch + kk * 16 + g4);
-      };
-      {
-        f4 da[4] = {}, dp[4] = {}, kk_[4] = {}, qk[4] = {};
-        mma<4, DV>(da, drop, [&](int kk, int n) { return dense(N, DV, n, kk); });
-        mma<4, DV>(dp, dout, [&](int kk, int n) { return dense(N, DV, n, kk); });
-        mma<4, DK>(kk_, [&](int kk) { return along(kt, DK + 4, wave * 16, kk, lane); },
-                   [&](int kk, int n) { return along(kt, DK + 4, n * 16, kk, lane); });
-        mma<4, DK>(qk, [&](int kk) { return along(qt, DK + 4, wave * 16, kk, lane); },
-                   [&](int kk, int n) { return along(kt, DK + 4, n * 16, kk, lane); });
-        float down[4] = {};
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = r0 + r;
-          float across_row = 0.0f, with_beta = 0.0f;
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const int j = n * 16 + i16;
-            const float d = j <= i ? between(s, i, j) : 0.0f;
-            const float dA = j < i ? -da[n][r] * d : 0.0f, dP = dp[n][r] * d;
-            const float unit_kk = kk_[n][r] * (s.rk[i] * s.rk[j]);
-            const float m = dA * s.beta[i] * unit_kk + dP * (qk[n][r] * (s.rq[i] * s.rk[j]));
-            across_row += m;
-            down[n] += m;
-            with_beta += dA * unit_kk;
-            e1[i * CP + j] = dP;
-            e2[i * CP + j] = dA * s.beta[i];
-          }
-          dg[r] += sum16(across_row);
-          dbeta[r] += sum16(with_beta);
-        }
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          float x = down[n];
-          x += __shfl_xor(x, 16);
-          x += __shfl_xor(x, 32);
-          if (lane < 16) col[wave * C + n * 16 + i16] = x;
-        }
-      }
-      float last[4];
-      {
-        f4 os[NK] = {}, rs[NK] = {}, ns[NK] = {};
-        mma<NK, DV>(os, dout, [&](int kk, int n) { return dense(S, DV, n, kk); });
-        mma<NK, DV>(rs, drop, [&](int kk, int n) { return dense(S, DV, n, kk); });
-        mma<NK, DV>(ns, [&](int kk) { return dense(N, DV, wave, kk); },
-                    [&](int kk, int n) { return dense(dS, DV, n, kk); });
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = r0 + r;
-          float o = 0.0f, d = 0.0f, e = 0.0f;
-#pragma unroll
-          for (int n = 0; n < NK; ++n) {
-            const float kv = kt[i * (DK + 4) + n * 16 + i16], qv = qt[i * (DK + 4) + n * 16 + i16];
-            o += os[n][r] * qv;
-            d += rs[n][r] * kv;
-            e += ns[n][r] * kv;
-          }
-          o = sum16(o) * (s.rq[i] * s.since[i]);
-          d = sum16(d) * (s.rk[i] * s.since[i]);
-          last[r] = sum16(e) * (s.rk[i] * s.left[i]);
-          dbeta[r] -= d;
-          dg[r] += o - d * s.beta[i] - last[r];
-#pragma unroll
-          for (int n = 0; n < NK; ++n) {
-            dq[n][r] += os[n][r] * (s.since[i] * a.scale);
-            dk[n][r] += ns[n][r] * s.left[i] - rs[n][r] * (s.since[i] * s.beta[i]);
-          }
-        }
-      }
-      {
-        // <dS, S>, a quarter in each wave
-        float x = 0.0f;
-        for (int i = threadIdx.x; i < DK * DV / 4; i += 256) {
-          const f4 u = *reinterpret_cast<const f4*>(S + i * 4);
-          const f4 v = *reinterpret_cast<const f4*>(dS + i * 4);
-          x += u[0] * v[0] + u[1] * v[1] + u[2] * v[2] + u[3] * v[3];
-        }
-        x *= s.since[C - 1];
-        if (i16 == 0) x += last[0] + last[1] + last[2] + last[3];
-#pragma unroll
-        for (int m = 1; m < 64; m *= 2) x += __shfl_xor(x, m);
-        if (lane == 0) tail[wave] = x;
-        if (i16 == 0)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) dsum[r0 + r] = dg[r];
-      }
+      oq = across_g(oq) * (rq * since);
+      rsk = across_g(rsk) * (rk * since);
+      nsk = across_g(nsk) * (rk * left);
+      over = across_g(over);
+      down = across_g(down);
+      with_beta = across_g(with_beta);
+      if (g == 0) s.dsum[own] = over - down - nsk + oq - rsk * beta;
+      const float lasts = over16(nsk, Sum());
+      if (lane == 0) s.tail[w] = lasts, s.tail[4 + w] = tail * s.dec.since[C - 1];
       __syncthreads();
-      mma<NK, C>(dq,
-                 [&](int kk) {
-                   f4 v = along(e1, CP, wave * 16, kk, lane);
+      if (g == 0 && own < rows) {
+        float x = with_beta - rsk;
 #pragma unroll
-                   for (int j = 0; j < 4; ++j) v[j] *= s.rk[kk * 16 + g4 + j] * a.scale;
-                   return v;
-                 },
-                 [&](int kk, int n) { return across(kt, DK + 4, n * 16, kk, lane); });
-      mma<NK, C>(dk,
-                 [&](int kk) {
-                   f4 v = across(e1, CP, wave * 16, kk, lane);
-#pragma unroll
-                   for (int j = 0; j < 4; ++j) v[j] *= s.rq[kk * 16 + g4 + j];
-                   return v;
-                 },
-                 [&](int kk, int n) { return across(qt, DK + 4, n * 16, kk, lane); });
-      mma<NK, C>(dk,
-                 [&](int kk) {
-                   f4 v = along(e2, CP, wave * 16, kk, lane) + across(e2, CP, wave * 16, kk, lane);
-#pragma unroll
-                   for (int j = 0; j < 4; ++j) v[j] *= s.rk[kk * 16 + g4 + j];
-                   return v;
-                 },
-                 [&](int kk, int n) { return across(kt, DK + 4, n * 16, kk, lane); });
-      if (i16 == 0)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (r0 + r < rows)
-            ((float*)ga.dbeta.d)[p.l * ga.dbeta.lane + (int64_t)(p.c * C + r0 + r) * ga.dbeta.row +
-                                 vh] = r0 + r < p.n ? dbeta[r] : 0.0f;
-      if (wave == 0) {
+        for (int i = 0; i < 8; ++i) x += s.dot[i][own];
+        ((float*)ga.dbeta.d)[p.l * ga.dbeta.lane + (int64_t)(p.c * C + own) * ga.dbeta.row + vh] =
+            own < p.n ? x : 0.0f;
+      }
+      if (w == 0) {
         // dg: the sums of dG from each position to the chunk's last
-        double x = (double)dsum[lane] - (double)col[lane] - (double)col[C + lane] -
-                   (double)col[2 * C + lane] - (double)col[3 * C + lane];
-        if (lane == C - 1) x += (double)tail[0] + tail[1] + tail[2] + tail[3];
+        double x = (double)s.dsum[lane];
+        if (lane == C - 1)
+          for (int i = 0; i < 8; ++i) x += (double)s.tail[i];
 #pragma unroll
         for (int m = 1; m < C; m *= 2) {
           const double y = __shfl_down(x, m);
@@ -894,47 +1112,60 @@ __global__ __launch_bounds__(256) void delta_grad_last_kernel(const DeltaGradArg
               lane < p.n ? (float)x : 0.0f;
       }
     }
-    // through the rows' lengths: d = r (d^ - u (u . d^)), u the unit row
+    bring_kq(true);
+    {
+      // e: q's part below (rows j), k's above (rows i); the own tile has both
+      f4 ek[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = r0 + r;
-      if (i >= rows) continue;
-      const int64_t t = p.c * C + i;
-      T* oq = (T*)ga.dq.d + p.l * ga.dq.lane + t * ga.dq.row + (int64_t)kh * a.dk;
-      T* ok = (T*)ga.dk.d + p.l * ga.dk.lane + t * ga.dk.row + (int64_t)kh * a.dk;
-      float fq = 0.0f, fk = 0.0f, rq = 1.0f, rk = 1.0f;
-      const bool live = i < p.n;
-      if (live && a.unit) {
+      for (int m = 0; m < 4; ++m) {
+        ek[m] = m == w ? mid_e : (m > w ? e[m] : ZERO);
+        e[m] = m <= w ? e[m] : ZERO;
+      }
+      Frag<FULL> ef[2], kf[2], ff[2];
 #pragma unroll
-        for (int n = 0; n < NK; ++n) {
-          fq += dq[n][r] * qt[i * (DK + 4) + n * 16 + i16];
-          fk += dk[n][r] * kt[i * (DK + 4) + n * 16 + i16];
-        }
-        rk = s.rk[i];
-        // the scale is in s.rq too
-        float ss = 0.0f;
-#pragma unroll
-        for (int n = 0; n < NK; ++n) {
-          const float x = qt[i * (DK + 4) + n * 16 + i16];
-          ss += x * x;
-        }
-        rq = 1.0f / __builtin_sqrtf(sum16(ss) + EPS);
-        fq = sum16(fq) * rq * rq;
-        fk = sum16(fk) * rk * rk;
+      for (int u = 0; u < 2; ++u) {
+        ef[u] = full<T>(e[2 * u], e[2 * u + 1]);
+        kf[u] = full<T>(ek[2 * u], ek[2 * u + 1]);
+        ff[u] = full<T>(f[2 * u], f[2 * u + 1]);
       }
 #pragma unroll
-      for (int n = 0; n < NK; ++n) {
-        const int j = n * 16 + i16;
-        if (j >= a.dk) continue;
-        float x = 0.0f, y = 0.0f;
-        if (live) {
-          x = rq * (dq[n][r] - qt[i * (DK + 4) + j] * fq);
-          y = rk * (dk[n][r] - kt[i * (DK + 4) + j] * fk);
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const Frag<P> kt = get<P>(s.k.a, m * 2 + u, sl);
+          mma<T>(dq[m], kt, ef[u]);
+          mma<T>(dk[m], kt, ff[u]);
+          mma<T>(dk[m], get<P>(s.k.b, m * 2 + u, sl), kf[u]);
         }
-        st1(oq + j, x);
-        st1(ok + j, y);
+    }
+    // through the rows' lengths: d = r (d^ - u (u . d^)), u the unit row
+    float fq = 0.0f, fk = 0.0f, rq = 1.0f, rk = 1.0f;
+    if (a.unit) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          fq += dq[m][r] * qo[m][r];
+          fk += dk[m][r] * ko[m][r];
+        }
+      rk = s.rk[own];
+      rq = 1.0f / __builtin_sqrtf(s.ssq[own] + EPS);
+      fq = fold16(fq, fq);
+      fk = fold16(fk, fk);
+      fq = fold32(fq, fq) * rq * rq;
+      fk = fold32(fk, fk) * rk * rk;
+    }
+    if (own < rows) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const bool live = own < p.n;
+        st4(row_at<T>(ga.dq, p, kh, a.dk, own), m * 16 + g4, a.dk, wide_out,
+            live ? (dq[m] - qo[m] * fq) * rq : ZERO);
+        st4(row_at<T>(ga.dk, p, kh, a.dk, own), m * 16 + g4, a.dk, wide_out,
+            live ? (dk[m] - ko[m] * fk) * rk : ZERO);
       }
     }
+    __syncthreads();
   }
 }
 
@@ -959,7 +1190,7 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const DeltaArgs a, uint
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
       const int row = y + RG * i;
-      st[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+      st[i] = ZERO;
       if (a.state_in && row < a.dk)
         st[i] = ld4(a.state_in + state + (int64_t)row * a.dv, 4 * x, a.dv, wide_state);
     }
@@ -996,7 +1227,7 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const DeltaArgs a, uint
           kq[buf][wave][lane + 64 * i] = wave ? qv[i] * rq : kv[i] * rk;
       }
       __syncthreads();
-      f4 sk = {0.0f, 0.0f, 0.0f, 0.0f}, sq = sk;
+      f4 sk = ZERO, sq = ZERO;
 #pragma unroll
       for (int i = 0; i < RPT; ++i) {
         sk += st[i] * kq[buf][0][y + RG * i];
@@ -1045,25 +1276,16 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const DeltaArgs a, uint
 // widths that the kernels are built for
 int built(int d) { return d <= 64 ? 64 : 128; }
 int chunks_of(int T) { return (T + C - 1) / C; }
-int64_t record_floats(int dk, int dv) {
-  const int k = built(dk), v = built(dv);
-  return (int64_t)k * v + C * v + C * k + C * C;
-}
-int64_t grad_record_floats(int dk, int dv) {
-  return (int64_t)built(dk) * built(dv) + C * built(dv);
-}
+// S and N of a chunk, dS and dR of it
+int64_t record_floats(int dk, int dv) { return (int64_t)dv * (built(dk) + C); }
 
 // Positions taken one after the other rather than in chunks.
 bool by_steps(int T) { return T <= 4; }
 
 template <typename F>
-hipError_t for_widths(int dk, int dv, F&& f) {
-  using std::integral_constant;
-  if (built(dk) == 64)
-    return built(dv) == 64 ? f(integral_constant<int, 64>(), integral_constant<int, 64>())
-                           : f(integral_constant<int, 64>(), integral_constant<int, 128>());
-  return built(dv) == 64 ? f(integral_constant<int, 128>(), integral_constant<int, 64>())
-                         : f(integral_constant<int, 128>(), integral_constant<int, 128>());
+hipError_t for_width(int dk, F&& f) {
+  if (built(dk) == 64) return f(std::integral_constant<int, 64>());
+  return f(std::integral_constant<int, 128>());
 }
 
 template <typename K>
@@ -1074,18 +1296,18 @@ hipError_t room(K kernel, size_t bytes) {
 }
 uint32_t grid(uint64_t blocks) { return (uint32_t)std::min<uint64_t>(blocks, MAX_BLOCKS); }
 
-bool wide_rows(const RowsIn& r, int d, int size) {
+template <typename R>
+bool wide_rows(const R& r, int d, int size) {
   return rows_by_16(r.d, r.lane, r.row, d, size);
 }
 
 template <typename T>
 hipError_t delta_of(const DeltaArgs& a, hipStream_t s) {
   const int size = sizeof(T);
-  const bool wide = wide_rows(a.qr, a.dk, size) && wide_rows(a.k, a.dk, size) &&
-                    wide_rows(a.v, a.dv, size);
   const uint64_t heads = (uint64_t)a.q.lanes * a.HV;
   if (by_steps(a.q.T) && !a.saved) {
-    const bool wide_state = a.dv % 4 == 0 && (uintptr_t)a.state_in % 16 == 0;
+    const bool wide = wide_rows(a.v, a.dv, size);
+    const bool wide_state = a.dv % 4 == 0;  // states are 16-byte aligned
     auto go = [&](auto kernel) {
       BOA_LAUNCH(kernel, grid(heads), 256, 0, s, a, heads, wide, wide_state);
       return hipGetLastError();
@@ -1094,22 +1316,19 @@ hipError_t delta_of(const DeltaArgs& a, hipStream_t s) {
       return a.dv <= 64 ? go(delta_step_kernel<T, 64, 16>) : go(delta_step_kernel<T, 64, 32>);
     return a.dv <= 64 ? go(delta_step_kernel<T, 128, 16>) : go(delta_step_kernel<T, 128, 32>);
   }
-  return for_widths(a.dk, a.dv, [&](auto dk, auto dv) {
-    constexpr int DK = dk, DV = dv, D = DK > DV ? DK : DV;
-    const int chunks = chunks_of(a.q.T);
-    float* rec = a.saved ? a.saved : (float*)a.work;
+  return for_width(a.dk, [&](auto dk) {
+    constexpr int DK = dk;
+    const bool wide = wide_rows(a.qr, a.dk, size) && wide_rows(a.k, a.dk, size);
+    const int chunks = chunks_of(a.q.T), tiles = (a.dv + 63) / 64;
+    unsigned char* prep = (unsigned char*)a.work;
     const uint64_t all = heads * chunks;
-    BOA_LAUNCH((delta_prep_kernel<T, DK, DV>), grid(all), 256, 0, s, a, rec, chunks, all, wide);
+    BOA_LAUNCH((delta_prep_kernel<T, DK, false>), grid(all), 256, 0, s, a, prep, chunks, all, wide);
     hipError_t e = hipGetLastError();
     if (e) return e;
-    const uint64_t tiles = heads * (DV / BV);
-    BOA_LAUNCH((delta_chain_kernel<T, DK, DV>), grid(tiles), 256, 0, s, a, rec, chunks, tiles,
-               wide);
-    if ((e = hipGetLastError())) return e;
-    const size_t lds = 4 * (C * (DK + 4) + C * (D + 4) + C * CP) + sizeof(Coef);
-    if ((e = room(delta_out_kernel<T, DK, DV>, lds))) return e;
-    BOA_LAUNCH((delta_out_kernel<T, DK, DV>), grid(all), 256, lds, s, a, (const float*)rec, chunks,
-               all, wide);
+    const size_t lds = sizeof(ChainLds<T, DK, false>);
+    if ((e = room(delta_chain_kernel<T, DK>, lds))) return e;
+    BOA_LAUNCH((delta_chain_kernel<T, DK>), grid(heads * tiles), 256, lds, s, a,
+               (const unsigned char*)prep, a.saved, chunks, tiles, heads * tiles, wide);
     return hipGetLastError();
   });
 }
@@ -1118,32 +1337,30 @@ template <typename T>
 hipError_t delta_grad_of(const DeltaGradArgs& ga, hipStream_t s) {
   const DeltaArgs& a = ga.f;
   const int size = sizeof(T);
-  const bool wide = wide_rows(a.qr, a.dk, size) && wide_rows(a.k, a.dk, size) &&
-                    wide_rows(a.v, a.dv, size) && wide_rows(ga.dout, a.dv, size);
+  const bool wide = wide_rows(a.qr, a.dk, size) && wide_rows(a.k, a.dk, size);
+  const bool wide_last = wide && wide_rows(a.v, a.dv, size) && wide_rows(ga.dout, a.dv, size);
+  const bool wide_out = wide_rows(ga.dq, a.dk, size) && wide_rows(ga.dk, a.dk, size) &&
+                        wide_rows(ga.dv, a.dv, size);
   const uint64_t heads = (uint64_t)a.q.lanes * a.HV;
-  return for_widths(a.dk, a.dv, [&](auto dk, auto dv) {
-    constexpr int DK = dk, DV = dv, D = DK > DV ? DK : DV;
-    const int chunks = chunks_of(a.q.T);
-    const float* rec = a.saved;
-    float* grec = (float*)a.work;
+  return for_width(a.dk, [&](auto dk) {
+    constexpr int DK = dk;
+    const int chunks = chunks_of(a.q.T), tiles = (a.dv + 63) / 64;
     const uint64_t all = heads * chunks;
-    size_t lds = 4 * (C * (DK + 4) + C * (D + 4) + C * CP) + sizeof(Coef);
-    hipError_t e = room(delta_grad_first_kernel<T, DK, DV>, lds);
+    unsigned char* prep = (unsigned char*)a.work;
+    float* grec = (float*)(prep + all * PREP_BYTES);
+    BOA_LAUNCH((delta_prep_kernel<T, DK, true>), grid(all), 256, 0, s, a, prep, chunks, all, wide);
+    hipError_t e = hipGetLastError();
     if (e) return e;
-    BOA_LAUNCH((delta_grad_first_kernel<T, DK, DV>), grid(all), 256, lds, s, ga, grec, chunks, all,
-               wide);
+    size_t lds = sizeof(ChainLds<T, DK, true>);
+    if ((e = room(delta_grad_chain_kernel<T, DK>, lds))) return e;
+    BOA_LAUNCH((delta_grad_chain_kernel<T, DK>), grid(heads * tiles), 256, lds, s, ga,
+               (const unsigned char*)prep, grec, chunks, tiles, heads * tiles, wide);
     if ((e = hipGetLastError())) return e;
-    const uint64_t tiles = heads * (DV / BV);
-    lds = 4 * (2 * C * (DK + 4) + DK * (BV + 4) + 2 * C * (BV + 4)) + sizeof(Coef);
-    if ((e = room(delta_grad_chain_kernel<T, DK, DV>, lds))) return e;
-    BOA_LAUNCH((delta_grad_chain_kernel<T, DK, DV>), grid(tiles), 256, lds, s, ga, rec, grec,
-               chunks, tiles, wide);
-    if ((e = hipGetLastError())) return e;
-    lds = 4 * (2 * C * (DK + 4) + C * (DV + 4) + 2 * C * CP + 5 * C + 4) + sizeof(Coef);
-    if ((e = room(delta_grad_last_kernel<T, DK, DV>, lds))) return e;
+    lds = sizeof(LastLds<T, DK>);
+    if ((e = room(delta_grad_last_kernel<T, DK>, lds))) return e;
     const uint64_t last = (uint64_t)a.q.lanes * a.H * chunks;
-    BOA_LAUNCH((delta_grad_last_kernel<T, DK, DV>), grid(last), 256, lds, s, ga, rec,
-               (const float*)grec, chunks, last, wide);
+    BOA_LAUNCH((delta_grad_last_kernel<T, DK>), grid(last), 256, lds, s, ga, (const float*)a.saved,
+               (const float*)grec, chunks, last, wide_last, wide_out);
     return hipGetLastError();
   });
 }
@@ -1156,9 +1373,7 @@ int64_t delta_saved_floats(int lanes, int T, int, int HV, int dk, int dv) {
 
 int64_t delta_work_bytes(int lanes, int T, int, int HV, int dk, int dv, bool grad) {
   const int64_t n = (int64_t)lanes * HV * chunks_of(T);
-  // a forward call without `saved` keeps its chunks' records here
-  const int64_t forward = by_steps(T) ? 0 : n * record_floats(dk, dv);
-  return 4 * (grad ? std::max(forward, n * grad_record_floats(dk, dv)) : forward);
+  return n * (PREP_BYTES + (grad ? 4 * record_floats(dk, dv) : 0));
 }
 
 hipError_t launch_delta(const DeltaArgs& a, hipStream_t s) {

@@ -206,7 +206,7 @@ def test_capture(codec):  # noqa: F811
     args = [d[n] for n in ("q", "k", "v", "g", "beta")]
 
     def step():
-        codec.delta_rule(*args, out, heads=1, d_state_in=d["state_in"], d_state_out=state,
+        codec.delta_rule(*args, out, w, heads=1, d_state_in=d["state_in"], d_state_out=state,
                          d_saved=saved)
         codec.delta_rule_grad(*args, saved, d["dout"], *g, w, heads=1, d_state_in=d["state_in"],
                               d_dstate_out=d["dstate_out"])

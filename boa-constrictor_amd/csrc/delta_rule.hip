@@ -70,31 +70,54 @@ __device__ __forceinline__ void st1(T* p, float x) {
   if constexpr (sizeof(T) == 4) *p = x;
   else *p = f32_to_bf16(x);
 }
-// four elements from column c on of a row of d, zero past d; wide: in one piece.
-// No branch (a load in one would wait for those before it): what is past d reads
-// the row's first or last element.
+// Four elements of a row as they lie in memory, from column c on of d; W: in one
+// piece (d and the addresses are multiples of 16 bytes).  No branch and no use of
+// what is loaded (either would wait for it): what lies past d is the row's first
+// or last elements, until `cut` clears it.
 template <typename T>
-__device__ __forceinline__ f4 ld4(const T* row, int c, int d, bool wide) {
-  f4 v;
-  if (wide) {
-    const T* p = row + (c < d ? c : 0);
-    if constexpr (sizeof(T) == 4) {
-      v = *reinterpret_cast<const f4*>(p);
+struct Raw {
+  using V = std::conditional_t<sizeof(T) == 4, f4, u2>;
+  V v;
+  template <bool W>
+  __device__ __forceinline__ void load(const T* row, int c, int d) {
+    if constexpr (W) {
+      v = *reinterpret_cast<const V*>(row + (c < d ? c : 0));
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = row[min(c + i, d - 1)];
     } else {
-      const u2 w = *reinterpret_cast<const u2*>(p);
-      v = f4{u2f(w[0] << 16), u2f(w[0] & 0xFFFF0000u), u2f(w[1] << 16), u2f(w[1] & 0xFFFF0000u)};
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        v[i] = row[min(c + 2 * i, d - 1)] | (uint32_t)row[min(c + 2 * i + 1, d - 1)] << 16;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = ld1(row + min(c + i, d - 1));
   }
+  // zero from element n on
+  template <bool W>
+  __device__ __forceinline__ void cut(int n) {
+    if constexpr (W || sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = c + i < d ? v[i] : 0.0f;
-  return v;
+      for (int i = 0; i < (int)(sizeof(V) / 4); ++i)
+        if (W ? n <= 0 : i >= n) v[i] = 0;
+    } else {
+      v[0] = n <= 0 ? 0 : (n == 1 ? v[0] & 0xFFFFu : v[0]);
+      v[1] = n <= 2 ? 0 : (n == 3 ? v[1] & 0xFFFFu : v[1]);
+    }
+  }
+  __device__ __forceinline__ f4 value() const {
+    if constexpr (sizeof(T) == 4) return v;
+    else return f4{u2f(v[0] << 16), u2f(v[0] & 0xFFFF0000u), u2f(v[1] << 16), u2f(v[1] & 0xFFFF0000u)};
+  }
+};
+template <typename T, bool W>
+__device__ __forceinline__ f4 ld4(const T* row, int c, int d) {
+  Raw<T> r;
+  r.template load<W>(row, c, d);
+  r.template cut<W>(d - c);
+  return r.value();
 }
-template <typename T>
-__device__ __forceinline__ void st4(T* row, int c, int d, bool wide, f4 v) {
-  if (wide) {
+template <typename T, bool W>
+__device__ __forceinline__ void st4(T* row, int c, int d, f4 v) {
+  if constexpr (W) {
     if (c >= d) return;
     if constexpr (sizeof(T) == 4) *reinterpret_cast<f4*>(row + c) = v;
     else *reinterpret_cast<u2*>(row + c) = u2{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
@@ -221,10 +244,9 @@ __device__ __forceinline__ void put(u4* tile, int U, int row, int k, f4 v) {
   }
 }
 
-// Four rows x four columns of a chunk's rows at a time, a thread: taken from
-// memory, and put as rows (k along them) or across (k over the positions).
+// Four rows x four columns of floats at a time, a thread
 struct Four {
-  f4 v[4];  // v[e]: row 4 pg + e
+  f4 v[4];
 };
 __device__ __forceinline__ Four turned(const Four& x) {
   Four t;
@@ -232,10 +254,10 @@ __device__ __forceinline__ Four turned(const Four& x) {
   for (int c = 0; c < 4; ++c) t.v[c] = f4{x.v[0][c], x.v[1][c], x.v[2][c], x.v[3][c]};
   return t;
 }
-template <typename T, int P>
-__device__ __forceinline__ void put_rows(u4* tile, int U, int row, int k, const Four& x) {
+template <typename T>
+__device__ __forceinline__ void put_full(u4* tile, int U, int row, int k, const Four& x) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) put<T, P>(tile, U, row + e, k, x.v[e]);
+  for (int e = 0; e < 4; ++e) put<T, Mode<T>::FULL>(tile, U, row + e, k, x.v[e]);
 }
 
 struct Place {
@@ -255,19 +277,60 @@ template <typename T>
 __device__ __forceinline__ T* row_at(const RowsOut& r, const Place& p, int h, int d, int row) {
   return (T*)r.d + p.l * r.lane + (int64_t)(p.c * C + row) * r.row + (int64_t)h * d;
 }
-// rows pos .. pos + 3, columns col .. col + 3; zero past the chunk's positions
-// (p.n of them, one at least) and past d
+// Rows pos .. pos + 3, columns col .. col + 3 of a chunk's rows, a thread: loaded,
+// later put as rows (k along them) or across (k over the positions), with zeros
+// past the chunk's positions and past d
 template <typename T>
-__device__ __forceinline__ Four four_of(const RowsIn& r, const Place& p, int h, int d, bool wide,
-                                        int pos, int col) {
-  Four x;
+struct Rows4 {
+  Raw<T> r[4];
+  template <bool W>
+  __device__ __forceinline__ void load(const RowsIn& from, const Place& p, int h, int d, int pos,
+                                       int col) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    x.v[e] = ld4(row_at<const T>(r, p, h, d, min(pos + e, p.n - 1)), col, d, wide);
+    for (int e = 0; e < 4; ++e)
+      r[e].template load<W>(row_at<const T>(from, p, h, d, min(pos + e, p.n - 1)), col, d);
+  }
+  // rows from n on and columns from d on
+  template <bool W>
+  __device__ __forceinline__ void cut(int n, int d) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (pos + e >= p.n) x.v[e] = ZERO;
-  return x;
+    for (int e = 0; e < 4; ++e) r[e].template cut<W>(e < n ? d : 0);
+  }
+  __device__ __forceinline__ Four values() const {
+    return Four{{r[0].value(), r[1].value(), r[2].value(), r[3].value()}};
+  }
+  __device__ __forceinline__ Rows4 turned() const {
+    Rows4 t;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) t.r[c].v = f4{r[0].v[c], r[1].v[c], r[2].v[c], r[3].v[c]};
+    } else {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t a = r[0].v[c], b = r[1].v[c], x = r[2].v[c], y = r[3].v[c];
+        t.r[2 * c].v = u2{__builtin_amdgcn_perm(b, a, 0x05040100), __builtin_amdgcn_perm(y, x, 0x05040100)};
+        t.r[2 * c + 1].v = u2{__builtin_amdgcn_perm(b, a, 0x07060302), __builtin_amdgcn_perm(y, x, 0x07060302)};
+      }
+    }
+    return t;
+  }
+  // as the rows `row` .. row + 3 of a tile, k .. k + 3
+  __device__ __forceinline__ void put(u4* tile, int U, int row, int k) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int block = (row + e) / 16 * U + k / 32, slot = slot_of((row + e) % 16, k / 4 % 4);
+      if constexpr (sizeof(T) == 4)
+        tile[(block * 2 + k / 16 % 2) * 64 + slot] = __builtin_bit_cast(u4, r[e].v);
+      else reinterpret_cast<u2*>(tile + block * 64 + slot)[k / 16 % 2] = r[e].v;
+    }
+  }
+};
+// one element as it lies in memory
+__device__ __forceinline__ uint32_t raw1(const float* p) { return f2u(*p); }
+__device__ __forceinline__ uint32_t raw1(const uint16_t* p) { return *p; }
+template <typename T>
+__device__ __forceinline__ float value1(uint32_t x) {
+  return sizeof(T) == 4 ? u2f(x) : u2f(x << 16);
 }
 
 // ---- what passes between the kernels, of a (lane, value head, chunk) -------
@@ -333,9 +396,9 @@ __device__ __forceinline__ void mma16(f4& acc, f4 x, f4 y) {
 
 // A block per (lane, value head, chunk): T and P as the chain reads them, and
 // the coefficients.
-template <typename T, int DK, bool TRANS>
+template <typename T, int DK, bool TRANS, bool W>
 __global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a, unsigned char* prep,
-                                                         int chunks, uint64_t blocks, bool wide) {
+                                                         int chunks, uint64_t blocks) {
   using M = Mode<T>;
   constexpr int U = DK / 32, P = M::ROWS;
   __shared__ u4 ka[4 * U * P * 64], qa[4 * U * P * 64];
@@ -352,18 +415,21 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a, unsi
     p.n = within(seq_len(a.q, p.l), p.c);
     if (!p.n) continue;
     const int kh = p.h / (a.HV / a.H);
-    Four k[DK / 64], q[DK / 64];
+    const int pos = tid / 16 * 4, col = tid % 16 * 4;
+    Rows4<T> k[DK / 64], q[DK / 64];
 #pragma unroll
     for (int i = 0; i < DK / 64; ++i) {
-      k[i] = four_of<T>(a.k, p, kh, a.dk, wide, tid / 16 * 4, i * 64 + tid % 16 * 4);
-      q[i] = four_of<T>(a.qr, p, kh, a.dk, wide, tid / 16 * 4, i * 64 + tid % 16 * 4);
+      k[i].template load<W>(a.k, p, kh, a.dk, pos, i * 64 + col);
+      q[i].template load<W>(a.qr, p, kh, a.dk, pos, i * 64 + col);
     }
     __syncthreads();
     decays_of(s, a, p);
 #pragma unroll
     for (int i = 0; i < DK / 64; ++i) {
-      put_rows<T, P>(ka, U, tid / 16 * 4, i * 64 + tid % 16 * 4, k[i]);
-      put_rows<T, P>(qa, U, tid / 16 * 4, i * 64 + tid % 16 * 4, q[i]);
+      k[i].template cut<W>(p.n - pos, a.dk - i * 64 - col);
+      q[i].template cut<W>(p.n - pos, a.dk - i * 64 - col);
+      k[i].put(ka, U, pos, i * 64 + col);
+      q[i].put(qa, U, pos, i * 64 + col);
     }
     for (int i = tid; i < C * CP; i += 256) tm[i] = 0.0f;
     __syncthreads();
@@ -497,12 +563,13 @@ struct ChainLds {
 template <typename T, int DK>
 struct ChainNext {
   static constexpr int IMG = (IMAGE<T> + 255) / 256;
-  Four k[DK / 64], q[DK / 64];
+  Rows4<T> k[DK / 64], q[DK / 64];
   u4 img[IMG];
   float coef[2];
+  template <bool W>
   __device__ __forceinline__ void load(const DeltaArgs& a, const unsigned char* prep, const Place& p,
-                                       int kh, bool wide) {
-    const int tid = threadIdx.x;
+                                       int kh) {
+    const int tid = threadIdx.x, pos = tid / 16 * 4, col = tid % 16 * 4;
 #pragma unroll
     for (int i = 0; i < IMG; ++i)
       img[i] = reinterpret_cast<const u4*>(prep)[min(tid + 256 * i, IMAGE<T> - 1)];
@@ -511,21 +578,23 @@ struct ChainNext {
     coef[1] = c[4 * C];
 #pragma unroll
     for (int i = 0; i < DK / 64; ++i) {
-      k[i] = four_of<T>(a.k, p, kh, a.dk, wide, tid / 16 * 4, i * 64 + tid % 16 * 4);
-      q[i] = four_of<T>(a.qr, p, kh, a.dk, wide, tid / 16 * 4, i * 64 + tid % 16 * 4);
+      k[i].template load<W>(a.k, p, kh, a.dk, pos, i * 64 + col);
+      q[i].template load<W>(a.qr, p, kh, a.dk, pos, i * 64 + col);
     }
   }
-  template <bool TRANS>
-  __device__ __forceinline__ void store(ChainLds<T, DK, TRANS>& s) const {
-    const int tid = threadIdx.x, pos = tid / 16 * 4;
-    constexpr int P = Mode<T>::ROWS;
+  // n: the chunk's positions
+  template <bool W, bool TRANS>
+  __device__ __forceinline__ void store(ChainLds<T, DK, TRANS>& s, int n, int dk) {
+    const int tid = threadIdx.x, pos = tid / 16 * 4, c4 = tid % 16 * 4;
 #pragma unroll
     for (int i = 0; i < DK / 64; ++i) {
-      const int col = i * 64 + tid % 16 * 4;
-      put_rows<T, P>(s.ka, DK / 32, pos, col, k[i]);
-      put_rows<T, P>(s.kt, 2, col, pos, turned(k[i]));
-      if (TRANS) put_rows<T, P>(s.q, 2, col, pos, turned(q[i]));
-      else put_rows<T, P>(s.q, DK / 32, pos, col, q[i]);
+      const int col = i * 64 + c4;
+      k[i].template cut<W>(n - pos, dk - col);
+      q[i].template cut<W>(n - pos, dk - col);
+      k[i].put(s.ka, DK / 32, pos, col);
+      k[i].turned().put(s.kt, 2, col, pos);
+      if (TRANS) q[i].turned().put(s.q, 2, col, pos);
+      else q[i].put(s.q, DK / 32, pos, col);
     }
 #pragma unroll
     for (int i = 0; i < IMG; ++i)
@@ -540,10 +609,10 @@ __device__ __forceinline__ f4 four_rows(const float* c, int t, int g) {
   return *reinterpret_cast<const f4*>(c + t * 16 + 4 * g);
 }
 
-template <typename T, int DK>
+template <typename T, int DK, bool W>
 __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_chain_kernel(
     const DeltaArgs a, const unsigned char* prep, float* rec, int chunks, int tiles,
-    uint64_t blocks, bool wide) {
+    uint64_t blocks) {
   using M = Mode<T>;
   constexpr int U = DK / 32, MT = DK / 16, FULL = M::FULL, P = M::ROWS;
   extern __shared__ __align__(16) unsigned char lds[];
@@ -570,27 +639,27 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_chain_kernel(
             st[m][r] = a.state_in[state + (int64_t)(m * 16 + 4 * g + r) * a.dv + col];
     }
     ChainNext<T, DK> next;
-    f4 v[4];
+    uint32_t v[4][4];
     auto bring = [&](int c) {
       p.c = c;
       p.n = within(len, c);
-      next.load(a, prep + (lh * chunks + c) * PREP_BYTES, p, kh, wide);
+      next.template load<W>(a, prep + (lh * chunks + c) * PREP_BYTES, p, kh);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          v[t][r] = ld1(row_at<const T>(a.v, p, p.h, a.dv, min(t * 16 + 4 * g + r, p.n - 1)) +
-                        min(col, a.dv - 1));
+          v[t][r] = raw1(row_at<const T>(a.v, p, p.h, a.dv, min(t * 16 + 4 * g + r, p.n - 1)) +
+                         min(col, a.dv - 1));
     };
     if (last > 0) bring(0);
     for (int c = 0; c < last; ++c) {
       __syncthreads();
-      next.store(s);
+      next.template store<W>(s, p.n, a.dk);
       f4 vc[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) vc[t][r] = mine ? v[t][r] : 0.0f;
+        for (int r = 0; r < 4; ++r) vc[t][r] = mine ? value1<T>(v[t][r]) : 0.0f;
       const int n = p.n;
       __syncthreads();
       if (c + 1 < last) bring(c + 1);
@@ -688,10 +757,10 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_chain_kernel(
 
 // The gradient's chain, from the last chunk to the first: dS and dR of every
 // chunk, both with a column of d_v after the other, as S and N are kept.
-template <typename T, int DK>
+template <typename T, int DK, bool W>
 __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_chain_kernel(
     const DeltaGradArgs ga, const unsigned char* prep, float* grec, int chunks, int tiles,
-    uint64_t blocks, bool wide) {
+    uint64_t blocks) {
   using M = Mode<T>;
   constexpr int U = DK / 32, MT = DK / 16, FULL = M::FULL, P = M::ROWS;
   extern __shared__ __align__(16) unsigned char lds[];
@@ -719,28 +788,28 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_chain_kernel
             st[m][r] = ga.dstate_out[state + (int64_t)(m * 16 + 4 * g + r) * a.dv + col];
     }
     ChainNext<T, DK> next;
-    f4 o[4];
+    uint32_t o[4][4];
     auto bring = [&](int c) {
       p.c = c;
       p.n = within(len, c);
-      next.load(a, prep + (lh * chunks + c) * PREP_BYTES, p, kh, wide);
+      next.template load<W>(a, prep + (lh * chunks + c) * PREP_BYTES, p, kh);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          o[t][r] = ld1(row_at<const T>(ga.dout, p, p.h, a.dv, min(t * 16 + 4 * g + r, p.n - 1)) +
-                        min(col, a.dv - 1));
+          o[t][r] = raw1(row_at<const T>(ga.dout, p, p.h, a.dv, min(t * 16 + 4 * g + r, p.n - 1)) +
+                         min(col, a.dv - 1));
     };
     if (last > 0) bring(last - 1);
     for (int c = last - 1; c >= 0; --c) {
       __syncthreads();
-      next.store(s);
+      next.template store<W>(s, p.n, a.dk);
       f4 dout[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          dout[t][r] = mine && t * 16 + 4 * g + r < p.n ? o[t][r] : 0.0f;
+          dout[t][r] = mine && t * 16 + 4 * g + r < p.n ? value1<T>(o[t][r]) : 0.0f;
       __syncthreads();
       if (c > 0) bring(c - 1);
       if (v0 >= a.dv) continue;
@@ -847,10 +916,9 @@ struct LastLds {
   float tail[8];
   Decays dec;
 };
-template <typename T, int DK>
-__global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_last_kernel(
-    const DeltaGradArgs ga, const float* rec, const float* grec, int chunks, uint64_t blocks,
-    bool wide, bool wide_out) {
+template <typename T, int DK, bool W>
+__global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
+    const DeltaGradArgs ga, const float* rec, const float* grec, int chunks, uint64_t blocks) {
   constexpr int U = DK / 32, MT = DK / 16, FULL = Mode<T>::FULL, P = Mode<T>::ROWS;
   extern __shared__ __align__(16) unsigned char lds[];
   const DeltaArgs& a = ga.f;
@@ -882,22 +950,25 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_last_kernel(
     }
     // K and Q as rows: their products, the lengths
     auto bring_kq = [&](bool across_) {
-      Four k[DK / 64], q[DK / 64];
+      const int pos = tid / 16 * 4, c4 = tid % 16 * 4;
+      Rows4<T> k[DK / 64], q[DK / 64];
 #pragma unroll
       for (int i = 0; i < DK / 64; ++i) {
-        k[i] = four_of<T>(a.k, p, kh, a.dk, wide, tid / 16 * 4, i * 64 + tid % 16 * 4);
-        q[i] = four_of<T>(a.qr, p, kh, a.dk, wide, tid / 16 * 4, i * 64 + tid % 16 * 4);
+        k[i].template load<W>(a.k, p, kh, a.dk, pos, i * 64 + c4);
+        q[i].template load<W>(a.qr, p, kh, a.dk, pos, i * 64 + c4);
       }
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < DK / 64; ++i) {
-        const int pos = tid / 16 * 4, col = i * 64 + tid % 16 * 4;
+        const int col = i * 64 + c4;
+        k[i].template cut<W>(p.n - pos, a.dk - col);
+        q[i].template cut<W>(p.n - pos, a.dk - col);
         if (across_) {
-          put_rows<T, P>(s.k.a, 2, col, pos, turned(k[i]));
-          put_rows<T, P>(s.k.b, 2, col, pos, turned(q[i]));
+          k[i].turned().put(s.k.a, 2, col, pos);
+          q[i].turned().put(s.k.b, 2, col, pos);
         } else {
-          put_rows<T, P>(s.k.a, U, pos, col, k[i]);
-          put_rows<T, P>(s.k.b, U, pos, col, q[i]);
+          k[i].put(s.k.a, U, pos, col);
+          q[i].put(s.k.b, U, pos, col);
         }
       }
       __syncthreads();
@@ -936,8 +1007,8 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_last_kernel(
     f4 qo[MT], ko[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      qo[m] = ld4(row_at<const T>(a.qr, p, kh, a.dk, min(own, p.n - 1)), m * 16 + g4, a.dk, wide);
-      ko[m] = ld4(row_at<const T>(a.k, p, kh, a.dk, min(own, p.n - 1)), m * 16 + g4, a.dk, wide);
+      qo[m] = ld4<T, W>(row_at<const T>(a.qr, p, kh, a.dk, min(own, p.n - 1)), m * 16 + g4, a.dk);
+      ko[m] = ld4<T, W>(row_at<const T>(a.k, p, kh, a.dk, min(own, p.n - 1)), m * 16 + g4, a.dk);
     }
     // what K and Q are multiplied with, and what comes from the states
     f4 e[4] = {}, mid_e = ZERO, f[4] = {}, dq[MT] = {}, dk[MT] = {};
@@ -953,12 +1024,13 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_last_kernel(
         // N and dR: 8 x 16 pieces of 4 columns x 4 positions; dO as many; S and dS
         // 8 x DK / 4
         const int half = tid / 128, pg = tid % 16, vg = tid / 16 % 8, v4 = v0 + vg * 4;
-        Four x, od, sx[DK / 64], dx[DK / 64];
+        Four x, sx[DK / 64];
+        Rows4<T> od;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           x.v[i] = *reinterpret_cast<const f4*>((half ? dR : N) +
                                                 (int64_t)min(v4 + i, a.dv - 1) * C + pg * 4);
-        od = four_of<T>(half ? a.v : ga.dout, p, vh, a.dv, wide, pg * 4, v4);
+        od.template load<W>(half ? a.v : ga.dout, p, vh, a.dv, pg * 4, v4);
 #pragma unroll
         for (int i = 0; i < DK / 64; ++i) {
           const int d4 = (i * 16 + tid % 16) * 4;
@@ -968,7 +1040,6 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_last_kernel(
             sx[i].v[j] = *reinterpret_cast<const f4*>((half ? dS : S) +
                                                       (int64_t)min(sv + j, a.dv - 1) * DK + d4);
         }
-        (void)dx;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (v4 + i >= a.dv) {
@@ -978,24 +1049,25 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_last_kernel(
           }
         __syncthreads();
         const Four xt = turned(x);  // rows: positions
-        put_rows<T, FULL>(half ? s.v.r : s.v.n, 1, pg * 4, vg * 4, xt);
+        od.template cut<W>(p.n - pg * 4, a.dv - v4);
+        put_full<T>(half ? s.v.r : s.v.n, 1, pg * 4, vg * 4, xt);
         if (half) {
           // dV, and dR . v
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const f4 d = xt.v[i] * od.v[i];
+            const f4 d = xt.v[i] * od.r[i].value();
             dots[i] += d[0] + d[1] + d[2] + d[3];
             const int pos = pg * 4 + i;
             if (pos < rows)
-              st4(row_at<T>(ga.dv, p, vh, a.dv, pos), v4, a.dv, wide_out,
-                  pos < p.n ? xt.v[i] * s.dec.beta[pos] : ZERO);
+              st4<T, W>(row_at<T>(ga.dv, p, vh, a.dv, pos), v4, a.dv,
+                        pos < p.n ? xt.v[i] * s.dec.beta[pos] : ZERO);
           }
         } else {
-          put_rows<T, P>(s.v.o, 1, pg * 4, vg * 4, od);
+          od.put(s.v.o, 1, pg * 4, vg * 4);
         }
 #pragma unroll
         for (int i = 0; i < DK / 64; ++i)
-          put_rows<T, FULL>(half ? s.v.d : s.v.s, 1, (i * 16 + tid % 16) * 4, vg * 4, turned(sx[i]));
+          put_full<T>(half ? s.v.d : s.v.s, 1, (i * 16 + tid % 16) * 4, vg * 4, turned(sx[i]));
         __syncthreads();
         const Frag<FULL> no = get<FULL>(s.v.n, w, sl), ro = get<FULL>(s.v.r, w, sl);
         const Frag<P> oo = get<P>(s.v.o, w, sl);
@@ -1159,10 +1231,10 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_last_kernel(
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         const bool live = own < p.n;
-        st4(row_at<T>(ga.dq, p, kh, a.dk, own), m * 16 + g4, a.dk, wide_out,
-            live ? (dq[m] - qo[m] * fq) * rq : ZERO);
-        st4(row_at<T>(ga.dk, p, kh, a.dk, own), m * 16 + g4, a.dk, wide_out,
-            live ? (dk[m] - ko[m] * fk) * rk : ZERO);
+        st4<T, W>(row_at<T>(ga.dq, p, kh, a.dk, own), m * 16 + g4, a.dk,
+                  live ? (dq[m] - qo[m] * fq) * rq : ZERO);
+        st4<T, W>(row_at<T>(ga.dk, p, kh, a.dk, own), m * 16 + g4, a.dk,
+                  live ? (dk[m] - ko[m] * fk) * rk : ZERO);
       }
     }
     __syncthreads();
@@ -1174,9 +1246,8 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_last_kernel(
 // columns 4 x .. 4 x + 3 of rows y + RG i.  With S^T k and S^T q of the state
 // before, o = scale (e^g S^T q + beta (k . q) e): one sum over the rows, and
 // one barrier, a position.
-template <typename T, int DK, int CX>
-__global__ __launch_bounds__(256) void delta_step_kernel(const DeltaArgs a, uint64_t blocks,
-                                                         bool wide, bool wide_state) {
+template <typename T, int DK, int CX, bool W>
+__global__ __launch_bounds__(256) void delta_step_kernel(const DeltaArgs a, uint64_t blocks) {
   constexpr int RG = 256 / CX, RPT = DK / RG;
   __shared__ __align__(16) float kq[2][2][DK];
   __shared__ __align__(16) f4 part[2][4][2][CX];
@@ -1192,7 +1263,7 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const DeltaArgs a, uint
       const int row = y + RG * i;
       st[i] = ZERO;
       if (a.state_in && row < a.dk)
-        st[i] = ld4(a.state_in + state + (int64_t)row * a.dv, 4 * x, a.dv, wide_state);
+        st[i] = ld4<float, W>(a.state_in + state + (int64_t)row * a.dv, 4 * x, a.dv);
     }
     for (int t = 0; t < len; ++t) {
       const int buf = t & 1;
@@ -1206,8 +1277,8 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const DeltaArgs a, uint
           kv[i] = ld1(kr + lane + 64 * i);
           qv[i] = ld1(qr + lane + 64 * i);
         }
-      const f4 v = ld4((const T*)a.v.d + l * a.v.lane + t * a.v.row + (int64_t)h * a.dv, 4 * x,
-                       a.dv, wide);
+      const f4 v = ld4<T, W>((const T*)a.v.d + l * a.v.lane + t * a.v.row + (int64_t)h * a.dv, 4 * x,
+                             a.dv);
       const float g = *((const float*)a.g.d + l * a.g.lane + t * a.g.row + h);
       const float beta = *((const float*)a.beta.d + l * a.beta.lane + t * a.beta.row + h);
       const float decay = exp_of(log_decay(g));
@@ -1260,14 +1331,7 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const DeltaArgs a, uint
       for (int i = 0; i < RPT; ++i) {
         const int row = y + RG * i;
         if (row >= a.dk) continue;
-        float* o = a.state_out + state + (int64_t)row * a.dv + 4 * x;
-        if (wide_state) {
-          if (4 * x < a.dv) *reinterpret_cast<f4*>(o) = st[i];
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (4 * x + j < a.dv) o[j] = st[i][j];
-        }
+        st4<float, W>(a.state_out + state + (int64_t)row * a.dv, 4 * x, a.dv, st[i]);
       }
     }
   }
@@ -1301,46 +1365,40 @@ bool wide_rows(const R& r, int d, int size) {
   return rows_by_16(r.d, r.lane, r.row, d, size);
 }
 
-template <typename T>
-hipError_t delta_of(const DeltaArgs& a, hipStream_t s) {
-  const int size = sizeof(T);
+template <typename T, bool W>
+hipError_t delta_steps_of(const DeltaArgs& a, hipStream_t s) {
   const uint64_t heads = (uint64_t)a.q.lanes * a.HV;
-  if (by_steps(a.q.T) && !a.saved) {
-    const bool wide = wide_rows(a.v, a.dv, size);
-    const bool wide_state = a.dv % 4 == 0;  // states are 16-byte aligned
-    auto go = [&](auto kernel) {
-      BOA_LAUNCH(kernel, grid(heads), 256, 0, s, a, heads, wide, wide_state);
-      return hipGetLastError();
-    };
-    if (built(a.dk) == 64)
-      return a.dv <= 64 ? go(delta_step_kernel<T, 64, 16>) : go(delta_step_kernel<T, 64, 32>);
-    return a.dv <= 64 ? go(delta_step_kernel<T, 128, 16>) : go(delta_step_kernel<T, 128, 32>);
-  }
+  auto go = [&](auto kernel) {
+    BOA_LAUNCH(kernel, grid(heads), 256, 0, s, a, heads);
+    return hipGetLastError();
+  };
+  if (built(a.dk) == 64)
+    return a.dv <= 64 ? go(delta_step_kernel<T, 64, 16, W>) : go(delta_step_kernel<T, 64, 32, W>);
+  return a.dv <= 64 ? go(delta_step_kernel<T, 128, 16, W>) : go(delta_step_kernel<T, 128, 32, W>);
+}
+
+template <typename T, bool W>
+hipError_t delta_of(const DeltaArgs& a, hipStream_t s) {
+  const uint64_t heads = (uint64_t)a.q.lanes * a.HV;
   return for_width(a.dk, [&](auto dk) {
     constexpr int DK = dk;
-    const bool wide = wide_rows(a.qr, a.dk, size) && wide_rows(a.k, a.dk, size);
     const int chunks = chunks_of(a.q.T), tiles = (a.dv + 63) / 64;
     unsigned char* prep = (unsigned char*)a.work;
     const uint64_t all = heads * chunks;
-    BOA_LAUNCH((delta_prep_kernel<T, DK, false>), grid(all), 256, 0, s, a, prep, chunks, all, wide);
+    BOA_LAUNCH((delta_prep_kernel<T, DK, false, W>), grid(all), 256, 0, s, a, prep, chunks, all);
     hipError_t e = hipGetLastError();
     if (e) return e;
     const size_t lds = sizeof(ChainLds<T, DK, false>);
-    if ((e = room(delta_chain_kernel<T, DK>, lds))) return e;
-    BOA_LAUNCH((delta_chain_kernel<T, DK>), grid(heads * tiles), 256, lds, s, a,
-               (const unsigned char*)prep, a.saved, chunks, tiles, heads * tiles, wide);
+    if ((e = room(delta_chain_kernel<T, DK, W>, lds))) return e;
+    BOA_LAUNCH((delta_chain_kernel<T, DK, W>), grid(heads * tiles), 256, lds, s, a,
+               (const unsigned char*)prep, a.saved, chunks, tiles, heads * tiles);
     return hipGetLastError();
   });
 }
 
-template <typename T>
+template <typename T, bool W>
 hipError_t delta_grad_of(const DeltaGradArgs& ga, hipStream_t s) {
   const DeltaArgs& a = ga.f;
-  const int size = sizeof(T);
-  const bool wide = wide_rows(a.qr, a.dk, size) && wide_rows(a.k, a.dk, size);
-  const bool wide_last = wide && wide_rows(a.v, a.dv, size) && wide_rows(ga.dout, a.dv, size);
-  const bool wide_out = wide_rows(ga.dq, a.dk, size) && wide_rows(ga.dk, a.dk, size) &&
-                        wide_rows(ga.dv, a.dv, size);
   const uint64_t heads = (uint64_t)a.q.lanes * a.HV;
   return for_width(a.dk, [&](auto dk) {
     constexpr int DK = dk;
@@ -1348,21 +1406,29 @@ hipError_t delta_grad_of(const DeltaGradArgs& ga, hipStream_t s) {
     const uint64_t all = heads * chunks;
     unsigned char* prep = (unsigned char*)a.work;
     float* grec = (float*)(prep + all * PREP_BYTES);
-    BOA_LAUNCH((delta_prep_kernel<T, DK, true>), grid(all), 256, 0, s, a, prep, chunks, all, wide);
+    BOA_LAUNCH((delta_prep_kernel<T, DK, true, W>), grid(all), 256, 0, s, a, prep, chunks, all);
     hipError_t e = hipGetLastError();
     if (e) return e;
     size_t lds = sizeof(ChainLds<T, DK, true>);
-    if ((e = room(delta_grad_chain_kernel<T, DK>, lds))) return e;
-    BOA_LAUNCH((delta_grad_chain_kernel<T, DK>), grid(heads * tiles), 256, lds, s, ga,
-               (const unsigned char*)prep, grec, chunks, tiles, heads * tiles, wide);
+    if ((e = room(delta_grad_chain_kernel<T, DK, W>, lds))) return e;
+    BOA_LAUNCH((delta_grad_chain_kernel<T, DK, W>), grid(heads * tiles), 256, lds, s, ga,
+               (const unsigned char*)prep, grec, chunks, tiles, heads * tiles);
     if ((e = hipGetLastError())) return e;
     lds = sizeof(LastLds<T, DK>);
-    if ((e = room(delta_grad_last_kernel<T, DK>, lds))) return e;
+    if ((e = room(delta_grad_last_kernel<T, DK, W>, lds))) return e;
     const uint64_t last = (uint64_t)a.q.lanes * a.H * chunks;
-    BOA_LAUNCH((delta_grad_last_kernel<T, DK>), grid(last), 256, lds, s, ga, (const float*)a.saved,
-               (const float*)grec, chunks, last, wide_last, wide_out);
+    BOA_LAUNCH((delta_grad_last_kernel<T, DK, W>), grid(last), 256, lds, s, ga,
+               (const float*)a.saved, (const float*)grec, chunks, last);
     return hipGetLastError();
   });
+}
+
+// f(row type, whether all rows can be moved 16 bytes at a time)
+template <typename F>
+hipError_t for_rows(bool bf16, bool wide, F&& f) {
+  using std::bool_constant;
+  if (bf16) return wide ? f(uint16_t(), bool_constant<true>()) : f(uint16_t(), bool_constant<false>());
+  return wide ? f(float(), bool_constant<true>()) : f(float(), bool_constant<false>());
 }
 
 }  // namespace
@@ -1377,11 +1443,23 @@ int64_t delta_work_bytes(int lanes, int T, int, int HV, int dk, int dv, bool gra
 }
 
 hipError_t launch_delta(const DeltaArgs& a, hipStream_t s) {
-  return a.bf16 ? delta_of<uint16_t>(a, s) : delta_of<float>(a, s);
+  const int size = a.bf16 ? 2 : 4;
+  if (by_steps(a.q.T) && !a.saved) {
+    const bool wide = wide_rows(a.v, a.dv, size) && a.dv % 4 == 0;  // states are 16-byte aligned
+    return for_rows(a.bf16, wide, [&](auto t, auto w) { return delta_steps_of<decltype(t), w>(a, s); });
+  }
+  const bool wide = wide_rows(a.qr, a.dk, size) && wide_rows(a.k, a.dk, size);
+  return for_rows(a.bf16, wide, [&](auto t, auto w) { return delta_of<decltype(t), w>(a, s); });
 }
 
-hipError_t launch_delta_grad(const DeltaGradArgs& a, hipStream_t s) {
-  return a.f.bf16 ? delta_grad_of<uint16_t>(a, s) : delta_grad_of<float>(a, s);
+hipError_t launch_delta_grad(const DeltaGradArgs& g, hipStream_t s) {
+  const DeltaArgs& a = g.f;
+  const int size = a.bf16 ? 2 : 4;
+  const bool wide = wide_rows(a.qr, a.dk, size) && wide_rows(a.k, a.dk, size) &&
+                    wide_rows(a.v, a.dv, size) && wide_rows(g.dout, a.dv, size) &&
+                    wide_rows(g.dq, a.dk, size) && wide_rows(g.dk, a.dk, size) &&
+                    wide_rows(g.dv, a.dv, size);
+  return for_rows(a.bf16, wide, [&](auto t, auto w) { return delta_grad_of<decltype(t), w>(g, s); });
 }
 
 }  // namespace boa

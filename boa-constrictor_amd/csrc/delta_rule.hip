@@ -215,6 +215,36 @@ __device__ __forceinline__ void mma(f4& acc, const Frag<PA>& a, const Frag<PB>& 
   }
 }
 
+// the same right operand under N left ones: products that do not wait for each
+// other, part by part
+template <typename T, int N, int PA, int PB>
+__device__ __forceinline__ void mma(f4 (&acc)[N], const Frag<PA> (&a)[N], const Frag<PB>& b) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const f4 y = __builtin_bit_cast(f4, b.p[h]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f4, a[n].p[h])[e], y[e],
+                                                        acc[n], 0, 0, 0);
+    }
+  } else {
+    typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+    for (int s = 2; s >= 0; --s)
+#pragma unroll
+      for (int i = 0; i < PA; ++i)
+        if (s - i >= 0 && s - i < PB)
+#pragma unroll
+          for (int n = 0; n < N; ++n)
+            acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a[n].p[i]),
+                                                             __builtin_bit_cast(b8, b.p[s - i]),
+                                                             acc[n], 0, 0, 0);
+  }
+}
+
 // ---- operands in LDS -------------------------------------------------------
 // A block is 16 rows x 32 of k as the lanes hold it, piece by piece, 16 bytes a
 // lane; a tile of U blocks across.  The lanes of g are turned by 4 g, so that
@@ -226,6 +256,12 @@ __device__ __forceinline__ Frag<P> get(const u4* tile, int block, int slot) {
 #pragma unroll
   for (int p = 0; p < P; ++p) r.p[p] = tile[(block * P + p) * 64 + slot];
   return r;
+}
+// blocks b0, b0 + step, ..
+template <int P, int N>
+__device__ __forceinline__ void get(Frag<P> (&r)[N], const u4* tile, int b0, int step, int slot) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) r[n] = get<P>(tile, b0 + n * step, slot);
 }
 // four values of one row, k .. k + 3 (k a multiple of 4)
 template <typename T, int P>
@@ -342,9 +378,21 @@ template <bool TRANS>
 __device__ __forceinline__ constexpr int tri_block(int t, int u) {
   return TRANS ? (t < 2 ? 2 * t + u : t + 2) : (t < 2 ? t : 2 * t - 2 + u);
 }
-template <bool TRANS>
-__device__ __forceinline__ constexpr bool tri_has(int t, int u) {
-  return TRANS ? (t < 2 || u == 1) : (t >= 2 || u == 0);
+// acc += triangle x b
+template <typename T, bool TRANS, int PB>
+__device__ __forceinline__ void triangle(f4 (&acc)[4], const u4* tri, const Frag<PB> (&b)[2],
+                                         int slot) {
+  constexpr int FULL = Mode<T>::FULL, U = TRANS ? 1 : 0;  // the 32 of k that all tiles have
+  Frag<FULL> x[4], y[2];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) x[t] = get<FULL>(tri, tri_block<TRANS>(t, U), slot);
+#pragma unroll
+  for (int t = 0; t < 2; ++t) y[t] = get<FULL>(tri, tri_block<TRANS>(TRANS ? t : 2 + t, 1 - U), slot);
+  mma<T>(acc, x, b[U]);
+  f4 two[2] = {acc[TRANS ? 0 : 2], acc[TRANS ? 1 : 3]};
+  mma<T>(two, y, b[1 - U]);
+  acc[TRANS ? 0 : 2] = two[0];
+  acc[TRANS ? 1 : 3] = two[1];
 }
 // Coefficients of the rows, floats: beta; beta e^G / |k|; e^(G_64 - G) / |k|;
 // scale e^G / |q|; then e^G_64.
@@ -610,7 +658,7 @@ __device__ __forceinline__ f4 four_rows(const float* c, int t, int g) {
 }
 
 template <typename T, int DK, bool W>
-__global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_chain_kernel(
+__global__ __launch_bounds__(256, 1) void delta_chain_kernel(
     const DeltaArgs a, const unsigned char* prep, float* rec, int chunks, int tiles,
     uint64_t blocks) {
   using M = Mode<T>;
@@ -676,13 +724,14 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_chain_kernel(
 #pragma unroll
         for (int u = 0; u < U; ++u) sf[u] = full<T>(st[2 * u], st[2 * u + 1]);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          x[t] = o[t] = ZERO;
+        for (int t = 0; t < 4; ++t) x[t] = o[t] = ZERO;
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            mma<T>(x[t], get<P>(s.ka, t * U + u, sl), sf[u]);
-            mma<T>(o[t], get<P>(s.q, t * U + u, sl), sf[u]);
-          }
+        for (int u = 0; u < U; ++u) {
+          Frag<P> k[4], q[4];
+          get<P>(k, s.ka, u, U, sl);
+          get<P>(q, s.q, u, U, sl);
+          mma<T>(x, k, sf[u]);
+          mma<T>(o, q, sf[u]);
         }
       }
       f4 nn[4];
@@ -694,12 +743,8 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_chain_kernel(
 #pragma unroll
         for (int u = 0; u < 2; ++u) rf[u] = full<T>(x[2 * u], x[2 * u + 1]);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          nn[t] = ZERO;
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-            if (tri_has<false>(t, u)) mma<T>(nn[t], get<FULL>(s.tri, tri_block<false>(t, u), sl), rf[u]);
-        }
+        for (int t = 0; t < 4; ++t) nn[t] = ZERO;
+        triangle<T, false>(nn, s.tri, rf, sl);
       }
       if (rec && mine) {
 #pragma unroll
@@ -711,13 +756,8 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_chain_kernel(
 #pragma unroll
         for (int u = 0; u < 2; ++u) nf[u] = full<T>(nn[2 * u], nn[2 * u + 1]);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          o[t] *= four_rows(s.coef + 3 * C, t, g);
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-            if (tri_has<false>(t, u))
-              mma<T>(o[t], get<FULL>(s.tri, TRI + tri_block<false>(t, u), sl), nf[u]);
-        }
+        for (int t = 0; t < 4; ++t) o[t] *= four_rows(s.coef + 3 * C, t, g);
+        triangle<T, false>(o, s.tri + TRI * FULL * 64, nf, sl);
         Place here = p;
         here.c = c;
 #pragma unroll
@@ -736,10 +776,12 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_chain_kernel(
                           nn[2 * u + 1] * four_rows(s.coef + 2 * C, 2 * u + 1, g));
         const float all = s.coef[4 * C];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          st[m] *= all;
+        for (int m = 0; m < MT; ++m) st[m] *= all;
 #pragma unroll
-          for (int u = 0; u < 2; ++u) mma<T>(st[m], get<P>(s.kt, m * 2 + u, sl), nf[u]);
+        for (int u = 0; u < 2; ++u) {
+          Frag<P> k[MT];
+          get<P>(k, s.kt, u, 2, sl);
+          mma<T>(st, k, nf[u]);
         }
       }
     }
@@ -758,7 +800,7 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_chain_kernel(
 // The gradient's chain, from the last chunk to the first: dS and dR of every
 // chunk, both with a column of d_v after the other, as S and N are kept.
 template <typename T, int DK, bool W>
-__global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_chain_kernel(
+__global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
     const DeltaGradArgs ga, const unsigned char* prep, float* grec, int chunks, int tiles,
     uint64_t blocks) {
   using M = Mode<T>;
@@ -828,16 +870,16 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_chain_kernel
 #pragma unroll
         for (int u = 0; u < 2; ++u) of[u] = rows_of<T>(dout[2 * u], dout[2 * u + 1]);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          dn[t] = ZERO;
+        for (int t = 0; t < 4; ++t) dn[t] = ZERO;
 #pragma unroll
-          for (int u = 0; u < U; ++u) mma<T>(dn[t], get<P>(s.ka, t * U + u, sl), sf[u]);
-          dn[t] *= four_rows(s.coef + 2 * C, t, g);
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-            if (tri_has<true>(t, u))
-              mma<T>(dn[t], get<FULL>(s.tri, TRI + tri_block<true>(t, u), sl), of[u]);
+        for (int u = 0; u < U; ++u) {
+          Frag<P> k[4];
+          get<P>(k, s.ka, u, U, sl);
+          mma<T>(dn, k, sf[u]);
         }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) dn[t] *= four_rows(s.coef + 2 * C, t, g);
+        triangle<T, true>(dn, s.tri + TRI * FULL * 64, of, sl);
       }
       f4 dr[4];
       {
@@ -845,12 +887,8 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_chain_kernel
 #pragma unroll
         for (int u = 0; u < 2; ++u) nf[u] = full<T>(dn[2 * u], dn[2 * u + 1]);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          dr[t] = ZERO;
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-            if (tri_has<true>(t, u)) mma<T>(dr[t], get<FULL>(s.tri, tri_block<true>(t, u), sl), nf[u]);
-        }
+        for (int t = 0; t < 4; ++t) dr[t] = ZERO;
+        triangle<T, true>(dr, s.tri, nf, sl);
       }
       if (mine) {
 #pragma unroll
@@ -868,13 +906,14 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_chain_kernel
         }
         const float all = s.coef[4 * C];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          st[m] *= all;
+        for (int m = 0; m < MT; ++m) st[m] *= all;
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            mma<T>(st[m], get<P>(s.q, m * 2 + u, sl), of[u]);
-            mma<T>(st[m], get<P>(s.kt, m * 2 + u, sl), rf[u]);
-          }
+        for (int u = 0; u < 2; ++u) {
+          Frag<P> k[MT], q[MT];
+          get<P>(q, s.q, u, 2, sl);
+          get<P>(k, s.kt, u, 2, sl);
+          mma<T>(st, q, of[u]);
+          mma<T>(st, k, rf[u]);
         }
       }
     }

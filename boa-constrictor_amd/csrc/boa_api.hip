@@ -1155,6 +1155,10 @@ struct TrainCheck {
     return p == s.u.d || p == s.delta.d || p == s.z.d || p == s.b.d || p == s.c.d || p == s.d_A ||
            p == s.d_D || p == s.d_delta_bias || p == s.d_state_in;
   }
+  // the delta rule's rows: 64 of them within 32 bits of bytes
+  void nearer(const boa_rows* r, const char* what) {
+    that(bad || r->row_stride <= (int64_t)1 << 23, "a row stride is over 2^23: ", what);
+  }
   // int8 rows
   void rows8(const boa_rows* r, int64_t width, bool written, const char* what) {
     const int keep = size;
@@ -1177,13 +1181,13 @@ struct TrainCheck {
     that(delta_sizes_ok(s->lanes, s->T, s->heads, s->v_heads, s->d_k, s->d_v),
          "v_heads has to be a multiple of heads, 1 .. 1024, d_k and d_v 1 .. 128");
     floats(s->d_lens, 4, true, "lens");
-    in(&s->q, "q"), near(&s->q, "q");
-    in(&s->k, "k"), near(&s->k, "k");
-    in(&s->v, "v"), near(&s->v, "v");
+    in(&s->q, "q"), nearer(&s->q, "q");
+    in(&s->k, "k"), nearer(&s->k, "k");
+    in(&s->v, "v"), nearer(&s->v, "v");
     const int keep = size;
     size = 4;
-    in(&s->g, "g"), near(&s->g, "g");
-    in(&s->beta, "beta"), near(&s->beta, "beta");
+    in(&s->g, "g"), nearer(&s->g, "g");
+    in(&s->beta, "beta"), nearer(&s->beta, "beta");
     size = keep;
     floats(s->d_state_in, 16, true, "state_in");
     a = DeltaArgs{};
@@ -2073,7 +2077,7 @@ int boa_delta_rule(boa_ctx* c, const boa_delta* d, const boa_rows* out, float* d
     DeltaArgs a{};
     k.delta(d, a);
     if (k.bad) return hipSuccess;
-    k.out(out, (int64_t)d->v_heads * d->d_v, "out"), k.near(out, "out");
+    k.out(out, (int64_t)d->v_heads * d->d_v, "out"), k.nearer(out, "out");
     k.floats(d_state_out, 16, true, "state_out");
     k.floats(d_saved, 16, true, "saved");
     k.that(k.bad || !k.delta_input(*d, out->d), "out is an input");
@@ -2098,15 +2102,15 @@ int boa_delta_rule_grad(boa_ctx* c, const boa_delta* d, const float* d_saved, co
     if (k.bad) return hipSuccess;
     const int64_t qk = (int64_t)d->heads * d->d_k;
     k.floats(d_saved, 16, false, "saved");
-    k.in(dout, "dout"), k.near(dout, "dout");
+    k.in(dout, "dout"), k.nearer(dout, "dout");
     k.floats(d_dstate_out, 4, true, "dstate_out");
-    k.out(&g->dq, qk, "dq"), k.near(&g->dq, "dq");
-    k.out(&g->dk, qk, "dk"), k.near(&g->dk, "dk");
-    k.out(&g->dv, (int64_t)d->v_heads * d->d_v, "dv"), k.near(&g->dv, "dv");
+    k.out(&g->dq, qk, "dq"), k.nearer(&g->dq, "dq");
+    k.out(&g->dk, qk, "dk"), k.nearer(&g->dk, "dk");
+    k.out(&g->dv, (int64_t)d->v_heads * d->d_v, "dv"), k.nearer(&g->dv, "dv");
     const int keep = k.size;
     k.size = 4;
-    k.out(&g->dg, d->v_heads, "dg"), k.near(&g->dg, "dg");
-    k.out(&g->dbeta, d->v_heads, "dbeta"), k.near(&g->dbeta, "dbeta");
+    k.out(&g->dg, d->v_heads, "dg"), k.nearer(&g->dg, "dg");
+    k.out(&g->dbeta, d->v_heads, "dbeta"), k.nearer(&g->dbeta, "dbeta");
     k.size = keep;
     k.floats(g->d_dstate_in, 4, true, "dstate_in");
     for (const void* p : {(const void*)g->dq.d, (const void*)g->dk.d, (const void*)g->dv.d,

@@ -78,17 +78,19 @@ template <typename T>
 struct Raw {
   using V = std::conditional_t<sizeof(T) == 4, f4, u2>;
   V v;
-  template <bool W>
-  __device__ __forceinline__ void load(const T* row, int c, int d) {
+  // from the element `row` on of what `from` gives by element
+  template <bool W, typename F>
+  __device__ __forceinline__ void load(const F& from, uint32_t row, int c, int d) {
     if constexpr (W) {
-      v = *reinterpret_cast<const V*>(row + (c < d ? c : 0));
+      v = *reinterpret_cast<const V*>(from.at(row + (c < d ? c : 0)));
     } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = row[min(c + i, d - 1)];
+      for (int i = 0; i < 4; ++i) v[i] = *from.at(row + min(c + i, d - 1));
     } else {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        v[i] = row[min(c + 2 * i, d - 1)] | (uint32_t)row[min(c + 2 * i + 1, d - 1)] << 16;
+        v[i] = *from.at(row + min(c + 2 * i, d - 1)) |
+               (uint32_t)*from.at(row + min(c + 2 * i + 1, d - 1)) << 16;
     }
   }
   // zero from element n on
@@ -103,15 +105,34 @@ struct Raw {
       v[1] = n <= 2 ? 0 : (n == 3 ? v[1] & 0xFFFFu : v[1]);
     }
   }
+  // as the first `left` elements (of four) from `element` on
+  template <bool W, typename F>
+  __device__ __forceinline__ void store(const F& to, uint32_t element, int left) const {
+    if constexpr (W) {
+      if (left > 0) *reinterpret_cast<V*>(to.at(element)) = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < left) {
+          if constexpr (sizeof(T) == 4) *to.at(element + i) = v[i];
+          else *to.at(element + i) = (uint16_t)(v[i / 2] >> (16 * (i % 2)));
+        }
+    }
+  }
   __device__ __forceinline__ f4 value() const {
     if constexpr (sizeof(T) == 4) return v;
     else return f4{u2f(v[0] << 16), u2f(v[0] & 0xFFFF0000u), u2f(v[1] << 16), u2f(v[1] & 0xFFFF0000u)};
   }
 };
+template <typename T>
+struct Plain {
+  const T* p;
+  __device__ __forceinline__ const T* at(uint32_t element) const { return p + element; }
+};
 template <typename T, bool W>
 __device__ __forceinline__ f4 ld4(const T* row, int c, int d) {
   Raw<T> r;
-  r.template load<W>(row, c, d);
+  r.template load<W>(Plain<T>{row}, 0, c, d);
   r.template cut<W>(d - c);
   return r.value();
 }
@@ -247,9 +268,10 @@ __device__ __forceinline__ void mma(f4 (&acc)[N], const Frag<PA> (&a)[N], const 
 
 // ---- operands in LDS -------------------------------------------------------
 // A block is 16 rows x 32 of k as the lanes hold it, piece by piece, 16 bytes a
-// lane; a tile of U blocks across.  The lanes of g are turned by 4 g, so that
-// writes of neighbouring k fall into different banks.
-__device__ __forceinline__ int slot_of(int i, int g) { return (i ^ (g << 2)) + 16 * g; }
+// lane; a tile of U blocks across.  The rows of each g are in another order, so
+// that four rows and four groups of k that are written at once fall into
+// different banks.
+__device__ __forceinline__ int slot_of(int i, int g) { return (i ^ g) + 16 * g; }
 template <int P>
 __device__ __forceinline__ Frag<P> get(const u4* tile, int block, int slot) {
   Frag<P> r;
@@ -296,6 +318,19 @@ __device__ __forceinline__ void put_full(u4* tile, int U, int row, int k, const 
   for (int e = 0; e < 4; ++e) put<T, Mode<T>::FULL>(tile, U, row + e, k, x.v[e]);
 }
 
+// a value that is the same in all lanes, kept in scalar registers
+__device__ __forceinline__ int same(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ uint64_t same(uint64_t x) {
+  return (uint64_t)(uint32_t)same((int)(x >> 32)) << 32 | (uint32_t)same((int)x);
+}
+template <typename T>
+__device__ __forceinline__ T* same(T* p) { return (T*)same((uint64_t)p); }
+// p[i] of elements of T, i of 32 bits beside a scalar address
+template <typename T, typename P>
+__device__ __forceinline__ T* at32(P* p, uint32_t i) {
+  return reinterpret_cast<T*>((char*)p + (uint64_t)(i * (uint32_t)sizeof(T)));
+}
+
 struct Place {
   int l, h, c;     // lane, head, chunk
   int n;           // positions of the chunk within the lane's length
@@ -304,27 +339,31 @@ __device__ __forceinline__ int within(int len, int c) {
   const int left = len - c * C;
   return left < 0 ? 0 : (left < C ? left : C);
 }
-// the first element of a chunk's row for a head of d columns
+// The rows of a chunk, one head of d columns: where the first begins and how far
+// apart they are.  All of it is the same in the whole block, so an element's
+// address is a scalar one plus 32 bits (64 rows with strides up to 2^23 elements).
 template <typename T>
-__device__ __forceinline__ T* row_at(const RowsIn& r, const Place& p, int h, int d, int row) {
-  return (T*)r.d + p.l * r.lane + (int64_t)(p.c * C + row) * r.row + (int64_t)h * d;
-}
-template <typename T>
-__device__ __forceinline__ T* row_at(const RowsOut& r, const Place& p, int h, int d, int row) {
-  return (T*)r.d + p.l * r.lane + (int64_t)(p.c * C + row) * r.row + (int64_t)h * d;
-}
+struct Chunk {
+  T* p;
+  uint32_t row;  // elements
+  template <typename R>
+  __device__ __forceinline__ Chunk(const R& r, const Place& at, int h, int d)
+      : p(same((T*)r.d + at.l * r.lane + (int64_t)at.c * C * r.row + (int64_t)h * d)),
+        row((uint32_t)r.row) {}
+  __device__ __forceinline__ T* at(uint32_t element) const { return at32<T>(p, element); }
+};
+
 // Rows pos .. pos + 3, columns col .. col + 3 of a chunk's rows, a thread: loaded,
 // later put as rows (k along them) or across (k over the positions), with zeros
 // past the chunk's positions and past d
 template <typename T>
 struct Rows4 {
   Raw<T> r[4];
+  // n: the chunk's positions, one at least
   template <bool W>
-  __device__ __forceinline__ void load(const RowsIn& from, const Place& p, int h, int d, int pos,
-                                       int col) {
+  __device__ __forceinline__ void load(const Chunk<const T>& from, int n, int d, int pos, int col) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      r[e].template load<W>(row_at<const T>(from, p, h, d, min(pos + e, p.n - 1)), col, d);
+    for (int e = 0; e < 4; ++e) r[e].template load<W>(from, min(pos + e, n - 1) * from.row, col, d);
   }
   // rows from n on and columns from d on
   template <bool W>
@@ -361,12 +400,17 @@ struct Rows4 {
     }
   }
 };
-// one element as it lies in memory
-__device__ __forceinline__ uint32_t raw1(const float* p) { return f2u(*p); }
-__device__ __forceinline__ uint32_t raw1(const uint16_t* p) { return *p; }
+// the rows that a lane holds of a 16 x 16 result: two of them, one under the other,
+// from an operand across their rows
 template <typename T>
-__device__ __forceinline__ float value1(uint32_t x) {
-  return sizeof(T) == 4 ? u2f(x) : u2f(x << 16);
+__device__ __forceinline__ void results_of(f4& a, f4& b, const Frag<Mode<T>::ROWS>& f) {
+  if constexpr (sizeof(T) == 4) {
+    a = __builtin_bit_cast(f4, f.p[0]);
+    b = __builtin_bit_cast(f4, f.p[1]);
+  } else {
+    a = Raw<T>{u2{f.p[0][0], f.p[0][1]}}.value();
+    b = Raw<T>{u2{f.p[0][2], f.p[0][3]}}.value();
+  }
 }
 
 // ---- what passes between the kernels, of a (lane, value head, chunk) -------
@@ -457,18 +501,18 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a, unsi
   const int i16 = lane % 16, g = lane / 16, g4 = 4 * g, sl = slot_of(i16, g);
   for (uint64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
     Place p;
-    p.c = (int)(b % chunks);
-    p.h = (int)(b / chunks % a.HV);
-    p.l = (int)(b / chunks / a.HV);
-    p.n = within(seq_len(a.q, p.l), p.c);
+    p.c = same((int)(b % chunks));
+    p.h = same((int)(b / chunks % a.HV));
+    p.l = same((int)(b / chunks / a.HV));
+    p.n = same(within(seq_len(a.q, p.l), p.c));
     if (!p.n) continue;
-    const int kh = p.h / (a.HV / a.H);
+    const int kh = same(p.h / (a.HV / a.H));
     const int pos = tid / 16 * 4, col = tid % 16 * 4;
     Rows4<T> k[DK / 64], q[DK / 64];
 #pragma unroll
     for (int i = 0; i < DK / 64; ++i) {
-      k[i].template load<W>(a.k, p, kh, a.dk, pos, i * 64 + col);
-      q[i].template load<W>(a.qr, p, kh, a.dk, pos, i * 64 + col);
+      k[i].template load<W>(Chunk<const T>(a.k, p, kh, a.dk), p.n, a.dk, pos, i * 64 + col);
+      q[i].template load<W>(Chunk<const T>(a.qr, p, kh, a.dk), p.n, a.dk, pos, i * 64 + col);
     }
     __syncthreads();
     decays_of(s, a, p);
@@ -599,46 +643,56 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a, unsi
 // ---- chain -----------------------------------------------------------------
 // A block per (lane, value head, 64 columns), a wave 16 of them.  Of a chunk the
 // block's LDS holds K as rows and across, Q as rows (the gradient's chain: across),
-// T and P (there: transposed) and the coefficients; the next chunk's are under
-// way in registers.  The state, 16 columns of it, stays in the wave's registers.
+// T and P (there: transposed), v across and the coefficients; the next chunk's are
+// under way in registers.  The state, 16 columns of it, stays in the wave's registers.
 template <typename T, int DK, bool TRANS>
 struct ChainLds {
   u4 ka[4 * (DK / 32) * Mode<T>::ROWS * 64], kt[DK / 16 * 2 * Mode<T>::ROWS * 64];
   u4 q[4 * (DK / 32) * Mode<T>::ROWS * 64];  // rows, or across: as many blocks
+  u4 v[4 * 2 * Mode<T>::ROWS * 64];  // v (dO), across: 16 columns a wave; then its results
   u4 tri[IMAGE<T>];
   float coef[COEF];
 };
 template <typename T, int DK>
 struct ChainNext {
   static constexpr int IMG = (IMAGE<T> + 255) / 256;
-  Rows4<T> k[DK / 64], q[DK / 64];
+  Rows4<T> k[DK / 64], q[DK / 64], v;
   u4 img[IMG];
   float coef[2];
   template <bool W>
   __device__ __forceinline__ void load(const DeltaArgs& a, const unsigned char* prep, const Place& p,
-                                       int kh) {
+                                       int kh, const RowsIn& rows, int v0) {
     const int tid = threadIdx.x, pos = tid / 16 * 4, col = tid % 16 * 4;
 #pragma unroll
     for (int i = 0; i < IMG; ++i)
-      img[i] = reinterpret_cast<const u4*>(prep)[min(tid + 256 * i, IMAGE<T> - 1)];
-    const float* c = reinterpret_cast<const float*>(prep + PREP_BYTES - COEF * 4);
-    coef[0] = c[tid];
-    coef[1] = c[4 * C];
+      img[i] = *at32<const u4>(prep, min(tid + 256 * i, IMAGE<T> - 1));
+    const unsigned char* c = prep + PREP_BYTES - COEF * 4;
+    coef[0] = *at32<const float>(c, tid);
+    coef[1] = *at32<const float>(c, 4 * C);
 #pragma unroll
     for (int i = 0; i < DK / 64; ++i) {
-      k[i].template load<W>(a.k, p, kh, a.dk, pos, i * 64 + col);
-      q[i].template load<W>(a.qr, p, kh, a.dk, pos, i * 64 + col);
+      k[i].template load<W>(Chunk<const T>(a.k, p, kh, a.dk), p.n, a.dk, pos, i * 64 + col);
+      q[i].template load<W>(Chunk<const T>(a.qr, p, kh, a.dk), p.n, a.dk, pos, i * 64 + col);
     }
+    v.template load<W>(Chunk<const T>(rows, p, p.h, a.dv), p.n, a.dv, pos, v0 + col);
   }
   // n: the chunk's positions
   template <bool W, bool TRANS>
-  __device__ __forceinline__ void store(ChainLds<T, DK, TRANS>& s, int n, int dk) {
+  __device__ __forceinline__ void store(ChainLds<T, DK, TRANS>& s, int n, int dk, int dv) {
     const int tid = threadIdx.x, pos = tid / 16 * 4, c4 = tid % 16 * 4;
+    // dv: columns of v left from the block's first one on
+    if (n < C || dv < 64) v.template cut<W>(n - pos, dv - c4);
+    v.turned().put(s.v, 2, c4, pos);
+    if (n < C || dk < DK) {
+#pragma unroll
+      for (int i = 0; i < DK / 64; ++i) {
+        k[i].template cut<W>(n - pos, dk - i * 64 - c4);
+        q[i].template cut<W>(n - pos, dk - i * 64 - c4);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < DK / 64; ++i) {
       const int col = i * 64 + c4;
-      k[i].template cut<W>(n - pos, dk - col);
-      q[i].template cut<W>(n - pos, dk - col);
       k[i].put(s.ka, DK / 32, pos, col);
       k[i].turned().put(s.kt, 2, col, pos);
       if (TRANS) q[i].turned().put(s.q, 2, col, pos);
@@ -657,23 +711,54 @@ __device__ __forceinline__ f4 four_rows(const float* c, int t, int g) {
   return *reinterpret_cast<const f4*>(c + t * 16 + 4 * g);
 }
 
+// A wave's 64 x 16 results as rows from column v0 on: each lane puts its column
+// into its slots of the wave's two blocks and takes four rows of four columns.
+template <typename T, bool W>
+__device__ __forceinline__ void put_result(u4* tile, const f4 (&o)[4], int wave, int lane, int slot,
+                                           const Chunk<T>& out, int n, int v0, int dv) {
+  constexpr int P = Mode<T>::ROWS;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const Frag<P> f = rows_of<T>(o[2 * u], o[2 * u + 1]);
+#pragma unroll
+    for (int p = 0; p < P; ++p) tile[((wave * 2 + u) * P + p) * 64 + slot] = f.p[p];
+  }
+  // the wave's own LDS accesses are in order; the compiler's have to be
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const int pg = lane / 4, cg = lane % 4, block = wave * 2 + pg / 8, h = pg / 4 % 2;
+  Rows4<T> x;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int s = slot_of(cg * 4 + c, pg % 4);
+    if constexpr (sizeof(T) == 4) x.r[c].v = __builtin_bit_cast(f4, tile[(block * 2 + h) * 64 + s]);
+    else x.r[c].v = reinterpret_cast<const u2*>(tile + block * 64 + s)[h];
+  }
+  x = x.turned();
+  const int col = v0 + cg * 4;
+  const uint32_t first = 4 * pg * out.row + col;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (4 * pg + e < n) x.r[e].template store<W>(out, first + e * out.row, dv - col);
+}
+
 template <typename T, int DK, bool W>
 __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
     const DeltaArgs a, const unsigned char* prep, float* rec, int chunks, int tiles,
-    uint64_t blocks) {
+    uint32_t blocks) {
   using M = Mode<T>;
   constexpr int U = DK / 32, MT = DK / 16, FULL = M::FULL, P = M::ROWS;
   extern __shared__ __align__(16) unsigned char lds[];
   ChainLds<T, DK, false>& s = *reinterpret_cast<ChainLds<T, DK, false>*>(lds);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i16 = lane % 16, g = lane / 16, sl = slot_of(i16, g);
-  for (uint64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const uint64_t lh = b / tiles;
+  for (uint32_t b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const uint32_t lh = same((int)(b / tiles));
     Place p;
-    p.h = (int)(lh % a.HV);
-    p.l = (int)(lh / a.HV);
-    const int kh = p.h / (a.HV / a.H), len = seq_len(a.q, p.l), last = (len + C - 1) / C;
-    const int v0 = (int)(b % tiles) * 64 + wave * 16, col = v0 + i16;
+    p.l = same((int)(lh / a.HV));
+    p.h = lh - p.l * a.HV;
+    const int kh = same(p.h / (a.HV / a.H)), len = same(seq_len(a.q, p.l)), last = (len + C - 1) / C;
+    const int vb = same((int)(b - lh * tiles) * 64), v0 = vb + wave * 16, col = v0 + i16;
     const bool mine = col < a.dv;
     const int64_t state = (int64_t)lh * a.dk * a.dv;
     f4 st[MT];
@@ -687,36 +772,24 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
             st[m][r] = a.state_in[state + (int64_t)(m * 16 + 4 * g + r) * a.dv + col];
     }
     ChainNext<T, DK> next;
-    uint32_t v[4][4];
     auto bring = [&](int c) {
       p.c = c;
       p.n = within(len, c);
-      next.template load<W>(a, prep + (lh * chunks + c) * PREP_BYTES, p, kh);
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          v[t][r] = raw1(row_at<const T>(a.v, p, p.h, a.dv, min(t * 16 + 4 * g + r, p.n - 1)) +
-                         min(col, a.dv - 1));
+      next.template load<W>(a, same(prep + ((uint64_t)lh * chunks + c) * PREP_BYTES), p, kh, a.v, vb);
     };
     if (last > 0) bring(0);
     for (int c = 0; c < last; ++c) {
       __syncthreads();
-      next.template store<W>(s, p.n, a.dk);
-      f4 vc[4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) vc[t][r] = mine ? value1<T>(v[t][r]) : 0.0f;
+      next.template store<W>(s, p.n, a.dk, a.dv - vb);
       const int n = p.n;
       __syncthreads();
       if (c + 1 < last) bring(c + 1);
       if (v0 >= a.dv) continue;
-      float* at = rec ? rec + (lh * chunks + c) * (int64_t)(a.dv * (DK + C)) : nullptr;
+      float* at = same(rec ? rec + ((int64_t)lh * chunks + c) * (a.dv * (DK + C)) : nullptr);
       if (rec && mine) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
-          *reinterpret_cast<f4*>(at + (int64_t)col * DK + m * 16 + 4 * g) = st[m];
+          *at32<f4>(at, col * (DK / 4) + m * 4 + g) = st[m];
       }
       f4 o[4], x[4];
       {
@@ -736,6 +809,10 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
       }
       f4 nn[4];
       {
+        f4 vc[4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          results_of<T>(vc[2 * u], vc[2 * u + 1], get<P>(s.v, wave * 2 + u, sl));
 #pragma unroll
         for (int t = 0; t < 4; ++t)
           x[t] = four_rows(s.coef, t, g) * vc[t] - four_rows(s.coef + C, t, g) * x[t];
@@ -746,11 +823,6 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
         for (int t = 0; t < 4; ++t) nn[t] = ZERO;
         triangle<T, false>(nn, s.tri, rf, sl);
       }
-      if (rec && mine) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-          *reinterpret_cast<f4*>(at + a.dv * DK + (int64_t)col * C + t * 16 + 4 * g) = nn[t];
-      }
       {
         Frag<FULL> nf[2];
 #pragma unroll
@@ -758,15 +830,6 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
 #pragma unroll
         for (int t = 0; t < 4; ++t) o[t] *= four_rows(s.coef + 3 * C, t, g);
         triangle<T, false>(o, s.tri + TRI * FULL * 64, nf, sl);
-        Place here = p;
-        here.c = c;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int row = t * 16 + 4 * g + r;
-            if (row < n && mine) st1(row_at<T>(a.out, here, p.h, a.dv, row) + col, o[t][r]);
-          }
       }
       {
         Frag<FULL> nf[2];
@@ -784,6 +847,14 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
           mma<T>(st, k, nf[u]);
         }
       }
+      if (rec && mine) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) *at32<f4>(at + a.dv * DK, col * (C / 4) + t * 4 + g) = nn[t];
+      }
+      // O, from a column to a row in each lane: through the wave's own part of v
+      Place here = p;
+      here.c = c;
+      put_result<T, W>(s.v, o, wave, lane, sl, Chunk<T>(a.out, here, p.h, a.dv), n, v0, a.dv);
     }
     if (a.state_out && mine) {
 #pragma unroll
@@ -802,7 +873,7 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
 template <typename T, int DK, bool W>
 __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
     const DeltaGradArgs ga, const unsigned char* prep, float* grec, int chunks, int tiles,
-    uint64_t blocks) {
+    uint32_t blocks) {
   using M = Mode<T>;
   constexpr int U = DK / 32, MT = DK / 16, FULL = M::FULL, P = M::ROWS;
   extern __shared__ __align__(16) unsigned char lds[];
@@ -810,13 +881,13 @@ __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
   ChainLds<T, DK, true>& s = *reinterpret_cast<ChainLds<T, DK, true>*>(lds);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i16 = lane % 16, g = lane / 16, sl = slot_of(i16, g);
-  for (uint64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const uint64_t lh = b / tiles;
+  for (uint32_t b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const uint32_t lh = same((int)(b / tiles));
     Place p;
-    p.h = (int)(lh % a.HV);
-    p.l = (int)(lh / a.HV);
-    const int kh = p.h / (a.HV / a.H), len = seq_len(a.q, p.l), last = (len + C - 1) / C;
-    const int v0 = (int)(b % tiles) * 64 + wave * 16, col = v0 + i16;
+    p.l = same((int)(lh / a.HV));
+    p.h = lh - p.l * a.HV;
+    const int kh = same(p.h / (a.HV / a.H)), len = same(seq_len(a.q, p.l)), last = (len + C - 1) / C;
+    const int vb = same((int)(b - lh * tiles) * 64), v0 = vb + wave * 16, col = v0 + i16;
     const bool mine = col < a.dv;
     const int64_t state = (int64_t)lh * a.dk * a.dv;
     f4 st[MT];
@@ -830,45 +901,33 @@ __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
             st[m][r] = ga.dstate_out[state + (int64_t)(m * 16 + 4 * g + r) * a.dv + col];
     }
     ChainNext<T, DK> next;
-    uint32_t o[4][4];
     auto bring = [&](int c) {
       p.c = c;
       p.n = within(len, c);
-      next.template load<W>(a, prep + (lh * chunks + c) * PREP_BYTES, p, kh);
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          o[t][r] = raw1(row_at<const T>(ga.dout, p, p.h, a.dv, min(t * 16 + 4 * g + r, p.n - 1)) +
-                         min(col, a.dv - 1));
+      next.template load<W>(a, same(prep + ((uint64_t)lh * chunks + c) * PREP_BYTES), p, kh, ga.dout, vb);
     };
     if (last > 0) bring(last - 1);
     for (int c = last - 1; c >= 0; --c) {
       __syncthreads();
-      next.template store<W>(s, p.n, a.dk);
-      f4 dout[4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          dout[t][r] = mine && t * 16 + 4 * g + r < p.n ? value1<T>(o[t][r]) : 0.0f;
+      next.template store<W>(s, p.n, a.dk, a.dv - vb);
       __syncthreads();
       if (c > 0) bring(c - 1);
       if (v0 >= a.dv) continue;
-      float* at = grec + (lh * chunks + c) * (int64_t)(a.dv * (DK + C));
+      float* at = same(grec + ((int64_t)lh * chunks + c) * (a.dv * (DK + C)));
       if (mine) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
-          *reinterpret_cast<f4*>(at + (int64_t)col * DK + m * 16 + 4 * g) = st[m];
+          *at32<f4>(at, col * (DK / 4) + m * 4 + g) = st[m];
       }
-      f4 dn[4];
+      f4 dn[4], dout[4];
       {
         Frag<FULL> sf[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) sf[u] = full<T>(st[2 * u], st[2 * u + 1]);
         Frag<P> of[2];
+        get<P>(of, s.v, wave * 2, 1, sl);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) of[u] = rows_of<T>(dout[2 * u], dout[2 * u + 1]);
+        for (int u = 0; u < 2; ++u) results_of<T>(dout[2 * u], dout[2 * u + 1], of[u]);
 #pragma unroll
         for (int t = 0; t < 4; ++t) dn[t] = ZERO;
 #pragma unroll
@@ -893,7 +952,7 @@ __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
       if (mine) {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
-          *reinterpret_cast<f4*>(at + a.dv * DK + (int64_t)col * C + t * 16 + 4 * g) = dr[t];
+          *at32<f4>(at + a.dv * DK, col * (C / 4) + t * 4 + g) = dr[t];
       }
       {
         Frag<FULL> of[2], rf[2];
@@ -967,10 +1026,10 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
   const int group = a.HV / a.H, own = w * 16 + i16;
   for (uint64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
     Place p;
-    p.c = (int)(b % chunks);
-    const int kh = (int)(b / chunks % a.H);
-    p.l = (int)(b / chunks / a.H);
-    p.n = within(seq_len(a.q, p.l), p.c);
+    p.c = same((int)(b % chunks));
+    const int kh = same((int)(b / chunks % a.H));
+    p.l = same((int)(b / chunks / a.H));
+    p.n = same(within(seq_len(a.q, p.l), p.c));
     const int rows = min(C, a.q.T - p.c * C);
     if (!p.n) {  // past the lane's length: zero
       for (int i = tid; i < rows * group; i += 256) {
@@ -980,10 +1039,10 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
       }
       const int wv = group * a.dv;
       for (int i = tid; i < rows * wv; i += 256)
-        st1(row_at<T>(ga.dv, p, kh, wv, i / wv) + i % wv, 0.0f);
+        st1(Chunk<T>(ga.dv, p, kh, wv).at(i / wv * (uint32_t)ga.dv.row + i % wv), 0.0f);
       for (int i = tid; i < rows * a.dk; i += 256) {
-        st1(row_at<T>(ga.dq, p, kh, a.dk, i / a.dk) + i % a.dk, 0.0f);
-        st1(row_at<T>(ga.dk, p, kh, a.dk, i / a.dk) + i % a.dk, 0.0f);
+        st1(Chunk<T>(ga.dq, p, kh, a.dk).at(i / a.dk * (uint32_t)ga.dq.row + i % a.dk), 0.0f);
+        st1(Chunk<T>(ga.dk, p, kh, a.dk).at(i / a.dk * (uint32_t)ga.dk.row + i % a.dk), 0.0f);
       }
       continue;
     }
@@ -993,8 +1052,8 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
       Rows4<T> k[DK / 64], q[DK / 64];
 #pragma unroll
       for (int i = 0; i < DK / 64; ++i) {
-        k[i].template load<W>(a.k, p, kh, a.dk, pos, i * 64 + c4);
-        q[i].template load<W>(a.qr, p, kh, a.dk, pos, i * 64 + c4);
+        k[i].template load<W>(Chunk<const T>(a.k, p, kh, a.dk), p.n, a.dk, pos, i * 64 + c4);
+        q[i].template load<W>(Chunk<const T>(a.qr, p, kh, a.dk), p.n, a.dk, pos, i * 64 + c4);
       }
       __syncthreads();
 #pragma unroll
@@ -1046,15 +1105,17 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
     f4 qo[MT], ko[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      qo[m] = ld4<T, W>(row_at<const T>(a.qr, p, kh, a.dk, min(own, p.n - 1)), m * 16 + g4, a.dk);
-      ko[m] = ld4<T, W>(row_at<const T>(a.k, p, kh, a.dk, min(own, p.n - 1)), m * 16 + g4, a.dk);
+      const Chunk<const T> qc(a.qr, p, kh, a.dk), kc(a.k, p, kh, a.dk);
+      const int row = min(own, p.n - 1);
+      qo[m] = ld4<T, W>(qc.at(row * qc.row), m * 16 + g4, a.dk);
+      ko[m] = ld4<T, W>(kc.at(row * kc.row), m * 16 + g4, a.dk);
     }
     // what K and Q are multiplied with, and what comes from the states
     f4 e[4] = {}, mid_e = ZERO, f[4] = {}, dq[MT] = {}, dk[MT] = {};
     for (int vh = kh * group; vh < (kh + 1) * group; ++vh) {
       p.h = vh;
       const int64_t at = (((int64_t)p.l * a.HV + vh) * chunks + p.c) * (a.dv * (DK + C));
-      const float *S = rec + at, *N = S + a.dv * DK, *dS = grec + at, *dR = dS + a.dv * DK;
+      const float *S = same(rec + at), *N = S + a.dv * DK, *dS = same(grec + at), *dR = dS + a.dv * DK;
       __syncthreads();
       decays_of(s.dec, a, p);
       f4 pp[4] = {}, aa[4] = {}, mid_p = ZERO, mid_a = ZERO, os[MT] = {}, rs[MT] = {}, ns[MT] = {};
@@ -1062,22 +1123,20 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
       for (int v0 = 0; v0 < a.dv; v0 += 32) {
         // N and dR: 8 x 16 pieces of 4 columns x 4 positions; dO as many; S and dS
         // 8 x DK / 4
-        const int half = tid / 128, pg = tid % 16, vg = tid / 16 % 8, v4 = v0 + vg * 4;
+        const int half = w / 2, pg = tid % 16, vg = tid / 16 % 8, v4 = v0 + vg * 4;
         Four x, sx[DK / 64];
         Rows4<T> od;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          x.v[i] = *reinterpret_cast<const f4*>((half ? dR : N) +
-                                                (int64_t)min(v4 + i, a.dv - 1) * C + pg * 4);
-        od.template load<W>(half ? a.v : ga.dout, p, vh, a.dv, pg * 4, v4);
+          x.v[i] = *at32<const f4>(half ? dR : N, min(v4 + i, a.dv - 1) * (C / 4) + pg);
+        od.template load<W>(Chunk<const T>(half ? a.v : ga.dout, p, vh, a.dv), p.n, a.dv, pg * 4, v4);
 #pragma unroll
         for (int i = 0; i < DK / 64; ++i) {
           const int d4 = (i * 16 + tid % 16) * 4;
           const int sv = v0 + (tid / 16 % 8) * 4;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            sx[i].v[j] = *reinterpret_cast<const f4*>((half ? dS : S) +
-                                                      (int64_t)min(sv + j, a.dv - 1) * DK + d4);
+            sx[i].v[j] = *at32<const f4>(half ? dS : S, min(sv + j, a.dv - 1) * (DK / 4) + d4 / 4);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -1098,7 +1157,7 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
             dots[i] += d[0] + d[1] + d[2] + d[3];
             const int pos = pg * 4 + i;
             if (pos < rows)
-              st4<T, W>(row_at<T>(ga.dv, p, vh, a.dv, pos), v4, a.dv,
+              st4<T, W>(Chunk<T>(ga.dv, p, vh, a.dv).at(pos * (uint32_t)ga.dv.row), v4, a.dv,
                         pos < p.n ? xt.v[i] * s.dec.beta[pos] : ZERO);
           }
         } else {
@@ -1270,9 +1329,9 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         const bool live = own < p.n;
-        st4<T, W>(row_at<T>(ga.dq, p, kh, a.dk, own), m * 16 + g4, a.dk,
+        st4<T, W>(Chunk<T>(ga.dq, p, kh, a.dk).at(own * (uint32_t)ga.dq.row), m * 16 + g4, a.dk,
                   live ? (dq[m] - qo[m] * fq) * rq : ZERO);
-        st4<T, W>(row_at<T>(ga.dk, p, kh, a.dk, own), m * 16 + g4, a.dk,
+        st4<T, W>(Chunk<T>(ga.dk, p, kh, a.dk).at(own * (uint32_t)ga.dk.row), m * 16 + g4, a.dk,
                   live ? (dk[m] - ko[m] * fk) * rk : ZERO);
       }
     }
@@ -1430,7 +1489,7 @@ hipError_t delta_of(const DeltaArgs& a, hipStream_t s) {
     const size_t lds = sizeof(ChainLds<T, DK, false>);
     if ((e = room(delta_chain_kernel<T, DK, W>, lds))) return e;
     BOA_LAUNCH((delta_chain_kernel<T, DK, W>), grid(heads * tiles), 256, lds, s, a,
-               (const unsigned char*)prep, a.saved, chunks, tiles, heads * tiles);
+               (const unsigned char*)prep, a.saved, chunks, tiles, (uint32_t)(heads * tiles));
     return hipGetLastError();
   });
 }
@@ -1451,7 +1510,7 @@ hipError_t delta_grad_of(const DeltaGradArgs& ga, hipStream_t s) {
     size_t lds = sizeof(ChainLds<T, DK, true>);
     if ((e = room(delta_grad_chain_kernel<T, DK, W>, lds))) return e;
     BOA_LAUNCH((delta_grad_chain_kernel<T, DK, W>), grid(heads * tiles), 256, lds, s, ga,
-               (const unsigned char*)prep, grec, chunks, tiles, heads * tiles);
+               (const unsigned char*)prep, grec, chunks, tiles, (uint32_t)(heads * tiles));
     if ((e = hipGetLastError())) return e;
     lds = sizeof(LastLds<T, DK>);
     if ((e = room(delta_grad_last_kernel<T, DK, W>, lds))) return e;
@@ -1487,7 +1546,8 @@ hipError_t launch_delta(const DeltaArgs& a, hipStream_t s) {
     const bool wide = wide_rows(a.v, a.dv, size) && a.dv % 4 == 0;  // states are 16-byte aligned
     return for_rows(a.bf16, wide, [&](auto t, auto w) { return delta_steps_of<decltype(t), w>(a, s); });
   }
-  const bool wide = wide_rows(a.qr, a.dk, size) && wide_rows(a.k, a.dk, size);
+  const bool wide = wide_rows(a.qr, a.dk, size) && wide_rows(a.k, a.dk, size) &&
+                    wide_rows(a.v, a.dv, size) && wide_rows(a.out, a.dv, size);
   return for_rows(a.bf16, wide, [&](auto t, auto w) { return delta_of<decltype(t), w>(a, s); });
 }
 

@@ -303,7 +303,8 @@ int boa_int8_matmul(boa_ctx* ctx, const boa_rows* x8, const float* d_scale8, con
  * (a multiple of heads, at most 1024) of d_v (1 .. 128); v_heads / heads
  * neighbouring heads of v share one of q and k.  g (log decays) and beta are
  * fp32 rows v_heads wide, whatever `precision` is.  unit_qk: q and k are
- * divided by their lengths sqrt(sum of squares + 1e-6) first.  A log decay
+ * divided by their lengths sqrt(sum of squares + 1e-6) first.  Row strides are
+ * at most 2^23.  A log decay
  * below -1e4 (-inf too) forgets the state.  States [lanes][v_heads][d_k][d_v]
  * fp32; d_state_in NULL is zero.  With T = 1 this is a decode step.  Positions
  * are taken 64 at a time: a value that is not finite spoils the results of its

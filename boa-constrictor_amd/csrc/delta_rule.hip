@@ -46,13 +46,23 @@ constexpr int CP = C + 4;      // pitch of a [64][64] tile of floats in LDS
 constexpr float EPS = 1e-6f;   // under the root of a row's length
 constexpr f4 ZERO = {0.0f, 0.0f, 0.0f, 0.0f};
 
-// e^x for x in 64 bits, to an fp32's precision whatever its size
-__device__ __forceinline__ float exp_of(double x) {
+// A sum of log decays in 64 bits as a power of two, a whole one and a fraction:
+// e^(a - b) then has an fp32's precision however large a and b are.
+struct Power {
+  int whole;
+  float part;
+};
+__device__ __forceinline__ Power power_of(double x) {
   const double y = x * 1.4426950408889634074;
-  const double n = __builtin_rint(y);
-  const float m = n > 1000.0 ? 1000.0f : (n < -1000.0 ? -1000.0f : (float)n);
-  const float e = __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f((float)(y - n)), (int)m);
-  return x != x ? (float)x : e;
+  const double n = __builtin_fmin(__builtin_fmax(__builtin_rint(y), -1e9), 1e9);
+  return Power{(int)n, (float)(y - n)};
+}
+__device__ __forceinline__ float raised(int whole, float part) {
+  return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(part), min(max(whole, -1000), 1000));
+}
+__device__ __forceinline__ float exp_of(double x) {
+  const Power p = power_of(x);
+  return raised(p.whole, p.part);
 }
 
 // the log decay as it is summed: below -1e4 nothing is left of a state
@@ -447,7 +457,8 @@ constexpr int64_t PREP_BYTES = 2 * TRI * 3 * 1024 + COEF * 4;  // the larger of 
 
 // the block's sums of log decays and betas, by its first wave
 struct Decays {
-  double sum[C];  // G
+  int whole[C];    // G, as a power of two
+  float part[C];
   float beta[C];
   float since[C];  // e^G
   float left[C];   // e^(G_64 - G)
@@ -465,7 +476,9 @@ __device__ __forceinline__ void decays_of(Decays& s, const DeltaArgs& a, const P
     if (i >= m) g += y;
   }
   const double all = __shfl(g, C - 1);
-  s.sum[i] = g;
+  const Power at = power_of(g);
+  s.whole[i] = at.whole;
+  s.part[i] = at.part;
   s.beta[i] = beta;
   s.since[i] = exp_of(g);
   s.left[i] = exp_of(all - g);
@@ -489,12 +502,18 @@ __device__ __forceinline__ void mma16(f4& acc, f4 x, f4 y) {
 // A block per (lane, value head, chunk): T and P as the chain reads them, and
 // the coefficients.
 template <typename T, int DK, bool TRANS, bool W>
-__global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a, unsigned char* prep,
+__global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 ? 4 : 2) void delta_prep_kernel(const DeltaArgs a, unsigned char* prep,
                                                          int chunks, uint64_t blocks) {
   using M = Mode<T>;
   constexpr int U = DK / 32, P = M::ROWS;
-  __shared__ u4 ka[4 * U * P * 64], qa[4 * U * P * 64];
-  __shared__ __align__(16) float am[C * CP], tm[C * CP];
+  constexpr int TILE = 4 * U * P * 64;
+  __shared__ union {
+    u4 kq[2 * TILE];  // K and Q, until their products are there
+    float t[C * CP];
+  } lds;
+  u4 *ka = lds.kq, *qa = lds.kq + TILE;
+  float* tm = lds.t;
+  __shared__ __align__(16) float am[C * CP];
   __shared__ float ssk[C], ssq[C], rk[C], rq[C];
   __shared__ Decays s;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -523,7 +542,6 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a, unsi
       k[i].put(ka, U, pos, i * 64 + col);
       q[i].put(qa, U, pos, i * 64 + col);
     }
-    for (int i = tid; i < C * CP; i += 256) tm[i] = 0.0f;
     __syncthreads();
     // this wave's 16 rows of K K^T and Q K^T up to the diagonal; Q Q^T for the
     // lengths, as K K^T's diagonal has those of k
@@ -550,6 +568,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a, unsi
       rk[tid] = a.unit ? 1.0f / __builtin_sqrtf(ssk[tid] + EPS) : 1.0f;
       rq[tid] = a.unit ? a.scale / __builtin_sqrtf(ssq[tid] + EPS) : a.scale;
     }
+    for (int i = tid; i < C * CP / 4; i += 256) reinterpret_cast<f4*>(tm)[i] = ZERO;
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < 4; ++n)
@@ -557,7 +576,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const DeltaArgs a, unsi
       for (int r = 0; r < 4; ++r) {
         const int i = wave * 16 + g4 + r, j = n * 16 + i16;
         float d = 0.0f;
-        if (n <= wave && j <= i) d = exp_of(s.sum[i] - s.sum[j]);
+        if (n <= wave && j <= i) d = raised(s.whole[i] - s.whole[j], s.part[i] - s.part[j]);
         am[i * CP + j] = n <= wave && j < i ? kk[n][r] * (s.beta[i] * rk[i] * rk[j] * d) : 0.0f;
         qk[n][r] = n <= wave && j <= i ? qk[n][r] * (rq[i] * rk[j] * d) : 0.0f;
       }
@@ -1010,21 +1029,47 @@ struct LastLds {
     } v;
   };
   float dot[8][C];  // dR . v, by groups of four columns
-  float ssk[C], ssq[C], rk[C], rq[C], dsum[C];
+  float rk[C], rq[C], dsum[C];
   float tail[8];
   Decays dec;
 };
+// The compiler moves nothing across: left alone it brings all of a loop's operands
+// in first, for which the registers do not suffice.
+__device__ __forceinline__ void apart() { __builtin_amdgcn_sched_barrier(0); }
+
+template <int P>
+__device__ __forceinline__ Frag<P> either(bool first, const Frag<P>& a, const Frag<P>& b) {
+  Frag<P> r;
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.p[p][i] = first ? a.p[p][i] : b.p[p][i];
+  return r;
+}
+__device__ __forceinline__ f4 either(bool first, f4 a, f4 b) {
+  return f4{first ? a[0] : b[0], first ? a[1] : b[1], first ? a[2] : b[2], first ? a[3] : b[3]};
+}
+__device__ __forceinline__ f4 one_of(const f4 (&x)[4], int w) {
+  return either(w < 2, either(w == 0, x[0], x[1]), either(w == 2, x[2], x[3]));
+}
+
 template <typename T, int DK, bool W>
-__global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
+__global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_last_kernel(
     const DeltaGradArgs ga, const float* rec, const float* grec, int chunks, uint64_t blocks) {
   constexpr int U = DK / 32, MT = DK / 16, FULL = Mode<T>::FULL, P = Mode<T>::ROWS;
   extern __shared__ __align__(16) unsigned char lds[];
   const DeltaArgs& a = ga.f;
   LastLds<T, DK>& s = *reinterpret_cast<LastLds<T, DK>*>(lds);
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int i16 = lane % 16, g = lane / 16, g4 = 4 * g, sl = slot_of(i16, g);
-  const int group = a.HV / a.H, own = w * 16 + i16;
+  const int group = a.HV / a.H;
   for (uint64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
+    // what follows from the thread's number is computed here, not kept from
+    // before the loop: there are no registers to keep it in
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, w = same(tid >> 6);
+    const int i16 = lane % 16, g = lane / 16, g4 = 4 * g, sl = slot_of(i16, g), own = w * 16 + i16;
+    // the wave again, but as a vector: what it decides by selects is no branch
+    const int wv = tid >> 6;
     Place p;
     p.c = same((int)(b % chunks));
     const int kh = same((int)(b / chunks % a.H));
@@ -1037,9 +1082,9 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
         ((float*)ga.dg.d)[p.l * ga.dg.lane + t * ga.dg.row + h] = 0.0f;
         ((float*)ga.dbeta.d)[p.l * ga.dbeta.lane + t * ga.dbeta.row + h] = 0.0f;
       }
-      const int wv = group * a.dv;
-      for (int i = tid; i < rows * wv; i += 256)
-        st1(Chunk<T>(ga.dv, p, kh, wv).at(i / wv * (uint32_t)ga.dv.row + i % wv), 0.0f);
+      const int wide = group * a.dv;
+      for (int i = tid; i < rows * wide; i += 256)
+        st1(Chunk<T>(ga.dv, p, kh, wide).at(i / wide * (uint32_t)ga.dv.row + i % wide), 0.0f);
       for (int i = tid; i < rows * a.dk; i += 256) {
         st1(Chunk<T>(ga.dq, p, kh, a.dk).at(i / a.dk * (uint32_t)ga.dq.row + i % a.dk), 0.0f);
         st1(Chunk<T>(ga.dk, p, kh, a.dk).at(i / a.dk * (uint32_t)ga.dk.row + i % a.dk), 0.0f);
@@ -1071,47 +1116,36 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
       }
       __syncthreads();
     };
-    bring_kq(false);
-    // kk: rows of tile m, column own; qk: m < w: q of own, k of tile m; m > w: q
-    // of tile m, k of own; the wave's own tile has both (mid: the second)
-    f4 kk[4] = {}, qk[4] = {}, mid_qk = ZERO;
-    {
-      f4 qq = ZERO;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const Frag<P> ko = get<P>(s.k.a, w * U + u, sl), qo = get<P>(s.k.b, w * U + u, sl);
-        mma<T>(qq, qo, qo);
-        mma<T>(mid_qk, qo, ko);
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          const Frag<P> km = get<P>(s.k.a, m * U + u, sl);
-          mma<T>(kk[m], km, ko);
-          if (m <= w) mma<T>(qk[m], km, qo);
-          else mma<T>(qk[m], get<P>(s.k.b, m * U + u, sl), ko);
-        }
-      }
-#pragma unroll
-      for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (m == w && g4 + r == i16) s.ssk[own] = kk[m][r], s.ssq[own] = qq[r];
-    }
-    __syncthreads();
-    if (tid < C) {
-      s.rk[tid] = a.unit ? 1.0f / __builtin_sqrtf(s.ssk[tid] + EPS) : 1.0f;
-      s.rq[tid] = a.unit ? a.scale / __builtin_sqrtf(s.ssq[tid] + EPS) : a.scale;
-    }
-    // this lane's columns of its own rows of q and k
+    // this lane's columns of its own rows of q and k; the rows' lengths from them
     f4 qo[MT], ko[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
+    auto bring_own = [&]() {
       const Chunk<const T> qc(a.qr, p, kh, a.dk), kc(a.k, p, kh, a.dk);
       const int row = min(own, p.n - 1);
-      qo[m] = ld4<T, W>(qc.at(row * qc.row), m * 16 + g4, a.dk);
-      ko[m] = ld4<T, W>(kc.at(row * kc.row), m * 16 + g4, a.dk);
-    }
-    // what K and Q are multiplied with, and what comes from the states
-    f4 e[4] = {}, mid_e = ZERO, f[4] = {}, dq[MT] = {}, dk[MT] = {};
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        qo[m] = ld4<T, W>(qc.at(row * qc.row), m * 16 + g4, a.dk);
+        ko[m] = ld4<T, W>(kc.at(row * kc.row), m * 16 + g4, a.dk);
+      }
+    };
+    auto across_g = [&](float x) {
+      x = fold16(x, x);
+      return fold32(x, x);
+    };
+    float ssq = 0.0f, ssk = 0.0f;
+    bring_own();
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        ssq += qo[m][r] * qo[m][r];
+        ssk += ko[m][r] * ko[m][r];
+      }
+    ssq = 1.0f / __builtin_sqrtf(across_g(ssq) + EPS);
+    const float rk = a.unit ? 1.0f / __builtin_sqrtf(across_g(ssk) + EPS) : 1.0f;
+    const float rq = a.unit ? ssq * a.scale : a.scale;
+    __syncthreads();
+    if (g == 0) s.rk[own] = rk, s.rq[own] = rq;
+    f4 dq[MT] = {}, dk[MT] = {};
     for (int vh = kh * group; vh < (kh + 1) * group; ++vh) {
       p.h = vh;
       const int64_t at = (((int64_t)p.l * a.HV + vh) * chunks + p.c) * (a.dv * (DK + C));
@@ -1146,6 +1180,7 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
             for (int j = 0; j < DK / 64; ++j) sx[j].v[i] = ZERO;
           }
         __syncthreads();
+        apart();
         const Four xt = turned(x);  // rows: positions
         od.template cut<W>(p.n - pg * 4, a.dv - v4);
         put_full<T>(half ? s.v.r : s.v.n, 1, pg * 4, vg * 4, xt);
@@ -1167,18 +1202,27 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
         for (int i = 0; i < DK / 64; ++i)
           put_full<T>(half ? s.v.d : s.v.s, 1, (i * 16 + tid % 16) * 4, vg * 4, turned(sx[i]));
         __syncthreads();
+        apart();
         const Frag<FULL> no = get<FULL>(s.v.n, w, sl), ro = get<FULL>(s.v.r, w, sl);
         const Frag<P> oo = get<P>(s.v.o, w, sl);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          if (m <= w) {
-            const Frag<FULL> nm = get<FULL>(s.v.n, m, sl);
-            mma<T>(pp[m], nm, oo);
-            mma<T>(aa[m], nm, ro);
+          // N of tile m with dO and dR of own, or dO and dR of tile m with N of own
+          mma<T>(aa[m], get<FULL>(m <= w ? s.v.n : s.v.r, m, sl), either(m <= wv, ro, no));
+          if constexpr (P == FULL) {
+            mma<T>(pp[m], get<P>(m <= w ? s.v.n : s.v.o, m, sl), either(m <= wv, oo, no));
           } else {
-            mma<T>(pp[m], get<P>(s.v.o, m, sl), no);
-            mma<T>(aa[m], get<FULL>(s.v.r, m, sl), no);
+            // one part of dO, three of N, whichever is on the left: the small first
+#pragma unroll
+            for (int i = FULL - 1; i >= 0; --i) {
+              Frag<1> x, y;
+              x.p[0] = *(m <= w ? s.v.n + (m * FULL + i) * 64 + sl : s.v.o + m * 64 + sl);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) y.p[0][j] = m <= wv ? oo.p[0][j] : no.p[i][j];
+              mma<T>(pp[m], x, y);
+            }
           }
+          apart();
         }
         mma<T>(mid_p, oo, no);
         mma<T>(mid_a, ro, no);
@@ -1188,6 +1232,7 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
           mma<T>(os[m], sm, oo);
           mma<T>(rs[m], sm, ro);
           mma<T>(ns[m], get<FULL>(s.v.d, m, sl), no);
+          apart();
         }
       }
       // <dS, S>: the two halves of the block hold one each, so from memory
@@ -1201,38 +1246,9 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
 #pragma unroll
         for (int i = 0; i < 4; ++i) s.dot[tid / 16 % 8][tid % 16 * 4 + i] = dots[i];
       }
-      const double G = s.dec.sum[own];
-      const float beta = s.dec.beta[own], rk = s.rk[own], rq = s.rq[own];
-      // sums over a row of dP P and dA A, over a column, and of dA k.k D
-      float over = 0.0f, down = 0.0f, with_beta = 0.0f;
-#pragma unroll
-      for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int o = m * 16 + g4 + r;
-          const double dG = s.dec.sum[o] - G;
-          const float d = exp_of(o < own ? -dG : dG), rko = s.rk[o], rqo = s.rq[o];
-          const float ukk = kk[m][r] * rk * rko;
-          if (m <= w) {  // own is the row, o the column
-            const float dP = o <= own ? pp[m][r] * d : 0.0f;
-            const float dA = o < own ? -aa[m][r] * d : 0.0f;
-            over += dP * (qk[m][r] * (rq * rko)) + dA * (beta * ukk);
-            with_beta += dA * ukk;
-            e[m][r] += dP * (rko * a.scale);
-            f[m][r] += dA * (beta * rko);
-          }
-          if (m >= w) {  // o is the row, own the column
-            const float p0 = m == w ? mid_p[r] : pp[m][r], a0 = m == w ? mid_a[r] : aa[m][r];
-            const float q0 = m == w ? mid_qk[r] : qk[m][r], bo = s.dec.beta[o];
-            const float dP = o >= own ? p0 * d : 0.0f;
-            const float dA = o > own ? -a0 * d : 0.0f;
-            down += dP * (q0 * (rqo * rk)) + dA * (bo * ukk);
-            if (m == w) mid_e[r] += dP * rqo;
-            else e[m][r] += dP * rqo;
-            f[m][r] += dA * (bo * rko);
-          }
-        }
       // from the states
+      bring_own();
+      const float beta = s.dec.beta[own];
       float oq = 0.0f, rsk = 0.0f, nsk = 0.0f;
       const float since = s.dec.since[own], left = s.dec.left[own];
 #pragma unroll
@@ -1246,13 +1262,58 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
         dq[m] += os[m] * (since * a.scale);
         dk[m] += ns[m] * left - rs[m] * (since * beta);
       }
-      auto across_g = [&](float x) {
-        x = fold16(x, x);
-        return fold32(x, x);
-      };
       oq = across_g(oq) * (rq * since);
       rsk = across_g(rsk) * (rk * since);
       nsk = across_g(nsk) * (rk * left);
+      // kk: rows of tile m, column own; qk: m <= w: q of own, k of tile m; m > w: q
+      // of tile m, k of own; the wave's own tile has both (mid: the second).  Which
+      // it is decides addresses and selects, not branches.
+      bring_kq(false);
+      f4 kk[4] = {}, qk[4] = {}, mid_qk = ZERO;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const Frag<P> kw = get<P>(s.k.a, w * U + u, sl), qw = get<P>(s.k.b, w * U + u, sl);
+        mma<T>(mid_qk, qw, kw);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          mma<T>(kk[m], get<P>(s.k.a, m * U + u, sl), kw);
+          mma<T>(qk[m], get<P>(m <= w ? s.k.a : s.k.b, m * U + u, sl), either(m <= wv, qw, kw));
+        }
+        apart();
+      }
+      // what K and Q are multiplied with
+      f4 e[4] = {}, mid_e = ZERO, f[4] = {}, mid_f = ZERO;
+      const int whole = s.dec.whole[own];
+      const float part = s.dec.part[own];
+      // sums over a row of dP P and dA A, over a column, and of dA k.k D
+      float over = 0.0f, down = 0.0f, with_beta = 0.0f;
+      auto element = [&](int o, bool row, float p0, float a0, float q0, float k0, f4& eo, f4& fo, int r) {
+        // row: own is the row and o the column, else the other way
+        const int dw = s.dec.whole[o] - whole;
+        const float dp = s.dec.part[o] - part;
+        const float d = raised(row ? -dw : dw, row ? -dp : dp);
+        const float rko = s.rk[o], rqo = s.rq[o], bo = s.dec.beta[o], ukk = k0 * rk * rko;
+        const float dP = (row ? o <= own : o >= own) ? p0 * d : 0.0f;
+        const float dA = (row ? o < own : o > own) ? -a0 * d : 0.0f;
+        const float br = row ? beta : bo;
+        const float both = dP * (q0 * (row ? rq * rko : rqo * rk)) + dA * (br * ukk);
+        over += row ? both : 0.0f;
+        down += row ? 0.0f : both;
+        with_beta += row ? dA * ukk : 0.0f;
+        eo[r] += dP * (row ? rko * a.scale : rqo);
+        fo[r] += dA * (br * rko);
+      };
+      const f4 mid_k = one_of(kk, wv);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          element(m * 16 + g4 + r, m <= wv, pp[m][r], aa[m][r], qk[m][r], kk[m][r], e[m], f[m], r);
+        apart();
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        element(w * 16 + g4 + r, false, mid_p[r], mid_a[r], mid_qk[r], mid_k[r], mid_e, mid_f, r);
       over = across_g(over);
       down = across_g(down);
       with_beta = across_g(with_beta);
@@ -1281,35 +1342,38 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
           ((float*)ga.dg.d)[p.l * ga.dg.lane + (int64_t)(p.c * C + lane) * ga.dg.row + vh] =
               lane < p.n ? (float)x : 0.0f;
       }
-    }
-    bring_kq(true);
-    {
-      // e: q's part below (rows j), k's above (rows i); the own tile has both
-      f4 ek[4];
+      bring_kq(true);
+      {
+        // e: q's part below (rows j), k's above (rows i); the own tile has both
+        f4 ek[4];
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        ek[m] = m == w ? mid_e : (m > w ? e[m] : ZERO);
-        e[m] = m <= w ? e[m] : ZERO;
-      }
-      Frag<FULL> ef[2], kf[2], ff[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        ef[u] = full<T>(e[2 * u], e[2 * u + 1]);
-        kf[u] = full<T>(ek[2 * u], ek[2 * u + 1]);
-        ff[u] = full<T>(f[2 * u], f[2 * u + 1]);
-      }
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < 4; ++m) {
+          ek[m] = either(m == wv, mid_e, either(m > wv, e[m], ZERO));
+          e[m] = either(m <= wv, e[m], ZERO);
+          f[m] += either(m == wv, mid_f, ZERO);
+        }
+        Frag<FULL> ef[2], kf[2], ff[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const Frag<P> kt = get<P>(s.k.a, m * 2 + u, sl);
-          mma<T>(dq[m], kt, ef[u]);
-          mma<T>(dk[m], kt, ff[u]);
-          mma<T>(dk[m], get<P>(s.k.b, m * 2 + u, sl), kf[u]);
+          ef[u] = full<T>(e[2 * u], e[2 * u + 1]);
+          kf[u] = full<T>(ek[2 * u], ek[2 * u + 1]);
+          ff[u] = full<T>(f[2 * u], f[2 * u + 1]);
         }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const Frag<P> kt = get<P>(s.k.a, m * 2 + u, sl);
+            mma<T>(dq[m], kt, ef[u]);
+            mma<T>(dk[m], kt, ff[u]);
+            mma<T>(dk[m], get<P>(s.k.b, m * 2 + u, sl), kf[u]);
+            apart();
+          }
+      }
     }
     // through the rows' lengths: d = r (d^ - u (u . d^)), u the unit row
-    float fq = 0.0f, fk = 0.0f, rq = 1.0f, rk = 1.0f;
+    bring_own();
+    float fq = 0.0f, fk = 0.0f;
     if (a.unit) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -1318,19 +1382,16 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
           fq += dq[m][r] * qo[m][r];
           fk += dk[m][r] * ko[m][r];
         }
-      rk = s.rk[own];
-      rq = 1.0f / __builtin_sqrtf(s.ssq[own] + EPS);
-      fq = fold16(fq, fq);
-      fk = fold16(fk, fk);
-      fq = fold32(fq, fq) * rq * rq;
-      fk = fold32(fk, fk) * rk * rk;
+      fq = across_g(fq) * ssq * ssq;
+      fk = across_g(fk) * rk * rk;
     }
+    const float by = a.unit ? ssq : 1.0f;
     if (own < rows) {
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         const bool live = own < p.n;
         st4<T, W>(Chunk<T>(ga.dq, p, kh, a.dk).at(own * (uint32_t)ga.dq.row), m * 16 + g4, a.dk,
-                  live ? (dq[m] - qo[m] * fq) * rq : ZERO);
+                  live ? (dq[m] - qo[m] * fq) * by : ZERO);
         st4<T, W>(Chunk<T>(ga.dk, p, kh, a.dk).at(own * (uint32_t)ga.dk.row), m * 16 + g4, a.dk,
                   live ? (dk[m] - ko[m] * fk) * rk : ZERO);
       }

@@ -278,15 +278,16 @@ __device__ __forceinline__ void mma(f4 (&acc)[N], const Frag<PA> (&a)[N], const 
 
 // ---- operands in LDS -------------------------------------------------------
 // A block is 16 rows x 32 of k as the lanes hold it, piece by piece, 16 bytes a
-// lane; a tile of U blocks across.  The rows of each g are in another order, so
-// that four rows and four groups of k that are written at once fall into
-// different banks.
+// lane; a tile of U blocks across.  The rows of each g, and of each block, are in
+// another order, so that what is written at once (rows of several blocks, or
+// groups of k) falls into different banks.
 __device__ __forceinline__ int slot_of(int i, int g) { return (i ^ g) + 16 * g; }
+__device__ __forceinline__ int slot_in(int block, int slot) { return slot ^ (block & 3); }
 template <int P>
 __device__ __forceinline__ Frag<P> get(const u4* tile, int block, int slot) {
   Frag<P> r;
 #pragma unroll
-  for (int p = 0; p < P; ++p) r.p[p] = tile[(block * P + p) * 64 + slot];
+  for (int p = 0; p < P; ++p) r.p[p] = tile[(block * P + p) * 64 + slot_in(block, slot)];
   return r;
 }
 // blocks b0, b0 + step, ..
@@ -298,7 +299,8 @@ __device__ __forceinline__ void get(Frag<P> (&r)[N], const u4* tile, int b0, int
 // four values of one row, k .. k + 3 (k a multiple of 4)
 template <typename T, int P>
 __device__ __forceinline__ void put(u4* tile, int U, int row, int k, f4 v) {
-  const int block = row / 16 * U + k / 32, h = k / 16 % 2, slot = slot_of(row % 16, k / 4 % 4);
+  const int block = row / 16 * U + k / 32, h = k / 16 % 2;
+  const int slot = slot_in(block, slot_of(row % 16, k / 4 % 4));
   if constexpr (sizeof(T) == 4) {
     tile[(block * 2 + h) * 64 + slot] = __builtin_bit_cast(u4, v);
   } else {
@@ -330,11 +332,9 @@ __device__ __forceinline__ void put_full(u4* tile, int U, int row, int k, const 
 
 // a value that is the same in all lanes, kept in scalar registers
 __device__ __forceinline__ int same(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ uint64_t same(uint64_t x) {
-  return (uint64_t)(uint32_t)same((int)(x >> 32)) << 32 | (uint32_t)same((int)x);
+__device__ __forceinline__ int64_t same(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)same((int)(x >> 32)) << 32 | (uint32_t)same((int)x));
 }
-template <typename T>
-__device__ __forceinline__ T* same(T* p) { return (T*)same((uint64_t)p); }
 // p[i] of elements of T, i of 32 bits beside a scalar address
 template <typename T, typename P>
 __device__ __forceinline__ T* at32(P* p, uint32_t i) {
@@ -358,7 +358,7 @@ struct Chunk {
   uint32_t row;  // elements
   template <typename R>
   __device__ __forceinline__ Chunk(const R& r, const Place& at, int h, int d)
-      : p(same((T*)r.d + at.l * r.lane + (int64_t)at.c * C * r.row + (int64_t)h * d)),
+      : p((T*)r.d + same(at.l * r.lane + (int64_t)at.c * C * r.row + (int64_t)h * d)),
         row((uint32_t)r.row) {}
   __device__ __forceinline__ T* at(uint32_t element) const { return at32<T>(p, element); }
 };
@@ -403,7 +403,8 @@ struct Rows4 {
   __device__ __forceinline__ void put(u4* tile, int U, int row, int k) const {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int block = (row + e) / 16 * U + k / 32, slot = slot_of((row + e) % 16, k / 4 % 4);
+      const int block = (row + e) / 16 * U + k / 32;
+      const int slot = slot_in(block, slot_of((row + e) % 16, k / 4 % 4));
       if constexpr (sizeof(T) == 4)
         tile[(block * 2 + k / 16 % 2) * 64 + slot] = __builtin_bit_cast(u4, r[e].v);
       else reinterpret_cast<u2*>(tile + block * 64 + slot)[k / 16 % 2] = r[e].v;
@@ -449,8 +450,9 @@ __device__ __forceinline__ void triangle(f4 (&acc)[4], const u4* tri, const Frag
   acc[TRANS ? 1 : 3] = two[1];
 }
 // Coefficients of the rows, floats: beta; beta e^G / |k|; e^(G_64 - G) / |k|;
-// scale e^G / |q|; then e^G_64.
-constexpr int COEF = 4 * C + 4;
+// scale e^G / |q|; then e^G_64; for the rows' gradients G as a power of two, e^G,
+// e^(G_64 - G), 1 / |k| and 1 / |q| as well.
+constexpr int CHAIN_COEF = 4 * C + 4, COEF = CHAIN_COEF + 6 * C;
 template <typename T>
 constexpr int IMAGE = 2 * TRI * Mode<T>::FULL * 64;  // 16-byte pieces of T and P
 constexpr int64_t PREP_BYTES = 2 * TRI * 3 * 1024 + COEF * 4;  // the larger of the types'
@@ -646,7 +648,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 ? 4 : 2) void delta
       }
       const Frag<M::FULL> f = full<T>(lo, hi);
 #pragma unroll
-      for (int i = 0; i < M::FULL; ++i) image[(job * M::FULL + i) * 64 + sl] = f.p[i];
+      for (int i = 0; i < M::FULL; ++i) image[(job * M::FULL + i) * 64 + slot_in(block, sl)] = f.p[i];
     }
     float* coef = reinterpret_cast<float*>(at + PREP_BYTES - COEF * 4);
     if (tid < C) {
@@ -655,6 +657,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 ? 4 : 2) void delta
       coef[2 * C + tid] = s.left[tid] * rk[tid];
       coef[3 * C + tid] = rq[tid] * s.since[tid];
       if (tid == C - 1) coef[4 * C] = s.since[tid];
+      if (TRANS) {
+        float* more = coef + CHAIN_COEF + tid;
+        more[0] = s.part[tid];
+        reinterpret_cast<int*>(more)[C] = s.whole[tid];
+        more[2 * C] = s.since[tid];
+        more[3 * C] = s.left[tid];
+        more[4 * C] = rk[tid];
+        more[5 * C] = a.unit ? 1.0f / __builtin_sqrtf(ssq[tid] + EPS) : 1.0f;
+      }
     }
   }
 }
@@ -670,7 +681,7 @@ struct ChainLds {
   u4 q[4 * (DK / 32) * Mode<T>::ROWS * 64];  // rows, or across: as many blocks
   u4 v[4 * 2 * Mode<T>::ROWS * 64];  // v (dO), across: 16 columns a wave; then its results
   u4 tri[IMAGE<T>];
-  float coef[COEF];
+  float coef[CHAIN_COEF];
 };
 template <typename T, int DK>
 struct ChainNext {
@@ -740,7 +751,8 @@ __device__ __forceinline__ void put_result(u4* tile, const f4 (&o)[4], int wave,
   for (int u = 0; u < 2; ++u) {
     const Frag<P> f = rows_of<T>(o[2 * u], o[2 * u + 1]);
 #pragma unroll
-    for (int p = 0; p < P; ++p) tile[((wave * 2 + u) * P + p) * 64 + slot] = f.p[p];
+    for (int p = 0; p < P; ++p)
+      tile[((wave * 2 + u) * P + p) * 64 + slot_in(wave * 2 + u, slot)] = f.p[p];
   }
   // the wave's own LDS accesses are in order; the compiler's have to be
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -749,7 +761,7 @@ __device__ __forceinline__ void put_result(u4* tile, const f4 (&o)[4], int wave,
   Rows4<T> x;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    const int s = slot_of(cg * 4 + c, pg % 4);
+    const int s = slot_in(block, slot_of(cg * 4 + c, pg % 4));
     if constexpr (sizeof(T) == 4) x.r[c].v = __builtin_bit_cast(f4, tile[(block * 2 + h) * 64 + s]);
     else x.r[c].v = reinterpret_cast<const u2*>(tile + block * 64 + s)[h];
   }
@@ -794,7 +806,7 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
     auto bring = [&](int c) {
       p.c = c;
       p.n = within(len, c);
-      next.template load<W>(a, same(prep + ((uint64_t)lh * chunks + c) * PREP_BYTES), p, kh, a.v, vb);
+      next.template load<W>(a, prep + same(((int64_t)lh * chunks + c) * PREP_BYTES), p, kh, a.v, vb);
     };
     if (last > 0) bring(0);
     for (int c = 0; c < last; ++c) {
@@ -804,7 +816,7 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
       __syncthreads();
       if (c + 1 < last) bring(c + 1);
       if (v0 >= a.dv) continue;
-      float* at = same(rec ? rec + ((int64_t)lh * chunks + c) * (a.dv * (DK + C)) : nullptr);
+      float* at = rec + same(((int64_t)lh * chunks + c) * (a.dv * (DK + C)));
       if (rec && mine) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
@@ -923,7 +935,7 @@ __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
     auto bring = [&](int c) {
       p.c = c;
       p.n = within(len, c);
-      next.template load<W>(a, same(prep + ((uint64_t)lh * chunks + c) * PREP_BYTES), p, kh, ga.dout, vb);
+      next.template load<W>(a, prep + same(((int64_t)lh * chunks + c) * PREP_BYTES), p, kh, ga.dout, vb);
     };
     if (last > 0) bring(last - 1);
     for (int c = last - 1; c >= 0; --c) {
@@ -932,7 +944,7 @@ __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
       __syncthreads();
       if (c > 0) bring(c - 1);
       if (v0 >= a.dv) continue;
-      float* at = same(grec + ((int64_t)lh * chunks + c) * (a.dv * (DK + C)));
+      float* at = grec + same(((int64_t)lh * chunks + c) * (a.dv * (DK + C)));
       if (mine) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
@@ -1029,10 +1041,15 @@ struct LastLds {
     } v;
   };
   float dot[8][C];  // dR . v, by groups of four columns
-  float rk[C], rq[C], dsum[C];
-  float tail[8];
-  Decays dec;
+  float dsum[C], tail[8];
+  struct {
+    float beta[C], unused[3 * C], all[4], part[C];
+    int whole[C];
+    float since[C], left[C], rk[C], uq[C];
+  } coef;
 };
+static_assert(sizeof(LastLds<float, 64>::coef) == COEF * 4, "as prep leaves them");
+
 // The compiler moves nothing across: left alone it brings all of a loop's operands
 // in first, for which the registers do not suffice.
 __device__ __forceinline__ void apart() { __builtin_amdgcn_sched_barrier(0); }
@@ -1053,9 +1070,37 @@ __device__ __forceinline__ f4 one_of(const f4 (&x)[4], int w) {
   return either(w < 2, either(w == 0, x[0], x[1]), either(w == 2, x[2], x[3]));
 }
 
+// What a thread brings of 32 columns of d_v: four columns of four positions of N
+// and v, or of dR and dO; four columns of two rows (of 64) of S and dS.
+template <typename T, int DK>
+struct LastNext {
+  Four x;
+  Rows4<T> rows;
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  f2 s[DK / 64][4], d[DK / 64][4];
+  template <bool W>
+  __device__ __forceinline__ void load(const float* S, const float* dS, const float* x_,
+                                       const Chunk<const T>& from, int n, int dv, int v0, int tid) {
+    const int pg = tid % 16, v4 = v0 + tid / 16 % 8 * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.v[i] = *at32<const f4>(x_, min(v4 + i, dv - 1) * (C / 4) + pg);
+    rows.template load<W>(from, n, dv, pg * 4, v4);
+    const int d2 = tid % 32, s4 = v0 + tid / 32 * 4;
+#pragma unroll
+    for (int i = 0; i < DK / 64; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t at = min(s4 + j, dv - 1) * (DK / 2) + i * 32 + d2;
+        s[i][j] = *at32<const f2>(S, at);
+        d[i][j] = *at32<const f2>(dS, at);
+      }
+  }
+};
+
 template <typename T, int DK, bool W>
-__global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_last_kernel(
-    const DeltaGradArgs ga, const float* rec, const float* grec, int chunks, uint64_t blocks) {
+__global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
+    const DeltaGradArgs ga, const unsigned char* prep, const float* rec, const float* grec,
+    int chunks, uint64_t blocks) {
   constexpr int U = DK / 32, MT = DK / 16, FULL = Mode<T>::FULL, P = Mode<T>::ROWS;
   extern __shared__ __align__(16) unsigned char lds[];
   const DeltaArgs& a = ga.f;
@@ -1091,118 +1136,90 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_last_kernel(
       }
       continue;
     }
-    // K and Q as rows: their products, the lengths
-    auto bring_kq = [&](bool across_) {
-      const int pos = tid / 16 * 4, c4 = tid % 16 * 4;
-      Rows4<T> k[DK / 64], q[DK / 64];
+    // K and Q, put twice: as rows, for their products, and across
+    Rows4<T> k[DK / 64], q[DK / 64];
+    const int kpos = tid / 16 * 4, kcol = tid % 16 * 4;
 #pragma unroll
-      for (int i = 0; i < DK / 64; ++i) {
-        k[i].template load<W>(Chunk<const T>(a.k, p, kh, a.dk), p.n, a.dk, pos, i * 64 + c4);
-        q[i].template load<W>(Chunk<const T>(a.qr, p, kh, a.dk), p.n, a.dk, pos, i * 64 + c4);
-      }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < DK / 64; ++i) {
-        const int col = i * 64 + c4;
-        k[i].template cut<W>(p.n - pos, a.dk - col);
-        q[i].template cut<W>(p.n - pos, a.dk - col);
-        if (across_) {
-          k[i].turned().put(s.k.a, 2, col, pos);
-          q[i].turned().put(s.k.b, 2, col, pos);
-        } else {
-          k[i].put(s.k.a, U, pos, col);
-          q[i].put(s.k.b, U, pos, col);
-        }
-      }
-      __syncthreads();
-    };
-    // this lane's columns of its own rows of q and k; the rows' lengths from them
-    f4 qo[MT], ko[MT];
-    auto bring_own = [&]() {
-      const Chunk<const T> qc(a.qr, p, kh, a.dk), kc(a.k, p, kh, a.dk);
-      const int row = min(own, p.n - 1);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        qo[m] = ld4<T, W>(qc.at(row * qc.row), m * 16 + g4, a.dk);
-        ko[m] = ld4<T, W>(kc.at(row * kc.row), m * 16 + g4, a.dk);
-      }
-    };
+    for (int i = 0; i < DK / 64; ++i) {
+      k[i].template load<W>(Chunk<const T>(a.k, p, kh, a.dk), p.n, a.dk, kpos, i * 64 + kcol);
+      q[i].template load<W>(Chunk<const T>(a.qr, p, kh, a.dk), p.n, a.dk, kpos, i * 64 + kcol);
+    }
     auto across_g = [&](float x) {
       x = fold16(x, x);
       return fold32(x, x);
     };
-    float ssq = 0.0f, ssk = 0.0f;
-    bring_own();
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        ssq += qo[m][r] * qo[m][r];
-        ssk += ko[m][r] * ko[m][r];
-      }
-    ssq = 1.0f / __builtin_sqrtf(across_g(ssq) + EPS);
-    const float rk = a.unit ? 1.0f / __builtin_sqrtf(across_g(ssk) + EPS) : 1.0f;
-    const float rq = a.unit ? ssq * a.scale : a.scale;
-    __syncthreads();
-    if (g == 0) s.rk[own] = rk, s.rq[own] = rq;
-    f4 dq[MT] = {}, dk[MT] = {};
+    f4 dq[MT] = {}, dk[MT] = {}, qo[MT], ko[MT];  // qo, ko: own rows of q and k
+    float rk = 0.0f, by = 0.0f;  // 1 / |k|, 1 / |q|
     for (int vh = kh * group; vh < (kh + 1) * group; ++vh) {
       p.h = vh;
-      const int64_t at = (((int64_t)p.l * a.HV + vh) * chunks + p.c) * (a.dv * (DK + C));
-      const float *S = same(rec + at), *N = S + a.dv * DK, *dS = same(grec + at), *dR = dS + a.dv * DK;
+      const int64_t record = same(((int64_t)p.l * a.HV + vh) * chunks + p.c);
+      const float *S = rec + record * (a.dv * (DK + C)), *N = S + a.dv * DK;
+      const float *dS = grec + record * (a.dv * (DK + C)), *dR = dS + a.dv * DK;
+      const unsigned char* coef = prep + ((record + 1) * PREP_BYTES - COEF * 4);
+      float co[(COEF + 255) / 256];
+#pragma unroll
+      for (int i = 0; i < (COEF + 255) / 256; ++i)
+        co[i] = *at32<const float>(coef, min(tid + 256 * i, COEF - 1));
+      // the block's first half takes N and dO, its second dR and v
+      const int half = w / 2, pg = tid % 16, vg = tid / 16 % 8;
+      const float* x_ = half ? dR : N;
+      const Chunk<const T> from(half ? a.v : ga.dout, p, vh, a.dv);
+      LastNext<T, DK> next;
+      next.template load<W>(S, dS, x_, from, p.n, a.dv, 0, tid);
       __syncthreads();
-      decays_of(s.dec, a, p);
+#pragma unroll
+      for (int i = 0; i < (COEF + 255) / 256; ++i)
+        if (tid + 256 * i < COEF) reinterpret_cast<float*>(&s.coef)[tid + 256 * i] = co[i];
       f4 pp[4] = {}, aa[4] = {}, mid_p = ZERO, mid_a = ZERO, os[MT] = {}, rs[MT] = {}, ns[MT] = {};
       float dots[4] = {}, tail = 0.0f;
       for (int v0 = 0; v0 < a.dv; v0 += 32) {
-        // N and dR: 8 x 16 pieces of 4 columns x 4 positions; dO as many; S and dS
-        // 8 x DK / 4
-        const int half = w / 2, pg = tid % 16, vg = tid / 16 % 8, v4 = v0 + vg * 4;
-        Four x, sx[DK / 64];
-        Rows4<T> od;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          x.v[i] = *at32<const f4>(half ? dR : N, min(v4 + i, a.dv - 1) * (C / 4) + pg);
-        od.template load<W>(Chunk<const T>(half ? a.v : ga.dout, p, vh, a.dv), p.n, a.dv, pg * 4, v4);
-#pragma unroll
-        for (int i = 0; i < DK / 64; ++i) {
-          const int d4 = (i * 16 + tid % 16) * 4;
-          const int sv = v0 + (tid / 16 % 8) * 4;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            sx[i].v[j] = *at32<const f4>(half ? dS : S, min(sv + j, a.dv - 1) * (DK / 4) + d4 / 4);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (v4 + i >= a.dv) {
-            x.v[i] = ZERO;
-#pragma unroll
-            for (int j = 0; j < DK / 64; ++j) sx[j].v[i] = ZERO;
-          }
         __syncthreads();
         apart();
-        const Four xt = turned(x);  // rows: positions
-        od.template cut<W>(p.n - pg * 4, a.dv - v4);
-        put_full<T>(half ? s.v.r : s.v.n, 1, pg * 4, vg * 4, xt);
-        if (half) {
-          // dV, and dR . v
+        {
+          const int v4 = v0 + vg * 4, s4 = v0 + tid / 32 * 4;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const f4 d = xt.v[i] * od.r[i].value();
-            dots[i] += d[0] + d[1] + d[2] + d[3];
-            const int pos = pg * 4 + i;
-            if (pos < rows)
-              st4<T, W>(Chunk<T>(ga.dv, p, vh, a.dv).at(pos * (uint32_t)ga.dv.row), v4, a.dv,
-                        pos < p.n ? xt.v[i] * s.dec.beta[pos] : ZERO);
-          }
-        } else {
-          od.put(s.v.o, 1, pg * 4, vg * 4);
-        }
+            if (v4 + i >= a.dv) next.x.v[i] = ZERO;
+            if (s4 + i >= a.dv)
 #pragma unroll
-        for (int i = 0; i < DK / 64; ++i)
-          put_full<T>(half ? s.v.d : s.v.s, 1, (i * 16 + tid % 16) * 4, vg * 4, turned(sx[i]));
+              for (int j = 0; j < DK / 64; ++j)
+                next.s[j][i] = next.d[j][i] = typename LastNext<T, DK>::f2{0.0f, 0.0f};
+          }
+          const Four xt = turned(next.x);  // rows: positions
+          next.rows.template cut<W>(p.n - pg * 4, a.dv - v4);
+          put_full<T>(half ? s.v.r : s.v.n, 1, pg * 4, vg * 4, xt);
+          if (half) {
+            // dV, and dR . v
+            const Chunk<T> out(ga.dv, p, vh, a.dv);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const f4 d = xt.v[i] * next.rows.r[i].value();
+              dots[i] += d[0] + d[1] + d[2] + d[3];
+              const int pos = pg * 4 + i;
+              if (pos < rows)
+                st4<T, W>(out.at(pos * out.row), v4, a.dv,
+                          pos < p.n ? xt.v[i] * s.coef.beta[pos] : ZERO);
+            }
+          } else {
+            next.rows.put(s.v.o, 1, pg * 4, vg * 4);
+          }
+          // S and dS: rows of d_k, columns of d_v along them; and <dS, S>
+#pragma unroll
+          for (int i = 0; i < DK / 64; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const f4 sv = {next.s[i][0][e], next.s[i][1][e], next.s[i][2][e], next.s[i][3][e]};
+              const f4 dv = {next.d[i][0][e], next.d[i][1][e], next.d[i][2][e], next.d[i][3][e]};
+              const f4 both = sv * dv;
+              tail += both[0] + both[1] + both[2] + both[3];
+              const int d = i * 64 + tid % 32 * 2 + e;
+              put<T, FULL>(s.v.s, 1, d, tid / 32 * 4, sv);
+              put<T, FULL>(s.v.d, 1, d, tid / 32 * 4, dv);
+            }
+        }
         __syncthreads();
         apart();
+        if (v0 + 32 < a.dv) next.template load<W>(S, dS, x_, from, p.n, a.dv, v0 + 32, tid);
         const Frag<FULL> no = get<FULL>(s.v.n, w, sl), ro = get<FULL>(s.v.r, w, sl);
         const Frag<P> oo = get<P>(s.v.o, w, sl);
 #pragma unroll
@@ -1216,7 +1233,7 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_last_kernel(
 #pragma unroll
             for (int i = FULL - 1; i >= 0; --i) {
               Frag<1> x, y;
-              x.p[0] = *(m <= w ? s.v.n + (m * FULL + i) * 64 + sl : s.v.o + m * 64 + sl);
+              x.p[0] = *((m <= w ? s.v.n + (m * FULL + i) * 64 : s.v.o + m * 64) + slot_in(m, sl));
 #pragma unroll
               for (int j = 0; j < 4; ++j) y.p[0][j] = m <= wv ? oo.p[0][j] : no.p[i][j];
               mma<T>(pp[m], x, y);
@@ -1235,22 +1252,45 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_last_kernel(
           apart();
         }
       }
-      // <dS, S>: the two halves of the block hold one each, so from memory
-      for (int i = tid; i < a.dv * DK / 4; i += 256) {
-        const f4 u = *reinterpret_cast<const f4*>(S + i * 4);
-        const f4 d = *reinterpret_cast<const f4*>(dS + i * 4);
-        tail += u[0] * d[0] + u[1] * d[1] + u[2] * d[2] + u[3] * d[3];
-      }
       tail = over64(tail, Sum());
-      if (tid >= 128) {
+      if (half) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s.dot[tid / 16 % 8][tid % 16 * 4 + i] = dots[i];
+        for (int i = 0; i < 4; ++i) s.dot[vg][pg * 4 + i] = dots[i];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < DK / 64; ++i) {
+        if (vh == kh * group) {
+          k[i].template cut<W>(p.n - kpos, a.dk - i * 64 - kcol);
+          q[i].template cut<W>(p.n - kpos, a.dk - i * 64 - kcol);
+        }
+        k[i].put(s.k.a, U, kpos, i * 64 + kcol);
+        q[i].put(s.k.b, U, kpos, i * 64 + kcol);
+      }
+      __syncthreads();
+      // kk: rows of tile m, column own; qk: m <= w: q of own, k of tile m; m > w: q
+      // of tile m, k of own; the wave's own tile has both (mid: the second).  Which
+      // it is decides addresses and selects, not branches.
+      f4 kk[4] = {}, qk[4] = {}, mid_qk = ZERO;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const Frag<P> kw = get<P>(s.k.a, w * U + u, sl), qw = get<P>(s.k.b, w * U + u, sl);
+        results_of<T>(ko[2 * u], ko[2 * u + 1], kw);
+        results_of<T>(qo[2 * u], qo[2 * u + 1], qw);
+        mma<T>(mid_qk, qw, kw);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          mma<T>(kk[m], get<P>(s.k.a, m * U + u, sl), kw);
+          mma<T>(qk[m], get<P>(m <= w ? s.k.a : s.k.b, m * U + u, sl), either(m <= wv, qw, kw));
+        }
+        apart();
       }
       // from the states
-      bring_own();
-      const float beta = s.dec.beta[own];
+      const float beta = s.coef.beta[own], since = s.coef.since[own], left = s.coef.left[own];
+      rk = s.coef.rk[own];
+      by = s.coef.uq[own];
+      const float rq = by * a.scale;
       float oq = 0.0f, rsk = 0.0f, nsk = 0.0f;
-      const float since = s.dec.since[own], left = s.dec.left[own];
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
 #pragma unroll
@@ -1265,34 +1305,18 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_last_kernel(
       oq = across_g(oq) * (rq * since);
       rsk = across_g(rsk) * (rk * since);
       nsk = across_g(nsk) * (rk * left);
-      // kk: rows of tile m, column own; qk: m <= w: q of own, k of tile m; m > w: q
-      // of tile m, k of own; the wave's own tile has both (mid: the second).  Which
-      // it is decides addresses and selects, not branches.
-      bring_kq(false);
-      f4 kk[4] = {}, qk[4] = {}, mid_qk = ZERO;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const Frag<P> kw = get<P>(s.k.a, w * U + u, sl), qw = get<P>(s.k.b, w * U + u, sl);
-        mma<T>(mid_qk, qw, kw);
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          mma<T>(kk[m], get<P>(s.k.a, m * U + u, sl), kw);
-          mma<T>(qk[m], get<P>(m <= w ? s.k.a : s.k.b, m * U + u, sl), either(m <= wv, qw, kw));
-        }
-        apart();
-      }
-      // what K and Q are multiplied with
+      // what K and Q are multiplied with; sums over a row of dP P and dA A, over a
+      // column, and of dA k.k D
       f4 e[4] = {}, mid_e = ZERO, f[4] = {}, mid_f = ZERO;
-      const int whole = s.dec.whole[own];
-      const float part = s.dec.part[own];
-      // sums over a row of dP P and dA A, over a column, and of dA k.k D
+      const int whole = s.coef.whole[own];
+      const float part = s.coef.part[own];
       float over = 0.0f, down = 0.0f, with_beta = 0.0f;
       auto element = [&](int o, bool row, float p0, float a0, float q0, float k0, f4& eo, f4& fo, int r) {
         // row: own is the row and o the column, else the other way
-        const int dw = s.dec.whole[o] - whole;
-        const float dp = s.dec.part[o] - part;
+        const int dw = s.coef.whole[o] - whole;
+        const float dp = s.coef.part[o] - part;
         const float d = raised(row ? -dw : dw, row ? -dp : dp);
-        const float rko = s.rk[o], rqo = s.rq[o], bo = s.dec.beta[o], ukk = k0 * rk * rko;
+        const float rko = s.coef.rk[o], rqo = s.coef.uq[o] * a.scale, bo = s.coef.beta[o], ukk = k0 * rk * rko;
         const float dP = (row ? o <= own : o >= own) ? p0 * d : 0.0f;
         const float dA = (row ? o < own : o > own) ? -a0 * d : 0.0f;
         const float br = row ? beta : bo;
@@ -1319,8 +1343,13 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_last_kernel(
       with_beta = across_g(with_beta);
       if (g == 0) s.dsum[own] = over - down - nsk + oq - rsk * beta;
       const float lasts = over16(nsk, Sum());
-      if (lane == 0) s.tail[w] = lasts, s.tail[4 + w] = tail * s.dec.since[C - 1];
+      if (lane == 0) s.tail[w] = lasts, s.tail[4 + w] = tail * s.coef.since[C - 1];
       __syncthreads();
+#pragma unroll
+      for (int i = 0; i < DK / 64; ++i) {
+        k[i].turned().put(s.k.a, 2, i * 64 + kcol, kpos);
+        q[i].turned().put(s.k.b, 2, i * 64 + kcol, kpos);
+      }
       if (g == 0 && own < rows) {
         float x = with_beta - rsk;
 #pragma unroll
@@ -1342,37 +1371,34 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_last_kernel(
           ((float*)ga.dg.d)[p.l * ga.dg.lane + (int64_t)(p.c * C + lane) * ga.dg.row + vh] =
               lane < p.n ? (float)x : 0.0f;
       }
-      bring_kq(true);
-      {
-        // e: q's part below (rows j), k's above (rows i); the own tile has both
-        f4 ek[4];
+      __syncthreads();
+      // e: q's part below (rows j), k's above (rows i); the own tile has both
+      f4 ek[4];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          ek[m] = either(m == wv, mid_e, either(m > wv, e[m], ZERO));
-          e[m] = either(m <= wv, e[m], ZERO);
-          f[m] += either(m == wv, mid_f, ZERO);
-        }
-        Frag<FULL> ef[2], kf[2], ff[2];
+      for (int m = 0; m < 4; ++m) {
+        ek[m] = either(m == wv, mid_e, either(m > wv, e[m], ZERO));
+        e[m] = either(m <= wv, e[m], ZERO);
+        f[m] += either(m == wv, mid_f, ZERO);
+      }
+      Frag<FULL> ef[2], kf[2], ff[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        ef[u] = full<T>(e[2 * u], e[2 * u + 1]);
+        kf[u] = full<T>(ek[2 * u], ek[2 * u + 1]);
+        ff[u] = full<T>(f[2 * u], f[2 * u + 1]);
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          ef[u] = full<T>(e[2 * u], e[2 * u + 1]);
-          kf[u] = full<T>(ek[2 * u], ek[2 * u + 1]);
-          ff[u] = full<T>(f[2 * u], f[2 * u + 1]);
+          const Frag<P> kt = get<P>(s.k.a, m * 2 + u, sl);
+          mma<T>(dq[m], kt, ef[u]);
+          mma<T>(dk[m], kt, ff[u]);
+          mma<T>(dk[m], get<P>(s.k.b, m * 2 + u, sl), kf[u]);
+          apart();
         }
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const Frag<P> kt = get<P>(s.k.a, m * 2 + u, sl);
-            mma<T>(dq[m], kt, ef[u]);
-            mma<T>(dk[m], kt, ff[u]);
-            mma<T>(dk[m], get<P>(s.k.b, m * 2 + u, sl), kf[u]);
-            apart();
-          }
-      }
     }
     // through the rows' lengths: d = r (d^ - u (u . d^)), u the unit row
-    bring_own();
     float fq = 0.0f, fk = 0.0f;
     if (a.unit) {
 #pragma unroll
@@ -1382,17 +1408,17 @@ __global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_grad_last_kernel(
           fq += dq[m][r] * qo[m][r];
           fk += dk[m][r] * ko[m][r];
         }
-      fq = across_g(fq) * ssq * ssq;
+      fq = across_g(fq) * by * by;
       fk = across_g(fk) * rk * rk;
     }
-    const float by = a.unit ? ssq : 1.0f;
     if (own < rows) {
+      const bool live = own < p.n;
+      const Chunk<T> oq_(ga.dq, p, kh, a.dk), ok_(ga.dk, p, kh, a.dk);
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        const bool live = own < p.n;
-        st4<T, W>(Chunk<T>(ga.dq, p, kh, a.dk).at(own * (uint32_t)ga.dq.row), m * 16 + g4, a.dk,
+        st4<T, W>(oq_.at(own * oq_.row), m * 16 + g4, a.dk,
                   live ? (dq[m] - qo[m] * fq) * by : ZERO);
-        st4<T, W>(Chunk<T>(ga.dk, p, kh, a.dk).at(own * (uint32_t)ga.dk.row), m * 16 + g4, a.dk,
+        st4<T, W>(ok_.at(own * ok_.row), m * 16 + g4, a.dk,
                   live ? (dk[m] - ko[m] * fk) * rk : ZERO);
       }
     }
@@ -1577,7 +1603,7 @@ hipError_t delta_grad_of(const DeltaGradArgs& ga, hipStream_t s) {
     if ((e = room(delta_grad_last_kernel<T, DK, W>, lds))) return e;
     const uint64_t last = (uint64_t)a.q.lanes * a.H * chunks;
     BOA_LAUNCH((delta_grad_last_kernel<T, DK, W>), grid(last), 256, lds, s, ga,
-               (const float*)a.saved, (const float*)grec, chunks, last);
+               (const unsigned char*)prep, (const float*)a.saved, (const float*)grec, chunks, last);
     return hipGetLastError();
   });
 }

@@ -1020,20 +1020,25 @@ __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
 }
 
 // ---- the rows' gradients of a chunk ----------------------------------------
-// A block per (lane, head of k, chunk) takes all value heads that share the head,
-// a wave 16 of the positions, "own".  Products over d_v come 32 columns at a
-// time, N, dR, dO, S and dS as left operands in LDS and this wave's own rows of
-// them (the same pieces) as right ones:
+// A block of eight waves per (lane, head of k, chunk) takes all value heads that
+// share the head.  Wave w of the first four and wave w of the other four have 16
+// of the positions, "own".  Products over d_v come 32 columns at a time, N, dR,
+// dO, S and dS as left operands in LDS and the own rows of them (the same pieces)
+// as right ones.  The first four waves take dP and dA,
 //   m < w:  dP^T, dA^T (rows j of tile m, column i own)      m > w:  dP, dA (rows i of tile m, column j own)
-// and both for the wave's own tile w; so sums over rows and over columns of dP P
+// and both for the own tile w, so that sums over rows and over columns of dP P
 // and dA A stay within the wave, and what K and Q are multiplied with lies as the
-// right operand.  dQ^T and dK^T [d_k][own] leave as four neighbouring columns a lane.
+// right operand; then those products.  The other four take what comes from the
+// states, dO S^T, dR S^T and N dS^T.  (By the same wave the two do not fit its
+// registers: 249 us for 32 x 1024 rows, 4 heads of 64 and 128 columns, not TBD.)
+// dQ^T and dK^T [d_k][own] leave as four neighbouring columns a lane.
 template <typename T, int DK>
 struct LastLds {
   static constexpr int P = Mode<T>::ROWS, FULL = Mode<T>::FULL;
   union {
     struct {
       u4 a[4 * (DK / 32) * P * 64], b[4 * (DK / 32) * P * 64];  // K, Q: rows; then across
+      f4 states[2 * DK / 16][4][64];  // what the first waves have of dQ and dK
     } k;
     struct {
       u4 n[4 * FULL * 64], r[4 * FULL * 64], o[4 * P * 64];
@@ -1041,7 +1046,7 @@ struct LastLds {
     } v;
   };
   float dot[8][C];  // dR . v, by groups of four columns
-  float dsum[C], tail[8];
+  float dsum[C], from[C], dots[C], tail[8];
   struct {
     float beta[C], unused[3 * C], all[4], part[C];
     int whole[C];
@@ -1070,27 +1075,31 @@ __device__ __forceinline__ f4 one_of(const f4 (&x)[4], int w) {
   return either(w < 2, either(w == 0, x[0], x[1]), either(w == 2, x[2], x[3]));
 }
 
-// What a thread brings of 32 columns of d_v: four columns of four positions of N
-// and v, or of dR and dO; four columns of two rows (of 64) of S and dS.
-template <typename T, int DK>
-struct LastNext {
+// What a thread brings of 32 columns of d_v: of the first 256, four columns of
+// four positions of N and dO, or of dR and v; of the others, four columns of two
+// rows (of 64) of S and dS.
+template <typename T>
+struct LastRows {
   Four x;
   Rows4<T> rows;
-  typedef float f2 __attribute__((ext_vector_type(2)));
-  f2 s[DK / 64][4], d[DK / 64][4];
   template <bool W>
-  __device__ __forceinline__ void load(const float* S, const float* dS, const float* x_,
-                                       const Chunk<const T>& from, int n, int dv, int v0, int tid) {
-    const int pg = tid % 16, v4 = v0 + tid / 16 % 8 * 4;
+  __device__ __forceinline__ void load(const float* x_, const Chunk<const T>& from, int n, int dv,
+                                       int v4, int pg) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x.v[i] = *at32<const f4>(x_, min(v4 + i, dv - 1) * (C / 4) + pg);
     rows.template load<W>(from, n, dv, pg * 4, v4);
-    const int d2 = tid % 32, s4 = v0 + tid / 32 * 4;
+  }
+};
+typedef float f2 __attribute__((ext_vector_type(2)));
+template <int DK>
+struct LastStates {
+  f2 s[DK / 64][4], d[DK / 64][4];
+  __device__ __forceinline__ void load(const float* S, const float* dS, int dv, int v4, int d2) {
 #pragma unroll
     for (int i = 0; i < DK / 64; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t at = min(s4 + j, dv - 1) * (DK / 2) + i * 32 + d2;
+        const uint32_t at = min(v4 + j, dv - 1) * (DK / 2) + i * 32 + d2;
         s[i][j] = *at32<const f2>(S, at);
         d[i][j] = *at32<const f2>(dS, at);
       }
@@ -1098,7 +1107,7 @@ struct LastNext {
 };
 
 template <typename T, int DK, bool W>
-__global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
+__global__ __launch_bounds__(512, 2) void delta_grad_last_kernel(
     const DeltaGradArgs ga, const unsigned char* prep, const float* rec, const float* grec,
     int chunks, uint64_t blocks) {
   constexpr int U = DK / 32, MT = DK / 16, FULL = Mode<T>::FULL, P = Mode<T>::ROWS;
@@ -1109,9 +1118,10 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
   for (uint64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
     // what follows from the thread's number is computed here, not kept from
     // before the loop: there are no registers to keep it in
-    int tid = threadIdx.x;
-    asm volatile("" : "+v"(tid));
-    const int lane = tid & 63, w = same(tid >> 6);
+    int all = threadIdx.x;
+    asm volatile("" : "+v"(all));
+    const bool states = same(all >> 8) != 0;
+    const int tid = all & 255, lane = tid & 63, w = same(tid >> 6);
     const int i16 = lane % 16, g = lane / 16, g4 = 4 * g, sl = slot_of(i16, g), own = w * 16 + i16;
     // the wave again, but as a vector: what it decides by selects is no branch
     const int wv = tid >> 6;
@@ -1122,75 +1132,65 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
     p.n = same(within(seq_len(a.q, p.l), p.c));
     const int rows = min(C, a.q.T - p.c * C);
     if (!p.n) {  // past the lane's length: zero
-      for (int i = tid; i < rows * group; i += 256) {
+      for (int i = all; i < rows * group; i += 512) {
         const int64_t t = p.c * C + i / group, h = kh * group + i % group;
         ((float*)ga.dg.d)[p.l * ga.dg.lane + t * ga.dg.row + h] = 0.0f;
         ((float*)ga.dbeta.d)[p.l * ga.dbeta.lane + t * ga.dbeta.row + h] = 0.0f;
       }
       const int wide = group * a.dv;
-      for (int i = tid; i < rows * wide; i += 256)
+      for (int i = all; i < rows * wide; i += 512)
         st1(Chunk<T>(ga.dv, p, kh, wide).at(i / wide * (uint32_t)ga.dv.row + i % wide), 0.0f);
-      for (int i = tid; i < rows * a.dk; i += 256) {
+      for (int i = all; i < rows * a.dk; i += 512) {
         st1(Chunk<T>(ga.dq, p, kh, a.dk).at(i / a.dk * (uint32_t)ga.dq.row + i % a.dk), 0.0f);
         st1(Chunk<T>(ga.dk, p, kh, a.dk).at(i / a.dk * (uint32_t)ga.dk.row + i % a.dk), 0.0f);
       }
       continue;
     }
-    // K and Q, put twice: as rows, for their products, and across
-    Rows4<T> k[DK / 64], q[DK / 64];
-    const int kpos = tid / 16 * 4, kcol = tid % 16 * 4;
-#pragma unroll
-    for (int i = 0; i < DK / 64; ++i) {
-      k[i].template load<W>(Chunk<const T>(a.k, p, kh, a.dk), p.n, a.dk, kpos, i * 64 + kcol);
-      q[i].template load<W>(Chunk<const T>(a.qr, p, kh, a.dk), p.n, a.dk, kpos, i * 64 + kcol);
-    }
     auto across_g = [&](float x) {
       x = fold16(x, x);
       return fold32(x, x);
     };
-    f4 dq[MT] = {}, dk[MT] = {}, qo[MT], ko[MT];  // qo, ko: own rows of q and k
-    float rk = 0.0f, by = 0.0f;  // 1 / |k|, 1 / |q|
-    for (int vh = kh * group; vh < (kh + 1) * group; ++vh) {
-      p.h = vh;
-      const int64_t record = same(((int64_t)p.l * a.HV + vh) * chunks + p.c);
-      const float *S = rec + record * (a.dv * (DK + C)), *N = S + a.dv * DK;
-      const float *dS = grec + record * (a.dv * (DK + C)), *dR = dS + a.dv * DK;
-      const unsigned char* coef = prep + ((record + 1) * PREP_BYTES - COEF * 4);
-      float co[(COEF + 255) / 256];
+    // Each four waves have a loop of their own, with as many barriers, so that
+    // neither keeps registers for the other.
+    if (!states) {
+      // K and Q, put twice: as rows, for their products, and across
+      Rows4<T> k[DK / 64], q[DK / 64];
+      const int kpos = tid / 16 * 4, kcol = tid % 16 * 4;
 #pragma unroll
-      for (int i = 0; i < (COEF + 255) / 256; ++i)
-        co[i] = *at32<const float>(coef, min(tid + 256 * i, COEF - 1));
-      // the block's first half takes N and dO, its second dR and v
-      const int half = w / 2, pg = tid % 16, vg = tid / 16 % 8;
-      const float* x_ = half ? dR : N;
-      const Chunk<const T> from(half ? a.v : ga.dout, p, vh, a.dv);
-      LastNext<T, DK> next;
-      next.template load<W>(S, dS, x_, from, p.n, a.dv, 0, tid);
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < (COEF + 255) / 256; ++i)
-        if (tid + 256 * i < COEF) reinterpret_cast<float*>(&s.coef)[tid + 256 * i] = co[i];
-      f4 pp[4] = {}, aa[4] = {}, mid_p = ZERO, mid_a = ZERO, os[MT] = {}, rs[MT] = {}, ns[MT] = {};
-      float dots[4] = {}, tail = 0.0f;
-      for (int v0 = 0; v0 < a.dv; v0 += 32) {
+      for (int i = 0; i < DK / 64; ++i) {
+        k[i].template load<W>(Chunk<const T>(a.k, p, kh, a.dk), p.n, a.dk, kpos, i * 64 + kcol);
+        q[i].template load<W>(Chunk<const T>(a.qr, p, kh, a.dk), p.n, a.dk, kpos, i * 64 + kcol);
+      }
+      for (int vh = kh * group; vh < (kh + 1) * group; ++vh) {
+        p.h = vh;
+        const int64_t record = same(((int64_t)p.l * a.HV + vh) * chunks + p.c);
+        const float *S = rec + record * (a.dv * (DK + C)), *N = S + a.dv * DK;
+        const float *dS = grec + record * (a.dv * (DK + C)), *dR = dS + a.dv * DK;
+        const unsigned char* coef = prep + ((record + 1) * PREP_BYTES - COEF * 4);
+        const float co0 = *at32<const float>(coef, min(all, COEF - 1));
+        const float co1 = *at32<const float>(coef, min(all + 512, COEF - 1));
         __syncthreads();
-        apart();
-        {
-          const int v4 = v0 + vg * 4, s4 = v0 + tid / 32 * 4;
+        reinterpret_cast<float*>(&s.coef)[min(all, COEF - 1)] = co0;
+        if (all + 512 < COEF) reinterpret_cast<float*>(&s.coef)[all + 512] = co1;
+        // the first two waves take N and dO, the others dR and v
+        const int half = w / 2, pg = tid % 16, vg = tid / 16 % 8;
+        const float* x_ = half ? dR : N;
+        const Chunk<const T> from(half ? a.v : ga.dout, p, vh, a.dv);
+        const Chunk<T> out(ga.dv, p, vh, a.dv);
+        LastRows<T> next;
+        next.template load<W>(x_, from, p.n, a.dv, vg * 4, pg);
+        f4 pp[4] = {}, aa[4] = {}, mid_p = ZERO, mid_a = ZERO;
+        f4 dots = ZERO;
+        for (int v0 = 0; v0 < a.dv; v0 += 32) {
+          const int v4 = v0 + vg * 4;
+          __syncthreads();
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (v4 + i >= a.dv) next.x.v[i] = ZERO;
-            if (s4 + i >= a.dv)
-#pragma unroll
-              for (int j = 0; j < DK / 64; ++j)
-                next.s[j][i] = next.d[j][i] = typename LastNext<T, DK>::f2{0.0f, 0.0f};
-          }
+          for (int i = 0; i < 4; ++i) next.x.v[i] = either(v4 + i < a.dv, next.x.v[i], ZERO);
           const Four xt = turned(next.x);  // rows: positions
           next.rows.template cut<W>(p.n - pg * 4, a.dv - v4);
           put_full<T>(half ? s.v.r : s.v.n, 1, pg * 4, vg * 4, xt);
           if (half) {
             // dV, and dR . v
-            const Chunk<T> out(ga.dv, p, vh, a.dv);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const f4 d = xt.v[i] * next.rows.r[i].value();
@@ -1203,223 +1203,275 @@ __global__ __launch_bounds__(256, 1) void delta_grad_last_kernel(
           } else {
             next.rows.put(s.v.o, 1, pg * 4, vg * 4);
           }
-          // S and dS: rows of d_k, columns of d_v along them; and <dS, S>
+          __syncthreads();
+          apart();
+          if (v0 + 32 < a.dv) next.template load<W>(x_, from, p.n, a.dv, v4 + 32, pg);
+          const Frag<FULL> no = get<FULL>(s.v.n, w, sl), ro = get<FULL>(s.v.r, w, sl);
+          const Frag<P> oo = get<P>(s.v.o, w, sl);
 #pragma unroll
-          for (int i = 0; i < DK / 64; ++i)
+          for (int m = 0; m < 4; ++m) {
+            // N of tile m with dO and dR of own, or dO and dR of tile m with N of own
+            mma<T>(aa[m], get<FULL>(m <= w ? s.v.n : s.v.r, m, sl), either(m <= wv, ro, no));
+            if constexpr (P == FULL) {
+              mma<T>(pp[m], get<P>(m <= w ? s.v.n : s.v.o, m, sl), either(m <= wv, oo, no));
+            } else {
+              // one part of dO, three of N, whichever is on the left: the small first
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const f4 sv = {next.s[i][0][e], next.s[i][1][e], next.s[i][2][e], next.s[i][3][e]};
-              const f4 dv = {next.d[i][0][e], next.d[i][1][e], next.d[i][2][e], next.d[i][3][e]};
-              const f4 both = sv * dv;
-              tail += both[0] + both[1] + both[2] + both[3];
-              const int d = i * 64 + tid % 32 * 2 + e;
-              put<T, FULL>(s.v.s, 1, d, tid / 32 * 4, sv);
-              put<T, FULL>(s.v.d, 1, d, tid / 32 * 4, dv);
+              for (int i = FULL - 1; i >= 0; --i) {
+                Frag<1> x, y;
+                x.p[0] = *((m <= w ? s.v.n + (m * FULL + i) * 64 : s.v.o + m * 64) + slot_in(m, sl));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y.p[0][j] = m <= wv ? oo.p[0][j] : no.p[i][j];
+                mma<T>(pp[m], x, y);
+              }
             }
+            apart();
+          }
+          mma<T>(mid_p, oo, no);
+          mma<T>(mid_a, ro, no);
+        }
+        if (half) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s.dot[vg][pg * 4 + i] = dots[i];
         }
         __syncthreads();
-        apart();
-        if (v0 + 32 < a.dv) next.template load<W>(S, dS, x_, from, p.n, a.dv, v0 + 32, tid);
-        const Frag<FULL> no = get<FULL>(s.v.n, w, sl), ro = get<FULL>(s.v.r, w, sl);
-        const Frag<P> oo = get<P>(s.v.o, w, sl);
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          // N of tile m with dO and dR of own, or dO and dR of tile m with N of own
-          mma<T>(aa[m], get<FULL>(m <= w ? s.v.n : s.v.r, m, sl), either(m <= wv, ro, no));
-          if constexpr (P == FULL) {
-            mma<T>(pp[m], get<P>(m <= w ? s.v.n : s.v.o, m, sl), either(m <= wv, oo, no));
-          } else {
-            // one part of dO, three of N, whichever is on the left: the small first
+        for (int i = 0; i < DK / 64; ++i) {
+          if (vh == kh * group) {
+            k[i].template cut<W>(p.n - kpos, a.dk - i * 64 - kcol);
+            q[i].template cut<W>(p.n - kpos, a.dk - i * 64 - kcol);
+          }
+          k[i].put(s.k.a, U, kpos, i * 64 + kcol);
+          q[i].put(s.k.b, U, kpos, i * 64 + kcol);
+        }
+        __syncthreads();
+        // kk: rows of tile m, column own; qk: m <= w: q of own, k of tile m; m > w: q
+        // of tile m, k of own; the wave's own tile has both (mid: the second).  Which
+        // it is decides addresses and selects, not branches.
+        f4 kk[4] = {}, qk[4] = {}, mid_qk = ZERO;
 #pragma unroll
-            for (int i = FULL - 1; i >= 0; --i) {
-              Frag<1> x, y;
-              x.p[0] = *((m <= w ? s.v.n + (m * FULL + i) * 64 : s.v.o + m * 64) + slot_in(m, sl));
+        for (int u = 0; u < U; ++u) {
+          const Frag<P> kw = get<P>(s.k.a, w * U + u, sl), qw = get<P>(s.k.b, w * U + u, sl);
+          mma<T>(mid_qk, qw, kw);
 #pragma unroll
-              for (int j = 0; j < 4; ++j) y.p[0][j] = m <= wv ? oo.p[0][j] : no.p[i][j];
-              mma<T>(pp[m], x, y);
-            }
+          for (int m = 0; m < 4; ++m) {
+            mma<T>(kk[m], get<P>(s.k.a, m * U + u, sl), kw);
+            mma<T>(qk[m], get<P>(m <= w ? s.k.a : s.k.b, m * U + u, sl), either(m <= wv, qw, kw));
           }
           apart();
         }
-        mma<T>(mid_p, oo, no);
-        mma<T>(mid_a, ro, no);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const Frag<FULL> sm = get<FULL>(s.v.s, m, sl);
-          mma<T>(os[m], sm, oo);
-          mma<T>(rs[m], sm, ro);
-          mma<T>(ns[m], get<FULL>(s.v.d, m, sl), no);
-          apart();
-        }
-      }
-      tail = over64(tail, Sum());
-      if (half) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s.dot[vg][pg * 4 + i] = dots[i];
-      }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < DK / 64; ++i) {
-        if (vh == kh * group) {
-          k[i].template cut<W>(p.n - kpos, a.dk - i * 64 - kcol);
-          q[i].template cut<W>(p.n - kpos, a.dk - i * 64 - kcol);
-        }
-        k[i].put(s.k.a, U, kpos, i * 64 + kcol);
-        q[i].put(s.k.b, U, kpos, i * 64 + kcol);
-      }
-      __syncthreads();
-      // kk: rows of tile m, column own; qk: m <= w: q of own, k of tile m; m > w: q
-      // of tile m, k of own; the wave's own tile has both (mid: the second).  Which
-      // it is decides addresses and selects, not branches.
-      f4 kk[4] = {}, qk[4] = {}, mid_qk = ZERO;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const Frag<P> kw = get<P>(s.k.a, w * U + u, sl), qw = get<P>(s.k.b, w * U + u, sl);
-        results_of<T>(ko[2 * u], ko[2 * u + 1], kw);
-        results_of<T>(qo[2 * u], qo[2 * u + 1], qw);
-        mma<T>(mid_qk, qw, kw);
+        // what K and Q are multiplied with; sums over a row of dP P and dA A, over a
+        // column, and of dA k.k D
+        f4 e[4] = {}, mid_e = ZERO, f[4] = {}, mid_f = ZERO;
+        const int whole = s.coef.whole[own];
+        const float part = s.coef.part[own], beta = s.coef.beta[own], rk = s.coef.rk[own];
+        const float rq = s.coef.uq[own] * a.scale;
+        float over = 0.0f, down = 0.0f, with_beta = 0.0f;
+        auto element = [&](int o, bool row, float p0, float a0, float q0, float k0, f4& eo, f4& fo,
+                           int r) {
+          // row: own is the row and o the column, else the other way
+          const int dw = s.coef.whole[o] - whole;
+          const float dp = s.coef.part[o] - part;
+          const float d = raised(row ? -dw : dw, row ? -dp : dp);
+          const float rko = s.coef.rk[o], rqo = s.coef.uq[o] * a.scale, bo = s.coef.beta[o];
+          const float ukk = k0 * rk * rko;
+          const float dP = (row ? o <= own : o >= own) ? p0 * d : 0.0f;
+          const float dA = (row ? o < own : o > own) ? -a0 * d : 0.0f;
+          const float br = row ? beta : bo;
+          const float both = dP * (q0 * (row ? rq * rko : rqo * rk)) + dA * (br * ukk);
+          over += row ? both : 0.0f;
+          down += row ? 0.0f : both;
+          with_beta += row ? dA * ukk : 0.0f;
+          eo[r] += dP * (row ? rko * a.scale : rqo);
+          fo[r] += dA * (br * rko);
+        };
+        const f4 mid_k = one_of(kk, wv);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          mma<T>(kk[m], get<P>(s.k.a, m * U + u, sl), kw);
-          mma<T>(qk[m], get<P>(m <= w ? s.k.a : s.k.b, m * U + u, sl), either(m <= wv, qw, kw));
-        }
-        apart();
-      }
-      // from the states
-      const float beta = s.coef.beta[own], since = s.coef.since[own], left = s.coef.left[own];
-      rk = s.coef.rk[own];
-      by = s.coef.uq[own];
-      const float rq = by * a.scale;
-      float oq = 0.0f, rsk = 0.0f, nsk = 0.0f;
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          oq += os[m][r] * qo[m][r];
-          rsk += rs[m][r] * ko[m][r];
-          nsk += ns[m][r] * ko[m][r];
-        }
-        dq[m] += os[m] * (since * a.scale);
-        dk[m] += ns[m] * left - rs[m] * (since * beta);
-      }
-      oq = across_g(oq) * (rq * since);
-      rsk = across_g(rsk) * (rk * since);
-      nsk = across_g(nsk) * (rk * left);
-      // what K and Q are multiplied with; sums over a row of dP P and dA A, over a
-      // column, and of dA k.k D
-      f4 e[4] = {}, mid_e = ZERO, f[4] = {}, mid_f = ZERO;
-      const int whole = s.coef.whole[own];
-      const float part = s.coef.part[own];
-      float over = 0.0f, down = 0.0f, with_beta = 0.0f;
-      auto element = [&](int o, bool row, float p0, float a0, float q0, float k0, f4& eo, f4& fo, int r) {
-        // row: own is the row and o the column, else the other way
-        const int dw = s.coef.whole[o] - whole;
-        const float dp = s.coef.part[o] - part;
-        const float d = raised(row ? -dw : dw, row ? -dp : dp);
-        const float rko = s.coef.rk[o], rqo = s.coef.uq[o] * a.scale, bo = s.coef.beta[o], ukk = k0 * rk * rko;
-        const float dP = (row ? o <= own : o >= own) ? p0 * d : 0.0f;
-        const float dA = (row ? o < own : o > own) ? -a0 * d : 0.0f;
-        const float br = row ? beta : bo;
-        const float both = dP * (q0 * (row ? rq * rko : rqo * rk)) + dA * (br * ukk);
-        over += row ? both : 0.0f;
-        down += row ? 0.0f : both;
-        with_beta += row ? dA * ukk : 0.0f;
-        eo[r] += dP * (row ? rko * a.scale : rqo);
-        fo[r] += dA * (br * rko);
-      };
-      const f4 mid_k = one_of(kk, wv);
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          element(m * 16 + g4 + r, m <= wv, pp[m][r], aa[m][r], qk[m][r], kk[m][r], e[m], f[m], r);
-        apart();
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        element(w * 16 + g4 + r, false, mid_p[r], mid_a[r], mid_qk[r], mid_k[r], mid_e, mid_f, r);
-      over = across_g(over);
-      down = across_g(down);
-      with_beta = across_g(with_beta);
-      if (g == 0) s.dsum[own] = over - down - nsk + oq - rsk * beta;
-      const float lasts = over16(nsk, Sum());
-      if (lane == 0) s.tail[w] = lasts, s.tail[4 + w] = tail * s.coef.since[C - 1];
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < DK / 64; ++i) {
-        k[i].turned().put(s.k.a, 2, i * 64 + kcol, kpos);
-        q[i].turned().put(s.k.b, 2, i * 64 + kcol, kpos);
-      }
-      if (g == 0 && own < rows) {
-        float x = with_beta - rsk;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x += s.dot[i][own];
-        ((float*)ga.dbeta.d)[p.l * ga.dbeta.lane + (int64_t)(p.c * C + own) * ga.dbeta.row + vh] =
-            own < p.n ? x : 0.0f;
-      }
-      if (w == 0) {
-        // dg: the sums of dG from each position to the chunk's last
-        double x = (double)s.dsum[lane];
-        if (lane == C - 1)
-          for (int i = 0; i < 8; ++i) x += (double)s.tail[i];
-#pragma unroll
-        for (int m = 1; m < C; m *= 2) {
-          const double y = __shfl_down(x, m);
-          if (lane + m < C) x += y;
-        }
-        if (lane < rows)
-          ((float*)ga.dg.d)[p.l * ga.dg.lane + (int64_t)(p.c * C + lane) * ga.dg.row + vh] =
-              lane < p.n ? (float)x : 0.0f;
-      }
-      __syncthreads();
-      // e: q's part below (rows j), k's above (rows i); the own tile has both
-      f4 ek[4];
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        ek[m] = either(m == wv, mid_e, either(m > wv, e[m], ZERO));
-        e[m] = either(m <= wv, e[m], ZERO);
-        f[m] += either(m == wv, mid_f, ZERO);
-      }
-      Frag<FULL> ef[2], kf[2], ff[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        ef[u] = full<T>(e[2 * u], e[2 * u + 1]);
-        kf[u] = full<T>(ek[2 * u], ek[2 * u + 1]);
-        ff[u] = full<T>(f[2 * u], f[2 * u + 1]);
-      }
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const Frag<P> kt = get<P>(s.k.a, m * 2 + u, sl);
-          mma<T>(dq[m], kt, ef[u]);
-          mma<T>(dk[m], kt, ff[u]);
-          mma<T>(dk[m], get<P>(s.k.b, m * 2 + u, sl), kf[u]);
+          for (int r = 0; r < 4; ++r)
+            element(m * 16 + g4 + r, m <= wv, pp[m][r], aa[m][r], qk[m][r], kk[m][r], e[m], f[m], r);
           apart();
         }
-    }
-    // through the rows' lengths: d = r (d^ - u (u . d^)), u the unit row
-    float fq = 0.0f, fk = 0.0f;
-    if (a.unit) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+        for (int r = 0; r < 4; ++r)
+          element(w * 16 + g4 + r, false, mid_p[r], mid_a[r], mid_qk[r], mid_k[r], mid_e, mid_f, r);
+        over = across_g(over);
+        down = across_g(down);
+        with_beta = across_g(with_beta);
+        if (g == 0) s.dsum[own] = over - down, s.dots[own] = with_beta;
+        __syncthreads();
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          fq += dq[m][r] * qo[m][r];
-          fk += dk[m][r] * ko[m][r];
+        for (int i = 0; i < DK / 64; ++i) {
+          k[i].turned().put(s.k.a, 2, i * 64 + kcol, kpos);
+          q[i].turned().put(s.k.b, 2, i * 64 + kcol, kpos);
         }
-      fq = across_g(fq) * by * by;
-      fk = across_g(fk) * rk * rk;
-    }
-    if (own < rows) {
-      const bool live = own < p.n;
-      const Chunk<T> oq_(ga.dq, p, kh, a.dk), ok_(ga.dk, p, kh, a.dk);
+        // e: q's part below (rows j), k's above (rows i); the own tile has both
+        f4 ek[4];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        st4<T, W>(oq_.at(own * oq_.row), m * 16 + g4, a.dk,
-                  live ? (dq[m] - qo[m] * fq) * by : ZERO);
-        st4<T, W>(ok_.at(own * ok_.row), m * 16 + g4, a.dk,
-                  live ? (dk[m] - ko[m] * fk) * rk : ZERO);
+        for (int m = 0; m < 4; ++m) {
+          ek[m] = either(m == wv, mid_e, either(m > wv, e[m], ZERO));
+          e[m] = either(m <= wv, e[m], ZERO);
+          f[m] += either(m == wv, mid_f, ZERO);
+        }
+        Frag<FULL> ef[2], kf[2], ff[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          ef[u] = full<T>(e[2 * u], e[2 * u + 1]);
+          kf[u] = full<T>(ek[2 * u], ek[2 * u + 1]);
+          ff[u] = full<T>(f[2 * u], f[2 * u + 1]);
+        }
+        __syncthreads();  // K and Q are there, across
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          f4 q0 = ZERO, k0 = ZERO;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const Frag<P> kt = get<P>(s.k.a, m * 2 + u, sl);
+            mma<T>(q0, kt, ef[u]);
+            mma<T>(k0, kt, ff[u]);
+            mma<T>(k0, get<P>(s.k.b, m * 2 + u, sl), kf[u]);
+          }
+          s.k.states[m][w][lane] = q0;
+          s.k.states[MT + m][w][lane] = k0;
+          apart();
+        }
+        __syncthreads();
+      }
+    } else {
+      f4 dq[MT] = {}, dk[MT] = {}, qo[MT], ko[MT];  // the other waves'; qo, ko: own rows of q and k
+      for (int vh = kh * group; vh < (kh + 1) * group; ++vh) {
+        p.h = vh;
+        const int64_t record = same(((int64_t)p.l * a.HV + vh) * chunks + p.c);
+        const float *S = rec + record * (a.dv * (DK + C)), *N = S + a.dv * DK;
+        const float *dS = grec + record * (a.dv * (DK + C)), *dR = dS + a.dv * DK;
+        const unsigned char* coef = prep + ((record + 1) * PREP_BYTES - COEF * 4);
+        const float co0 = *at32<const float>(coef, min(all, COEF - 1));
+        const float co1 = *at32<const float>(coef, min(all + 512, COEF - 1));
+        __syncthreads();
+        reinterpret_cast<float*>(&s.coef)[min(all, COEF - 1)] = co0;
+        if (all + 512 < COEF) reinterpret_cast<float*>(&s.coef)[all + 512] = co1;
+        const int d2 = tid % 32, vg = tid / 32;
+        LastStates<DK> next;
+        next.load(S, dS, a.dv, vg * 4, d2);
+        f4 os[MT] = {}, rs[MT] = {}, ns[MT] = {};
+        float tail = 0.0f;
+        for (int v0 = 0; v0 < a.dv; v0 += 32) {
+          const int v4 = v0 + vg * 4;
+          __syncthreads();
+          // rows of d_k, columns of d_v along them; and <dS, S>
+#pragma unroll
+          for (int i = 0; i < DK / 64; ++i)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              f4 sv, dv;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                sv[j] = v4 + j < a.dv ? next.s[i][j][r] : 0.0f;
+                dv[j] = v4 + j < a.dv ? next.d[i][j][r] : 0.0f;
+              }
+              const f4 both = sv * dv;
+              tail += both[0] + both[1] + both[2] + both[3];
+              put<T, FULL>(s.v.s, 1, i * 64 + d2 * 2 + r, vg * 4, sv);
+              put<T, FULL>(s.v.d, 1, i * 64 + d2 * 2 + r, vg * 4, dv);
+            }
+          __syncthreads();
+          apart();
+          if (v0 + 32 < a.dv) next.load(S, dS, a.dv, v4 + 32, d2);
+          const Frag<FULL> no = get<FULL>(s.v.n, w, sl), ro = get<FULL>(s.v.r, w, sl);
+          const Frag<P> oo = get<P>(s.v.o, w, sl);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            const Frag<FULL> sm = get<FULL>(s.v.s, m, sl);
+            mma<T>(os[m], sm, oo);
+            mma<T>(rs[m], sm, ro);
+            mma<T>(ns[m], get<FULL>(s.v.d, m, sl), no);
+            apart();
+          }
+        }
+        tail = over64(tail, Sum());
+        __syncthreads();
+        __syncthreads();  // K and Q are there
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          results_of<T>(ko[2 * u], ko[2 * u + 1], get<P>(s.k.a, w * U + u, sl));
+          results_of<T>(qo[2 * u], qo[2 * u + 1], get<P>(s.k.b, w * U + u, sl));
+        }
+        const float beta = s.coef.beta[own], since = s.coef.since[own], left = s.coef.left[own];
+        const float rk = s.coef.rk[own], rq = s.coef.uq[own] * a.scale;
+        float oq = 0.0f, rsk = 0.0f, nsk = 0.0f;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            oq += os[m][r] * qo[m][r];
+            rsk += rs[m][r] * ko[m][r];
+            nsk += ns[m][r] * ko[m][r];
+          }
+          dq[m] += os[m] * (since * a.scale);
+          dk[m] += ns[m] * left - rs[m] * (since * beta);
+        }
+        oq = across_g(oq) * (rq * since);
+        rsk = across_g(rsk) * (rk * since);
+        nsk = across_g(nsk) * (rk * left);
+        if (g == 0) s.from[own] = oq - nsk - rsk * beta;
+        const float lasts = over16(nsk, Sum());
+        if (lane == 0) s.tail[w] = lasts, s.tail[4 + w] = tail * s.coef.since[C - 1];
+        __syncthreads();
+        if (g == 0 && own < rows) {
+          float x = s.dots[own] - rsk;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x += s.dot[i][own];
+          ((float*)ga.dbeta.d)[p.l * ga.dbeta.lane + (int64_t)(p.c * C + own) * ga.dbeta.row + vh] =
+              own < p.n ? x : 0.0f;
+        }
+        __syncthreads();
+        if (w == 0) {
+          // dg: the sums of dG from each position to the chunk's last
+          double x = (double)s.dsum[lane] + (double)s.from[lane];
+          if (lane == C - 1)
+            for (int i = 0; i < 8; ++i) x += (double)s.tail[i];
+#pragma unroll
+          for (int m = 1; m < C; m *= 2) {
+            const double y = __shfl_down(x, m);
+            if (lane + m < C) x += y;
+          }
+          if (lane < rows)
+            ((float*)ga.dg.d)[p.l * ga.dg.lane + (int64_t)(p.c * C + lane) * ga.dg.row + vh] =
+                lane < p.n ? (float)x : 0.0f;
+        }
+        __syncthreads();
+        // the two parts meet
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          dq[m] += s.k.states[m][w][lane];
+          dk[m] += s.k.states[MT + m][w][lane];
+        }
+      }
+      // through the rows' lengths: d = r (d^ - u (u . d^)), u the unit row
+      float fq = 0.0f, fk = 0.0f;
+      const float rk = s.coef.rk[own], by = s.coef.uq[own];
+      if (a.unit) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            fq += dq[m][r] * qo[m][r];
+            fk += dk[m][r] * ko[m][r];
+          }
+        fq = across_g(fq) * by * by;
+        fk = across_g(fk) * rk * rk;
+      }
+      if (own < rows) {
+        const bool live = own < p.n;
+        const Chunk<T> oq_(ga.dq, p, kh, a.dk), ok_(ga.dk, p, kh, a.dk);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          st4<T, W>(oq_.at(own * oq_.row), m * 16 + g4, a.dk,
+                    live ? (dq[m] - qo[m] * fq) * by : ZERO);
+          st4<T, W>(ok_.at(own * ok_.row), m * 16 + g4, a.dk,
+                    live ? (dk[m] - ko[m] * fk) * rk : ZERO);
+        }
       }
     }
     __syncthreads();
@@ -1602,7 +1654,7 @@ hipError_t delta_grad_of(const DeltaGradArgs& ga, hipStream_t s) {
     lds = sizeof(LastLds<T, DK>);
     if ((e = room(delta_grad_last_kernel<T, DK, W>, lds))) return e;
     const uint64_t last = (uint64_t)a.q.lanes * a.H * chunks;
-    BOA_LAUNCH((delta_grad_last_kernel<T, DK, W>), grid(last), 256, lds, s, ga,
+    BOA_LAUNCH((delta_grad_last_kernel<T, DK, W>), grid(last), 512, lds, s, ga,
                (const unsigned char*)prep, (const float*)a.saved, (const float*)grec, chunks, last);
     return hipGetLastError();
   });

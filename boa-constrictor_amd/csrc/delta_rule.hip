@@ -773,34 +773,57 @@ __device__ __forceinline__ void put_result(u4* tile, const f4 (&o)[4], int wave,
     if (4 * pg + e < n) x.r[e].template store<W>(out, first + e * out.row, dv - col);
 }
 
-template <typename T, int DK, bool W>
+// Few sequences of many chunks are cut into segments.  A first pass takes each
+// from a zero state, and beside it (LOCAL's tiles past those of d_v) from the
+// columns of the identity without v: its last state is then what the segment adds
+// and what it makes of the state before it.  The combine kernel chains those, and
+// the main pass takes every segment from its own first state.
+struct Segments {
+  int n, chunks;  // segments of a sequence, chunks of a segment
+  float* local;   // [lane][v head][segment][64 tiles + d_k columns][d_k]
+  float* first;   // [lane][v head][segment][64 tiles columns][d_k]: the states it is taken from
+};
+
+template <typename T, int DK, bool W, bool LOCAL>
 __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
     const DeltaArgs a, const unsigned char* prep, float* rec, int chunks, int tiles,
-    uint32_t blocks) {
+    const Segments seg, uint32_t blocks) {
   using M = Mode<T>;
   constexpr int U = DK / 32, MT = DK / 16, FULL = M::FULL, P = M::ROWS;
   extern __shared__ __align__(16) unsigned char lds[];
   ChainLds<T, DK, false>& s = *reinterpret_cast<ChainLds<T, DK, false>*>(lds);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i16 = lane % 16, g = lane / 16, sl = slot_of(i16, g);
+  const int per = LOCAL ? tiles + DK / 64 : tiles;
   for (uint32_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const uint32_t lh = same((int)(b / tiles));
+    const uint32_t ls = same((int)(b / per)), lh = same((int)(ls / seg.n));
+    const int sg = ls - lh * seg.n;
     Place p;
     p.l = same((int)(lh / a.HV));
     p.h = lh - p.l * a.HV;
-    const int kh = same(p.h / (a.HV / a.H)), len = same(seq_len(a.q, p.l)), last = (len + C - 1) / C;
-    const int vb = same((int)(b - lh * tiles) * 64), v0 = vb + wave * 16, col = v0 + i16;
+    const int kh = same(p.h / (a.HV / a.H)), len = same(seq_len(a.q, p.l)), all = (len + C - 1) / C;
+    const int from = sg * seg.chunks, last = min(all, from + seg.chunks);
+    const int vb = same((int)(b - ls * per) * 64), v0 = vb + wave * 16, col = v0 + i16;
     const bool mine = col < a.dv;
+    const int left = LOCAL && vb >= tiles * 64 ? 0 : a.dv - vb;  // columns of v from vb on
     const int64_t state = (int64_t)lh * a.dk * a.dv;
     f4 st[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       st[m] = ZERO;
-      if (a.state_in && mine)
+      if constexpr (LOCAL) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (m * 16 + 4 * g + r == col - tiles * 64) st[m][r] = 1.0f;
+      } else if (seg.n > 1) {
+        st[m] = *at32<const f4>(seg.first + same((int64_t)ls * tiles * 64 * DK),
+                                col * (DK / 4) + m * 4 + g);
+      } else if (a.state_in && mine) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           if (m * 16 + 4 * g + r < a.dk)
             st[m][r] = a.state_in[state + (int64_t)(m * 16 + 4 * g + r) * a.dv + col];
+      }
     }
     ChainNext<T, DK> next;
     auto bring = [&](int c) {
@@ -808,16 +831,16 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
       p.n = within(len, c);
       next.template load<W>(a, prep + same(((int64_t)lh * chunks + c) * PREP_BYTES), p, kh, a.v, vb);
     };
-    if (last > 0) bring(0);
-    for (int c = 0; c < last; ++c) {
+    if (last > from) bring(from);
+    for (int c = from; c < last; ++c) {
       __syncthreads();
-      next.template store<W>(s, p.n, a.dk, a.dv - vb);
+      next.template store<W>(s, p.n, a.dk, left);
       const int n = p.n;
       __syncthreads();
       if (c + 1 < last) bring(c + 1);
-      if (v0 >= a.dv) continue;
+      if (!LOCAL && v0 >= a.dv) continue;
       float* at = rec + same(((int64_t)lh * chunks + c) * (a.dv * (DK + C)));
-      if (rec && mine) {
+      if (!LOCAL && rec && mine) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
           *at32<f4>(at, col * (DK / 4) + m * 4 + g) = st[m];
@@ -833,9 +856,11 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
         for (int u = 0; u < U; ++u) {
           Frag<P> k[4], q[4];
           get<P>(k, s.ka, u, U, sl);
-          get<P>(q, s.q, u, U, sl);
           mma<T>(x, k, sf[u]);
-          mma<T>(o, q, sf[u]);
+          if constexpr (!LOCAL) {
+            get<P>(q, s.q, u, U, sl);
+            mma<T>(o, q, sf[u]);
+          }
         }
       }
       f4 nn[4];
@@ -854,7 +879,7 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
         for (int t = 0; t < 4; ++t) nn[t] = ZERO;
         triangle<T, false>(nn, s.tri, rf, sl);
       }
-      {
+      if constexpr (!LOCAL) {
         Frag<FULL> nf[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) nf[u] = full<T>(nn[2 * u], nn[2 * u + 1]);
@@ -878,6 +903,7 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
           mma<T>(st, k, nf[u]);
         }
       }
+      if constexpr (LOCAL) continue;
       if (rec && mine) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) *at32<f4>(at + a.dv * DK, col * (C / 4) + t * 4 + g) = nn[t];
@@ -887,7 +913,11 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
       here.c = c;
       put_result<T, W>(s.v, o, wave, lane, sl, Chunk<T>(a.out, here, p.h, a.dv), n, v0, a.dv);
     }
-    if (a.state_out && mine) {
+    if constexpr (LOCAL) {
+      float* to = seg.local + same((int64_t)ls * (tiles * 64 + DK) * DK);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) *at32<f4>(to, col * (DK / 4) + m * 4 + g) = st[m];
+    } else if (a.state_out && mine && sg == max(0, (all - 1) / seg.chunks)) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -901,10 +931,10 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
 
 // The gradient's chain, from the last chunk to the first: dS and dR of every
 // chunk, both with a column of d_v after the other, as S and N are kept.
-template <typename T, int DK, bool W>
+template <typename T, int DK, bool W, bool LOCAL>
 __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
     const DeltaGradArgs ga, const unsigned char* prep, float* grec, int chunks, int tiles,
-    uint32_t blocks) {
+    const Segments seg, uint32_t blocks) {
   using M = Mode<T>;
   constexpr int U = DK / 32, MT = DK / 16, FULL = M::FULL, P = M::ROWS;
   extern __shared__ __align__(16) unsigned char lds[];
@@ -913,23 +943,30 @@ __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i16 = lane % 16, g = lane / 16, sl = slot_of(i16, g);
   for (uint32_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const uint32_t lh = same((int)(b / tiles));
+    const uint32_t ls = same((int)(b / tiles)), lh = same((int)(ls / seg.n));
+    const int sg = ls - lh * seg.n;
     Place p;
     p.l = same((int)(lh / a.HV));
     p.h = lh - p.l * a.HV;
-    const int kh = same(p.h / (a.HV / a.H)), len = same(seq_len(a.q, p.l)), last = (len + C - 1) / C;
-    const int vb = same((int)(b - lh * tiles) * 64), v0 = vb + wave * 16, col = v0 + i16;
+    const int kh = same(p.h / (a.HV / a.H)), len = same(seq_len(a.q, p.l)), all = (len + C - 1) / C;
+    const int from = sg * seg.chunks, last = min(all, from + seg.chunks);
+    const int vb = same((int)(b - ls * tiles) * 64), v0 = vb + wave * 16, col = v0 + i16;
     const bool mine = col < a.dv;
     const int64_t state = (int64_t)lh * a.dk * a.dv;
     f4 st[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       st[m] = ZERO;
-      if (ga.dstate_out && mine)
+      if constexpr (LOCAL) {
+      } else if (seg.n > 1) {
+        st[m] = *at32<const f4>(seg.first + same((int64_t)ls * tiles * 64 * DK),
+                                col * (DK / 4) + m * 4 + g);
+      } else if (ga.dstate_out && mine) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           if (m * 16 + 4 * g + r < a.dk)
             st[m][r] = ga.dstate_out[state + (int64_t)(m * 16 + 4 * g + r) * a.dv + col];
+      }
     }
     ChainNext<T, DK> next;
     auto bring = [&](int c) {
@@ -937,15 +974,15 @@ __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
       p.n = within(len, c);
       next.template load<W>(a, prep + same(((int64_t)lh * chunks + c) * PREP_BYTES), p, kh, ga.dout, vb);
     };
-    if (last > 0) bring(last - 1);
-    for (int c = last - 1; c >= 0; --c) {
+    if (last > from) bring(last - 1);
+    for (int c = last - 1; c >= from; --c) {
       __syncthreads();
       next.template store<W>(s, p.n, a.dk, a.dv - vb);
       __syncthreads();
-      if (c > 0) bring(c - 1);
+      if (c > from) bring(c - 1);
       if (v0 >= a.dv) continue;
       float* at = grec + same(((int64_t)lh * chunks + c) * (a.dv * (DK + C)));
-      if (mine) {
+      if (!LOCAL && mine) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
           *at32<f4>(at, col * (DK / 4) + m * 4 + g) = st[m];
@@ -980,7 +1017,7 @@ __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
         for (int t = 0; t < 4; ++t) dr[t] = ZERO;
         triangle<T, true>(dr, s.tri, nf, sl);
       }
-      if (mine) {
+      if (!LOCAL && mine) {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
           *at32<f4>(at + a.dv * DK, col * (C / 4) + t * 4 + g) = dr[t];
@@ -1007,7 +1044,11 @@ __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
         }
       }
     }
-    if (ga.dstate_in && mine) {
+    if constexpr (LOCAL) {
+      float* to = seg.local + same((int64_t)ls * tiles * 64 * DK);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) *at32<f4>(to, col * (DK / 4) + m * 4 + g) = st[m];
+    } else if (ga.dstate_in && mine && sg == 0) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -1016,6 +1057,64 @@ __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
             ga.dstate_in[state + (int64_t)(m * 16 + 4 * g + r) * a.dv + col] = st[m][r];
     }
     __syncthreads();
+  }
+}
+
+// The segments' first states, one from the other: S = M S + what the segment adds,
+// M its last states from the identity; or backwards, dS = M^T dS + what it adds.
+// A wave per 16 columns of a (lane, value head).
+template <int DK, bool BACK>
+__global__ __launch_bounds__(64) void delta_combine_kernel(const DeltaArgs a, const float* first,
+                                                           const float* moves, const float* adds,
+                                                           int adds_columns, float* states,
+                                                           int tiles, int segments, uint32_t blocks) {
+  constexpr int MT = DK / 16;
+  const int lane = threadIdx.x, i16 = lane % 16, g = lane / 16;
+  for (uint32_t b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const uint32_t lh = b / (4 * tiles);
+    const int col = (int)(b - lh * 4 * tiles) * 16 + i16;
+    f4 st[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      st[m] = ZERO;
+      if (first && col < a.dv)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (m * 16 + 4 * g + r < a.dk)
+            st[m][r] = first[((int64_t)lh * a.dk + m * 16 + 4 * g + r) * a.dv + col];
+    }
+    for (int i = 0; i < segments; ++i) {
+      const int64_t at = (int64_t)lh * segments + (BACK ? segments - 1 - i : i);
+      float* to = states + (at * tiles * 64 + col) * DK;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) *reinterpret_cast<f4*>(to + m * 16 + 4 * g) = st[m];
+      if (i + 1 == segments) break;
+      const float* move = moves + (at * (tiles * 64 + DK) + tiles * 64) * DK;
+      const float* add = adds + (at * adds_columns + col) * DK;
+      f4 x[MT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) x[m] = *reinterpret_cast<const f4*>(add + m * 16 + 4 * g);
+#pragma unroll
+      for (int n = 0; n < MT; ++n) {
+        f4 y[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          if constexpr (BACK) {
+            y[m] = *reinterpret_cast<const f4*>(move + (m * 16 + i16) * DK + n * 16 + 4 * g);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[m][j] = move[(n * 16 + 4 * g + j) * DK + m * 16 + i16];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+            x[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(y[m][j], st[n][j], x[m], 0, 0, 0);
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) st[m] = x[m];
+    }
   }
 }
 
@@ -1580,6 +1679,27 @@ int chunks_of(int T) { return (T + C - 1) / C; }
 // S and N of a chunk, dS and dR of it
 int64_t record_floats(int dk, int dv) { return (int64_t)dv * (built(dk) + C); }
 
+// Segments of a sequence: as many as keep the two passes (about 4 and 6.5 us a
+// chunk) and the chain of the segments (2 us each) together shortest, where there
+// are CUs for them and they come to three at least.
+struct Cut {
+  int n, chunks;
+};
+Cut segments_of(int64_t heads, int chunks, int dk, int dv) {
+  const int tiles = (dv + 63) / 64 + built(dk) / 64;
+  int64_t n = 1;
+  while ((n + 1) * (n + 1) <= 5 * (int64_t)chunks) ++n;
+  n = std::min<int64_t>(n, 256 / (heads * tiles));
+  if (chunks < 16 || n < 3) return {1, chunks};
+  const int each = (int)((chunks + n - 1) / n);
+  return {(chunks + each - 1) / each, each};
+}
+// floats of Segments::local (of the gradient: without the identity's columns) and first
+int64_t local_floats(int64_t heads, const Cut& c, int dk, int dv, bool moves) {
+  if (c.n == 1) return 0;
+  return heads * c.n * ((dv + 63) / 64 * 64 + (moves ? built(dk) : 0)) * built(dk);
+}
+
 // Positions taken one after the other rather than in chunks.
 bool by_steps(int T) { return T <= 4; }
 
@@ -1626,9 +1746,28 @@ hipError_t delta_of(const DeltaArgs& a, hipStream_t s) {
     hipError_t e = hipGetLastError();
     if (e) return e;
     const size_t lds = sizeof(ChainLds<T, DK, false>);
-    if ((e = room(delta_chain_kernel<T, DK, W>, lds))) return e;
-    BOA_LAUNCH((delta_chain_kernel<T, DK, W>), grid(heads * tiles), 256, lds, s, a,
-               (const unsigned char*)prep, a.saved, chunks, tiles, (uint32_t)(heads * tiles));
+    const Cut cut = segments_of(heads, chunks, a.dk, a.dv);
+    Segments seg{cut.n, cut.chunks, nullptr, nullptr};
+    if (cut.n > 1) {
+      seg.first = (float*)(prep + all * PREP_BYTES);
+      // where the gradient follows, it needs what the segments make of a state
+      seg.local = a.saved ? a.saved + all * record_floats(a.dk, a.dv)
+                          : seg.first + local_floats(heads, cut, a.dk, a.dv, false);
+      const uint32_t blocks = (uint32_t)(heads * cut.n * (tiles + DK / 64));
+      if ((e = room(delta_chain_kernel<T, DK, W, true>, lds))) return e;
+      BOA_LAUNCH((delta_chain_kernel<T, DK, W, true>), blocks, 256, lds, s, a,
+                 (const unsigned char*)prep, (float*)nullptr, chunks, tiles, seg, blocks);
+      if ((e = hipGetLastError())) return e;
+      const uint32_t waves = (uint32_t)(heads * tiles * 4);
+      BOA_LAUNCH((delta_combine_kernel<DK, false>), waves, 64, 0, s, a, a.state_in,
+                 (const float*)seg.local, (const float*)seg.local, tiles * 64 + DK, seg.first, tiles,
+                 cut.n, waves);
+      if ((e = hipGetLastError())) return e;
+    }
+    if ((e = room(delta_chain_kernel<T, DK, W, false>, lds))) return e;
+    const uint64_t blocks = heads * cut.n * tiles;
+    BOA_LAUNCH((delta_chain_kernel<T, DK, W, false>), grid(blocks), 256, lds, s, a,
+               (const unsigned char*)prep, a.saved, chunks, tiles, seg, (uint32_t)blocks);
     return hipGetLastError();
   });
 }
@@ -1647,9 +1786,26 @@ hipError_t delta_grad_of(const DeltaGradArgs& ga, hipStream_t s) {
     hipError_t e = hipGetLastError();
     if (e) return e;
     size_t lds = sizeof(ChainLds<T, DK, true>);
-    if ((e = room(delta_grad_chain_kernel<T, DK, W>, lds))) return e;
-    BOA_LAUNCH((delta_grad_chain_kernel<T, DK, W>), grid(heads * tiles), 256, lds, s, ga,
-               (const unsigned char*)prep, grec, chunks, tiles, (uint32_t)(heads * tiles));
+    const Cut cut = segments_of(heads, chunks, a.dk, a.dv);
+    Segments seg{cut.n, cut.chunks, nullptr, nullptr};
+    if (cut.n > 1) {
+      seg.first = grec + all * record_floats(a.dk, a.dv);
+      seg.local = seg.first + local_floats(heads, cut, a.dk, a.dv, false);
+      const uint32_t blocks = (uint32_t)(heads * cut.n * tiles);
+      if ((e = room(delta_grad_chain_kernel<T, DK, W, true>, lds))) return e;
+      BOA_LAUNCH((delta_grad_chain_kernel<T, DK, W, true>), blocks, 256, lds, s, ga,
+                 (const unsigned char*)prep, grec, chunks, tiles, seg, blocks);
+      if ((e = hipGetLastError())) return e;
+      const uint32_t waves = (uint32_t)(heads * tiles * 4);
+      BOA_LAUNCH((delta_combine_kernel<DK, true>), waves, 64, 0, s, a, ga.dstate_out,
+                 (const float*)(a.saved + all * record_floats(a.dk, a.dv)), (const float*)seg.local,
+                 tiles * 64, seg.first, tiles, cut.n, waves);
+      if ((e = hipGetLastError())) return e;
+    }
+    if ((e = room(delta_grad_chain_kernel<T, DK, W, false>, lds))) return e;
+    const uint64_t blocks = heads * cut.n * tiles;
+    BOA_LAUNCH((delta_grad_chain_kernel<T, DK, W, false>), grid(blocks), 256, lds, s, ga,
+               (const unsigned char*)prep, grec, chunks, tiles, seg, (uint32_t)blocks);
     if ((e = hipGetLastError())) return e;
     lds = sizeof(LastLds<T, DK>);
     if ((e = room(delta_grad_last_kernel<T, DK, W>, lds))) return e;
@@ -1671,12 +1827,21 @@ hipError_t for_rows(bool bf16, bool wide, F&& f) {
 }  // namespace
 
 int64_t delta_saved_floats(int lanes, int T, int, int HV, int dk, int dv) {
-  return (int64_t)lanes * HV * chunks_of(T) * record_floats(dk, dv);
+  const int64_t heads = (int64_t)lanes * HV;
+  const int chunks = chunks_of(T);
+  return heads * chunks * record_floats(dk, dv) +
+         local_floats(heads, segments_of(heads, chunks, dk, dv), dk, dv, true);
 }
 
 int64_t delta_work_bytes(int lanes, int T, int, int HV, int dk, int dv, bool grad) {
-  const int64_t n = (int64_t)lanes * HV * chunks_of(T);
-  return n * (PREP_BYTES + (grad ? 4 * record_floats(dk, dv) : 0));
+  const int64_t heads = (int64_t)lanes * HV;
+  const int chunks = chunks_of(T);
+  const Cut cut = segments_of(heads, chunks, dk, dv);
+  const int64_t first = local_floats(heads, cut, dk, dv, false);
+  // what a forward call needs, and a gradient's as well if it is to be one's
+  int64_t floats = first + local_floats(heads, cut, dk, dv, true);
+  if (grad) floats = std::max(floats, heads * chunks * record_floats(dk, dv) + 2 * first);
+  return heads * chunks * PREP_BYTES + 4 * floats;
 }
 
 hipError_t launch_delta(const DeltaArgs& a, hipStream_t s) {

@@ -97,6 +97,34 @@ def recurrence(s, heads, scale, unit, live, grad=False):
     return got, grads
 
 
+def _segment(lanes, hv, T, dk, dv):
+    """chunks of a segment: few long sequences are cut, each segment taken from a
+    zero state and from the identity first"""
+    chunks, wide = -(-T // C), 64 if dk <= 64 else 128
+    n = int((5 * chunks) ** 0.5)
+    n = min(n, 256 // (lanes * hv * (-(-dv // 64) + wide // 64)))
+    return chunks if chunks < 16 or n < 3 else -(-chunks // n)
+
+
+def _firsts(S, step, free, dk, chunks, each, back):
+    """The segments' first states from the first one's: step(c, S) is a chunk's,
+    free(c, S) without what it adds."""
+    order = range(0, chunks, each)
+    firsts = {}
+    for at in (reversed(order) if back else order):
+        firsts[at] = S
+        local = M(torch.zeros_like(S.val))
+        eye = torch.eye(dk, dtype=torch.float64).expand(*S.val.shape[:-2], dk, dk)
+        move = M(eye)
+        inside = range(at, min(at + each, chunks))
+        for c in inside:  # the moves are the forward pass's, whichever way they are used
+            move = free(c, move)
+        for c in (reversed(inside) if back else inside):
+            local = step(c, local)
+        S = (move.t if back else move) @ S + local
+    return firsts
+
+
 def _chunked(t, heads, live):
     lanes, T, width = t.shape
     n = -(-T // C)
@@ -143,8 +171,18 @@ def bounds(s, heads, scale, unit, live, grad=False):
           else torch.zeros((lanes, hv, dk, dv), dtype=torch.float64))
     kl, all_ = k * left, at(since, slice(None))
     all_ = M(since.val[:, :, :, -1:], since.err[:, :, :, -1:])
+    each = _segment(lanes, hv, T, dk, dv)
+    zero = M(torch.zeros((), dtype=torch.float64))
+
+    def step(c, S, add=True):
+        N = (at(Un, c) if add else zero) - at(W, c) @ S
+        return S * at(all_, c) + at(kl, c).t @ N
+
+    free = lambda c, S: step(c, S, False)  # noqa: E731
+    firsts = {} if each == n else _firsts(S, step, free, dk, n, each, False)
     Ss, Ns = [], []
     for c in range(n):
+        S = firsts.get(c, S)
         Ss.append(S)
         Ns.append(at(Un, c) - at(W, c) @ S)
         S = S * at(all_, c) + at(kl, c).t @ Ns[-1]
@@ -157,8 +195,15 @@ def bounds(s, heads, scale, unit, live, grad=False):
     dN = P.t @ dO
     dS = M(s["dstate_out"].double() if s.get("dstate_out") is not None
            else torch.zeros((lanes, hv, dk, dv), dtype=torch.float64))
+    def back(c, dS):
+        d = at(dN, c) + at(kl, c) @ dS
+        return dS * at(all_, c) + at(qs, c).t @ at(dO, c) - at(W, c).t @ d
+
+    lasts = {} if each == n else _firsts(dS, back, free, dk, n, each, True)
     dSs, dNs = [], []
     for c in reversed(range(n)):
+        if c == n - 1 or (c + 1) % each == 0:
+            dS = lasts.get(c // each * each, dS)
         dSs.append(dS)
         dNs.append(at(dN, c) + at(kl, c) @ dS)
         dS = dS * at(all_, c) + at(qs, c).t @ at(dO, c) - at(W, c).t @ dNs[-1]

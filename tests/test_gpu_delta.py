@@ -101,7 +101,10 @@ SHAPES = [  # lanes, T, heads, v heads, d_k, d_v, layout, lens, kind
     (1, 65, 2, 2, 128, 64, "time", "full", "plain"), (3, 130, 1, 2, 80, 80, "wide", "ragged", "plain"),
     (3, 129, 2, 4, 128, 128, "dense", "ragged", "same"), (2, 200, 1, 3, 33, 100, "odd", "ragged", "reset"),
     (5, 70, 2, 2, 64, 128, "dense", "ragged", "none"), (2, 300, 1, 1, 127, 7, "odd", "ragged", "plain"),
-    (1, 513, 1, 1, 64, 64, "dense", "full", "plain")]
+    (1, 513, 1, 1, 64, 64, "dense", "full", "plain"),
+    # cut into segments
+    (1, 1100, 1, 1, 64, 64, "dense", "full", "plain"), (2, 1029, 1, 2, 33, 80, "odd", "ragged", "reset"),
+    (3, 1500, 1, 2, 80, 70, "wide", "ragged", "same"), (1, 2000, 2, 2, 128, 128, "dense", "full", "none")]
 
 
 @pytest.mark.parametrize("train", [False, True])
@@ -125,7 +128,7 @@ def test_raw_rows_and_no_states(codec, dtype, T):  # noqa: F811
     compare(got, s, 1, live, scale=1.7, unit=False)
 
 
-@pytest.mark.parametrize("T", [1, 4, 150])
+@pytest.mark.parametrize("T", [1, 4, 150, 1200])
 def test_states_in_place(codec, T):  # noqa: F811
     s, g = inputs(3, T, 1, 2, 64, 128, F32)
     lens = lens_of("ragged", 3, T, g)
@@ -133,7 +136,7 @@ def test_states_in_place(codec, T):  # noqa: F811
     compare(got, s, 1, live)
 
 
-@pytest.mark.parametrize("T,at", [(200, 64), (200, 77), (130, 3)])
+@pytest.mark.parametrize("T,at", [(200, 64), (200, 77), (130, 3), (1200, 1100)])
 def test_pieces_make_the_whole(codec, T, at):  # noqa: F811
     """A sequence in two calls, the state handed on."""
     s, _ = inputs(2, T, 1, 2, 64, 64, F32)

@@ -780,7 +780,8 @@ __device__ __forceinline__ void put_result(u4* tile, const f4 (&o)[4], int wave,
 // the main pass takes every segment from its own first state.
 struct Segments {
   int n, chunks;  // segments of a sequence, chunks of a segment
-  float* local;   // [lane][v head][segment][64 tiles + d_k columns][d_k]
+  float* local;   // [lane][v head][segment][64 tiles + 2 d_k][d_k]: a row for each column;
+                  // the identity's as rows, too
   float* first;   // [lane][v head][segment][64 tiles columns][d_k]: the states it is taken from
 };
 
@@ -914,9 +915,15 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
       put_result<T, W>(s.v, o, wave, lane, sl, Chunk<T>(a.out, here, p.h, a.dv), n, v0, a.dv);
     }
     if constexpr (LOCAL) {
-      float* to = seg.local + same((int64_t)ls * (tiles * 64 + DK) * DK);
+      float* to = seg.local + same((int64_t)ls * (tiles * 64 + 2 * DK) * DK);
 #pragma unroll
       for (int m = 0; m < MT; ++m) *at32<f4>(to, col * (DK / 4) + m * 4 + g) = st[m];
+      if (vb >= tiles * 64)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            to[(tiles * 64 + DK + m * 16 + 4 * g + r) * DK + col - tiles * 64] = st[m][r];
     } else if (a.state_out && mine && sg == max(0, (all - 1) / seg.chunks)) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -1062,59 +1069,65 @@ __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
 
 // The segments' first states, one from the other: S = M S + what the segment adds,
 // M its last states from the identity; or backwards, dS = M^T dS + what it adds.
-// A wave per 16 columns of a (lane, value head).
+// A block per 16 columns of a (lane, value head), a quarter of the rows a wave; the
+// next segment's M is under way while the states pass through LDS.
 template <int DK, bool BACK>
-__global__ __launch_bounds__(64) void delta_combine_kernel(const DeltaArgs a, const float* first,
-                                                           const float* moves, const float* adds,
-                                                           int adds_columns, float* states,
-                                                           int tiles, int segments, uint32_t blocks) {
-  constexpr int MT = DK / 16;
-  const int lane = threadIdx.x, i16 = lane % 16, g = lane / 16;
+__global__ __launch_bounds__(256) void delta_combine_kernel(const DeltaArgs a, const float* first,
+                                                            const float* moves, const float* adds,
+                                                            int adds_columns, float* states,
+                                                            int tiles, int segments, uint32_t blocks) {
+  constexpr int MT = DK / 16, MW = MT / 4;
+  __shared__ f4 now[2][MT][64];
+  const int tid = threadIdx.x, lane = tid & 63, w = same(tid >> 6), i16 = lane % 16, g = lane / 16;
   for (uint32_t b = blockIdx.x; b < blocks; b += gridDim.x) {
     const uint32_t lh = b / (4 * tiles);
     const int col = (int)(b - lh * 4 * tiles) * 16 + i16;
-    f4 st[MT];
+    f4 st[MW], add[MW], move[MW][MT];
+    auto bring = [&](int i) {
+      const int64_t at = (int64_t)lh * segments + (BACK ? segments - 1 - i : i);
+      const float* m_ = moves + (at * (tiles * 64 + 2 * DK) + tiles * 64 + (BACK ? 0 : DK)) * DK;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
+      for (int m = 0; m < MW; ++m) {
+        const int row = (w * MW + m) * 16;
+        add[m] = *reinterpret_cast<const f4*>(adds + (at * adds_columns + col) * DK + row + 4 * g);
+#pragma unroll
+        for (int n = 0; n < MT; ++n)
+          move[m][n] = *reinterpret_cast<const f4*>(m_ + (row + i16) * DK + n * 16 + 4 * g);
+      }
+    };
+#pragma unroll
+    for (int m = 0; m < MW; ++m) {
       st[m] = ZERO;
+      const int row = (w * MW + m) * 16 + 4 * g;
       if (first && col < a.dv)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (m * 16 + 4 * g + r < a.dk)
-            st[m][r] = first[((int64_t)lh * a.dk + m * 16 + 4 * g + r) * a.dv + col];
+          if (row + r < a.dk) st[m][r] = first[((int64_t)lh * a.dk + row + r) * a.dv + col];
     }
+    bring(0);
     for (int i = 0; i < segments; ++i) {
       const int64_t at = (int64_t)lh * segments + (BACK ? segments - 1 - i : i);
-      float* to = states + (at * tiles * 64 + col) * DK;
 #pragma unroll
-      for (int m = 0; m < MT; ++m) *reinterpret_cast<f4*>(to + m * 16 + 4 * g) = st[m];
-      if (i + 1 == segments) break;
-      const float* move = moves + (at * (tiles * 64 + DK) + tiles * 64) * DK;
-      const float* add = adds + (at * adds_columns + col) * DK;
-      f4 x[MT];
-#pragma unroll
-      for (int m = 0; m < MT; ++m) x[m] = *reinterpret_cast<const f4*>(add + m * 16 + 4 * g);
+      for (int m = 0; m < MW; ++m) {
+        now[i % 2][w * MW + m][lane] = st[m];
+        *reinterpret_cast<f4*>(states + (at * tiles * 64 + col) * DK + (w * MW + m) * 16 + 4 * g) =
+            st[m];
+        st[m] = add[m];
+      }
+      __syncthreads();
 #pragma unroll
       for (int n = 0; n < MT; ++n) {
-        f4 y[MT];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          if constexpr (BACK) {
-            y[m] = *reinterpret_cast<const f4*>(move + (m * 16 + i16) * DK + n * 16 + 4 * g);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[m][j] = move[(n * 16 + 4 * g + j) * DK + m * 16 + i16];
-          }
-        }
+        const f4 y = now[i % 2][n][lane];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int m = 0; m < MT; ++m)
-            x[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(y[m][j], st[n][j], x[m], 0, 0, 0);
+          for (int m = 0; m < MW; ++m)
+            st[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(move[m][n][j], y[j], st[m], 0, 0, 0);
       }
-#pragma unroll
-      for (int m = 0; m < MT; ++m) st[m] = x[m];
+      // (of the last segment nothing is needed, nor is there one after it)
+      if (i + 2 < segments) bring(i + 1);
     }
+    __syncthreads();
   }
 }
 
@@ -1679,8 +1692,8 @@ int chunks_of(int T) { return (T + C - 1) / C; }
 // S and N of a chunk, dS and dR of it
 int64_t record_floats(int dk, int dv) { return (int64_t)dv * (built(dk) + C); }
 
-// Segments of a sequence: as many as keep the two passes (about 4 and 6.5 us a
-// chunk) and the chain of the segments (2 us each) together shortest, where there
+// Segments of a sequence: as many as keep the two passes (about 5 and 6.5 us a
+// chunk) and the chain of the segments (0.75 us each) together shortest, where there
 // are CUs for them and they come to three at least.
 struct Cut {
   int n, chunks;
@@ -1688,16 +1701,16 @@ struct Cut {
 Cut segments_of(int64_t heads, int chunks, int dk, int dv) {
   const int tiles = (dv + 63) / 64 + built(dk) / 64;
   int64_t n = 1;
-  while ((n + 1) * (n + 1) <= 5 * (int64_t)chunks) ++n;
+  while ((n + 1) * (n + 1) <= 16 * (int64_t)chunks) ++n;
   n = std::min<int64_t>(n, 256 / (heads * tiles));
-  if (chunks < 16 || n < 3) return {1, chunks};
+  if (chunks < 8 || n < 3) return {1, chunks};
   const int each = (int)((chunks + n - 1) / n);
   return {(chunks + each - 1) / each, each};
 }
 // floats of Segments::local (of the gradient: without the identity's columns) and first
 int64_t local_floats(int64_t heads, const Cut& c, int dk, int dv, bool moves) {
   if (c.n == 1) return 0;
-  return heads * c.n * ((dv + 63) / 64 * 64 + (moves ? built(dk) : 0)) * built(dk);
+  return heads * c.n * ((dv + 63) / 64 * 64 + (moves ? 2 * built(dk) : 0)) * built(dk);
 }
 
 // Positions taken one after the other rather than in chunks.
@@ -1758,10 +1771,10 @@ hipError_t delta_of(const DeltaArgs& a, hipStream_t s) {
       BOA_LAUNCH((delta_chain_kernel<T, DK, W, true>), blocks, 256, lds, s, a,
                  (const unsigned char*)prep, (float*)nullptr, chunks, tiles, seg, blocks);
       if ((e = hipGetLastError())) return e;
-      const uint32_t waves = (uint32_t)(heads * tiles * 4);
-      BOA_LAUNCH((delta_combine_kernel<DK, false>), waves, 64, 0, s, a, a.state_in,
-                 (const float*)seg.local, (const float*)seg.local, tiles * 64 + DK, seg.first, tiles,
-                 cut.n, waves);
+      const uint32_t columns = (uint32_t)(heads * tiles * 4);
+      BOA_LAUNCH((delta_combine_kernel<DK, false>), columns, 256, 0, s, a, a.state_in,
+                 (const float*)seg.local, (const float*)seg.local, tiles * 64 + 2 * DK, seg.first,
+                 tiles, cut.n, columns);
       if ((e = hipGetLastError())) return e;
     }
     if ((e = room(delta_chain_kernel<T, DK, W, false>, lds))) return e;
@@ -1796,10 +1809,10 @@ hipError_t delta_grad_of(const DeltaGradArgs& ga, hipStream_t s) {
       BOA_LAUNCH((delta_grad_chain_kernel<T, DK, W, true>), blocks, 256, lds, s, ga,
                  (const unsigned char*)prep, grec, chunks, tiles, seg, blocks);
       if ((e = hipGetLastError())) return e;
-      const uint32_t waves = (uint32_t)(heads * tiles * 4);
-      BOA_LAUNCH((delta_combine_kernel<DK, true>), waves, 64, 0, s, a, ga.dstate_out,
+      const uint32_t columns = (uint32_t)(heads * tiles * 4);
+      BOA_LAUNCH((delta_combine_kernel<DK, true>), columns, 256, 0, s, a, ga.dstate_out,
                  (const float*)(a.saved + all * record_floats(a.dk, a.dv)), (const float*)seg.local,
-                 tiles * 64, seg.first, tiles, cut.n, waves);
+                 tiles * 64, seg.first, tiles, cut.n, columns);
       if ((e = hipGetLastError())) return e;
     }
     if ((e = room(delta_grad_chain_kernel<T, DK, W, false>, lds))) return e;

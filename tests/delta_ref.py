@@ -101,9 +101,9 @@ def _segment(lanes, hv, T, dk, dv):
     """chunks of a segment: few long sequences are cut, each segment taken from a
     zero state and from the identity first"""
     chunks, wide = -(-T // C), 64 if dk <= 64 else 128
-    n = int((5 * chunks) ** 0.5)
+    n = int((16 * chunks) ** 0.5)
     n = min(n, 256 // (lanes * hv * (-(-dv // 64) + wide // 64)))
-    return chunks if chunks < 16 or n < 3 else -(-chunks // n)
+    return chunks if chunks < 8 or n < 3 else -(-chunks // n)
 
 
 def _firsts(S, step, free, dk, chunks, each, back):

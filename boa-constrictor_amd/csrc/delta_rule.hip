@@ -1114,6 +1114,7 @@ __global__ __launch_bounds__(256) void delta_combine_kernel(const DeltaArgs a, c
             st[m];
         st[m] = add[m];
       }
+      if (i + 1 == segments) break;
       __syncthreads();
 #pragma unroll
       for (int n = 0; n < MT; ++n) {
@@ -1124,8 +1125,7 @@ __global__ __launch_bounds__(256) void delta_combine_kernel(const DeltaArgs a, c
           for (int m = 0; m < MW; ++m)
             st[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(move[m][n][j], y[j], st[m], 0, 0, 0);
       }
-      // (of the last segment nothing is needed, nor is there one after it)
-      if (i + 2 < segments) bring(i + 1);
+      bring(min(i + 1, segments - 2));  // (none after the last)
     }
     __syncthreads();
   }
@@ -1203,6 +1203,7 @@ struct LastRows {
   }
 };
 typedef float f2 __attribute__((ext_vector_type(2)));
+typedef int i4 __attribute__((ext_vector_type(4)));
 template <int DK>
 struct LastStates {
   f2 s[DK / 64][4], d[DK / 64][4];
@@ -1379,35 +1380,38 @@ __global__ __launch_bounds__(512, 2) void delta_grad_last_kernel(
         const float part = s.coef.part[own], beta = s.coef.beta[own], rk = s.coef.rk[own];
         const float rq = s.coef.uq[own] * a.scale;
         float over = 0.0f, down = 0.0f, with_beta = 0.0f;
-        auto element = [&](int o, bool row, float p0, float a0, float q0, float k0, f4& eo, f4& fo,
-                           int r) {
-          // row: own is the row and o the column, else the other way
-          const int dw = s.coef.whole[o] - whole;
-          const float dp = s.coef.part[o] - part;
-          const float d = raised(row ? -dw : dw, row ? -dp : dp);
-          const float rko = s.coef.rk[o], rqo = s.coef.uq[o] * a.scale, bo = s.coef.beta[o];
-          const float ukk = k0 * rk * rko;
-          const float dP = (row ? o <= own : o >= own) ? p0 * d : 0.0f;
-          const float dA = (row ? o < own : o > own) ? -a0 * d : 0.0f;
-          const float br = row ? beta : bo;
-          const float both = dP * (q0 * (row ? rq * rko : rqo * rk)) + dA * (br * ukk);
-          over += row ? both : 0.0f;
-          down += row ? 0.0f : both;
-          with_beta += row ? dA * ukk : 0.0f;
-          eo[r] += dP * (row ? rko * a.scale : rqo);
-          fo[r] += dA * (br * rko);
+        // of the four o = at .. at + 3; row: own is the row and o the column, else the
+        // other way
+        auto elements = [&](int at, bool row, f4 p4, f4 a4, f4 q4, f4 k4, f4& eo, f4& fo) {
+          const i4 whole4 = *reinterpret_cast<const i4*>(s.coef.whole + at);
+          const f4 part4 = *reinterpret_cast<const f4*>(s.coef.part + at);
+          const f4 rk4 = *reinterpret_cast<const f4*>(s.coef.rk + at);
+          const f4 rq4 = *reinterpret_cast<const f4*>(s.coef.uq + at) * a.scale;
+          const f4 b4 = *reinterpret_cast<const f4*>(s.coef.beta + at);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int o = at + r, dw = whole4[r] - whole;
+            const float dp = part4[r] - part;
+            const float d = raised(row ? -dw : dw, row ? -dp : dp);
+            const float ukk = k4[r] * rk * rk4[r];
+            const float dP = (row ? o <= own : o >= own) ? p4[r] * d : 0.0f;
+            const float dA = (row ? o < own : o > own) ? -a4[r] * d : 0.0f;
+            const float br = row ? beta : b4[r];
+            const float both = dP * (q4[r] * (row ? rq * rk4[r] : rq4[r] * rk)) + dA * (br * ukk);
+            over += row ? both : 0.0f;
+            down += row ? 0.0f : both;
+            with_beta += row ? dA * ukk : 0.0f;
+            eo[r] += dP * (row ? rk4[r] * a.scale : rq4[r]);
+            fo[r] += dA * (br * rk4[r]);
+          }
         };
         const f4 mid_k = one_of(kk, wv);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            element(m * 16 + g4 + r, m <= wv, pp[m][r], aa[m][r], qk[m][r], kk[m][r], e[m], f[m], r);
+          elements(m * 16 + g4, m <= wv, pp[m], aa[m], qk[m], kk[m], e[m], f[m]);
           apart();
         }
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          element(w * 16 + g4 + r, false, mid_p[r], mid_a[r], mid_qk[r], mid_k[r], mid_e, mid_f, r);
+        elements(w * 16 + g4, false, mid_p, mid_a, mid_qk, mid_k, mid_e, mid_f);
         over = across_g(over);
         down = across_g(down);
         with_beta = across_g(with_beta);

@@ -199,11 +199,11 @@ __global__ __launch_bounds__(256) void sample_kernel(const SampleArgs a, uint32_
         if (x[j] == top) byte = 4 * lane + j;
       byte = wave_all(byte, lane, Min32());
     } else {
-      const double temperature = (double)h.temperature;
+      const double sharp = 1.0 / (double)h.temperature;
       double w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        w[j] = ::exp((x[j] - top) / temperature);
+        w[j] = ::exp((x[j] - top) * sharp);
         if (w[j] < (double)h.min_p) w[j] = 0.0;
       }
       const bool by_k = h.top_k >= 1.0f && h.top_k < 256.0f, by_p = h.top_p < 1.0f;
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256) void sample_kernel(const SampleArgs a, uint32_
           double v[4], total;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            v[j] = by_k && !((float)(4 * lane + j) < h.top_k) ? 0.0 : ::exp((s[j] - top) / temperature);
+            v[j] = by_k && !((float)(4 * lane + j) < h.top_k) ? 0.0 : ::exp((s[j] - top) * sharp);
           double at = wave_before(v[0] + v[1] + v[2] + v[3], lane, total);
           const double enough = (double)h.top_p * total;
           bool out[4];

@@ -2082,7 +2082,7 @@ int boa_delta_rule(boa_ctx* c, const boa_delta* d, const boa_rows* out, float* d
     k.floats(d_saved, 16, true, "saved");
     k.that(k.bad || !k.delta_input(*d, out->d), "out is an input");
     k.work(d_work, work_bytes, boa_delta_rule_work_bytes(d->lanes, d->T, d->heads, d->v_heads,
-                                                         d->d_k, d->d_v, 0));
+                                                         d->d_k, d->d_v, d_saved != nullptr));
     if (k.bad) return hipSuccess;
     a.out = k.to(*out);
     a.state_out = d_state_out;

@@ -1698,7 +1698,12 @@ int64_t record_floats(int dk, int dv) { return (int64_t)dv * (built(dk) + C); }
 
 // Segments of a sequence: as many as keep the two passes (about 5 and 6.5 us a
 // chunk) and the chain of the segments (0.75 us each) together shortest, where there
-// are CUs for them and they come to three at least.
+// are CUs for them and they come to three at least.  With and without, us:
+//   positions:                      384           512          1024          4096
+//   2 of 64 x 64, fp32           37 and 54     38 and 66    44 and 115    69 and 411
+//   8 of 128 x 128, bf16         53 and 49     59 and 59    69 and 99    127 and 336
+//   32 of 64 x 64, bf16          45 and 42     48 and 51    65 and 86    160 and 280
+// so from 8 chunks on, where none is slower.
 struct Cut {
   int n, chunks;
 };
@@ -1717,8 +1722,15 @@ int64_t local_floats(int64_t heads, const Cut& c, int dk, int dv, bool moves) {
   return heads * c.n * ((dv + 63) / 64 * 64 + (moves ? 2 * built(dk) : 0)) * built(dk);
 }
 
-// Positions taken one after the other rather than in chunks.
-bool by_steps(int T) { return T <= 4; }
+// Positions taken one after the other rather than in chunks: what a position takes
+// (1.4 us where few states wait for their rows, 2.5 at 64 lanes of 8 states of 128 x
+// 128) against a chunk's three kernels.  Measured, us:
+//   positions:                           4             8            16
+//   1 lane, 2 of 64 x 64, fp32      10 and 22     14 and 22     25 and 22
+//   the same, bf16                  10 and 19     15 and 19     27 and 20
+//   64 lanes, 8 of 128 x 128, bf16  22 and 72     32 and 72     52 and 72
+//   1000 lanes, 4 of 64 x 128       78 and 455   115 and 457   191 and 459
+bool by_steps(int T) { return T <= 12; }
 
 template <typename F>
 hipError_t for_width(int dk, F&& f) {
@@ -1851,6 +1863,7 @@ int64_t delta_saved_floats(int lanes, int T, int, int HV, int dk, int dv) {
 }
 
 int64_t delta_work_bytes(int lanes, int T, int, int HV, int dk, int dv, bool grad) {
+  if (!grad && by_steps(T)) return 0;
   const int64_t heads = (int64_t)lanes * HV;
   const int chunks = chunks_of(T);
   const Cut cut = segments_of(heads, chunks, dk, dv);

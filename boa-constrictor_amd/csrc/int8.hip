@@ -296,7 +296,11 @@ hipError_t int8_of(const Int8Args& a, hipStream_t s) {
   const int ksteps = steps_of(a.K);
   const uint32_t rt = (rows + 127) / 128, ct = (a.N + 127) / 128;
   const bool wide_out = rows_by_16(a.out.d, a.out.lane, a.out.row, a.N, sizeof(T));
-  if ((uint64_t)rt * ct < 256) {
+  // Tiles of 32 x 32 while those of 128 x 128 leave most CUs without work.  Small
+  // and large, us: 1024 rows, N 1032, K 256 (72 large tiles) 5.3 and 6.0; 512 rows,
+  // 2064, 512 (68) 6.4 and 7.6; 6000, 256, 256 (94) 6.8 and 6.1; 768, 2064, 512
+  // (102) 9.0 and 7.6; 64, 2064, 512 (17) 3.9 and 7.2.
+  if ((uint64_t)rt * ct < 80) {
     const uint32_t frt = (rows + 31) / 32, fct = (a.N + 31) / 32;
     const uint32_t blocks = (uint32_t)std::min<uint64_t>((uint64_t)frt * fct, MAX_BLOCKS);
     BOA_LAUNCH((int8_few_kernel<T, WIDE>), blocks, 256, 0, s, a, rows, ksteps, frt, fct);

@@ -381,8 +381,9 @@ hipError_t norm_of(const NormArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-// Blocks of the gradient: as many as the CUs hold at eight waves a SIMD, each
-// with its own partial sums
+// Blocks of the gradient, each with its own partial sums: with 512, 1024, 2048 of
+// them 79, 61, 57 us (130,250 x 256, fp32), 13, 15, 22 (8103 x 512, bf16) and 40,
+// 39, 44 (32,768 x 1024, bf16)
 constexpr uint32_t GRAD_BLOCKS = 1024;
 uint32_t grad_blocks(int64_t rows, int G) {
   return (uint32_t)std::min<int64_t>((rows * G + 255) / 256, GRAD_BLOCKS);

@@ -306,8 +306,11 @@ int boa_int8_matmul(boa_ctx* ctx, const boa_rows* x8, const float* d_scale8, con
  * divided by their lengths sqrt(sum of squares + 1e-6) first.  Row strides are
  * at most 2^23.  A log decay
  * below -1e4 (-inf too) forgets the state.  States [lanes][v_heads][d_k][d_v]
- * fp32; d_state_in NULL is zero.  With T = 1 this is a decode step.  Positions
- * are taken 64 at a time: a value that is not finite spoils the results of its
+ * fp32; d_state_in NULL is zero.  With T = 1 this is a decode step.  The order of
+ * sums follows from the sizes (T, and for few long sequences lanes and v_heads
+ * too), so the same sequence in another batch may differ in its last bits; the
+ * same call gives the same bits.  Positions
+ * are taken up to 64 at a time: a value that is not finite spoils the results of its
  * lane and head from the first of its 64 on, and none of other lanes. */
 typedef struct {
     int32_t lanes, T, heads, v_heads, d_k, d_v, precision, unit_qk;
@@ -335,6 +338,8 @@ int boa_delta_rule_grad(boa_ctx* ctx, const boa_delta* d, const float* d_saved,
                         const boa_delta_grads* grads, void* d_work, int64_t work_bytes);
 int64_t boa_delta_rule_saved_floats(int32_t lanes, int32_t T, int32_t heads, int32_t v_heads,
                                     int32_t d_k, int32_t d_v);
+/* Of both calls: grad 0 for the rule without d_saved (0 bytes where T is small),
+ * 1 for it with d_saved and for its gradient. */
 int64_t boa_delta_rule_work_bytes(int32_t lanes, int32_t T, int32_t heads, int32_t v_heads,
                                   int32_t d_k, int32_t d_v, int32_t grad);
 

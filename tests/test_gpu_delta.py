@@ -101,7 +101,8 @@ SHAPES = [  # lanes, T, heads, v heads, d_k, d_v, layout, lens, kind
     (1, 65, 2, 2, 128, 64, "time", "full", "plain"), (3, 130, 1, 2, 80, 80, "wide", "ragged", "plain"),
     (3, 129, 2, 4, 128, 128, "dense", "ragged", "same"), (2, 200, 1, 3, 33, 100, "odd", "ragged", "reset"),
     (5, 70, 2, 2, 64, 128, "dense", "ragged", "none"), (2, 300, 1, 1, 127, 7, "odd", "ragged", "plain"),
-    (1, 513, 1, 1, 64, 64, "dense", "full", "plain"),
+    (1, 513, 1, 1, 64, 64, "dense", "full", "plain"), (3, 12, 1, 2, 100, 36, "dense", "ragged", "same"),
+    (2, 9, 2, 2, 64, 64, "odd", "ragged", "reset"), (4, 13, 1, 1, 128, 128, "time", "ragged", "tiny"),
     # cut into segments
     (1, 1100, 1, 1, 64, 64, "dense", "full", "plain"), (2, 1029, 1, 2, 33, 80, "odd", "ragged", "reset"),
     (3, 1500, 1, 2, 80, 70, "wide", "ragged", "same"), (1, 2000, 2, 2, 128, 128, "dense", "full", "none")]
@@ -237,24 +238,30 @@ def test_capture(codec):  # noqa: F811
 
 def test_refusals(codec):  # noqa: F811
     z = lambda *n, dt=F32: torch.zeros(n, dtype=dt, device="cuda")  # noqa: E731
-    ok = dict(q=z(2, 8, 64), k=z(2, 8, 64), v=z(2, 8, 128), g=z(2, 8, 2), beta=z(2, 8, 2),
-              out=z(2, 8, 128), w=work(boa_hip.delta_rule_work_bytes(2, 8, 1, 2, 64, 64)), heads=1)
+    ok = dict(q=z(2, 20, 64), k=z(2, 20, 64), v=z(2, 20, 128), g=z(2, 20, 2), beta=z(2, 20, 2),
+              out=z(2, 20, 128), w=work(boa_hip.delta_rule_work_bytes(2, 20, 1, 2, 64, 64)), heads=1)
 
     def call(**new):
         a = dict(ok, **new)
         codec.delta_rule(a["q"], a["k"], a["v"], a["g"], a["beta"], a["out"], a["w"],
                          heads=a["heads"], d_state_in=a.get("state_in"),
-                         d_state_out=a.get("state_out"))
+                         d_state_out=a.get("state_out"), d_saved=a.get("saved"))
 
     call()
+    # few positions need no workspace, unless what the gradient needs is to be kept
+    few = dict(ok, **{n: ok[n][:, :12] for n in ("q", "k", "v", "g", "beta", "out")})
+    assert boa_hip.delta_rule_work_bytes(2, 12, 1, 2, 64, 64) == 0
+    call(**dict(few, w=None))
+    with pytest.raises(boa_hip.BoaError, match="workspace"):
+        call(**dict(few, w=None, saved=z(boa_hip.delta_rule_saved_floats(2, 12, 1, 2, 64, 64))))
     for bad, why in [(dict(w=None), "workspace"), (dict(w=ok["w"][:-16]), "workspace"),
-                     (dict(out=ok["v"]), "input"), (dict(out=z(2, 8, 64).repeat(1, 1, 1)), "out"),
-                     (dict(q=z(2, 8, 64, dt=BF16)), "k"), (dict(g=z(2, 8, 2, dt=BF16)), "g"),
-                     (dict(q=z(2, 8, 192), k=z(2, 8, 192)), "128"),
-                     (dict(q=z(2, 8, 192), k=z(2, 8, 192), heads=3), "multiple"),
+                     (dict(out=ok["v"]), "input"), (dict(out=z(2, 20, 64).repeat(1, 1, 1)), "out"),
+                     (dict(q=z(2, 20, 64, dt=BF16)), "k"), (dict(g=z(2, 20, 2, dt=BF16)), "g"),
+                     (dict(q=z(2, 20, 192), k=z(2, 20, 192)), "128"),
+                     (dict(q=z(2, 20, 192), k=z(2, 20, 192), heads=3), "multiple"),
                      (dict(heads=0), "heads"), (dict(heads=5), "heads"),
                      (dict(state_in=z(2, 2, 64, 32)), "state_in"),
-                     (dict(q=z(2, 8, 64).cpu()), "cpu"),
-                     (dict(out=z(1, 8, 128).expand(2, 8, 128)), "overlap")]:
+                     (dict(q=z(2, 20, 64).cpu()), "cpu"),
+                     (dict(out=z(1, 20, 128).expand(2, 20, 128)), "overlap")]:
         with pytest.raises((boa_hip.BoaError, ValueError), match=why):
             call(**bad)

@@ -1378,40 +1378,48 @@ __global__ __launch_bounds__(512, 2) void delta_grad_last_kernel(
         f4 e[4] = {}, mid_e = ZERO, f[4] = {}, mid_f = ZERO;
         const int whole = s.coef.whole[own];
         const float part = s.coef.part[own], beta = s.coef.beta[own], rk = s.coef.rk[own];
-        const float rq = s.coef.uq[own] * a.scale;
+        const float uq = s.coef.uq[own];
         float over = 0.0f, down = 0.0f, with_beta = 0.0f;
         // of the four o = at .. at + 3; row: own is the row and o the column, else the
-        // other way
-        auto elements = [&](int at, bool row, f4 p4, f4 a4, f4 q4, f4 k4, f4& eo, f4& fo) {
+        // other way.  Of a tile that is not the wave's own all elements count.
+        auto elements = [&](int at, bool row, bool whole_tile, f4 p4, f4 a4, f4 q4, f4 k4, f4& eo,
+                            f4& fo) {
           const i4 whole4 = *reinterpret_cast<const i4*>(s.coef.whole + at);
           const f4 part4 = *reinterpret_cast<const f4*>(s.coef.part + at);
           const f4 rk4 = *reinterpret_cast<const f4*>(s.coef.rk + at);
-          const f4 rq4 = *reinterpret_cast<const f4*>(s.coef.uq + at) * a.scale;
+          const f4 rq4 = *reinterpret_cast<const f4*>(s.coef.uq + at);
           const f4 b4 = *reinterpret_cast<const f4*>(s.coef.beta + at);
+          const f4 of_k = either(row, rk4, rq4) * a.scale, of_b = either(row, f4{beta, beta, beta, beta}, b4);
+          // what lies below the diagonal by how much
+          const int flip = row ? -1 : 0;
+          const float signf = row ? -1.0f : 1.0f;
+          const int by = whole_tile ? C : ((at - own) ^ flip) - flip;
+          float with_q = 0.0f, with_k = 0.0f, kb = 0.0f;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int o = at + r, dw = whole4[r] - whole;
-            const float dp = part4[r] - part;
-            const float d = raised(row ? -dw : dw, row ? -dp : dp);
-            const float ukk = k4[r] * rk * rk4[r];
-            const float dP = (row ? o <= own : o >= own) ? p4[r] * d : 0.0f;
-            const float dA = (row ? o < own : o > own) ? -a4[r] * d : 0.0f;
-            const float br = row ? beta : b4[r];
-            const float both = dP * (q4[r] * (row ? rq * rk4[r] : rq4[r] * rk)) + dA * (br * ukk);
-            over += row ? both : 0.0f;
-            down += row ? 0.0f : both;
-            with_beta += row ? dA * ukk : 0.0f;
-            eo[r] += dP * (row ? rk4[r] * a.scale : rq4[r]);
-            fo[r] += dA * (br * rk4[r]);
+            const float d = raised(((whole4[r] - whole) ^ flip) - flip, (part4[r] - part) * signf);
+            const int below = by + (r ^ flip) - flip;
+            const float dP = below >= 0 ? p4[r] * d : 0.0f;
+            const float dA = below > 0 ? -a4[r] * d : 0.0f;
+            const float e = dP * of_k[r], f = dA * rk4[r], fk = f * k4[r];
+            eo[r] += e;
+            fo[r] += f * of_b[r];
+            with_q += e * q4[r];
+            with_k += fk;
+            kb += fk * of_b[r];
           }
+          const float both = with_q * (row ? uq : rk) + kb * rk;
+          over += row ? both : 0.0f;
+          down += row ? 0.0f : both;
+          with_beta += row ? with_k * rk : 0.0f;
         };
         const f4 mid_k = one_of(kk, wv);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          elements(m * 16 + g4, m <= wv, pp[m], aa[m], qk[m], kk[m], e[m], f[m]);
+          elements(m * 16 + g4, m <= wv, m != wv, pp[m], aa[m], qk[m], kk[m], e[m], f[m]);
           apart();
         }
-        elements(w * 16 + g4, false, mid_p, mid_a, mid_qk, mid_k, mid_e, mid_f);
+        elements(w * 16 + g4, false, false, mid_p, mid_a, mid_qk, mid_k, mid_e, mid_f);
         over = across_g(over);
         down = across_g(down);
         with_beta = across_g(with_beta);
@@ -1496,12 +1504,17 @@ __global__ __launch_bounds__(512, 2) void delta_grad_last_kernel(
           if (v0 + 32 < a.dv) next.load(S, dS, a.dv, v4 + 32, d2);
           const Frag<FULL> no = get<FULL>(s.v.n, w, sl), ro = get<FULL>(s.v.r, w, sl);
           const Frag<P> oo = get<P>(s.v.o, w, sl);
+          Frag<FULL> sm = get<FULL>(s.v.s, 0, sl), dm = get<FULL>(s.v.d, 0, sl);
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
-            const Frag<FULL> sm = get<FULL>(s.v.s, m, sl);
+            // the next ones are under way
+            Frag<FULL> s1, d1;
+            if (m + 1 < MT) s1 = get<FULL>(s.v.s, m + 1, sl), d1 = get<FULL>(s.v.d, m + 1, sl);
             mma<T>(os[m], sm, oo);
             mma<T>(rs[m], sm, ro);
-            mma<T>(ns[m], get<FULL>(s.v.d, m, sl), no);
+            mma<T>(ns[m], dm, no);
+            sm = s1;
+            dm = d1;
             apart();
           }
         }

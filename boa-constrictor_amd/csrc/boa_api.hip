@@ -2117,6 +2117,7 @@ int boa_delta_rule_grad(boa_ctx* c, const boa_delta* d, const float* d_saved, co
                           (const void*)g->dg.d, (const void*)g->dbeta.d})
       k.that(k.bad || (!k.delta_input(*d, p) && p != dout->d && p != d_saved),
              "a gradient is an input");
+    k.that(k.bad || !g->d_dstate_in || g->d_dstate_in != d_saved, "dstate_in is saved");
     k.work(d_work, work_bytes, boa_delta_rule_work_bytes(d->lanes, d->T, d->heads, d->v_heads,
                                                          d->d_k, d->d_v, 1));
     if (k.bad) return hipSuccess;

@@ -1611,8 +1611,9 @@ __global__ __launch_bounds__(512, 2) void delta_grad_last_kernel(
 // ---- few positions, one after the other ------------------------------------
 // A block per (lane, value head): 256 threads hold the state, thread (x, y)
 // columns 4 x .. 4 x + 3 of rows y + RG i.  With S^T k and S^T q of the state
-// before, o = scale (e^g S^T q + beta (k . q) e): one sum over the rows, and
-// one barrier, a position.
+// before, o = scale (e^g S^T q + beta (k . q) e): one sum over the rows and
+// two barriers a position.  Bound by the states, read and written once: 1000 lanes
+// of 4 of 64 x 128, one position, 50 us, 5.2 TB/s, as fast as a copy.
 template <typename T, int DK, int CX, bool W>
 __global__ __launch_bounds__(256) void delta_step_kernel(const DeltaArgs a, uint64_t blocks) {
   constexpr int RG = 256 / CX, RPT = DK / RG;

@@ -202,6 +202,51 @@ def test_the_batch_does_not_matter(codec):  # noqa: F811
         assert torch.equal(one[0], many[lane])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_capture(codec, dtype):  # noqa: F811
+    """Norm in both forms, its gradient in place and the product, replayed on new
+    values between eager calls."""
+    lanes, T, width, n = 5, 37, 256, 130
+    new = lambda *s, dt=dtype: torch.zeros(s, dtype=dt, device="cuda")  # noqa: E731
+    x, res, dy = new(lanes, T, width), new(lanes, T, width), new(lanes, T, width)
+    total, out, dx, y = new(lanes, T, width), new(lanes, T, width), new(lanes, T, width), new(lanes, T, n)
+    x8, s8 = new(lanes, T, width, dt=torch.int8), new(lanes, T, dt=F32)
+    w, dw, ws = torch.ones((width,), device="cuda"), new(width, dt=F32), torch.ones((n,), device="cuda")
+    packed = work(boa_hip.int8_pack_bytes(n, width))
+    codec.int8_pack(torch.randint(-127, 128, (n, width), dtype=torch.int8, device="cuda"), packed)
+    wk = work(boa_hip.rms_norm_grad_work_bytes(lanes, T, width))
+
+    def step():
+        codec.rms_norm(x, out, d_weight=w, d_residual=res, d_sum=total, d_out8=x8, d_scale8=s8)
+        codec.int8_matmul(x8, s8, packed, ws, y)
+        dx.copy_(dy)
+        codec.rms_norm_grad(total, dx, dx, wk, d_weight=w, d_dweight=dw)
+
+    results = [total, out, x8, s8, y, dx, dw]
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        codec.set_stream(torch.cuda.current_stream().cuda_stream)
+        step()
+    codec.set_stream(torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        for t in (x, res, dy, w):
+            t.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [t.clone() for t in results]
+        for t in results:
+            t.zero_()
+        step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(replayed, results))
+        apart = torch.zeros_like(dx)  # not into dout itself
+        dw.zero_()
+        codec.rms_norm_grad(total, dy, apart, wk, d_weight=w, d_dweight=dw)
+        torch.cuda.synchronize()
+        assert torch.equal(apart, dx) and torch.equal(dw, replayed[-1])
+
+
 def test_refusals(codec):  # noqa: F811
     z = lambda *n, dt=F32: torch.zeros(n, dtype=dt, device="cuda")  # noqa: E731
     x, i8 = z(2, 4, 64), z(2, 4, 64, dt=torch.int8)

@@ -122,6 +122,28 @@ def test_a_share_of_each(codec):  # noqa: F811
     assert (share - torch.softmax(x[0, 0].double(), -1) * n).abs().max() <= 1.01
 
 
+@pytest.mark.parametrize("how", [dict(), dict(top_k=30), dict(top_p=0.5), dict(top_k=30, top_p=0.5)])
+def test_an_infinite_temperature(codec, how):  # noqa: F811
+    """Every byte that is not ruled out is as likely as the others."""
+    n = 600
+    x = torch.full((1, n, 256), -math.inf)
+    x[..., 100:200] = torch.randn((100,), generator=torch.Generator().manual_seed(4))
+    u = (torch.arange(n, dtype=torch.float64) / n).float().view(1, n)
+    for settings in (dict(temperature=math.inf, **how),
+                     dict(d_params=torch.tensor([[math.inf, how.get("top_k", 0), how.get("top_p", 1.0),
+                                                  0.0]], device="cuda"))):
+        out = torch.full((1, n), 7, dtype=torch.uint8, device="cuda")
+        logp = torch.full((1, n), 7.5, device="cuda")
+        codec.sample_bytes(dev(x), dev(u), out, d_logp=logp, **settings)
+        kept = (30 if "top_k" in how else 100) * (0.5 if "top_p" in how else 1)
+        ranked = torch.sort(x[0, 0], descending=True)[1][:int(kept)].sort()[0]
+        share = torch.arange(1, len(ranked) + 1, dtype=torch.float64)
+        want = ranked[(share <= u[0].double()[:, None] * kept).sum(1)]
+        assert torch.equal(out[0].cpu().long(), want)
+        # a logarithm's value, rounded once
+        assert (logp.cpu().double() + math.log(kept)).abs().max() <= 2.0 ** -24 * math.log(kept)
+
+
 def test_capture(codec):  # noqa: F811
     x, u = torch.randn((9, 1, 256), device="cuda"), torch.rand((9, 1), device="cuda")
     out, logp = torch.zeros((9, 1), dtype=torch.uint8, device="cuda"), torch.zeros((9, 1), device="cuda")

@@ -502,7 +502,10 @@ __device__ __forceinline__ void mma16(f4& acc, f4 x, f4 y) {
 }
 
 // A block per (lane, value head, chunk): T and P as the chain reads them, and
-// the coefficients.
+// the coefficients.  Bound by a block's chain of steps (the substitution of 16
+// columns, then the products between blocks) and by the 39 KB that it writes: 2048
+// chunks of 64 columns of k 46 us, 1.8 TB/s.  All chunks are at hand at once, so as
+// many blocks as the registers allow share a CU: four (bf16, d_k up to 64) or two.
 template <typename T, int DK, bool TRANS, bool W>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 ? 4 : 2) void delta_prep_kernel(const DeltaArgs a, unsigned char* prep,
                                                          int chunks, uint64_t blocks) {
@@ -785,6 +788,14 @@ struct Segments {
   float* first;   // [lane][v head][segment][64 tiles columns][d_k]: the states it is taken from
 };
 
+// The states from chunk to chunk and O.  A block's four waves, 16 columns of S, N
+// and O each, share K, Q, T, P and v in LDS (69 KB for bf16 rows and d_k up to 64,
+// 117 KB at 128); S stays in registers as the next product's right operand, so a
+// wave has no exchange with others but the barriers around a chunk's loads, which
+// are a chunk ahead.  Bound by the latency of a chunk's chain of dependent products
+// (S -> R -> N -> S), with one wave a SIMD: 6.2 us a chunk of bf16 rows (98 us for
+// 32 x 1024, 4 heads of 64 and 128 columns, of which the matrix instructions take a
+// fifth), 6.5 of fp32 ones.
 template <typename T, int DK, bool W, bool LOCAL>
 __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
     const DeltaArgs a, const unsigned char* prep, float* rec, int chunks, int tiles,
@@ -937,7 +948,8 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
 }
 
 // The gradient's chain, from the last chunk to the first: dS and dR of every
-// chunk, both with a column of d_v after the other, as S and N are kept.
+// chunk, both with a column of d_v after the other, as S and N are kept.  Bound as
+// the forward chain: 90 us for 32 x 1024, 4 heads of 64 and 128 columns.
 template <typename T, int DK, bool W, bool LOCAL>
 __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
     const DeltaGradArgs ga, const unsigned char* prep, float* grec, int chunks, int tiles,
@@ -1070,7 +1082,9 @@ __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
 // The segments' first states, one from the other: S = M S + what the segment adds,
 // M its last states from the identity; or backwards, dS = M^T dS + what it adds.
 // A block per 16 columns of a (lane, value head), a quarter of the rows a wave; the
-// next segment's M is under way while the states pass through LDS.
+// next segment's M is under way while the states pass through LDS.  Bound by the
+// latency of one step: 63 segments of 64 columns 48 us (with one wave a block, which
+// reads M's columns as they lie, 245).
 template <int DK, bool BACK>
 __global__ __launch_bounds__(256) void delta_combine_kernel(const DeltaArgs a, const float* first,
                                                             const float* moves, const float* adds,
@@ -1143,7 +1157,11 @@ __global__ __launch_bounds__(256) void delta_combine_kernel(const DeltaArgs a, c
 // right operand; then those products.  The other four take what comes from the
 // states, dO S^T, dR S^T and N dS^T.  (By the same wave the two do not fit its
 // registers: forward and gradient of 4 x 777 rows, 4 heads of 128 and 8 of 128
-// columns, 341 us and not 319.)
+// columns, 341 us and not 319.)  Bound by the two roles' waits for each other and by
+// the LDS between products: 194 us for 32 x 1024 rows, 4 heads of 64 and 128 columns,
+// 2.7 TB/s; the matrix instructions take a tenth.  K and Q kept in LDS rather than
+// in registers: 234; the products' operands brought one tile ahead in the first four
+// waves: 218.
 // dQ^T and dK^T [d_k][own] leave as four neighbouring columns a lane.
 template <typename T, int DK>
 struct LastLds {

@@ -790,7 +790,7 @@ struct Segments {
 
 // The states from chunk to chunk and O.  A block's four waves, 16 columns of S, N
 // and O each, share K, Q, T, P and v in LDS (69 KB for bf16 rows and d_k up to 64,
-// 117 KB at 128); S stays in registers as the next product's right operand, so a
+// 93 KB at 128); S stays in registers as the next product's right operand, so a
 // wave has no exchange with others but the barriers around a chunk's loads, which
 // are a chunk ahead.  Bound by the latency of a chunk's chain of dependent products
 // (S -> R -> N -> S), with one wave a SIMD: 6.2 us a chunk of bf16 rows (98 us for

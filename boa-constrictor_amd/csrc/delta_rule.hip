@@ -792,10 +792,12 @@ struct Segments {
 // and O each, share K, Q, T, P and v in LDS (69 KB for bf16 rows and d_k up to 64,
 // 93 KB at 128); S stays in registers as the next product's right operand, so a
 // wave has no exchange with others but the barriers around a chunk's loads, which
-// are a chunk ahead.  Bound by the latency of a chunk's chain of dependent products
-// (S -> R -> N -> S), with one wave a SIMD: 6.2 us a chunk of bf16 rows (98 us for
-// 32 x 1024, 4 heads of 64 and 128 columns, of which the matrix instructions take a
-// fifth), 6.5 of fp32 ones.
+// are a chunk ahead.  6 us a chunk, of which the matrix instructions take a fifth.
+// Where S and N are kept for the gradient, their bytes bound it: 98 us for 32 x 1024
+// bf16 rows, 4 heads of 64 and 128 columns, 150 KB a chunk, 80 of them written, 3.1
+// TB/s.  Else the latency of a chunk's dependent products (S -> R -> N -> S), with one
+// wave a SIMD.  O by a second wave beside the one that carries S: 102 us there, and a
+// prefill of 64 x 521, 8 heads of 128 x 128, 255 us in all and not 240.
 template <typename T, int DK, bool W, bool LOCAL>
 __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
     const DeltaArgs a, const unsigned char* prep, float* rec, int chunks, int tiles,
@@ -949,7 +951,7 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
 
 // The gradient's chain, from the last chunk to the first: dS and dR of every
 // chunk, both with a column of d_v after the other, as S and N are kept.  Bound as
-// the forward chain: 90 us for 32 x 1024, 4 heads of 64 and 128 columns.
+// the forward chain: 90 us for 32 x 1024, 4 heads of 64 and 128 columns, 3.0 TB/s.
 template <typename T, int DK, bool W, bool LOCAL>
 __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
     const DeltaGradArgs ga, const unsigned char* prep, float* grec, int chunks, int tiles,
@@ -1159,7 +1161,7 @@ __global__ __launch_bounds__(256) void delta_combine_kernel(const DeltaArgs a, c
 // registers: forward and gradient of 4 x 777 rows, 4 heads of 128 and 8 of 128
 // columns, 341 us and not 319.)  Bound by the two roles' waits for each other and by
 // the LDS between products: 194 us for 32 x 1024 rows, 4 heads of 64 and 128 columns,
-// 2.7 TB/s; the matrix instructions take a tenth.  K and Q kept in LDS rather than
+// 2.2 TB/s; the matrix instructions take a tenth.  K and Q kept in LDS rather than
 // in registers: 234; the products' operands brought one tile ahead in the first four
 // waves: 218.
 // dQ^T and dK^T [d_k][own] leave as four neighbouring columns a lane.

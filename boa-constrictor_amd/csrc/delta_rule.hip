@@ -508,7 +508,8 @@ __device__ __forceinline__ void mma16(f4& acc, f4 x, f4 y) {
 // many blocks as the registers allow share a CU: four (bf16, d_k up to 64) or two.
 template <typename T, int DK, bool TRANS, bool W>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 ? 4 : 2) void delta_prep_kernel(const DeltaArgs a, unsigned char* prep,
-                                                         int chunks, uint64_t blocks) {
+                                                         int chunks, uint32_t* order,
+                                                         uint64_t blocks) {
   using M = Mode<T>;
   constexpr int U = DK / 32, P = M::ROWS;
   constexpr int TILE = 4 * U * P * 64;
@@ -523,6 +524,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 ? 4 : 2) void delta
   __shared__ Decays s;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i16 = lane % 16, g = lane / 16, g4 = 4 * g, sl = slot_of(i16, g);
+  // the lanes' order, the longest first, for the chain
+  for (int l = blockIdx.x; order && l < a.q.lanes; l += gridDim.x) {
+    const int own = seq_len(a.q, l);
+    int rank = 0;
+    for (int j0 = 0; j0 < a.q.lanes; j0 += 256) {
+      const int j = j0 + tid, other = seq_len(a.q, min(j, a.q.lanes - 1));
+      rank += __syncthreads_count(j < a.q.lanes && (other > own || (other == own && j < l)));
+    }
+    if (tid == 0) order[rank] = l;
+  }
   for (uint64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
     Place p;
     p.c = same((int)(b % chunks));
@@ -801,7 +812,7 @@ struct Segments {
 template <typename T, int DK, bool W, bool LOCAL>
 __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
     const DeltaArgs a, const unsigned char* prep, float* rec, int chunks, int tiles,
-    const Segments seg, uint32_t blocks) {
+    const Segments seg, const uint32_t* order, uint32_t blocks) {
   using M = Mode<T>;
   constexpr int U = DK / 32, MT = DK / 16, FULL = M::FULL, P = M::ROWS;
   extern __shared__ __align__(16) unsigned char lds[];
@@ -810,11 +821,13 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
   const int i16 = lane % 16, g = lane / 16, sl = slot_of(i16, g);
   const int per = LOCAL ? tiles + DK / 64 : tiles;
   for (uint32_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const uint32_t ls = same((int)(b / per)), lh = same((int)(ls / seg.n));
-    const int sg = ls - lh * seg.n;
+    const uint32_t ls = same((int)(b / per)), nth = same((int)(ls / seg.n));
+    const int sg = ls - nth * seg.n;
     Place p;
-    p.l = same((int)(lh / a.HV));
-    p.h = lh - p.l * a.HV;
+    p.l = same((int)(nth / a.HV));
+    p.h = nth - p.l * a.HV;
+    if (order) p.l = same((int)order[p.l]);
+    const uint32_t lh = (uint32_t)p.l * a.HV + p.h;
     const int kh = same(p.h / (a.HV / a.H)), len = same(seq_len(a.q, p.l)), all = (len + C - 1) / C;
     const int from = sg * seg.chunks, last = min(all, from + seg.chunks);
     const int vb = same((int)(b - ls * per) * 64), v0 = vb + wave * 16, col = v0 + i16;
@@ -955,7 +968,7 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
 template <typename T, int DK, bool W, bool LOCAL>
 __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
     const DeltaGradArgs ga, const unsigned char* prep, float* grec, int chunks, int tiles,
-    const Segments seg, uint32_t blocks) {
+    const Segments seg, const uint32_t* order, uint32_t blocks) {
   using M = Mode<T>;
   constexpr int U = DK / 32, MT = DK / 16, FULL = M::FULL, P = M::ROWS;
   extern __shared__ __align__(16) unsigned char lds[];
@@ -964,11 +977,13 @@ __global__ __launch_bounds__(256, 1) void delta_grad_chain_kernel(
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i16 = lane % 16, g = lane / 16, sl = slot_of(i16, g);
   for (uint32_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-    const uint32_t ls = same((int)(b / tiles)), lh = same((int)(ls / seg.n));
-    const int sg = ls - lh * seg.n;
+    const uint32_t ls = same((int)(b / tiles)), nth = same((int)(ls / seg.n));
+    const int sg = ls - nth * seg.n;
     Place p;
-    p.l = same((int)(lh / a.HV));
-    p.h = lh - p.l * a.HV;
+    p.l = same((int)(nth / a.HV));
+    p.h = nth - p.l * a.HV;
+    if (order) p.l = same((int)order[p.l]);
+    const uint32_t lh = (uint32_t)p.l * a.HV + p.h;
     const int kh = same(p.h / (a.HV / a.H)), len = same(seq_len(a.q, p.l)), all = (len + C - 1) / C;
     const int from = sg * seg.chunks, last = min(all, from + seg.chunks);
     const int vb = same((int)(b - ls * tiles) * 64), v0 = vb + wave * 16, col = v0 + i16;
@@ -1757,6 +1772,13 @@ int64_t local_floats(int64_t heads, const Cut& c, int dk, int dv, bool moves) {
   return heads * c.n * ((dv + 63) / 64 * 64 + (moves ? 2 * built(dk) : 0)) * built(dk);
 }
 
+// Lanes of different lengths: the chains take the longest first where there are more
+// blocks than CUs, so that none starts late (64 x 521, 8 heads of 128 x 128, lengths
+// up to that: 145 and 168 us).  `at`: where the order is kept, of lanes' size.
+uint32_t* order_of(const DeltaArgs& a, uint64_t blocks, int chunks, const Cut& cut, void* at) {
+  return a.q.lens && cut.n == 1 && chunks > 1 && blocks > 256 ? (uint32_t*)at : nullptr;
+}
+
 // Positions taken one after the other rather than in chunks: what a position takes
 // (1.4 us where few states wait for their rows, 2.5 at 64 lanes of 8 states of 128 x
 // 128) against a chunk's three kernels.  Measured, us:
@@ -1806,11 +1828,13 @@ hipError_t delta_of(const DeltaArgs& a, hipStream_t s) {
     const int chunks = chunks_of(a.q.T), tiles = (a.dv + 63) / 64;
     unsigned char* prep = (unsigned char*)a.work;
     const uint64_t all = heads * chunks;
-    BOA_LAUNCH((delta_prep_kernel<T, DK, false, W>), grid(all), 256, 0, s, a, prep, chunks, all);
+    const Cut cut = segments_of(heads, chunks, a.dk, a.dv);
+    uint32_t* order = order_of(a, heads * tiles, chunks, cut, prep + all * PREP_BYTES);
+    BOA_LAUNCH((delta_prep_kernel<T, DK, false, W>), grid(all), 256, 0, s, a, prep, chunks, order,
+               all);
     hipError_t e = hipGetLastError();
     if (e) return e;
     const size_t lds = sizeof(ChainLds<T, DK, false>);
-    const Cut cut = segments_of(heads, chunks, a.dk, a.dv);
     Segments seg{cut.n, cut.chunks, nullptr, nullptr};
     if (cut.n > 1) {
       seg.first = (float*)(prep + all * PREP_BYTES);
@@ -1820,7 +1844,8 @@ hipError_t delta_of(const DeltaArgs& a, hipStream_t s) {
       const uint32_t blocks = (uint32_t)(heads * cut.n * (tiles + DK / 64));
       if ((e = room(delta_chain_kernel<T, DK, W, true>, lds))) return e;
       BOA_LAUNCH((delta_chain_kernel<T, DK, W, true>), blocks, 256, lds, s, a,
-                 (const unsigned char*)prep, (float*)nullptr, chunks, tiles, seg, blocks);
+                 (const unsigned char*)prep, (float*)nullptr, chunks, tiles, seg,
+                 (const uint32_t*)nullptr, blocks);
       if ((e = hipGetLastError())) return e;
       const uint32_t columns = (uint32_t)(heads * tiles * 4);
       BOA_LAUNCH((delta_combine_kernel<DK, false>), columns, 256, 0, s, a, a.state_in,
@@ -1831,7 +1856,8 @@ hipError_t delta_of(const DeltaArgs& a, hipStream_t s) {
     if ((e = room(delta_chain_kernel<T, DK, W, false>, lds))) return e;
     const uint64_t blocks = heads * cut.n * tiles;
     BOA_LAUNCH((delta_chain_kernel<T, DK, W, false>), grid(blocks), 256, lds, s, a,
-               (const unsigned char*)prep, a.saved, chunks, tiles, seg, (uint32_t)blocks);
+               (const unsigned char*)prep, a.saved, chunks, tiles, seg,
+               (const uint32_t*)order, (uint32_t)blocks);
     return hipGetLastError();
   });
 }
@@ -1846,11 +1872,14 @@ hipError_t delta_grad_of(const DeltaGradArgs& ga, hipStream_t s) {
     const uint64_t all = heads * chunks;
     unsigned char* prep = (unsigned char*)a.work;
     float* grec = (float*)(prep + all * PREP_BYTES);
-    BOA_LAUNCH((delta_prep_kernel<T, DK, true, W>), grid(all), 256, 0, s, a, prep, chunks, all);
+    const Cut cut = segments_of(heads, chunks, a.dk, a.dv);
+    uint32_t* order =
+        order_of(a, heads * tiles, chunks, cut, grec + all * record_floats(a.dk, a.dv));
+    BOA_LAUNCH((delta_prep_kernel<T, DK, true, W>), grid(all), 256, 0, s, a, prep, chunks, order,
+               all);
     hipError_t e = hipGetLastError();
     if (e) return e;
     size_t lds = sizeof(ChainLds<T, DK, true>);
-    const Cut cut = segments_of(heads, chunks, a.dk, a.dv);
     Segments seg{cut.n, cut.chunks, nullptr, nullptr};
     if (cut.n > 1) {
       seg.first = grec + all * record_floats(a.dk, a.dv);
@@ -1858,7 +1887,8 @@ hipError_t delta_grad_of(const DeltaGradArgs& ga, hipStream_t s) {
       const uint32_t blocks = (uint32_t)(heads * cut.n * tiles);
       if ((e = room(delta_grad_chain_kernel<T, DK, W, true>, lds))) return e;
       BOA_LAUNCH((delta_grad_chain_kernel<T, DK, W, true>), blocks, 256, lds, s, ga,
-                 (const unsigned char*)prep, grec, chunks, tiles, seg, blocks);
+                 (const unsigned char*)prep, grec, chunks, tiles, seg,
+                 (const uint32_t*)nullptr, blocks);
       if ((e = hipGetLastError())) return e;
       const uint32_t columns = (uint32_t)(heads * tiles * 4);
       BOA_LAUNCH((delta_combine_kernel<DK, true>), columns, 256, 0, s, a, ga.dstate_out,
@@ -1869,7 +1899,8 @@ hipError_t delta_grad_of(const DeltaGradArgs& ga, hipStream_t s) {
     if ((e = room(delta_grad_chain_kernel<T, DK, W, false>, lds))) return e;
     const uint64_t blocks = heads * cut.n * tiles;
     BOA_LAUNCH((delta_grad_chain_kernel<T, DK, W, false>), grid(blocks), 256, lds, s, ga,
-               (const unsigned char*)prep, grec, chunks, tiles, seg, (uint32_t)blocks);
+               (const unsigned char*)prep, grec, chunks, tiles, seg,
+               (const uint32_t*)order, (uint32_t)blocks);
     if ((e = hipGetLastError())) return e;
     lds = sizeof(LastLds<T, DK>);
     if ((e = room(delta_grad_last_kernel<T, DK, W>, lds))) return e;
@@ -1906,6 +1937,7 @@ int64_t delta_work_bytes(int lanes, int T, int, int HV, int dk, int dv, bool gra
   // what a forward call needs, and a gradient's as well if it is to be one's
   int64_t floats = first + local_floats(heads, cut, dk, dv, true);
   if (grad) floats = std::max(floats, heads * chunks * record_floats(dk, dv) + 2 * first);
+  if (cut.n == 1) floats += (lanes + 3) / 4 * 4;  // the lanes' order
   return heads * chunks * PREP_BYTES + 4 * floats;
 }
 

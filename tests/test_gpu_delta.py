@@ -103,6 +103,8 @@ SHAPES = [  # lanes, T, heads, v heads, d_k, d_v, layout, lens, kind
     (5, 70, 2, 2, 64, 128, "dense", "ragged", "none"), (2, 300, 1, 1, 127, 7, "odd", "ragged", "plain"),
     (1, 513, 1, 1, 64, 64, "dense", "full", "plain"), (3, 12, 1, 2, 100, 36, "dense", "ragged", "same"),
     (2, 9, 2, 2, 64, 64, "odd", "ragged", "reset"), (4, 13, 1, 1, 128, 128, "time", "ragged", "tiny"),
+    # more blocks than CUs: the longest lanes first
+    (70, 150, 2, 4, 33, 20, "dense", "ragged", "plain"), (300, 70, 1, 1, 16, 100, "wide", "ragged", "reset"),
     # cut into segments
     (1, 1100, 1, 1, 64, 64, "dense", "full", "plain"), (2, 1029, 1, 2, 33, 80, "odd", "ragged", "reset"),
     (3, 1500, 1, 2, 80, 70, "wide", "ragged", "same"), (1, 2000, 2, 2, 128, 128, "dense", "full", "none")]

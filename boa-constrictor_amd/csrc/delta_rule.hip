@@ -505,9 +505,10 @@ __device__ __forceinline__ void mma16(f4& acc, f4 x, f4 y) {
 // the coefficients.  Bound by a block's chain of steps (the substitution of 16
 // columns, then the products between blocks) and by the 39 KB that it writes: 2048
 // chunks of 64 columns of k 46 us, 1.8 TB/s.  All chunks are at hand at once, so as
-// many blocks as the registers allow share a CU: four (bf16, d_k up to 64) or two.
+// many blocks as registers and LDS allow share a CU: four for bf16 rows and d_k up to
+// 64, three at 128 (two: 74 and not 54 us for the prompts of 64 x 521, 8 heads).
 template <typename T, int DK, bool TRANS, bool W>
-__global__ __launch_bounds__(256, sizeof(T) == 2 && DK == 64 ? 4 : 2) void delta_prep_kernel(const DeltaArgs a, unsigned char* prep,
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? (DK == 64 ? 4 : 3) : 2) void delta_prep_kernel(const DeltaArgs a, unsigned char* prep,
                                                          int chunks, uint32_t* order,
                                                          uint64_t blocks) {
   using M = Mode<T>;

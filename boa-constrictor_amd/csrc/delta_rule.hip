@@ -751,6 +751,10 @@ struct ChainNext {
   }
 };
 
+// The compiler moves nothing across: left alone it brings all of a loop's operands
+// in first, for which the registers do not suffice.
+__device__ __forceinline__ void apart() { __builtin_amdgcn_sched_barrier(0); }
+
 // rows 4 g .. of tile t of a [64] array
 __device__ __forceinline__ f4 four_rows(const float* c, int t, int g) {
   return *reinterpret_cast<const f4*>(c + t * 16 + 4 * g);
@@ -801,8 +805,9 @@ struct Segments {
 };
 
 // The states from chunk to chunk and O.  A block's four waves, 16 columns of S, N
-// and O each, share K, Q, T, P and v in LDS (69 KB for bf16 rows and d_k up to 64,
-// 93 KB at 128); S stays in registers as the next product's right operand, so a
+// and O each, share K, Q, T, P and v in LDS (69 KB for bf16 rows and d_k up to 64, so
+// that two blocks share a CU: forward of 64 x 512, 4 heads of 64 and 128 columns, 105
+// us and not 123; 93 KB at 128, one block); S stays in registers as the next product's right operand, so a
 // wave has no exchange with others but the barriers around a chunk's loads, which
 // are a chunk ahead.  6 us a chunk, of which the matrix instructions take a fifth.
 // Where S and N are kept for the gradient, their bytes bound it: 98 us for 32 x 1024
@@ -811,17 +816,20 @@ struct Segments {
 // wave a SIMD.  O by a second wave beside the one that carries S: 102 us there, and a
 // prefill of 64 x 521, 8 heads of 128 x 128, 255 us in all and not 240.
 template <typename T, int DK, bool W, bool LOCAL>
-__global__ __launch_bounds__(256, 1) void delta_chain_kernel(
+__global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_chain_kernel(
     const DeltaArgs a, const unsigned char* prep, float* rec, int chunks, int tiles,
     const Segments seg, const uint32_t* order, uint32_t blocks) {
   using M = Mode<T>;
   constexpr int U = DK / 32, MT = DK / 16, FULL = M::FULL, P = M::ROWS;
   extern __shared__ __align__(16) unsigned char lds[];
   ChainLds<T, DK, false>& s = *reinterpret_cast<ChainLds<T, DK, false>*>(lds);
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int i16 = lane % 16, g = lane / 16, sl = slot_of(i16, g);
   const int per = LOCAL ? tiles + DK / 64 : tiles;
   for (uint32_t b = blockIdx.x; b < blocks; b += gridDim.x) {
+    // (computed here, not kept from before the loop, for which registers lack)
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, wave = same(tid >> 6);
+    const int i16 = lane % 16, g = lane / 16, sl = slot_of(i16, g);
     const uint32_t ls = same((int)(b / per)), nth = same((int)(ls / seg.n));
     const int sg = ls - nth * seg.n;
     Place p;
@@ -875,20 +883,19 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
       }
       f4 o[4], x[4];
       {
-        Frag<FULL> sf[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) sf[u] = full<T>(st[2 * u], st[2 * u + 1]);
 #pragma unroll
         for (int t = 0; t < 4; ++t) x[t] = o[t] = ZERO;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+          const Frag<FULL> sf = full<T>(st[2 * u], st[2 * u + 1]);
           Frag<P> k[4], q[4];
           get<P>(k, s.ka, u, U, sl);
-          mma<T>(x, k, sf[u]);
+          mma<T>(x, k, sf);
           if constexpr (!LOCAL) {
             get<P>(q, s.q, u, U, sl);
-            mma<T>(o, q, sf[u]);
+            mma<T>(o, q, sf);
           }
+          if constexpr (DK == 64) apart();
         }
       }
       f4 nn[4];
@@ -929,6 +936,7 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(
           Frag<P> k[MT];
           get<P>(k, s.kt, u, 2, sl);
           mma<T>(st, k, nf[u]);
+          if constexpr (DK == 64) apart();
         }
       }
       if constexpr (LOCAL) continue;
@@ -1203,10 +1211,6 @@ struct LastLds {
   } coef;
 };
 static_assert(sizeof(LastLds<float, 64>::coef) == COEF * 4, "as prep leaves them");
-
-// The compiler moves nothing across: left alone it brings all of a loop's operands
-// in first, for which the registers do not suffice.
-__device__ __forceinline__ void apart() { __builtin_amdgcn_sched_barrier(0); }
 
 template <int P>
 __device__ __forceinline__ Frag<P> either(bool first, const Frag<P>& a, const Frag<P>& b) {

@@ -381,9 +381,6 @@ struct Rows4 {
 #pragma unroll
     for (int e = 0; e < 4; ++e) r[e].template cut<W>(e < n ? d : 0);
   }
-  __device__ __forceinline__ Four values() const {
-    return Four{{r[0].value(), r[1].value(), r[2].value(), r[3].value()}};
-  }
   __device__ __forceinline__ Rows4 turned() const {
     Rows4 t;
     if constexpr (sizeof(T) == 4) {
@@ -506,11 +503,12 @@ __device__ __forceinline__ void mma16(f4& acc, f4 x, f4 y) {
 // columns, then the products between blocks) and by the 39 KB that it writes: 2048
 // chunks of 64 columns of k 46 us, 1.8 TB/s.  All chunks are at hand at once, so as
 // many blocks as registers and LDS allow share a CU: four for bf16 rows and d_k up to
-// 64, three at 128 (two: 74 and not 54 us for the prompts of 64 x 521, 8 heads).
+// 64, three at 128 (two: 74 and not 59 us for the prompts of 64 x 521, 8 heads); two
+// or three for fp32 rows, one at 128, whose K and Q take 64 KB.
 template <typename T, int DK, bool TRANS, bool W>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? (DK == 64 ? 4 : 3) : 2) void delta_prep_kernel(const DeltaArgs a, unsigned char* prep,
-                                                         int chunks, uint32_t* order,
-                                                         uint64_t blocks) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? (DK == 64 ? 4 : 3) : DK == 64 ? 2 : 1)
+void delta_prep_kernel(const DeltaArgs a, unsigned char* prep, int chunks, uint32_t* order,
+                       uint64_t blocks) {
   using M = Mode<T>;
   constexpr int U = DK / 32, P = M::ROWS;
   constexpr int TILE = 4 * U * P * 64;
@@ -807,9 +805,10 @@ struct Segments {
 // The states from chunk to chunk and O.  A block's four waves, 16 columns of S, N
 // and O each, share K, Q, T, P and v in LDS (69 KB for bf16 rows and d_k up to 64, so
 // that two blocks share a CU: forward of 64 x 512, 4 heads of 64 and 128 columns, 105
-// us and not 123; 93 KB at 128, one block); S stays in registers as the next product's right operand, so a
-// wave has no exchange with others but the barriers around a chunk's loads, which
-// are a chunk ahead.  6 us a chunk, of which the matrix instructions take a fifth.
+// us and not 123; 93 KB at 128, one block).  S stays in registers as the next
+// product's right operand, so a wave has no exchange with others but the barriers
+// around a chunk's loads, which are a chunk ahead.  6 us a chunk, of which the matrix
+// instructions take a fifth.
 // Where S and N are kept for the gradient, their bytes bound it: 98 us for 32 x 1024
 // bf16 rows, 4 heads of 64 and 128 columns, 150 KB a chunk, 80 of them written, 3.1
 // TB/s.  Else the latency of a chunk's dependent products (S -> R -> N -> S), with one
@@ -1508,8 +1507,8 @@ __global__ __launch_bounds__(512, 2) void delta_grad_last_kernel(
       for (int vh = kh * group; vh < (kh + 1) * group; ++vh) {
         p.h = vh;
         const int64_t record = same(((int64_t)p.l * a.HV + vh) * chunks + p.c);
-        const float *S = rec + record * (a.dv * (DK + C)), *N = S + a.dv * DK;
-        const float *dS = grec + record * (a.dv * (DK + C)), *dR = dS + a.dv * DK;
+        const float *S = rec + record * (a.dv * (DK + C));
+        const float* dS = grec + record * (a.dv * (DK + C));
         const unsigned char* coef = prep + ((record + 1) * PREP_BYTES - COEF * 4);
         const float co0 = *at32<const float>(coef, min(all, COEF - 1));
         const float co1 = *at32<const float>(coef, min(all + 512, COEF - 1));

@@ -6,6 +6,8 @@
 // so q does not depend on r.  t and q are computed in 64 bits: a value next to
 // the border of two steps goes to the side that the formula puts it on.
 //   dh = r (w dy - n mean(n w dy)) + dsum,  n = h r;      dw = sum of rows dy n
+// Sums are in fp32; where squares of a row would leave its range, they are taken
+// again from the row times a power of two.
 //
 // All of it is bound by the rows' bytes: a row is read once, held in registers
 // by G threads of U vectors each (16 bytes a vector, or single elements where
@@ -88,6 +90,28 @@ struct Most {  // NaN wins
   __device__ X operator()(X a, X b) const { return a != a ? a : (b > a || b != b ? b : a); }
 };
 
+// r of a row, as n = h before r after: the two others are 1, or a power of two on
+// the side where no product leaves fp32's range.  half: the square root of both.
+struct Root {
+  float before, r, after, half;
+  __device__ __forceinline__ float of(float h) const { return h * before * r * after; }
+};
+// squares(s): this thread's sum of (s h)^2.  From LEAST on, squares below the least
+// normal number are off by less than 2^-40 of the mean; up to MOST no sum of 8192 of
+// them overflows, and a NaN goes either way.
+template <int G, typename F>
+__device__ __forceinline__ Root root_of(const F& squares, int width, float eps, float* part) {
+  constexpr float LEAST = 0x1p-110f, MOST = 0x1p100f;
+  const float mean = row_all<G>(squares(1.0f), Sum(), part) / (float)width + eps;
+  if (mean >= LEAST && mean < MOST) return {1.0f, 1.0f / __builtin_sqrtf(mean), 1.0f, 1.0f};
+  const bool small = mean < LEAST;
+  const float s = small ? 0x1p90f : 0x1p-80f;
+  const float again = row_all<G>(squares(s), Sum(), part) / (float)width + eps * s * s;
+  const float r = 1.0f / __builtin_sqrtf(again);
+  if (small) return {s, r, 1.0f, 0x1p45f};
+  return {1.0f, r, s, 0x1p-40f};
+}
+
 // 127 t / top to the nearest whole number.  f is the quotient in fp32, off by
 // under 5e-5 (h, t, the step and the product are rounded, 127 being the most);
 // where that leaves the number open, t and the product are taken in 64 bits, and
@@ -145,20 +169,27 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a, uint32_t ro
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if ((u * G + g) * V >= a.width) h[u][j] = hr[u][j] = 0.0f;
-    float ss = 0.0f, most = 0.0f;
+    float most = 0.0f;
+    if constexpr (OUT8) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float s = h[u][j] + hr[u][j];
-        ss += s * s;
-        if constexpr (OUT8) most = Most()(most, __builtin_fabsf(s * w[u][j]));
-      }
-    float rn = 1.0f;
-    if (a.norm) {
-      ss = row_all<G>(ss, Sum(), (float*)part);
-      rn = 1.0f / __builtin_sqrtf(ss / (float)a.width + a.eps);
+        for (int j = 0; j < V; ++j)
+          most = Most()(most, __builtin_fabsf((h[u][j] + hr[u][j]) * w[u][j]));
     }
+    Root rn = {1.0f, 1.0f, 1.0f, 1.0f};
+    if (a.norm)
+      rn = root_of<G>([&](float by) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float s = (h[u][j] + hr[u][j]) * by;
+            ss += s * s;
+          }
+        return ss;
+      }, a.width, a.eps, (float*)part);
     if (a.sum.d && live) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -176,7 +207,7 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a, uint32_t ro
         if (i < a.width) {
           float y[V];
 #pragma unroll
-          for (int j = 0; j < V; ++j) y[j] = (h[u][j] + hr[u][j]) * rn * w[u][j];
+          for (int j = 0; j < V; ++j) y[j] = rn.of(h[u][j] + hr[u][j]) * w[u][j];
           store_row<V>((T*)a.out.d + l * a.out.lane + t * a.out.row + i, y);
         }
       }
@@ -219,7 +250,8 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a, uint32_t ro
             }
           }
         }
-        if (g == 0) a.scale8[r] = (float)(top * (double)rn / 127.0);
+        if (g == 0)
+          a.scale8[r] = (float)(top * (double)rn.before * (double)rn.r * (double)rn.after / 127.0);
       }
     }
   }
@@ -253,7 +285,6 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(const NormGradArgs a, ui
     const T* hp = (const T*)a.h.d + l * a.h.lane + t * a.h.row;
     const T* dp = (const T*)a.dout.d + l * a.dout.lane + t * a.dout.row;
     const T* sp = a.dsum.d ? (const T*)a.dsum.d + l * a.dsum.lane + t * a.dsum.row : nullptr;
-    float ss = 0.0f, c = 0.0f;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -273,17 +304,33 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(const NormGradArgs a, ui
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if ((u * G + g) * V >= a.width) h[u][j] = dy[u][j] = 0.0f;
+    const Root rn = root_of<G>([&](float by) {
+      float ss = 0.0f;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        ss += h[u][j] * h[u][j];
-        c += h[u][j] * (w[u][j] * dy[u][j]);
-      }
-    ss = row_all<G>(ss, Sum(), part);
-    c = row_all<G>(c, Sum(), part);
-    const float rn = 1.0f / __builtin_sqrtf(ss / (float)a.width + a.eps);
-    const float m = c * rn / (float)a.width;  // mean of n w dy
+        for (int j = 0; j < V; ++j) {
+          const float s = h[u][j] * by;
+          ss += s * s;
+        }
+      return ss;
+    }, a.width, a.eps, part);
+    // sum of x w dy
+    auto along = [&](auto x) {
+      float c = 0.0f;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < V; ++j) c += x(h[u][j]) * (w[u][j] * dy[u][j]);
+      return row_all<G>(c, Sum(), part);
+    };
+    // the mean of n w dy: r taken out of the sum, unless its terms or their sum
+    // leave fp32's range
+    const float c = along([](float x) { return x; }), cr = c * rn.r;
+    float m = cr / (float)a.width;
+    if (live && (rn.half != 1.0f || !(__builtin_fabsf(c) >= 0x1p-100f) ||
+                 !(__builtin_fabsf(cr) >= 0x1p-110f) || !(__builtin_fabsf(cr) < 0x1p120f)))
+      m = along([&](float x) { return rn.of(x); }) / (float)a.width;
     if (there) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -291,9 +338,10 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(const NormGradArgs a, ui
         float dx[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float n = h[u][j] * rn;
+          const float n = rn.of(h[u][j]);
           if (live) dw[u][j] += dy[u][j] * n;
-          dx[j] = live ? rn * (w[u][j] * dy[u][j] - n * m) + ds[u][j] : 0.0f;
+          const float d = (w[u][j] * dy[u][j] - n * m) * rn.half * rn.r * rn.half;
+          dx[j] = live ? d + ds[u][j] : 0.0f;
         }
         if (i < a.width) store_row<V>((T*)a.dx.d + l * a.dx.lane + t * a.dx.row + i, dx);
       }

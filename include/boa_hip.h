@@ -264,6 +264,8 @@ int64_t boa_next_byte_loss_work_bytes(int32_t lanes, int32_t T);
  * with d_scale8 [lanes][T], the out rows in 8 bits: of t = h weight,
  * out8 = rint(127 t / max |t|) and scale8 = max |t| r / 127, so that out8
  * scale8 is out within half a step.  A boa_rows of int8 has strides in bytes.
+ * Rows may have any values whose h is finite: squares beyond fp32's range are
+ * scaled.  (A scale8 below 2^-126 has steps of 2^-149, as fp32 has there.)
  * A row of zeros has scale 0 (NaN where eps is 0), one with a value that is not
  * finite scale NaN or infinity. */
 int boa_rms_norm(boa_ctx* ctx, const boa_rows* x, const boa_rows* residual, const float* d_weight,

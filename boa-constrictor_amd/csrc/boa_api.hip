@@ -16,6 +16,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -1168,6 +1169,17 @@ struct TrainCheck {
     near(r, what);
     size = keep;
   }
+  // outputs (and a workspace) that begin where another or an input does; the
+  // pointers of those that are not there are NULL
+  void apart(std::initializer_list<const void*> outs, std::initializer_list<const void*> ins) {
+    if (bad) return;
+    for (auto o = outs.begin(); o != outs.end(); ++o) {
+      if (!*o) continue;
+      for (auto i = ins.begin(); i != ins.end(); ++i) that(*o != *i, "an output is an input");
+      for (auto p = outs.begin(); p != o; ++p) that(*o != *p, "an output is another output");
+    }
+  }
+  static const void* at(const boa_rows* r) { return r ? r->d : nullptr; }
   // an output that may be an input only with the same strides
   void same_or_other(const boa_rows* o, const boa_rows* i, const char* what) {
     that(bad || !o || !i || o->d != i->d ||
@@ -1205,10 +1217,6 @@ struct TrainCheck {
     a.g = from(s->g);
     a.beta = from(s->beta);
     a.state_in = s->d_state_in;
-  }
-  static bool delta_input(const boa_delta& s, const void* p) {
-    return p == s.q.d || p == s.k.d || p == s.v.d || p == s.g.d || p == s.beta.d ||
-           p == s.d_state_in;
   }
 };
 
@@ -1940,18 +1948,11 @@ int boa_rms_norm(boa_ctx* c, const boa_rows* x, const boa_rows* residual, const 
       k.out(sum, width, "sum"), k.near(sum, "sum");
       k.same_or_other(sum, x, "sum"), k.same_or_other(sum, residual, "sum");
     }
-    if (out) {
-      k.out(out, width, "out"), k.near(out, "out");
-      k.that(k.bad || (out->d != x->d && (!residual || out->d != residual->d) &&
-                       (!sum || out->d != sum->d)), "out is an input or another output");
-    }
-    if (out8) {
-      k.rows8(out8, width, true, "out8");
-      k.floats(d_scale8, 4, false, "scale8");
-      k.that(k.bad || (out8->d != x->d && (!residual || out8->d != residual->d) &&
-                       (!sum || out8->d != sum->d) && (!out || out8->d != out->d)),
-             "out8 is an input or another output");
-    }
+    if (out) k.out(out, width, "out"), k.near(out, "out");
+    if (out8) k.rows8(out8, width, true, "out8"), k.floats(d_scale8, 4, false, "scale8");
+    const void* scale8 = out8 ? d_scale8 : nullptr;
+    k.apart({k.at(out), k.at(out8), scale8}, {k.at(x), k.at(residual), k.at(sum), d_weight, d_lens});
+    k.apart({k.at(sum)}, {d_weight, d_lens});
     if (k.bad) return hipSuccess;
     NormArgs a{};
     a.q = Seqs{lanes, T, d_lens};
@@ -1984,11 +1985,11 @@ int boa_rms_norm_grad(boa_ctx* c, const boa_rows* h, const float* d_weight, cons
     k.in(dout, "dout"), k.near(dout, "dout");
     if (dsum) k.in(dsum, "dsum"), k.near(dsum, "dsum");
     k.out(dx, width, "dx"), k.near(dx, "dx");
-    k.that(k.bad || dx->d != h->d, "dx is an input");
     k.same_or_other(dx, dout, "dx"), k.same_or_other(dx, dsum, "dx");
     k.floats(d_dweight, 4, true, "dweight");
-    k.that(k.bad || !d_dweight || d_dweight != d_weight, "dweight is an input");
     if (d_dweight) k.work(d_work, work_bytes, boa_rms_norm_grad_work_bytes(lanes, T, width));
+    k.apart({k.at(dx), d_dweight, d_dweight ? d_work : nullptr}, {k.at(h), d_weight, d_lens});
+    k.apart({d_dweight, d_dweight ? d_work : nullptr}, {k.at(dout), k.at(dsum)});
     if (k.bad) return hipSuccess;
     NormGradArgs a{};
     a.q = Seqs{lanes, T, d_lens};
@@ -2015,7 +2016,7 @@ int boa_int8_rows(boa_ctx* c, const boa_rows* x, const int32_t* d_lens, int32_t 
     k.floats(d_lens, 4, true, "lens");
     k.rows8(out8, width, true, "out8");
     k.floats(d_scale8, 4, false, "scale8");
-    k.that(k.bad || out8->d != x->d, "out8 is an input");
+    k.apart({k.at(out8), d_scale8}, {k.at(x), d_lens});
     if (k.bad) return hipSuccess;
     NormArgs a{};
     a.q = Seqs{lanes, T, d_lens};
@@ -2053,8 +2054,7 @@ int boa_int8_matmul(boa_ctx* c, const boa_rows* x8, const float* d_scale8, const
     k.floats(d_wscale, 4, false, "wscale");
     k.floats(d_bias, 4, true, "bias");
     k.out(out, n, "out"), k.near(out, "out");
-    k.that(k.bad || (out->d != x8->d && out->d != d_packed && out->d != d_scale8 &&
-                     out->d != d_wscale && out->d != d_bias), "out is an input");
+    k.apart({k.at(out)}, {k.at(x8), d_scale8, d_lens, d_packed, d_wscale, d_bias});
     if (k.bad) return hipSuccess;
     Int8Args a{};
     a.q = Seqs{lanes, T, d_lens};
@@ -2080,9 +2080,12 @@ int boa_delta_rule(boa_ctx* c, const boa_delta* d, const boa_rows* out, float* d
     k.out(out, (int64_t)d->v_heads * d->d_v, "out"), k.nearer(out, "out");
     k.floats(d_state_out, 16, true, "state_out");
     k.floats(d_saved, 16, true, "saved");
-    k.that(k.bad || !k.delta_input(*d, out->d), "out is an input");
-    k.work(d_work, work_bytes, boa_delta_rule_work_bytes(d->lanes, d->T, d->heads, d->v_heads,
-                                                         d->d_k, d->d_v, d_saved != nullptr));
+    const int64_t need = boa_delta_rule_work_bytes(d->lanes, d->T, d->heads, d->v_heads, d->d_k,
+                                                   d->d_v, d_saved != nullptr);
+    k.work(d_work, work_bytes, need);
+    k.apart({k.at(out), d_saved, need > 0 ? d_work : nullptr},
+            {d->q.d, d->k.d, d->v.d, d->g.d, d->beta.d, d->d_state_in, d->d_lens, d_state_out});
+    k.apart({d_state_out}, {d->q.d, d->k.d, d->v.d, d->g.d, d->beta.d, d->d_lens});
     if (k.bad) return hipSuccess;
     a.out = k.to(*out);
     a.state_out = d_state_out;
@@ -2113,13 +2116,13 @@ int boa_delta_rule_grad(boa_ctx* c, const boa_delta* d, const float* d_saved, co
     k.out(&g->dbeta, d->v_heads, "dbeta"), k.nearer(&g->dbeta, "dbeta");
     k.size = keep;
     k.floats(g->d_dstate_in, 4, true, "dstate_in");
-    for (const void* p : {(const void*)g->dq.d, (const void*)g->dk.d, (const void*)g->dv.d,
-                          (const void*)g->dg.d, (const void*)g->dbeta.d})
-      k.that(k.bad || (!k.delta_input(*d, p) && p != dout->d && p != d_saved),
-             "a gradient is an input");
-    k.that(k.bad || !g->d_dstate_in || g->d_dstate_in != d_saved, "dstate_in is saved");
     k.work(d_work, work_bytes, boa_delta_rule_work_bytes(d->lanes, d->T, d->heads, d->v_heads,
                                                          d->d_k, d->d_v, 1));
+    k.apart({g->dq.d, g->dk.d, g->dv.d, g->dg.d, g->dbeta.d, d_work},
+            {d->q.d, d->k.d, d->v.d, d->g.d, d->beta.d, d->d_state_in, d->d_lens, d_saved,
+             k.at(dout), d_dstate_out, g->d_dstate_in});
+    k.apart({g->d_dstate_in}, {d->q.d, d->k.d, d->v.d, d->g.d, d->beta.d, d->d_lens, d_saved,
+                               k.at(dout)});
     if (k.bad) return hipSuccess;
     a.f.saved = const_cast<float*>(d_saved);
     a.f.work = d_work;
@@ -2154,9 +2157,7 @@ int boa_sample_bytes(boa_ctx* c, const boa_rows* logits, const float* d_bias,
     k.bytes(d_bytes, byte_stride, "bytes");
     k.that(lanes == 1 || byte_stride >= T, "rows overlap: ", "bytes");
     k.floats(d_logp, 4, true, "logp");
-    k.that(k.bad || ((const void*)d_bytes != logits->d && (const void*)d_bytes != d_uniform &&
-                     (const void*)d_logp != logits->d && (!d_logp || d_logp != d_uniform)),
-           "an output is an input");
+    k.apart({d_bytes, d_logp}, {k.at(logits), d_bias, d_uniform, d_lens, d_params});
     if (k.bad) return hipSuccess;
     SampleArgs a{};
     a.q = Seqs{lanes, T, d_lens};

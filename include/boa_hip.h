@@ -254,7 +254,9 @@ int64_t boa_next_byte_loss_work_bytes(int32_t lanes, int32_t T);
 /* The recurrence of predictors that keep a matrix of associations instead of
  * the scan's vector, what stands around it in a block, and the choice of a
  * byte.  Rows, lane lengths, strides, types, workspaces, streams and capture
- * are as for the training operators above; row strides are at most 2^25. */
+ * are as for the training operators above; row strides are at most 2^25.  An
+ * output (or a workspace) that is an input or another output is refused, but for
+ * those named as in place below. */
 
 /* Root-mean-square norm of x + residual:
  *   h = x + residual    r = 1 / sqrt(mean h^2 + eps)    out = h r weight

@@ -2011,7 +2011,7 @@ int boa_int8_rows(boa_ctx* c, const boa_rows* x, const int32_t* d_lens, int32_t 
                   int32_t width, int32_t precision, const boa_rows* out8, float* d_scale8) {
   return train_call(c, "boa_int8_rows", [&](TrainCheck& k) {
     k.sizes(lanes, T, precision);
-    k.that(width >= 1 && width <= 8192, "width has to be 1 .. 8192");
+    k.that(width >= 1 && width <= 16384, "width has to be 1 .. 16384");
     k.in(x, "x"), k.near(x, "x");
     k.floats(d_lens, 4, true, "lens");
     k.rows8(out8, width, true, "out8");

@@ -134,6 +134,9 @@ template <typename T, int V, int G, int U, bool OUT8>
 __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a, uint32_t rows) {
   __shared__ double part[4];
   constexpr int R = 256 / G;  // rows of a block
+  // over 8192 columns: rows in 8 bits and nothing else, so neither weights nor a
+  // residual take registers
+  constexpr bool PLAIN = G * U * V > 8192;
   const int g = threadIdx.x % G;
   const uint32_t len = a.q.T;
   float w[U][V];
@@ -142,14 +145,14 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a, uint32_t ro
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int i = (u * G + g) * V + j;
-      w[u][j] = i < a.width ? (a.weight ? a.weight[i] : 1.0f) : 0.0f;
+      w[u][j] = PLAIN ? 1.0f : i < a.width ? (a.weight ? a.weight[i] : 1.0f) : 0.0f;
     }
   for (uint64_t b = (uint64_t)blockIdx.x * R; b < rows; b += (uint64_t)gridDim.x * R) {
     const uint64_t r = b + threadIdx.x / G;
     const uint32_t l = r < rows ? (uint32_t)r / len : 0, t = r < rows ? (uint32_t)r - l * len : 0;
     const bool live = r < rows && (int)t < seq_len(a.q, l);
     const T* x = (const T*)a.x.d + l * a.x.lane + t * a.x.row;
-    const T* res = a.res.d ? (const T*)a.res.d + l * a.res.lane + t * a.res.row : nullptr;
+    const T* res = !PLAIN && a.res.d ? (const T*)a.res.d + l * a.res.lane + t * a.res.row : nullptr;
     float h[U][V], hr[U][V];
     // no branch between a row's loads, each of which would wait for the last:
     // threads past its end read its first elements
@@ -178,7 +181,7 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a, uint32_t ro
           most = Most()(most, __builtin_fabsf((h[u][j] + hr[u][j]) * w[u][j]));
     }
     Root rn = {1.0f, 1.0f, 1.0f, 1.0f};
-    if (a.norm)
+    if (!PLAIN && a.norm)
       rn = root_of<G>([&](float by) {
         float ss = 0.0f;
 #pragma unroll
@@ -190,7 +193,7 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a, uint32_t ro
           }
         return ss;
       }, a.width, a.eps, (float*)part);
-    if (a.sum.d && live) {
+    if (!PLAIN && a.sum.d && live) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int i = (u * G + g) * V;
@@ -200,7 +203,7 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a, uint32_t ro
         if (i < a.width) store_row<V>((T*)a.sum.d + l * a.sum.lane + t * a.sum.row + i, s);
       }
     }
-    if (a.out.d && live) {
+    if (!PLAIN && a.out.d && live) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int i = (u * G + g) * V;
@@ -420,11 +423,18 @@ hipError_t norm_of(const NormArgs& a, hipStream_t s) {
   auto go = [&](auto G, auto U) {
     // eight blocks a CU, which keep the weight in registers from row to row
     const uint32_t blocks = std::min<uint32_t>(((uint64_t)rows * G + 255) / 256, 2048);
-    if (a.out8.d)
-      BOA_LAUNCH((norm_kernel<T, V, G, U, true>), blocks, 256, 0, s, a, rows);
-    else
-      BOA_LAUNCH((norm_kernel<T, V, G, U, false>), blocks, 256, 0, s, a, rows);
+    if constexpr (G * U * V <= 8192)
+      if (!a.out8.d) {
+        BOA_LAUNCH((norm_kernel<T, V, G, U, false>), blocks, 256, 0, s, a, rows);
+        return;
+      }
+    BOA_LAUNCH((norm_kernel<T, V, G, U, true>), blocks, 256, 0, s, a, rows);
   };
+  // rows in 8 bits without a norm may be as wide as the product takes them, 16384
+  if (a.width > 8192) {
+    go(std::integral_constant<int, 256>(), std::integral_constant<int, 64 / V>());
+    return hipGetLastError();
+  }
   const Shape sh = shape_of((a.width + V - 1) / V);
   if constexpr (V == 1) {
     if (sh.U == 32) {

@@ -284,7 +284,8 @@ int boa_rms_norm_grad(boa_ctx* ctx, const boa_rows* h, const float* d_weight,
                       const boa_rows* dx, float* d_dweight, void* d_work, int64_t work_bytes);
 int64_t boa_rms_norm_grad_work_bytes(int32_t lanes, int32_t T, int32_t width);
 
-/* Rows in 8 bits: out8 = rint(127 x / max |x|), scale8 = max |x| / 127. */
+/* Rows (1 .. 16384 wide) in 8 bits: out8 = rint(127 x / max |x|), scale8 =
+ * max |x| / 127. */
 int boa_int8_rows(boa_ctx* ctx, const boa_rows* x, const int32_t* d_lens, int32_t lanes, int32_t T,
                   int32_t width, int32_t precision, const boa_rows* out8, float* d_scale8);
 /* Weights [n][k] int8 (n 1 .. 65536 output channels, k 1 .. 16384), laid out

@@ -314,7 +314,10 @@ int boa_int8_matmul(boa_ctx* ctx, const boa_rows* x8, const float* d_scale8, con
  * fp32; d_state_in NULL is zero.  With T = 1 this is a decode step.  The order of
  * sums follows from the sizes (T, and for few long sequences lanes and v_heads
  * too), so the same sequence in another batch may differ in its last bits; the
- * same call gives the same bits.  Positions
+ * same call gives the same bits.  Up to 12 positions without d_saved are taken
+ * one after the other: the same bits as in single steps, in any batch.  Longer
+ * calls sum in another order, so what has to agree bit for bit, as an encoder and
+ * a decoder, has to take both in calls of up to 12.  Positions
  * are taken up to 64 at a time: a value that is not finite spoils the results of its
  * lane and head from the first of its 64 on, and none of other lanes. */
 typedef struct {

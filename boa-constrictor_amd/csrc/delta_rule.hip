@@ -1779,8 +1779,16 @@ int64_t local_floats(int64_t heads, const Cut& c, int dk, int dv, bool moves) {
 // Lanes of different lengths: the chains take the longest first where there are more
 // blocks than CUs, so that none starts late (64 x 521, 8 heads of 128 x 128, lengths
 // up to that: 145 and 168 us).  `at`: where the order is kept, of lanes' size.
+// Each lane is ranked among all of them, which takes what it brings from about 4000
+// lanes on and far more beyond.  With and without the order, whole calls of lanes up to
+// T long, one head of 64 x 64, bf16, us:
+//   lanes:       1000          2000          4000            16,000        65,535
+//   T = 100   69 and  69   125 and 120   271 and  249   1,388 and   938   11,763 and 3,779
+//   T = 520  184 and 207   355 and 380   721 and  717   3,117 and 2,702
+constexpr int ORDER_LANES = 2048;
 uint32_t* order_of(const DeltaArgs& a, uint64_t blocks, int chunks, const Cut& cut, void* at) {
-  return a.q.lens && cut.n == 1 && chunks > 1 && blocks > 256 ? (uint32_t*)at : nullptr;
+  return a.q.lens && cut.n == 1 && chunks > 1 && blocks > 256 && a.q.lanes <= ORDER_LANES
+             ? (uint32_t*)at : nullptr;
 }
 
 // Positions taken one after the other rather than in chunks: what a position takes
@@ -1941,7 +1949,7 @@ int64_t delta_work_bytes(int lanes, int T, int, int HV, int dk, int dv, bool gra
   // what a forward call needs, and a gradient's as well if it is to be one's
   int64_t floats = first + local_floats(heads, cut, dk, dv, true);
   if (grad) floats = std::max(floats, heads * chunks * record_floats(dk, dv) + 2 * first);
-  if (cut.n == 1) floats += (lanes + 3) / 4 * 4;  // the lanes' order
+  if (cut.n == 1) floats += std::min((lanes + 3) / 4 * 4, ORDER_LANES);  // the lanes' order
   return heads * chunks * PREP_BYTES + 4 * floats;
 }
 

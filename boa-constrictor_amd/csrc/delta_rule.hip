@@ -805,7 +805,9 @@ struct Segments {
 // The states from chunk to chunk and O.  A block's four waves, 16 columns of S, N
 // and O each, share K, Q, T, P and v in LDS (69 KB for bf16 rows and d_k up to 64, so
 // that two blocks share a CU: forward of 64 x 512, 4 heads of 64 and 128 columns, 105
-// us and not 123; 93 KB at 128, one block).  S stays in registers as the next
+// us and not 123; 93 KB at 128 and 91 KB for fp32 rows, one block: there a bound of two
+// saves registers only, which aligned rows do not lack and for which others spill, 227
+// and not 209 us for 64 x 512 fp32 rows in odd places).  S stays in registers as the next
 // product's right operand, so a wave has no exchange with others but the barriers
 // around a chunk's loads, which are a chunk ahead.  6 us a chunk, of which the matrix
 // instructions take a fifth.
@@ -815,7 +817,7 @@ struct Segments {
 // wave a SIMD.  O by a second wave beside the one that carries S: 102 us there, and a
 // prefill of 64 x 521, 8 heads of 128 x 128, 255 us in all and not 240.
 template <typename T, int DK, bool W, bool LOCAL>
-__global__ __launch_bounds__(256, DK == 64 ? 2 : 1) void delta_chain_kernel(
+__global__ __launch_bounds__(256, DK == 64 && (sizeof(T) == 2 || W) ? 2 : 1) void delta_chain_kernel(
     const DeltaArgs a, const unsigned char* prep, float* rec, int chunks, int tiles,
     const Segments seg, const uint32_t* order, uint32_t blocks) {
   using M = Mode<T>;

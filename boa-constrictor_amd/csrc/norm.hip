@@ -90,26 +90,32 @@ struct Most {  // NaN wins
   __device__ X operator()(X a, X b) const { return a != a ? a : (b > a || b != b ? b : a); }
 };
 
-// r of a row, as n = h before r after: the two others are 1, or a power of two on
-// the side where no product leaves fp32's range.  half: the square root of both.
+// A row's r: n = h r, where h may have been multiplied by a power of two, and what
+// the formula has r before is multiplied by `first` and by `second`, of which no
+// product leaves fp32's range before the result does.
 struct Root {
-  float before, r, after, half;
-  __device__ __forceinline__ float of(float h) const { return h * before * r * after; }
+  float r, first, second;
 };
-// squares(s): this thread's sum of (s h)^2.  From LEAST on, squares below the least
-// normal number are off by less than 2^-40 of the mean; up to MOST no sum of 8192 of
-// them overflows, and a NaN goes either way.
-template <int G, typename F>
-__device__ __forceinline__ Root root_of(const F& squares, int width, float eps, float* part) {
+// From the mean of h^2 plus eps as it is.  From LEAST on, squares below the least
+// normal number are off by less than 2^-40 of it; up to MOST no sum of 8192 of them
+// overflows.  Else scale(f) multiplies the row by f, and squares() sums it again (a
+// NaN goes either way): what f = 2^-71 takes from small elements is under 2^-129 of n.
+template <int G, typename S, typename F>
+__device__ __forceinline__ Root root_of(float mean, const S& scale, const F& squares, int width,
+                                        float eps, float* part) {
   constexpr float LEAST = 0x1p-110f, MOST = 0x1p100f;
-  const float mean = row_all<G>(squares(1.0f), Sum(), part) / (float)width + eps;
-  if (mean >= LEAST && mean < MOST) return {1.0f, 1.0f / __builtin_sqrtf(mean), 1.0f, 1.0f};
-  const bool small = mean < LEAST;
-  const float s = small ? 0x1p90f : 0x1p-80f;
-  const float again = row_all<G>(squares(s), Sum(), part) / (float)width + eps * s * s;
-  const float r = 1.0f / __builtin_sqrtf(again);
-  if (small) return {s, r, 1.0f, 0x1p45f};
-  return {1.0f, r, s, 0x1p-40f};
+  // a branch for the wave, whose other rows are multiplied by one: a divergent one
+  // takes registers for h twice
+  Root rn = {1.0f / __builtin_sqrtf(mean), 1.0f, 1.0f};
+  const bool small = mean < LEAST, within = mean >= LEAST && mean < MOST;
+  if (__any(!within)) {
+    const float f = within ? 1.0f : small ? 0x1p90f : 0x1p-71f;
+    scale(f);
+    rn.r = 1.0f / __builtin_sqrtf(row_all<G>(squares(), Sum(), part) / (float)width + eps * f * f);
+    if (!within) rn.first = small ? 0x1p45f : 0x1p-35f, rn.second = small ? 0x1p45f : 0x1p-36f;
+  }
+  rn.first *= rn.r;
+  return rn;
 }
 
 // 127 t / top to the nearest whole number.  f is the quotient in fp32, off by
@@ -130,8 +136,10 @@ __device__ __forceinline__ int step_of(float f, float x, float res, float w, dou
 // row is read once.  Bound by the bytes: 65,000 of 130,250 x 256 fp32 rows, two in
 // and two out, 53 us (5.0 TB/s); 33,360 x 512 bf16 rows with a sum and 8 bits, 36 us
 // (3.3 TB/s), where the quotients near a border, in 64 bits, take part of it.
+// (The bound: 64 registers and eight waves a SIMD for two vectors of bf16; left to
+// itself the compiler takes 66, and 39,000 x 256 rows 22 us and not 21.)
 template <typename T, int V, int G, int U, bool OUT8>
-__global__ __launch_bounds__(256) void norm_kernel(const NormArgs a, uint32_t rows) {
+__global__ __launch_bounds__(256, !OUT8 && V == 8 && U == 2 ? 8 : 1) void norm_kernel(const NormArgs a, uint32_t rows) {
   __shared__ double part[4];
   constexpr int R = 256 / G;  // rows of a block
   // over 8192 columns: rows in 8 bits and nothing else, so neither weights nor a
@@ -172,37 +180,41 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a, uint32_t ro
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if ((u * G + g) * V >= a.width) h[u][j] = hr[u][j] = 0.0f;
-    float most = 0.0f;
-    if constexpr (OUT8) {
+    // only rows in 8 bits need x and the residual for themselves
+    if constexpr (!OUT8) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          most = Most()(most, __builtin_fabsf((h[u][j] + hr[u][j]) * w[u][j]));
+        for (int j = 0; j < V; ++j) h[u][j] += hr[u][j];
     }
-    Root rn = {1.0f, 1.0f, 1.0f, 1.0f};
-    if (!PLAIN && a.norm)
-      rn = root_of<G>([&](float by) {
-        float ss = 0.0f;
+    auto sum = [&](int u, int j) { return OUT8 ? h[u][j] + hr[u][j] : h[u][j]; };
+    auto squares = [&] {
+      float ss = 0.0f;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float s = (h[u][j] + hr[u][j]) * by;
-            ss += s * s;
-          }
-        return ss;
-      }, a.width, a.eps, (float*)part);
+        for (int j = 0; j < V; ++j) ss += sum(u, j) * sum(u, j);
+      return ss;
+    };
+    float mean = 0.0f, rn = 1.0f;
+    if (!PLAIN && a.norm) mean = row_all<G>(squares(), Sum(), (float*)part) / (float)a.width + a.eps;
     if (!PLAIN && a.sum.d && live) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int i = (u * G + g) * V;
         float s[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) s[j] = h[u][j] + hr[u][j];
+        for (int j = 0; j < V; ++j) s[j] = sum(u, j);
         if (i < a.width) store_row<V>((T*)a.sum.d + l * a.sum.lane + t * a.sum.row + i, s);
       }
     }
+    if (!PLAIN && a.norm)
+      rn = root_of<G>(mean, [&](float f) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < V; ++j) h[u][j] *= f, OUT8 ? hr[u][j] *= f : 0.0f;
+      }, squares, a.width, a.eps, (float*)part).r;
     if (!PLAIN && a.out.d && live) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -210,12 +222,18 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a, uint32_t ro
         if (i < a.width) {
           float y[V];
 #pragma unroll
-          for (int j = 0; j < V; ++j) y[j] = rn.of(h[u][j] + hr[u][j]) * w[u][j];
+          for (int j = 0; j < V; ++j) y[j] = sum(u, j) * rn * w[u][j];
           store_row<V>((T*)a.out.d + l * a.out.lane + t * a.out.row + i, y);
         }
       }
     }
     if constexpr (OUT8) {
+      float most = 0.0f;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          most = Most()(most, __builtin_fabsf(sum(u, j) * w[u][j]));
       most = row_all<G>(most, Most(), (float*)part);
       // the greatest in 64 bits is among those next to the greatest in fp32
       // (all of them, where fp32 has few digits left or none)
@@ -253,8 +271,7 @@ __global__ __launch_bounds__(256) void norm_kernel(const NormArgs a, uint32_t ro
             }
           }
         }
-        if (g == 0)
-          a.scale8[r] = (float)(top * (double)rn.before * (double)rn.r * (double)rn.after / 127.0);
+        if (g == 0) a.scale8[r] = (float)(top * (double)rn / 127.0);
       }
     }
   }
@@ -307,33 +324,42 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(const NormGradArgs a, ui
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if ((u * G + g) * V >= a.width) h[u][j] = dy[u][j] = 0.0f;
-    const Root rn = root_of<G>([&](float by) {
+    auto squares = [&] {
       float ss = 0.0f;
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float s = h[u][j] * by;
-          ss += s * s;
-        }
+        for (int j = 0; j < V; ++j) ss += h[u][j] * h[u][j];
       return ss;
-    }, a.width, a.eps, part);
-    // sum of x w dy
-    auto along = [&](auto x) {
-      float c = 0.0f;
+    };
+    const float mean = row_all<G>(squares(), Sum(), part) / (float)a.width + a.eps;
+    float c = 0.0f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < V; ++j) c += h[u][j] * (w[u][j] * dy[u][j]);
+    c = row_all<G>(c, Sum(), part);
+    const Root rn = root_of<G>(mean, [&](float f) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < V; ++j) c += x(h[u][j]) * (w[u][j] * dy[u][j]);
-      return row_all<G>(c, Sum(), part);
-    };
+        for (int j = 0; j < V; ++j) h[u][j] *= f;
+    }, squares, a.width, a.eps, part);
     // the mean of n w dy: r taken out of the sum, unless its terms or their sum
     // leave fp32's range
-    const float c = along([](float x) { return x; }), cr = c * rn.r;
+    const float cr = c * rn.r;
     float m = cr / (float)a.width;
-    if (live && (rn.half != 1.0f || !(__builtin_fabsf(c) >= 0x1p-100f) ||
-                 !(__builtin_fabsf(cr) >= 0x1p-110f) || !(__builtin_fabsf(cr) < 0x1p120f)))
-      m = along([&](float x) { return rn.of(x); }) / (float)a.width;
+    const bool within = rn.second == 1.0f && __builtin_fabsf(c) >= 0x1p-100f &&
+                        __builtin_fabsf(cr) >= 0x1p-110f && __builtin_fabsf(cr) < 0x1p120f;
+    if (__any(live && !within)) {
+      c = 0.0f;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < V; ++j) c += h[u][j] * (rn.r * w[u][j]) * dy[u][j];
+      c = row_all<G>(c, Sum(), part) / (float)a.width;
+      if (!within) m = c;
+    }
     if (there) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -341,9 +367,9 @@ __global__ __launch_bounds__(256) void norm_grad_kernel(const NormGradArgs a, ui
         float dx[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float n = rn.of(h[u][j]);
+          const float n = h[u][j] * rn.r;
           if (live) dw[u][j] += dy[u][j] * n;
-          const float d = (w[u][j] * dy[u][j] - n * m) * rn.half * rn.r * rn.half;
+          const float d = rn.first * (w[u][j] * dy[u][j] - n * m) * rn.second;
           dx[j] = live ? d + ds[u][j] : 0.0f;
         }
         if (i < a.width) store_row<V>((T*)a.dx.d + l * a.dx.lane + t * a.dx.row + i, dx);

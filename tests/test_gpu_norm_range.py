@@ -94,3 +94,23 @@ def test_rows_without_gradients(codec):  # noqa: F811
     one = torch.ones((1, 1, 256), device="cuda")
     codec.rms_norm_grad(dev(x[2:3, 1:2]), dev(dy[2:3, 1:2]), one, eps=1e-6)
     assert torch.equal(one[0, 0], dx[2, 1])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("width", [64, 256, 4096])
+def test_rows_do_not_matter_to_each_other(codec, width, dtype):  # noqa: F811
+    """A row's bits are the same alone as beside rows of any size."""
+    x, g = rows(width, dtype, 7)
+    x, dy = dev(x), dev(torch.randn(x.shape, generator=g).to(dtype))
+
+    def run(x, dy):
+        out, dx, q = torch.zeros_like(x), torch.zeros_like(x), torch.zeros_like(x, dtype=torch.int8)
+        s8 = torch.zeros(x.shape[:2], device="cuda")
+        codec.rms_norm(x, out, d_out8=q, d_scale8=s8, eps=2.0 ** -116)
+        codec.rms_norm_grad(x, dy, dx, eps=2.0 ** -116)
+        return out, dx, q, s8
+
+    whole = run(x, dy)
+    for i in range(len(SIZES)):
+        for a, b in zip(run(x[:, i:i + 1].clone(), dy[:, i:i + 1].clone()), whole):
+            assert torch.equal(a, b[:, i:i + 1])

@@ -452,7 +452,8 @@ __device__ __forceinline__ void triangle(f4 (&acc)[4], const u4* tri, const Frag
 constexpr int CHAIN_COEF = 4 * C + 4, COEF = CHAIN_COEF + 6 * C;
 template <typename T>
 constexpr int IMAGE = 2 * TRI * Mode<T>::FULL * 64;  // 16-byte pieces of T and P
-constexpr int64_t PREP_BYTES = 2 * TRI * 3 * 1024 + COEF * 4;  // the larger of the types'
+// the larger of the types': bf16's, 39 KB; fp32 rows leave a third of it unused
+constexpr int64_t PREP_BYTES = 2 * TRI * 3 * 1024 + COEF * 4;
 
 // the block's sums of log decays and betas, by its first wave
 struct Decays {
@@ -809,8 +810,8 @@ struct Segments {
 // saves registers only, which aligned rows do not lack and for which others spill, 227
 // and not 209 us for 64 x 512 fp32 rows in odd places).  S stays in registers as the next
 // product's right operand, so a wave has no exchange with others but the barriers
-// around a chunk's loads, which are a chunk ahead.  6 us a chunk, of which the matrix
-// instructions take a fifth.
+// around a chunk's loads, which are a chunk ahead.  6 us a chunk; the matrix
+// instructions take 0.15 (d_k up to 64, with S and N kept) to 0.18 of the SIMDs' time.
 // Where S and N are kept for the gradient, their bytes bound it: 98 us for 32 x 1024
 // bf16 rows, 4 heads of 64 and 128 columns, 150 KB a chunk, 80 of them written, 3.1
 // TB/s.  Else the latency of a chunk's dependent products (S -> R -> N -> S), with one
@@ -1186,9 +1187,12 @@ __global__ __launch_bounds__(256) void delta_combine_kernel(const DeltaArgs a, c
 // registers: forward and gradient of 4 x 777 rows, 4 heads of 128 and 8 of 128
 // columns, 341 us and not 319.)  Bound by the two roles' waits for each other and by
 // the LDS between products: 194 us for 32 x 1024 rows, 4 heads of 64 and 128 columns,
-// 2.2 TB/s; the matrix instructions take a tenth.  K and Q kept in LDS rather than
+// 2.2 TB/s; the matrix instructions take 0.14.  K and Q kept in LDS rather than
 // in registers: 234; the products' operands brought one tile ahead in the first four
-// waves: 218.
+// waves: 218.  At 128 columns of k the second role's seven arrays (dq, dk, qo, ko, os,
+// rs, ns) are 224 registers: 218 to 272 are spilled, 600 to 700 bytes a lane, and with
+// 208 blocks of two value heads each a ragged 4 x 777 rows take 93 us.  At 64 columns
+// 31 (bf16, aligned) to 77 (fp32, not) are spilled.
 // dQ^T and dK^T [d_k][own] leave as four neighbouring columns a lane.
 template <typename T, int DK>
 struct LastLds {
@@ -1654,7 +1658,8 @@ __global__ __launch_bounds__(512, 2) void delta_grad_last_kernel(
 // columns 4 x .. 4 x + 3 of rows y + RG i.  With S^T k and S^T q of the state
 // before, o = scale (e^g S^T q + beta (k . q) e): one sum over the rows and
 // two barriers a position.  Bound by the states, read and written once: 1000 lanes
-// of 4 of 64 x 128, one position, 50 us, 5.2 TB/s, as fast as a copy.
+// of 4 of 64 x 128, one position, 58 us, 4.6 TB/s (a copy: 5.1); 50 where the caches
+// hold a part of the states.
 template <typename T, int DK, int CX, bool W>
 __global__ __launch_bounds__(256) void delta_step_kernel(const DeltaArgs a, uint64_t blocks) {
   constexpr int RG = 256 / CX, RPT = DK / RG;
@@ -1801,6 +1806,10 @@ uint32_t* order_of(const DeltaArgs& a, uint64_t blocks, int chunks, const Cut& c
 //   the same, bf16                  10 and 19     15 and 19     27 and 20
 //   64 lanes, 8 of 128 x 128, bf16  22 and 72     32 and 72     52 and 72
 //   1000 lanes, 4 of 64 x 128       78 and 455   115 and 457   191 and 459
+// T alone decides: what a call needs and whether its bits are those of single steps
+// must not depend on the batch, which a server fills as it can.  12 is where few lanes
+// break even; many lanes would up to about 40 positions, and pay up to 2.4 times in
+// between.
 bool by_steps(int T) { return T <= 12; }
 
 template <typename F>

@@ -151,17 +151,20 @@ __device__ __forceinline__ void put_results(const Int8Args& a, i32x4 (&acc)[4][4
   }
 }
 
-// Many rows: a block of four waves takes 128 rows x `group` tiles of 128
-// channels, a wave 64 x 64 of a tile (128 x 64, for which the weights would have
-// to come half as often, does not fit the registers of two waves a SIMD: 110 us
-// and not 71 for 33,360 x 2064 x 512, bf16).  64 KS of K at a time the rows lie in LDS
-// (all of K up to 512, brought once for the block's tiles); the weights come
-// straight from the caches into registers, one or two steps ahead and across
-// tiles.  Two blocks a CU, so one's stores overlap the other's products.  Blocks
-// that follow each other on an XCD take the groups of one row tile, whose rows
-// its L2 then holds.  33,360 x 2064 x 512, bf16: 71 us, 1.0 Pop/s and 2.2 TB/s;
-// bound by eight steps of products and then as much work for the results, which
-// two blocks a CU overlap only in part.
+// Many rows: a block of four waves takes 128 rows x `group` tiles of 128 channels, a
+// wave 64 x 64 of a tile (128 x 64, for which the weights would have to come half as
+// often, does not fit the registers of two waves a SIMD: 110 us and not 71 for 33,360 x
+// 2064 x 512, bf16, rows in the caches).  64 KS of K at a time the rows lie in LDS (all
+// of K up to 512, brought once for the block's tiles); the weights come straight from
+// the caches into registers, one or two steps ahead and across tiles.  Two blocks a CU,
+// so one's stores overlap the other's products.  Blocks that follow each other on an
+// XCD take the groups of one row tile, whose rows its L2 then holds.  33,360 x 2064 x
+// 512, bf16: 82 us, 0.86 Pop/s and 1.9 TB/s (73 with the same rows and results again,
+// which the caches hold); fp32 results 122.  Bound by eight steps of products, a fifth
+// of the time, and then as much work for the results, which two blocks a CU overlap
+// only in part.  Rows that are not wide are put together byte by byte, for which the
+// form of KS = 3 spills 112 to 118 registers and those of 5 .. 8 keep 128 bytes a lane
+// in scratch.
 template <typename T, int KS, bool WIDE>
 __global__ __launch_bounds__(256, 2) void int8_kernel(const Int8Args a, uint32_t rows, int ksteps,
                                                       uint32_t row_tiles, uint32_t col_tiles,

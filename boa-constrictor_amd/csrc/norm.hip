@@ -135,9 +135,10 @@ __device__ __forceinline__ int step_of(float f, float x, float res, float w, dou
 // G threads a row, which stays in registers from the sums to the results, so each
 // row is read once.  Bound by the bytes: 65,000 of 130,250 x 256 fp32 rows, two in
 // and two out, 53 us (5.0 TB/s); 33,360 x 512 bf16 rows with a sum and 8 bits, 36 us
-// (3.3 TB/s), where the quotients near a border, in 64 bits, take part of it.
+// (3.3 TB/s), 21 without the 8 bits: 480 vector instructions a row are issued 0.6 of
+// the time.
 // (The bound: 64 registers and eight waves a SIMD for two vectors of bf16; left to
-// itself the compiler takes 66, and 39,000 x 256 rows 22 us and not 21.)
+// itself the compiler takes 66, and 39,000 x 256 rows 24 us and not 21.)
 template <typename T, int V, int G, int U, bool OUT8>
 __global__ __launch_bounds__(256, !OUT8 && V == 8 && U == 2 ? 8 : 1) void norm_kernel(const NormArgs a, uint32_t rows) {
   __shared__ double part[4];
@@ -474,7 +475,8 @@ hipError_t norm_of(const NormArgs& a, hipStream_t s) {
 
 // Blocks of the gradient, each with its own partial sums: with 512, 1024, 2048 of
 // them 79, 61, 57 us (130,250 x 256, fp32), 13, 15, 22 (8103 x 512, bf16) and 40,
-// 39, 44 (32,768 x 1024, bf16)
+// 39, 44 (32,768 x 1024, bf16), all without dsum and with h as dout, too: 1024 is
+// never far from the best
 constexpr uint32_t GRAD_BLOCKS = 1024;
 uint32_t grad_blocks(int64_t rows, int G) {
   return (uint32_t)std::min<int64_t>((rows * G + 255) / 256, GRAD_BLOCKS);

@@ -144,7 +144,7 @@ __device__ __forceinline__ void sort_wave(double (&x)[4], int lane) {
 // A wave per row, bytes 4 i .. 4 i + 3 in lane i.  Bound by the vector
 // instructions, which the SIMDs issue without a pause: 1500 a row, of them 600 the
 // sort's where top_k or top_p ask for it, most others the exponentials' and the
-// sums' in 64 bits.  32,500 rows: 86 us; 64 rows: 7 us, what a launch takes.
+// sums' in 64 bits.  32,500 rows: 87 us; 64 rows: 7 us, what a launch takes.
 template <typename T>
 __global__ __launch_bounds__(256) void sample_kernel(const SampleArgs a, uint32_t rows, bool wide) {
   const int lane = threadIdx.x & 63;

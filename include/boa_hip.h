@@ -296,7 +296,8 @@ int64_t boa_int8_pack_bytes(int32_t n, int32_t k);
 /* out = scale8 wscale sum_k x8 w + bias: int8 rows x8 (k wide) with a scale
  * each, packed weights with a scale for each channel, d_bias [n] or NULL; out
  * rows (n wide) of the type `precision`.  The sums are exact, so a lane's
- * results do not depend on the other lanes or their number. */
+ * results do not depend on the other lanes or their number.  The two scales are
+ * multiplied first: their product has to be within fp32's normal range. */
 int boa_int8_matmul(boa_ctx* ctx, const boa_rows* x8, const float* d_scale8, const int32_t* d_lens,
                     int32_t lanes, int32_t T, int32_t k, const void* d_packed,
                     const float* d_wscale, int32_t n, const float* d_bias, int32_t precision,
@@ -308,7 +309,8 @@ int boa_int8_matmul(boa_ctx* ctx, const boa_rows* x8, const float* d_scale8, con
  * (a multiple of heads, at most 1024) of d_v (1 .. 128); v_heads / heads
  * neighbouring heads of v share one of q and k.  g (log decays) and beta are
  * fp32 rows v_heads wide, whatever `precision` is.  unit_qk: q and k are
- * divided by their lengths sqrt(sum of squares + 1e-6) first.  Row strides are
+ * divided by their lengths sqrt(sum of squares + 1e-6) first; the squares are
+ * summed in fp32, so values have to be below 1e18.  Row strides are
  * at most 2^23.  A log decay
  * below -1e4 (-inf too) forgets the state.  States [lanes][v_heads][d_k][d_v]
  * fp32; d_state_in NULL is zero.  With T = 1 this is a decode step.  The order of
@@ -347,7 +349,11 @@ int boa_delta_rule_grad(boa_ctx* ctx, const boa_delta* d, const float* d_saved,
 int64_t boa_delta_rule_saved_floats(int32_t lanes, int32_t T, int32_t heads, int32_t v_heads,
                                     int32_t d_k, int32_t d_v);
 /* Of both calls: grad 0 for the rule without d_saved (0 bytes where T is small),
- * 1 for it with d_saved and for its gradient. */
+ * 1 for it with d_saved and for its gradient.  Both grow with the positions: for
+ * every 64 of them, lane and head of v 39 KB of workspace, and where the gradient is
+ * wanted 4 d_v (d_k + 64) bytes (d_k as 64 or 128) of workspace and as many saved.
+ * Long prompts of many lanes are better taken in pieces, the states handed on: 64
+ * lanes of 16,384 with 8 heads ask for 5 GB at once. */
 int64_t boa_delta_rule_work_bytes(int32_t lanes, int32_t T, int32_t heads, int32_t v_heads,
                                   int32_t d_k, int32_t d_v, int32_t grad);
 

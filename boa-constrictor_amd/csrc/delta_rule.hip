@@ -818,7 +818,8 @@ struct Segments {
 // wave a SIMD.  O by a second wave beside the one that carries S: 102 us there, and a
 // prefill of 64 x 521, 8 heads of 128 x 128, 255 us in all and not 240.
 template <typename T, int DK, bool W, bool LOCAL>
-__global__ __launch_bounds__(256, DK == 64 && (sizeof(T) == 2 || W) ? 2 : 1) void delta_chain_kernel(
+__global__ __launch_bounds__(256, DK == 64 && (sizeof(T) == 2 || W) ? 2 : 1)
+void delta_chain_kernel(
     const DeltaArgs a, const unsigned char* prep, float* rec, int chunks, int tiles,
     const Segments seg, const uint32_t* order, uint32_t blocks) {
   using M = Mode<T>;

@@ -140,7 +140,8 @@ __device__ __forceinline__ int step_of(float f, float x, float res, float w, dou
 // (The bound: 64 registers and eight waves a SIMD for two vectors of bf16; left to
 // itself the compiler takes 66, and 39,000 x 256 rows 24 us and not 21.)
 template <typename T, int V, int G, int U, bool OUT8>
-__global__ __launch_bounds__(256, !OUT8 && V == 8 && U == 2 ? 8 : 1) void norm_kernel(const NormArgs a, uint32_t rows) {
+__global__ __launch_bounds__(256, !OUT8 && V == 8 && U == 2 ? 8 : 1) void norm_kernel(
+    const NormArgs a, uint32_t rows) {
   __shared__ double part[4];
   constexpr int R = 256 / G;  // rows of a block
   // over 8192 columns: rows in 8 bits and nothing else, so neither weights nor a
